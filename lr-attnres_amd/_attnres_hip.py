@@ -30,6 +30,7 @@ PHASE1_MAX_QUERIES = 16
 PHASE_MAX_DIM = 4096
 SITE_LOGITS_MAX_QUERIES = 256
 SITE_LOGITS_MAX_RANK = 128
+QKV_ROTARY_MAX_HEAD_DIM = 1024
 FLT_EPSILON = float(torch.finfo(torch.float32).eps)
 
 
@@ -225,6 +226,22 @@ class ValueKeyDesc(ctypes.Structure):
                 ("norm_eps", c_float), ("values", POINTER(c_void_p)), ("value_row_stride", POINTER(c_int64))]
 
 
+class QkvRotaryDesc(ctypes.Structure):
+    """attnres_qkv_rotary_desc (include/attnres_sublayers.h)."""
+    _fields_ = [("dtype", c_int32), ("table_dtype", c_int32), ("batch", c_int64), ("tokens", c_int64),
+                ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("qk_norm", c_int32),
+                ("norm_eps", c_float), ("qkv", c_void_p), ("batch_stride", c_int64), ("token_stride", c_int64),
+                ("sin", c_void_p), ("cos", c_void_p), ("table_rows", c_int64), ("table_row_stride", c_int64),
+                ("positions", c_void_p), ("positions_batch_stride", c_int64), ("positions_token_stride", c_int64),
+                ("start", c_int64)]
+
+
+class SwigluDesc(ctypes.Structure):
+    """attnres_swiglu_desc (include/attnres_sublayers.h)."""
+    _fields_ = [("dtype", c_int32), ("n_tok", c_int64), ("dim", c_int32), ("hidden", c_int32), ("x", c_void_p),
+                ("x_row_stride", c_int64), ("weight", c_void_p), ("weight_row_stride", c_int64)]
+
+
 def load() -> ctypes.CDLL:
     """Load the HIP library once; raise with a build hint if it is missing."""
     global _lib
@@ -322,6 +339,22 @@ def load() -> ctypes.CDLL:
     lib.attnres_value_keys_backward.argtypes = [POINTER(ValueKeyDesc), c_void_p, c_int32, POINTER(c_void_p), c_void_p,
                                                 POINTER(c_float), POINTER(c_void_p), c_void_p, c_void_p, c_size_t,
                                                 c_void_p]
+    lib.attnres_qkv_rotary_forward.restype = c_int
+    lib.attnres_qkv_rotary_forward.argtypes = [POINTER(QkvRotaryDesc), c_void_p, c_void_p, c_void_p]
+    lib.attnres_qkv_rotary_backward.restype = c_int
+    lib.attnres_qkv_rotary_backward.argtypes = [POINTER(QkvRotaryDesc), POINTER(c_void_p), POINTER(c_int64), c_void_p,
+                                                c_void_p]
+    lib.attnres_swiglu_saved_row_stride.restype = c_int64
+    lib.attnres_swiglu_saved_row_stride.argtypes = [POINTER(SwigluDesc)]
+    lib.attnres_swiglu_forward_workspace_size.restype = c_size_t
+    lib.attnres_swiglu_forward_workspace_size.argtypes = [POINTER(SwigluDesc)]
+    lib.attnres_swiglu_backward_workspace_size.restype = c_size_t
+    lib.attnres_swiglu_backward_workspace_size.argtypes = [POINTER(SwigluDesc), c_int32, c_int32]
+    lib.attnres_swiglu_forward.restype = c_int
+    lib.attnres_swiglu_forward.argtypes = [POINTER(SwigluDesc), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.attnres_swiglu_backward.restype = c_int
+    lib.attnres_swiglu_backward.argtypes = [POINTER(SwigluDesc), c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_size_t, c_void_p]
     lib.attnres_kernel_timing.restype = c_int
     lib.attnres_kernel_timing.argtypes = [c_int]
     lib.attnres_test_phase2_block_layout.restype = c_int
@@ -1115,3 +1148,85 @@ def value_keys_backward(d: ValueKey, weight, grad_keys, keys, inv_rms, want_valu
                                          _ptr(dw), _ptr(ws), ws_bytes, _stream(dev))
     _check(rc, "value keys backward")
     return dvals, dw
+
+
+# ------------------------------------------------------------------ the sublayers around the reads
+
+def qkv_rotary_desc(qkv, sin, cos, positions, start: int, q_heads: int, kv_heads: int, qk_norm: bool) -> QkvRotaryDesc:
+    """qkv [B, T, (q_heads + 2 kv_heads) Dh] with a contiguous last dim; sin, cos [rows, Dh / 2] of one row stride;
+    positions [B, T] int64 or None."""
+    B, T, C = qkv.shape
+    d = QkvRotaryDesc()
+    d.dtype, d.table_dtype = DTYPE_CODE[qkv.dtype], DTYPE_CODE[sin.dtype]
+    d.batch, d.tokens = B, T
+    d.q_heads, d.kv_heads, d.head_dim = q_heads, kv_heads, C // (q_heads + 2 * kv_heads)
+    d.qk_norm, d.norm_eps = int(qk_norm), FLT_EPSILON
+    d.qkv = qkv.data_ptr()
+    # (a dimension of one is never stepped over: its stride may be anything)
+    d.batch_stride, d.token_stride = qkv.stride(0) if B > 1 else 0, qkv.stride(1) if T > 1 else 0
+    d.sin, d.cos = sin.data_ptr(), cos.data_ptr()
+    d.table_rows, d.table_row_stride = sin.size(0), sin.stride(0) if sin.size(0) > 1 else sin.size(1)
+    if positions is not None:
+        d.positions = positions.data_ptr()
+        d.positions_batch_stride, d.positions_token_stride = positions.stride()
+    d.start = start
+    return d
+
+
+def qkv_rotary_forward(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm):
+    """(q [B, q_heads, T, Dh], k [B, kv_heads, T, Dh])"""
+    d = qkv_rotary_desc(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm)
+    q = qkv.new_empty((d.batch, q_heads, d.tokens, d.head_dim))
+    k = qkv.new_empty((d.batch, kv_heads, d.tokens, d.head_dim))
+    _check(load().attnres_qkv_rotary_forward(ctypes.byref(d), _ptr(q), _ptr(k), _stream(qkv.device)),
+           "qkv rotary forward")
+    return q, k
+
+
+def qkv_rotary_backward(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm, grads):
+    """The projection's gradient [B, T, C] from those of q, k and v ([B, heads, T, Dh], or None)."""
+    d = qkv_rotary_desc(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm)
+    grads = [g if g is None or g.stride(-1) == 1 or g.size(-1) == 1 else g.contiguous() for g in grads]
+    ptrs = (c_void_p * 3)(*[None if g is None else g.data_ptr() for g in grads])
+    strides = (c_int64 * 9)()
+    for i, g in enumerate(grads):
+        for j in range(3):
+            strides[3 * i + j] = 0 if g is None or g.size(j) == 1 else g.stride(j)
+    out = qkv.new_empty(qkv.shape)
+    _check(load().attnres_qkv_rotary_backward(ctypes.byref(d), ptrs, strides, _ptr(out), _stream(qkv.device)),
+           "qkv rotary backward")
+    return out
+
+
+def swiglu_desc(x, weight) -> SwigluDesc:
+    """x [n, D] and weight [2 F, D], contiguous last dims"""
+    d = SwigluDesc()
+    d.dtype, d.n_tok, d.dim, d.hidden = DTYPE_CODE[x.dtype], x.size(0), x.size(1), weight.size(0) // 2
+    d.x, d.x_row_stride = x.data_ptr(), x.stride(0) if x.size(0) > 1 else x.size(1)
+    d.weight, d.weight_row_stride = weight.data_ptr(), weight.stride(0)
+    return d
+
+
+def swiglu_forward(x, weight, save: bool):
+    """(h [n, F], what the backward needs of the projections, or None)"""
+    lib, d = load(), swiglu_desc(x, weight)
+    h = x.new_empty((d.n_tok, d.hidden))
+    saved = x.new_empty((2, d.n_tok, lib.attnres_swiglu_saved_row_stride(ctypes.byref(d)))) if save else None
+    n = lib.attnres_swiglu_forward_workspace_size(ctypes.byref(d))
+    ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
+    _check(lib.attnres_swiglu_forward(ctypes.byref(d), _ptr(h), _ptr(saved), _ptr(ws), n, _stream(x.device)),
+           "swiglu forward")
+    return h, saved
+
+
+def swiglu_backward(x, weight, saved, grad_h, want_dx: bool, want_dweight: bool):
+    """(dx [n, D] or None, dweight [2 F, D] or None)"""
+    lib, d = load(), swiglu_desc(x, weight)
+    dx = x.new_empty((d.n_tok, d.dim)) if want_dx else None
+    dw = x.new_empty((2 * d.hidden, d.dim)) if want_dweight else None
+    n = lib.attnres_swiglu_backward_workspace_size(ctypes.byref(d), int(want_dx), int(want_dweight))
+    ws = torch.empty((max(n, 1),), dtype=torch.uint8, device=x.device)
+    _check(lib.attnres_swiglu_backward(ctypes.byref(d), _ptr(grad_h), grad_h.stride(0) if d.n_tok > 1 else d.hidden,
+                                       _ptr(saved), _ptr(dx), _ptr(dw), _ptr(ws), n, _stream(x.device)),
+           "swiglu backward")
+    return dx, dw

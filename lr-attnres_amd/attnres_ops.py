@@ -341,7 +341,7 @@ _NATIVE = None
 _BOUND = {name: getattr(_hip, name) for name in (
     "forward", "backward", "phase1_forward", "phase1_backward_sites", "phase1_bank_forward", "phase1_bank_backward",
     "phase2_forward", "phase2_backward", "accum_read_forward", "accum_read_backward", "block_accum_forward",
-    "block_accum_backward")}
+    "block_accum_backward", "qkv_rotary_forward", "qkv_rotary_backward", "swiglu_forward", "swiglu_backward")}
 
 
 def _native(fwd: str, bwd: str):
@@ -1848,3 +1848,214 @@ def lrid_block_accumulate_read(projected: Tensor, partial_value: Optional[Tensor
             bool(normalize_output), float(logit_scale), bias_value, scale_value, bool(scale_key), qrow)
     value, key, out = _AccumReadFn.apply(meta, y, pv, pk, bank, inter, lse, bias_t, scale_t)
     return value.view(B, T, D), key.view(B, T, R), out.view(B, T, D)
+
+
+# ------------------------------------------------------------------ the sublayers around the reads
+
+@torch.library.custom_op("attnres_hip::qkv_rotary", mutates_args=())
+def _qkv_rotary_op(qkv: Tensor, sin: Tensor, cos: Tensor, positions: Optional[Tensor], start: int, q_heads: int,
+                   kv_heads: int, qk_norm: bool) -> tuple[Tensor, Tensor]:
+    with _device_ctx(qkv.device):
+        return _hip.qkv_rotary_forward(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm)
+
+
+@_qkv_rotary_op.register_fake
+def _qkv_rotary_fake(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm):
+    B, T, C = qkv.shape
+    Dh = C // (q_heads + 2 * kv_heads)
+    return qkv.new_empty((B, q_heads, T, Dh)), qkv.new_empty((B, kv_heads, T, Dh))
+
+
+@torch.library.custom_op("attnres_hip::qkv_rotary_backward", mutates_args=())
+def _qkv_rotary_backward_op(qkv: Tensor, sin: Tensor, cos: Tensor, positions: Optional[Tensor], grad_q: Optional[Tensor],
+                            grad_k: Optional[Tensor], start: int, q_heads: int, kv_heads: int,
+                            qk_norm: bool) -> Tensor:
+    with _device_ctx(qkv.device):
+        return _hip.qkv_rotary_backward(qkv, sin, cos, positions, start, q_heads, kv_heads, qk_norm,
+                                        [grad_q, grad_k, None])
+
+
+@_qkv_rotary_backward_op.register_fake
+def _qkv_rotary_backward_fake(qkv, sin, cos, positions, grad_q, grad_k, start, q_heads, kv_heads, qk_norm):
+    return qkv.new_empty(qkv.shape)
+
+
+def _qkv_rotary_setup_context(ctx, inputs, output):
+    qkv, sin, cos, positions, *ctx.args = inputs
+    ctx.save_for_backward(qkv, sin, cos, positions)
+
+
+def _qkv_rotary_backward(ctx, grad_q, grad_k):
+    qkv, sin, cos, positions = ctx.saved_tensors
+    # (a saved-tensor hook may give back another layout)
+    qkv, sin, cos = _last_dense(qkv), sin.contiguous(), cos.contiguous()
+    d = _qkv_rotary_backward_op(qkv, sin, cos, positions, grad_q, grad_k, *ctx.args)
+    return d, None, None, None, None, None, None, None
+
+
+_qkv_rotary_op.register_autograd(_qkv_rotary_backward, setup_context=_qkv_rotary_setup_context)
+
+
+def _last_dense(t: Tensor) -> Tensor:
+    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _weight_rows(t: Tensor) -> Tensor:
+    return t if (t.size(1) == 1 or t.stride(1) == 1) and t.stride(0) >= t.size(1) else t.contiguous()
+
+
+_POSITION_TYPES = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
+
+
+def qkv_norm_rotary(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, positions=None,
+                    num_kv_heads: Optional[int] = None, qk_norm: bool = True):
+    """Attention's heads from a fused query / key / value projection, in one HIP pass each way.
+
+    Not in the reference's op module: the reference's attention does this as a split, three transposes, ``norm`` of the
+    query and key heads and ``rope.rotate`` of both (model.py:478-506, 28-31, 291-313), about a dozen passes over them.
+
+    ``qkv`` [B, T, (num_heads + 2 num_kv_heads) Dh]: query, key and value heads (``num_kv_heads``: as many as query heads
+    unless given).  Query and key heads are rms-normed over Dh (``qk_norm``; torch's default eps) and rotated by interleaved
+    pairs, all in fp32 with one rounding to the dtype (the reference rounds the normed head, each product and each sum).
+    ``sin``, ``cos``: tables [..., rows, Dh / 2] (as ``RotaryEmbedding``'s buffers), fp32 or in ``qkv``'s dtype.
+    ``positions``: None (token t takes row t), an int (row ``positions`` + t), or an integer tensor [T] or [B, T] of rows;
+    a row outside the tables gives NaN in that token's queries and keys (a tensor's values are not looked at on the host).
+
+    Returns ``q`` [B, num_heads, T, Dh] and ``k`` [B, num_kv_heads, T, Dh], dense, and ``v`` [B, num_kv_heads, T, Dh], a
+    view into ``qkv`` (not to be modified in place while a gradient is to come).  The backward writes the projection's
+    whole gradient, the values' part included; ``sin`` and ``cos`` take none.
+    """
+    what = "qkv_norm_rotary"
+    H, K = int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads)
+    nat = _native("qkv_rotary_forward", "qkv_rotary_backward")
+    if nat:
+        out = nat.qkv_rotary(qkv, H, K, sin, cos, positions, bool(qk_norm))
+        if out is not None:
+            return out
+    if qkv.dim() != 3:
+        raise RuntimeError(f"{what}: qkv must be [B, T, heads * head_dim], got {tuple(qkv.shape)}")
+    if qkv.dtype not in _ALLOWED:
+        raise RuntimeError(f"{what}: dtype {qkv.dtype} is not supported (fp32, bf16, fp16)")
+    if H < 1 or K < 1:
+        raise RuntimeError(f"{what}: num_heads and num_kv_heads must be >= 1, got {H} and {K}")
+    B, T, C = qkv.shape
+    if C == 0 or C % (H + 2 * K) != 0 or (C // (H + 2 * K)) % 2 != 0:
+        raise RuntimeError(f"{what}: {C} columns are not {H} + 2 * {K} heads of an even width")
+    Dh = C // (H + 2 * K)
+    if Dh > _hip.QKV_ROTARY_MAX_HEAD_DIM:
+        raise RuntimeError(f"{what}: head width {Dh} above {_hip.QKV_ROTARY_MAX_HEAD_DIM}")
+    for name, t in (("sin", sin), ("cos", cos)):
+        if t.dim() < 2 or t.size(-1) != Dh // 2:
+            raise RuntimeError(f"{what}: {name} must be [..., rows, {Dh // 2}], got {tuple(t.shape)}")
+        if t.requires_grad:
+            raise RuntimeError(f"{what}: {name} takes no gradient")
+        if not t.is_floating_point():
+            raise RuntimeError(f"{what}: {name} must be a floating-point table, got {t.dtype}")
+    if sin.shape != cos.shape:
+        raise RuntimeError(f"{what}: sin {tuple(sin.shape)} and cos {tuple(cos.shape)} differ in shape")
+    dev = _check_gpu([qkv, sin, cos], what)
+    table = qkv.dtype if sin.dtype == cos.dtype == qkv.dtype else torch.float32
+    sin, cos = (t.to(table).reshape(-1, Dh // 2).contiguous() for t in (sin, cos))
+    rows, start, at = sin.size(0), 0, None
+    if isinstance(positions, Tensor):
+        if positions.dtype not in _POSITION_TYPES:
+            raise RuntimeError(f"{what}: positions must be integers, got {positions.dtype}")
+        if positions.shape != (T,) and positions.shape != (B, T):
+            raise RuntimeError(f"{what}: positions must be [{T}] or [{B}, {T}], got {tuple(positions.shape)}")
+        _check_gpu([qkv, positions], what)
+        at = positions.to(torch.int64).expand(B, T)
+    elif positions is not None:
+        if isinstance(positions, bool) or not isinstance(positions, int):
+            raise RuntimeError(f"{what}: positions must be None, an int or an integer tensor, got {type(positions)}")
+        start = positions
+    if at is None and B * T > 0 and (start < 0 or start + T > rows):
+        raise RuntimeError(f"{what}: rows {start} .. {start + T - 1} are outside the tables' {rows}")
+    qkv = _last_dense(qkv)
+    v = qkv[..., (H + K) * Dh:].view(B, T, K, Dh).transpose(1, 2)
+    if B * T == 0:  # nothing to compute; differentiable all the same
+        return (qkv[..., :H * Dh].reshape(B, T, H, Dh).transpose(1, 2),
+                qkv[..., H * Dh:(H + K) * Dh].reshape(B, T, K, Dh).transpose(1, 2), v)
+    q, k = _qkv_rotary_op(qkv, sin, cos, at, start, H, K, bool(qk_norm))
+    return q, k, v
+
+
+@torch.library.custom_op("attnres_hip::swiglu", mutates_args=())
+def _swiglu_op(x: Tensor, weight: Tensor, save: bool) -> tuple[Tensor, Tensor]:
+    with _device_ctx(x.device):
+        h, saved = _hip.swiglu_forward(x, weight, save)
+    return h, saved if saved is not None else x.new_empty((0,))
+
+
+@_swiglu_op.register_fake
+def _swiglu_fake(x, weight, save):
+    n, F_ = x.size(0), weight.size(0) // 2
+    step = 16 if x.dtype == torch.float32 else 32  # (hidden columns of a k step of the products)
+    return x.new_empty((n, F_)), x.new_empty((2, n, (F_ + step - 1) // step * step) if save else (0,))
+
+
+@torch.library.custom_op("attnres_hip::swiglu_backward", mutates_args=())
+def _swiglu_backward_op(x: Tensor, weight: Tensor, saved: Tensor, grad_h: Tensor, want_dx: bool,
+                        want_dweight: bool) -> tuple[Tensor, Tensor]:
+    with _device_ctx(x.device):
+        dx, dw = _hip.swiglu_backward(x, weight, saved, grad_h, want_dx, want_dweight)
+    return tuple(t if t is not None else x.new_empty((0,)) for t in (dx, dw))
+
+
+@_swiglu_backward_op.register_fake
+def _swiglu_backward_fake(x, weight, saved, grad_h, want_dx, want_dweight):
+    return x.new_empty(x.shape if want_dx else (0,)), x.new_empty(weight.shape if want_dweight else (0,))
+
+
+def _swiglu_setup_context(ctx, inputs, output):
+    x, weight, _ = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, weight, output[1])
+
+
+def _swiglu_backward(ctx, grad_h, grad_saved):
+    if grad_h is None:
+        return None, None, None
+    x, weight, saved = ctx.saved_tensors
+    want = ctx.needs_input_grad
+    # (a saved-tensor hook may give back another layout)
+    dx, dw = _swiglu_backward_op(_last_dense(x), _weight_rows(weight), saved.contiguous(), _last_dense(grad_h), want[0],
+                                 want[1])
+    return dx if want[0] else None, dw if want[1] else None, None
+
+
+_swiglu_op.register_autograd(_swiglu_backward, setup_context=_swiglu_setup_context)
+
+
+def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
+    """A gated feed-forward block up to its output projection: ``(x @ W_up^T) * silu(x @ W_gate^T)``.
+
+    Not in the reference's op module: the reference's MLP does this as a linear layer, a chunk, ``silu`` and a product
+    (model.py:572-589).  Here the matrix-core kernel that forms both projections applies the activation and the product to
+    the fp32 sums, with one rounding to the dtype; the backward forms the projections' gradient in one pass and multiplies
+    it by the weight and the input.
+
+    ``x`` [..., D]; ``weight`` [2 F, D], rows ``[0, F)`` up and ``[F, 2 F)`` gate (``nn.Linear(D, 2 F, bias=False).weight``
+    with ``[up, gate] = fc1(x).chunk(2)``), taken in ``x``'s dtype.  Returns [..., F].  For the backward both projections
+    are kept in the dtype, as the linear layer's output would be.
+    """
+    what = "swiglu_projection"
+    nat = _native("swiglu_forward", "swiglu_backward")
+    if nat:
+        out = nat.swiglu(x, weight)
+        if out is not None:
+            return out
+    if x.dim() < 1:
+        raise RuntimeError(f"{what}: x must be [..., D]")
+    if x.dtype not in _ALLOWED:
+        raise RuntimeError(f"{what}: dtype {x.dtype} is not supported (fp32, bf16, fp16)")
+    D = x.size(-1)
+    if weight.dim() != 2 or weight.size(1) != D or weight.size(0) < 2 or weight.size(0) % 2 != 0 or D < 1:
+        raise RuntimeError(f"{what}: weight must be [2 F, {D}], got {tuple(weight.shape)}")
+    if not weight.is_floating_point():
+        raise RuntimeError(f"{what}: weight must be a floating-point tensor, got {weight.dtype}")
+    _check_gpu([x, weight], what)
+    w = _weight_rows(weight.to(x.dtype))
+    rows = _last_dense(x.reshape(-1, D))
+    save = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+    h, _ = _swiglu_op(rows, w, save)
+    return h.view(*x.shape[:-1], w.size(0) // 2)

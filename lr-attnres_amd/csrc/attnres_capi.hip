@@ -14,6 +14,7 @@
 #include "attnres_launch.h"
 #include "attnres_lr_split.h"
 #include "attnres_params.h"
+#include "attnres_sublayers.h"
 
 using namespace attnres;
 
@@ -69,6 +70,20 @@ int fail(int code, const char* fmt, ...) {
   g_last_error = buf;
   return code;
 }
+
+}  // namespace
+
+int attnres::api_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return code;
+}
+
+namespace {
 
 int elem_size(int dtype) { return dtype == ATTNRES_DTYPE_F32 ? 4 : 2; }
 

@@ -1,0 +1,402 @@
+// C ABI of the sublayer kernels: argument checks, kernel selection and launch
+// geometry.  Declared in include/attnres_sublayers.h.
+#include <string.h>
+
+#include "../../include/attnres_sublayers.h"
+#include "attnres_sublayers.h"
+#include "attnres_swiglu.h"
+
+using namespace attnres;
+
+namespace {
+
+int es_of(int dtype) { return dtype == ATTNRES_DTYPE_F32 ? 4 : 2; }
+bool known(int dtype) {
+  return dtype == ATTNRES_DTYPE_F32 || dtype == ATTNRES_DTYPE_BF16 || dtype == ATTNRES_DTYPE_F16;
+}
+bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+
+int check_rotary(const attnres_qkv_rotary_desc* d) {
+  if (!d) return api_fail(ATTNRES_EINVAL, "desc is NULL");
+  if (!known(d->dtype)) return api_fail(ATTNRES_EINVAL, "unknown dtype %d", d->dtype);
+  if (d->table_dtype != ATTNRES_DTYPE_F32 && d->table_dtype != d->dtype)
+    return api_fail(ATTNRES_EINVAL, "table dtype %d is neither fp32 nor the values' %d", d->table_dtype, d->dtype);
+  if (d->batch < 0 || d->tokens < 0)
+    return api_fail(ATTNRES_EINVAL, "batch=%lld, tokens=%lld must be >= 0", (long long)d->batch, (long long)d->tokens);
+  if (d->q_heads < 1 || d->kv_heads < 1 || d->q_heads > (1 << 20) || d->kv_heads > (1 << 20))
+    return api_fail(ATTNRES_EINVAL, "q_heads=%d, kv_heads=%d must be >= 1", d->q_heads, d->kv_heads);
+  if (d->head_dim < 2 || d->head_dim % 2)
+    return api_fail(ATTNRES_EINVAL, "head_dim=%d must be even and >= 2", d->head_dim);
+  if (d->head_dim > ATTNRES_QKV_ROTARY_MAX_HEAD_DIM)
+    return api_fail(ATTNRES_EUNSUPPORTED, "head_dim=%d above %d", d->head_dim, ATTNRES_QKV_ROTARY_MAX_HEAD_DIM);
+  if (d->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (d->batch > INT64_MAX / d->tokens || d->batch * d->tokens > (int64_t)1 << 40)
+    return api_fail(ATTNRES_EUNSUPPORTED, "too many tokens");
+  if (!d->qkv || !d->sin || !d->cos) return api_fail(ATTNRES_EINVAL, "qkv / sin / cos is NULL");
+  if (d->batch_stride < 0 || d->token_stride < 0)
+    return api_fail(ATTNRES_EINVAL, "batch_stride and token_stride must be >= 0");
+  if (d->table_rows < 1) return api_fail(ATTNRES_EINVAL, "table_rows=%lld < 1", (long long)d->table_rows);
+  if (d->table_row_stride < d->head_dim / 2)
+    return api_fail(ATTNRES_EINVAL, "table_row_stride=%lld below head_dim / 2 = %d", (long long)d->table_row_stride,
+                    d->head_dim / 2);
+  if (!d->positions && (d->start < 0 || d->start > d->table_rows - d->tokens))
+    return api_fail(ATTNRES_EINVAL, "rows %lld .. %lld are outside the tables' %lld", (long long)d->start,
+                    (long long)(d->start + d->tokens - 1), (long long)d->table_rows);
+  return ATTNRES_OK;
+}
+
+void fill_rotary(const attnres_qkv_rotary_desc* d, QkvRotaryParams* p) {
+  memset(p, 0, sizeof(*p));
+  p->qkv = d->qkv;
+  p->b_stride = d->batch_stride;
+  p->t_stride = d->token_stride;
+  p->n_tok = d->batch * d->tokens;
+  p->tokens = d->tokens;
+  p->q_heads = d->q_heads;
+  p->kv_heads = d->kv_heads;
+  p->head_dim = d->head_dim;
+  p->qk_norm = d->qk_norm != 0;
+  p->eps = d->norm_eps;
+  p->sin = d->sin;
+  p->cos = d->cos;
+  p->table_rows = d->table_rows;
+  p->table_stride = d->table_row_stride;
+  p->pos = d->positions;
+  p->pos_b_stride = d->positions_batch_stride;
+  p->pos_t_stride = d->positions_token_stride;
+  p->start = d->start;
+}
+
+// The widest vector that every row starts at a multiple of, and the lanes that
+// cover a head with it; vec 1 is the general kernel (any alignment).
+void rotary_layout(const attnres_qkv_rotary_desc* d, const QkvRotaryParams& p, int* vec, int* lanes, int* chunks) {
+  const int es = es_of(d->dtype), ts = es_of(d->table_dtype), Dh = d->head_dim;
+  for (int v = es == 4 ? 4 : 8; v >= 2; v /= 2) {
+    bool ok = Dh % v == 0 && aligned(p.qkv, (int64_t)v * es) && p.b_stride % v == 0 && p.t_stride % v == 0 &&
+              aligned(p.sin, (int64_t)v / 2 * ts) && aligned(p.cos, (int64_t)v / 2 * ts) &&
+              p.table_stride % (v / 2) == 0 && aligned(p.q, (int64_t)v * es) && aligned(p.k, (int64_t)v * es) &&
+              aligned(p.dqkv, (int64_t)v * es);
+    for (int i = 0; i < 3 && ok; ++i) {
+      if (!p.grad[i]) continue;
+      ok = aligned(p.grad[i], (int64_t)v * es);
+      for (int j = 0; j < 3; ++j) ok = ok && p.grad_stride[i][j] % v == 0;
+    }
+    if (!ok) continue;
+    *chunks = 1;
+    for (*lanes = v == 8 ? 4 : v == 4 ? 8 : 32; *lanes <= (v == 8 ? 32 : 64); *lanes *= 2)
+      if (*lanes * v >= Dh) {
+        *vec = v;
+        return;
+      }
+    if (v == 2 && Dh <= 256) {
+      *vec = 2;
+      *lanes = 64;
+      *chunks = 2;
+      return;
+    }
+  }
+  *vec = *lanes = *chunks = 1;
+}
+
+}  // namespace
+
+extern "C" int attnres_qkv_rotary_forward(const attnres_qkv_rotary_desc* d, void* q, void* k, void* stream) {
+  if (int rc = check_rotary(d)) return rc;
+  if (d->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (!q || !k) return api_fail(ATTNRES_EINVAL, "q / k is NULL");
+  QkvRotaryParams p;
+  fill_rotary(d, &p);
+  p.q = q;
+  p.k = k;
+  int vec, lanes, chunks;
+  rotary_layout(d, p, &vec, &lanes, &chunks);
+  const hipError_t err = launch_qkv_rotary(d->dtype, d->table_dtype == ATTNRES_DTYPE_F32, false, p, vec, lanes, chunks,
+                                           (hipStream_t)stream);
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "qkv rotary forward launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}
+
+extern "C" int attnres_qkv_rotary_backward(const attnres_qkv_rotary_desc* d, const void* const* grads,
+                                           const int64_t* strides, void* dqkv, void* stream) {
+  if (int rc = check_rotary(d)) return rc;
+  if (d->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (!grads || !strides || !dqkv) return api_fail(ATTNRES_EINVAL, "grads / strides / dqkv is NULL");
+  QkvRotaryParams p;
+  fill_rotary(d, &p);
+  for (int i = 0; i < 3; ++i) {
+    p.grad[i] = grads[i];
+    for (int j = 0; j < 3; ++j) {
+      p.grad_stride[i][j] = grads[i] ? strides[3 * i + j] : 0;
+      if (p.grad_stride[i][j] < 0) return api_fail(ATTNRES_EINVAL, "negative gradient stride");
+    }
+  }
+  p.dqkv = dqkv;
+  int vec, lanes, chunks;
+  rotary_layout(d, p, &vec, &lanes, &chunks);
+  const hipError_t err = launch_qkv_rotary(d->dtype, d->table_dtype == ATTNRES_DTYPE_F32, true, p, vec, lanes, chunks,
+                                           (hipStream_t)stream);
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "qkv rotary backward launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}
+
+// ---------------------------------------------------------------- gated feed-forward
+
+namespace {
+
+constexpr int kCus = 256;
+
+struct SwLayout {
+  int es, per, step;   // bytes of a value, values of a chunk and of a k step
+  int Fp;              // hidden, in whole steps
+  int Dp;              // dim, in whole chunks
+  bool x_ok, w_ok;     // the products can read the operand as it is
+};
+
+int round_up(int v, int to) { return (v + to - 1) / to * to; }
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+SwLayout sw_layout(const attnres_swiglu_desc* d) {
+  SwLayout l;
+  l.es = es_of(d->dtype);
+  l.per = 16 / l.es;
+  l.step = kSwStepBytes / l.es;
+  l.Fp = round_up(d->hidden, l.step);
+  l.Dp = round_up(d->dim, l.per);
+  // direct loads of 16 bytes; a tile's rows within 32-bit offsets of its first one
+  const int64_t far = ((int64_t)1 << 32) / (256 * l.es) - d->dim;
+  l.x_ok = d->dim % l.per == 0 && aligned(d->x, 16) && d->x_row_stride % l.per == 0 && d->x_row_stride < far;
+  l.w_ok = d->dim % l.per == 0 && aligned(d->weight, 16) && d->weight_row_stride % l.per == 0 &&
+           d->weight_row_stride < far &&
+           (int64_t)2 * d->hidden * d->weight_row_stride * l.es < (int64_t)1 << 32;
+  return l;
+}
+
+// Tile and splits of a product with `steps` k steps: the least time in a simple
+// model, in units of a 256 x 256 tile's step.  A launch runs in rounds of as many
+// workgroups as the CUs hold; a split's sums are written and read once more.
+struct SwShape {
+  int tile, tiles_m, tiles_n, splits, steps;
+};
+constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128};
+
+SwShape sw_shape(int form, int64_t M, int N, int steps) {
+  // a step's and a tile's fixed cost, and the workgroups of a CU
+  constexpr double kStepCost[3] = {1.0, 0.40, 0.28}, kFixed[3] = {12.0, 6.0, 4.0};
+  constexpr int kPerCu[3] = {1, 2, 3};
+  SwShape best{};
+  double least = 1e300;
+  for (int t = 0; t < 3; ++t) {
+    const int cols = form == kFwd ? kTileN[t] / 2 : kTileN[t];
+    const int tm = (int)((M + kTileM[t] - 1) / kTileM[t]), tn = (N + cols - 1) / cols;
+    for (int splits = 1; splits <= 64; ++splits) {
+      const int per = (steps + splits - 1) / splits;
+      if (splits > 1 && (per < 4 || (steps + per - 1) / per != splits)) continue;
+      const int64_t wgs = (int64_t)tm * tn * splits;
+      if (wgs > (1 << 24)) continue;
+      const double rounds = (double)((wgs + kCus - 1) / kCus);  // tiles that one CU works on
+      const double together = rounds < kPerCu[t] ? rounds : kPerCu[t];
+      // co-resident workgroups share the CU: full rate only with all of them there
+      double cost = (per * kStepCost[t] + kFixed[t]) * (rounds / together) * (1.0 + 0.75 * (together - 1));
+      if (splits > 1) {
+        const double bytes = (double)wgs * kTileM[t] * kTileN[t] * 4 * 2;
+        cost += 12.0 + bytes / 2.0e6;  // a second launch; about 4 TB/s against 0.5 us a step
+      }
+      if (cost < least) {
+        least = cost;
+        best = SwShape{t, tm, tn, splits, per};
+      }
+    }
+  }
+  return best;
+}
+
+size_t sw_partials(const SwShape& s) {
+  return s.splits > 1 ? up256((size_t)s.splits * s.tiles_m * s.tiles_n * kTileM[s.tile] * kTileN[s.tile] * 4) : 0;
+}
+
+int check_swiglu(const attnres_swiglu_desc* d) {
+  if (!d) return api_fail(ATTNRES_EINVAL, "desc is NULL");
+  if (!known(d->dtype)) return api_fail(ATTNRES_EINVAL, "unknown dtype %d", d->dtype);
+  if (d->n_tok < 0) return api_fail(ATTNRES_EINVAL, "n_tok=%lld < 0", (long long)d->n_tok);
+  if (d->dim < 1 || d->hidden < 1) return api_fail(ATTNRES_EINVAL, "dim=%d, hidden=%d must be >= 1", d->dim, d->hidden);
+  if (d->n_tok > INT32_MAX / 2 || d->dim > (1 << 20) || d->hidden > (1 << 20) ||
+      (int64_t)2 * round_up(d->hidden, 32) * round_up(d->dim, 8) * es_of(d->dtype) >= (int64_t)1 << 32)
+    return api_fail(ATTNRES_EUNSUPPORTED, "n_tok=%lld, dim=%d, hidden=%d: outside the kernels' 32-bit offsets",
+                    (long long)d->n_tok, d->dim, d->hidden);
+  if (d->n_tok == 0) return ATTNRES_OK;
+  if (!d->x || !d->weight) return api_fail(ATTNRES_EINVAL, "x / weight is NULL");
+  if (d->n_tok > 1 && d->x_row_stride < 0) return api_fail(ATTNRES_EINVAL, "x_row_stride < 0");
+  if (d->weight_row_stride < d->dim)
+    return api_fail(ATTNRES_EINVAL, "weight_row_stride=%lld < dim=%d", (long long)d->weight_row_stride, d->dim);
+  return ATTNRES_OK;
+}
+
+SwShape fwd_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
+  return sw_shape(kFwd, d->n_tok, d->hidden, (d->dim + l.step - 1) / l.step);
+}
+SwShape dx_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
+  return sw_shape(kDx, d->n_tok, d->dim, 2 * l.Fp / l.step);
+}
+SwShape dw_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
+  return sw_shape(kDw, 2 * l.Fp, d->dim, (int)((d->n_tok + l.step - 1) / l.step));
+}
+
+size_t packed_x(const attnres_swiglu_desc* d, const SwLayout& l) {
+  return l.x_ok ? 0 : up256((size_t)d->n_tok * l.Dp * l.es);
+}
+size_t packed_w(const attnres_swiglu_desc* d, const SwLayout& l) {
+  return l.w_ok ? 0 : up256((size_t)2 * d->hidden * l.Dp * l.es);
+}
+
+// an operand as the products read it: where it is, or copied to `to`
+hipError_t sw_operand(const attnres_swiglu_desc* d, const SwLayout& l, bool weight, char* to, hipStream_t st,
+                      const void** at, int64_t* stride) {
+  const bool ok = weight ? l.w_ok : l.x_ok;
+  *at = weight ? d->weight : d->x;
+  *stride = weight ? d->weight_row_stride : d->x_row_stride;
+  if (ok) return hipSuccess;
+  SwPackParams k{};
+  k.from = *at;
+  k.from_stride = *stride;
+  k.to = to;
+  k.rows = weight ? (int64_t)2 * d->hidden : d->n_tok;
+  k.to_stride = l.Dp;
+  k.cols = d->dim;
+  *at = to;
+  *stride = l.Dp;
+  return launch_swiglu_pack(d->dtype, k, st);
+}
+
+void set_shape(const SwShape& s, SwGemmParams* g) {
+  g->tiles_m = s.tiles_m;
+  g->tiles_n = s.tiles_n;
+  g->splits = s.splits;
+  g->steps = s.steps;
+}
+
+}  // namespace
+
+extern "C" int64_t attnres_swiglu_saved_row_stride(const attnres_swiglu_desc* d) {
+  return d && known(d->dtype) && d->hidden >= 1 && d->hidden <= (1 << 20) ? sw_layout(d).Fp : 0;
+}
+
+extern "C" size_t attnres_swiglu_forward_workspace_size(const attnres_swiglu_desc* d) {
+  if (check_swiglu(d) || d->n_tok == 0) return 0;
+  const SwLayout l = sw_layout(d);
+  return packed_x(d, l) + packed_w(d, l) + sw_partials(fwd_shape(d, l));
+}
+
+extern "C" size_t attnres_swiglu_backward_workspace_size(const attnres_swiglu_desc* d, int32_t want_dx, int32_t want_dw) {
+  if (check_swiglu(d) || d->n_tok == 0) return 0;
+  const SwLayout l = sw_layout(d);
+  const size_t a = want_dx ? sw_partials(dx_shape(d, l)) : 0, b = want_dw ? sw_partials(dw_shape(d, l)) : 0;
+  return up256((size_t)d->n_tok * 2 * l.Fp * l.es) + (want_dw ? packed_x(d, l) : 0) + (want_dx ? packed_w(d, l) : 0) +
+         (a > b ? a : b);
+}
+
+extern "C" int attnres_swiglu_forward(const attnres_swiglu_desc* d, void* h, void* saved, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  if (int rc = check_swiglu(d)) return rc;
+  if (d->n_tok == 0) return ATTNRES_OK;
+  if (!h) return api_fail(ATTNRES_EINVAL, "h is NULL");
+  if (saved && !aligned(saved, 16)) return api_fail(ATTNRES_EINVAL, "saved is not aligned to 16 bytes");
+  const SwLayout l = sw_layout(d);
+  const SwShape s = fwd_shape(d, l);
+  const size_t px = packed_x(d, l), pw = packed_w(d, l), need = px + pw + sw_partials(s);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  if (!s.steps) return api_fail(ATTNRES_EUNSUPPORTED, "too many tiles");
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  SwGemmParams g{};
+  hipError_t err = sw_operand(d, l, false, ws, st, &g.q, &g.q_stride);
+  if (err == hipSuccess) err = sw_operand(d, l, true, ws + px, st, &g.p, &g.p_stride);
+  g.M = (int)d->n_tok;
+  g.N = g.F = g.n_out = d->hidden;
+  g.Fp = l.Fp;
+  g.K = l.Dp;
+  set_shape(s, &g);
+  g.out = h;
+  g.out_stride = d->hidden;
+  g.out_vec = d->hidden % l.per == 0 && aligned(h, 16);
+  g.saved = saved;
+  g.saved_stride = l.Fp;
+  g.partials = (float*)(ws + px + pw);
+  if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kFwd, s.tile, g, st);
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu forward launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}
+
+extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void* grad_h, int64_t grad_row_stride,
+                                       const void* saved, void* dx, void* dweight, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  if (int rc = check_swiglu(d)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  hipError_t err = hipSuccess;
+  if (d->n_tok == 0) {
+    if (dweight) err = launch_swiglu_clear(d->dtype, dweight, (int64_t)2 * d->hidden * d->dim, st);
+    if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu backward launch failed: %s", hipGetErrorString(err));
+    return ATTNRES_OK;
+  }
+  if (!dx && !dweight) return ATTNRES_OK;
+  if (!grad_h || !saved) return api_fail(ATTNRES_EINVAL, "grad_h / saved is NULL");
+  if (!aligned(saved, 16)) return api_fail(ATTNRES_EINVAL, "saved is not aligned to 16 bytes");
+  if (grad_row_stride < 0) return api_fail(ATTNRES_EINVAL, "grad_row_stride < 0");
+  const SwLayout l = sw_layout(d);
+  const SwShape sx = dx_shape(d, l), sw = dw_shape(d, l);
+  if (!sx.steps || !sw.steps) return api_fail(ATTNRES_EUNSUPPORTED, "too many tiles");
+  const size_t need = attnres_swiglu_backward_workspace_size(d, dx != nullptr, dweight != nullptr);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  char* ws = (char*)workspace;
+  const size_t pd = up256((size_t)d->n_tok * 2 * l.Fp * l.es), px = dweight ? packed_x(d, l) : 0,
+               pw = dx ? packed_w(d, l) : 0;
+  SwGradParams e{};
+  e.dh = grad_h;
+  e.dh_stride = grad_row_stride;
+  e.saved = saved;
+  e.d = ws;
+  e.n = d->n_tok;
+  e.F = d->hidden;
+  e.Fp = l.Fp;
+  e.vec = aligned(grad_h, 16) && grad_row_stride % l.per == 0;
+  err = launch_swiglu_grad(d->dtype, e, st);
+  if (dx && err == hipSuccess) {
+    SwGemmParams g{};
+    err = sw_operand(d, l, true, ws + pd + px, st, &g.p, &g.p_stride);
+    g.q = ws;
+    g.q_stride = 2 * l.Fp;
+    g.M = (int)d->n_tok;
+    g.N = l.w_ok ? d->dim : l.Dp;
+    g.K = 2 * l.Fp;
+    g.F = d->hidden;
+    g.Fp = l.Fp;
+    set_shape(sx, &g);
+    g.out = dx;
+    g.out_stride = d->dim;
+    g.n_out = d->dim;
+    g.out_vec = d->dim % l.per == 0 && aligned(dx, 16);
+    g.partials = (float*)(ws + pd + px + pw);
+    if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kDx, sx.tile, g, st);
+  }
+  if (dweight && err == hipSuccess) {
+    SwGemmParams g{};
+    err = sw_operand(d, l, false, ws + pd, st, &g.p, &g.p_stride);
+    g.q = ws;
+    g.q_stride = 2 * l.Fp;
+    g.M = 2 * l.Fp;
+    g.N = l.x_ok ? d->dim : l.Dp;
+    g.K = (int)d->n_tok;
+    g.F = d->hidden;
+    g.Fp = l.Fp;
+    set_shape(sw, &g);
+    g.out = dweight;
+    g.out_stride = d->dim;
+    g.n_out = d->dim;
+    g.out_vec = d->dim % l.per == 0 && aligned(dweight, 16);
+    g.partials = (float*)(ws + pd + px + pw);
+    if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kDw, sw.tile, g, st);
+  }
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu backward launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}

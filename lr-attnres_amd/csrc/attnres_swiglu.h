@@ -1,0 +1,202 @@
+// The matrix-core product of the gated feed-forward kernels (attnres_swiglu*.hip).
+//
+//   C[m, n] = sum_k Q[m, k] P[n, k]
+// in three forms:
+//   kFwd  P = W, Q = x (both with k contiguous), k over dim: a tile's P rows are half
+//         up and half gate rows of the same hidden columns, so that a lane ends with
+//         u and z of one element and forms u silu(z) in its registers
+//   kDx   P = W^T, Q = [du dz], k over both halves of the hidden dimension
+//   kDw   P = x^T, Q = [du dz]^T, k over tokens
+//
+// Tile.  Four waves, 2 x 2, each with a quarter of the BM x BN tile as 32 x 32 MFMA
+// tiles.  P is the MFMA's row operand, so that a lane holds for one m (lane % 32)
+// groups of 4 consecutive n.  k runs in steps of 64 bytes through kStages stages of
+// LDS, filled by loads that write LDS directly (16 bytes a lane; no registers), three
+// steps ahead; a wave reads the fragments of the next half step while the matrix
+// cores work on this one.  One barrier a step: behind it the next stage has landed
+// (each wave waited for its own loads) and nobody reads the oldest one any more.
+//
+// LDS layouts (a stage holds R rows of 64 bytes, or 32 / 16 rows of R values):
+//   k contiguous: the 16-byte chunks of row r are swapped by f(r) = (r / 2 % 4) ^ (r /
+//     8 % 2): the 8 (or 16) rows that a read serves at once then lie in all banks
+//   k strided, 16-bit: 32-byte units of row k are swapped by s(k) = 2 (k % 4) ^ (k / 2 %
+//     2) for the transposing reads (4 rows x 32 bytes per 16 lanes)
+//   k strided, fp32: rows as they are; a fragment's values are read one by one
+// The direct loads write LDS in lane order, so the swaps are made in the addresses
+// that the lanes read from.
+//
+// k beyond its end (dim not a whole number of steps, the last tokens, hidden columns
+// that fill no step) is loaded from a block of zeros, so that both operands vanish
+// there and no value behind the end is touched.
+#pragma once
+
+#include "attnres_device.h"
+#include "attnres_sublayers.h"
+
+namespace attnres {
+
+enum SwForm { kFwd = 0, kDx = 1, kDw = 2 };
+
+constexpr int kSwStages = 4;
+constexpr int kSwStepBytes = 64;  // of k, per row: 32 16-bit values, 16 fp32
+
+struct SwGemmParams {
+  const void* p;            // fwd / dx: W; dw: x
+  const void* q;            // fwd: x; dx / dw: [du dz], rows of 2 Fp
+  int64_t p_stride, q_stride;
+  int32_t M, N;             // rows / columns of the product (fwd: N = hidden; else in whole chunks)
+  int32_t n_out;            // columns of the output
+  int32_t K;                // fwd: dim, dx: 2 Fp, dw: tokens
+  int32_t F, Fp;            // hidden, and rounded up to a whole number of steps
+  int32_t tiles_m, tiles_n;
+  int32_t splits, steps;    // k steps of a split
+  void* out;                // [M, N] (dw: rows of the padded halves are left out)
+  int64_t out_stride;
+  int32_t out_vec;          // whole 16-byte stores to out
+  void* saved;              // fwd: u and z, [2, M, saved_stride], or null
+  int64_t saved_stride;
+  float* partials;          // splits > 1: [splits, tiles, BM * BN] in the kernel's own order
+};
+
+hipError_t launch_swiglu_gemm(int dtype, int form, int tile, const SwGemmParams& p, hipStream_t st);
+
+// [du dz] of the backward, rows of 2 Fp with zeros behind each half's F columns
+struct SwGradParams {
+  const void* dh;           // [n, F], rows of dh_stride
+  const void* saved;        // u and z [2, n, Fp]
+  void* d;                  // [n, 2 Fp]
+  int64_t n, dh_stride;
+  int32_t F, Fp;
+  int32_t vec;              // whole 16-byte loads of dh
+};
+hipError_t launch_swiglu_grad(int dtype, const SwGradParams& p, hipStream_t st);
+
+// rows x cols values to rows of to_stride, zeros behind the columns
+struct SwPackParams {
+  const void* from;
+  void* to;
+  int64_t rows, from_stride, to_stride;
+  int32_t cols;
+};
+hipError_t launch_swiglu_pack(int dtype, const SwPackParams& p, hipStream_t st);
+hipError_t launch_swiglu_clear(int dtype, void* to, int64_t values, hipStream_t st);
+
+// ---------------------------------------------------------------------- device
+
+template <class DT> struct SwElem {  // 16-byte fragments and their MFMA
+  static constexpr int kSize = sizeof(typename DT::S);
+  static constexpr int kPer = 16 / kSize;                // values in a chunk
+  static constexpr int kStep = kSwStepBytes / kSize;     // k of a step
+};
+
+typedef float sw_f16 __attribute__((ext_vector_type(16)));
+typedef float sw_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 sw_bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 sw_h8 __attribute__((ext_vector_type(8)));
+typedef short sw_s4 __attribute__((ext_vector_type(4)));
+
+// acc += P-fragment x Q-fragment: lane l holds 16 bytes of row l % 32, the lower
+// half of the lanes the first 16 bytes of k, the upper the next.  fp32: four
+// products of 2 k each, the same permutation of k on both sides.
+template <class DT>
+__device__ __forceinline__ void sw_mfma(const u32x4& a, const u32x4& b, sw_f16& c) {
+  if constexpr (DT::kCode == 1) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sw_bf8, a), __builtin_bit_cast(sw_bf8, b), c, 0, 0, 0);
+  } else if constexpr (DT::kCode == 2) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(sw_h8, a), __builtin_bit_cast(sw_h8, b), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+  }
+}
+
+// 16 bytes a lane from global memory straight to LDS: lane l's to lds + 16 l.  No
+// register is written, so nothing in flight can overwrite one; the waits are the
+// kernel's own (sw_wait).
+__device__ __forceinline__ void sw_dma(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void sw_dma64(const char* at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "s"(lds) : "memory", "m0");
+}
+// this wave's LDS reads are done and at most N of its loads are under way; then all waves meet
+template <int N>
+__device__ __forceinline__ void sw_wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+// One operand of R rows (values along m or n) in LDS.  T: k strided in memory.
+template <class DT, int R, bool T>
+struct SwOperand {
+  using E = SwElem<DT>;
+  static constexpr int kBytes = R * kSwStepBytes;         // of a stage
+  static constexpr int kLoads = R / 64;                   // direct loads of a thread per step
+  static constexpr int kRowChunks = R / E::kPer;          // strided: chunks of a row of R values
+  static constexpr int kUnitMask = R / 16 - 1;            // strided 16-bit: 32-byte units of a row
+  uint32_t off[kLoads];   // byte offsets of this thread's chunks from the step's base
+  int kr[kLoads];         // and their k: chunk * kPer (contiguous) or row (strided)
+  uint32_t rd[4];         // byte addresses of this lane's fragments
+
+  __device__ static int f_row(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+  __device__ static int s_row(int k) { return ((2 * (k & 3)) ^ ((k >> 1) & 1)) & kUnitMask; }
+
+  // row / first k and chunk of load i of a thread
+  __device__ __forceinline__ static void place(int i, int tid, int* row, int* chunk) {
+    const int q = i * 256 + tid;
+    if constexpr (!T) {
+      *row = q >> 2;
+      *chunk = (q & 3) ^ f_row(*row);
+    } else {
+      *row = q / kRowChunks;
+      const int c = q % kRowChunks;
+      if constexpr (E::kSize == 2) *chunk = (((c >> 1) ^ s_row(*row)) << 1) | (c & 1);
+      else *chunk = c;
+    }
+  }
+
+  // where this lane's fragments begin: rd by half step (contiguous), by 32-row group (strided)
+  __device__ __forceinline__ void place_reads(int row0, int lane, uint32_t base) {
+    if constexpr (!T) {
+      const int r = row0 + (lane & 31);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) rd[kk] = base + r * 64 + (((2 * kk + (lane >> 5)) ^ f_row(r)) * 16);
+    } else if constexpr (E::kSize == 2) {
+      const int g = lane >> 4, i = lane & 15;
+      const int k = (g >> 1) * 8 + (i >> 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int unit = (row0 + 32 * j) / 16 + (g & 1);
+        rd[j] = base + k * (R * 2) + ((unit ^ s_row(k)) & kUnitMask) * 32 + (i & 3) * 8;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rd[j] = base + (4 * (lane >> 5)) * (R * 4) + (row0 + 32 * j + (lane & 31)) * 4;
+    }
+  }
+
+  // the fragment of 32-row group j, half step kk, of the stage at `stage`
+  __device__ __forceinline__ u32x4 read(const char* lds, uint32_t stage, int kk, int j) const {
+    if constexpr (!T) {
+      return *(const u32x4*)(lds + stage + rd[kk] + j * 2048);
+    } else if constexpr (E::kSize == 2) {
+      typedef __attribute__((address_space(3))) sw_s4 lds_s4;
+      const char* at = lds + stage + rd[j] + kk * 16 * (R * 2);
+      const sw_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+      const sw_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 4 * (R * 2)));
+      const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+      return u32x4{a.x, a.y, b.x, b.y};
+    } else {
+      const char* at = lds + stage + rd[j] + kk * 8 * (R * 4);
+      u32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *(const uint32_t*)(at + e * (R * 4));
+      return v;
+    }
+  }
+};
+
+}  // namespace attnres

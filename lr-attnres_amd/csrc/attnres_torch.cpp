@@ -31,6 +31,7 @@
 
 #include "../../include/attnres_hip.h"
 #include "../../include/attnres_phase1_bank.h"
+#include "../../include/attnres_sublayers.h"
 
 namespace {
 
@@ -48,7 +49,9 @@ struct Lib {
   X(attnres_phase1_bank_forward) X(attnres_phase1_bank_backward) X(attnres_phase1_bank_backward_workspace_size)    \
   X(attnres_phase2_forward) X(attnres_phase2_backward) X(attnres_phase2_backward_workspace_size)                   \
   X(attnres_accum_read_forward) X(attnres_accum_read_backward) X(attnres_block_accum_forward)                      \
-  X(attnres_block_accum_backward)
+  X(attnres_block_accum_backward) X(attnres_qkv_rotary_forward) X(attnres_qkv_rotary_backward)                     \
+  X(attnres_swiglu_saved_row_stride) X(attnres_swiglu_forward_workspace_size)                                      \
+  X(attnres_swiglu_backward_workspace_size) X(attnres_swiglu_forward) X(attnres_swiglu_backward)
   ATTNRES_FNS(ATTNRES_FN)
 } lib;
 
@@ -1045,6 +1048,8 @@ py::object block_accum(const py::object& projected, const py::object& partial_va
   return py::make_tuple(res[0], res[1]);
 }
 
+#include "attnres_torch_sublayers.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_attnres_torch, m) {
@@ -1055,4 +1060,6 @@ PYBIND11_MODULE(_attnres_torch, m) {
   m.def("phase2", &merge_read);
   m.def("accum_read", &accum_read);
   m.def("block_accum", &block_accum);
+  m.def("qkv_rotary", &qkv_rotary);
+  m.def("swiglu", &swiglu);
 }
