@@ -67,7 +67,7 @@ int attnres_qkv_rotary_backward(const attnres_qkv_rotary_desc* desc, const void*
  */
 typedef struct attnres_swiglu_desc {
   int32_t dtype;          /* ATTNRES_DTYPE_* */
-  int64_t n_tok;          /* 0 is allowed: the forward launches nothing, the backward clears dweight */
+  int64_t n_tok;          /* at most 2^22; 0 is allowed: the forward launches nothing, the backward clears dweight */
   int32_t dim;
   int32_t hidden;
   const void* x;          /* [n_tok, dim], contiguous last dimension */
@@ -76,17 +76,16 @@ typedef struct attnres_swiglu_desc {
   int64_t weight_row_stride;
 } attnres_swiglu_desc;
 
-/* Elements between the rows of the projections that the forward saves: hidden,
- * rounded up to what the kernels store whole.  Host computation. */
-int64_t attnres_swiglu_saved_row_stride(const attnres_swiglu_desc* desc);
+/* Bytes of what the forward keeps of u and z for the backward (its own layout; more
+ * bits than the 16-bit dtypes hold).  Host computation. */
+size_t attnres_swiglu_saved_size(const attnres_swiglu_desc* desc);
 
 /* Workspace bytes of the forward / of the backward (host computation). */
 size_t attnres_swiglu_forward_workspace_size(const attnres_swiglu_desc* desc);
 size_t attnres_swiglu_backward_workspace_size(const attnres_swiglu_desc* desc, int32_t want_dx, int32_t want_dweight);
 
-/* h [n_tok, hidden] dense.  saved: NULL, or [2, n_tok, saved_row_stride] in dtype,
- * aligned to 16 bytes: u and z, rounded, for the backward.  workspace aligned to
- * 256 bytes. */
+/* h [n_tok, hidden] dense.  saved: NULL, or attnres_swiglu_saved_size bytes aligned to
+ * 16, for the backward.  workspace aligned to 256 bytes. */
 int attnres_swiglu_forward(const attnres_swiglu_desc* desc, void* h, void* saved, void* workspace,
                            size_t workspace_bytes, void* stream);
 

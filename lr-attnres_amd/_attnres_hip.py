@@ -344,8 +344,8 @@ def load() -> ctypes.CDLL:
     lib.attnres_qkv_rotary_backward.restype = c_int
     lib.attnres_qkv_rotary_backward.argtypes = [POINTER(QkvRotaryDesc), POINTER(c_void_p), POINTER(c_int64), c_void_p,
                                                 c_void_p]
-    lib.attnres_swiglu_saved_row_stride.restype = c_int64
-    lib.attnres_swiglu_saved_row_stride.argtypes = [POINTER(SwigluDesc)]
+    lib.attnres_swiglu_saved_size.restype = c_size_t
+    lib.attnres_swiglu_saved_size.argtypes = [POINTER(SwigluDesc)]
     lib.attnres_swiglu_forward_workspace_size.restype = c_size_t
     lib.attnres_swiglu_forward_workspace_size.argtypes = [POINTER(SwigluDesc)]
     lib.attnres_swiglu_backward_workspace_size.restype = c_size_t
@@ -1211,7 +1211,8 @@ def swiglu_forward(x, weight, save: bool):
     """(h [n, F], what the backward needs of the projections, or None)"""
     lib, d = load(), swiglu_desc(x, weight)
     h = x.new_empty((d.n_tok, d.hidden))
-    saved = x.new_empty((2, d.n_tok, lib.attnres_swiglu_saved_row_stride(ctypes.byref(d)))) if save else None
+    saved = torch.empty((lib.attnres_swiglu_saved_size(ctypes.byref(d)),), dtype=torch.uint8,
+                        device=x.device) if save else None
     n = lib.attnres_swiglu_forward_workspace_size(ctypes.byref(d))
     ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
     _check(lib.attnres_swiglu_forward(ctypes.byref(d), _ptr(h), _ptr(saved), _ptr(ws), n, _stream(x.device)),

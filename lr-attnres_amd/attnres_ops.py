@@ -1983,14 +1983,16 @@ def qkv_norm_rotary(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, posit
 def _swiglu_op(x: Tensor, weight: Tensor, save: bool) -> tuple[Tensor, Tensor]:
     with _device_ctx(x.device):
         h, saved = _hip.swiglu_forward(x, weight, save)
-    return h, saved if saved is not None else x.new_empty((0,))
+    return h, saved if saved is not None else torch.empty((0,), dtype=torch.uint8, device=x.device)
 
 
 @_swiglu_op.register_fake
 def _swiglu_fake(x, weight, save):
     n, F_ = x.size(0), weight.size(0) // 2
-    step = 16 if x.dtype == torch.float32 else 32  # (hidden columns of a k step of the products)
-    return x.new_empty((n, F_)), x.new_empty((2, n, (F_ + step - 1) // step * step) if save else (0,))
+    # attnres_swiglu_saved_size: hidden columns in groups of 32, bytes of a pair (u, z)
+    pair = {torch.float32: 8, torch.bfloat16: 5, torch.float16: 6}[x.dtype]
+    size = n * ((F_ + 31) // 32 * 32) * pair if save else 0
+    return x.new_empty((n, F_)), x.new_empty((size,), dtype=torch.uint8)
 
 
 @torch.library.custom_op("attnres_hip::swiglu_backward", mutates_args=())
@@ -2036,7 +2038,7 @@ def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
 
     ``x`` [..., D]; ``weight`` [2 F, D], rows ``[0, F)`` up and ``[F, 2 F)`` gate (``nn.Linear(D, 2 F, bias=False).weight``
     with ``[up, gate] = fc1(x).chunk(2)``), taken in ``x``'s dtype.  Returns [..., F].  For the backward both projections
-    are kept in the dtype, as the linear layer's output would be.
+    are kept, in the 16-bit dtypes with 12 (bf16) or 16 (fp16) significant bits: 5 or 6 bytes for each of the [..., F].
     """
     what = "swiglu_projection"
     nat = _native("swiglu_forward", "swiglu_backward")

@@ -1,5 +1,6 @@
 // C ABI of the sublayer kernels: argument checks, kernel selection and launch
 // geometry.  Declared in include/attnres_sublayers.h.
+#include <stdlib.h>
 #include <string.h>
 
 #include "../../include/attnres_sublayers.h"
@@ -147,9 +148,10 @@ constexpr int kCus = 256;
 
 struct SwLayout {
   int es, per, step;   // bytes of a value, values of a chunk and of a k step
-  int Fp;              // hidden, in whole steps
+  int Fp;              // hidden, in whole steps and rows of a store
   int Dp;              // dim, in whole chunks
   bool x_ok, w_ok;     // the products can read the operand as it is
+  bool w_ok_dx;        // and dx the weight: its halves fill k steps
 };
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
@@ -160,7 +162,7 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
   l.es = es_of(d->dtype);
   l.per = 16 / l.es;
   l.step = kSwStepBytes / l.es;
-  l.Fp = round_up(d->hidden, l.step);
+  l.Fp = round_up(d->hidden, kSwRows);
   l.Dp = round_up(d->dim, l.per);
   // direct loads of 16 bytes; a tile's rows within 32-bit offsets of its first one
   const int64_t far = ((int64_t)1 << 32) / (256 * l.es) - d->dim;
@@ -168,6 +170,7 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
   l.w_ok = d->dim % l.per == 0 && aligned(d->weight, 16) && d->weight_row_stride % l.per == 0 &&
            d->weight_row_stride < far &&
            (int64_t)2 * d->hidden * d->weight_row_stride * l.es < (int64_t)1 << 32;
+  l.w_ok_dx = l.w_ok && d->hidden == l.Fp;
   return l;
 }
 
@@ -177,28 +180,28 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
 struct SwShape {
   int tile, tiles_m, tiles_n, splits, steps;
 };
-constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128};
 
 SwShape sw_shape(int form, int64_t M, int N, int steps) {
   // a step's and a tile's fixed cost, and the workgroups of a CU
-  constexpr double kStepCost[3] = {1.0, 0.40, 0.28}, kFixed[3] = {12.0, 6.0, 4.0};
-  constexpr int kPerCu[3] = {1, 2, 3};
+  constexpr double kStepCost[kSwTiles] = {1.0, 0.70, 0.40, 0.28}, kFixed[kSwTiles] = {12.0, 7.0, 6.0, 4.0};
+  static const int force = getenv("SW_TILE") ? atoi(getenv("SW_TILE")) : -1;
   SwShape best{};
   double least = 1e300;
-  for (int t = 0; t < 3; ++t) {
-    const int cols = form == kFwd ? kTileN[t] / 2 : kTileN[t];
-    const int tm = (int)((M + kTileM[t] - 1) / kTileM[t]), tn = (N + cols - 1) / cols;
+  for (int t = 0; t < kSwTiles; ++t) {
+    if (force >= 0 && t != force) continue;
+    const int cols = form == kFwd ? kSwTileN[t] / 2 : kSwTileN[t];
+    const int tm = (int)((M + kSwTileM[t] - 1) / kSwTileM[t]), tn = (N + cols - 1) / cols;
     for (int splits = 1; splits <= 64; ++splits) {
       const int per = (steps + splits - 1) / splits;
       if (splits > 1 && (per < 4 || (steps + per - 1) / per != splits)) continue;
       const int64_t wgs = (int64_t)tm * tn * splits;
       if (wgs > (1 << 24)) continue;
       const double rounds = (double)((wgs + kCus - 1) / kCus);  // tiles that one CU works on
-      const double together = rounds < kPerCu[t] ? rounds : kPerCu[t];
+      const double together = rounds < sw_per_cu(kSwTileM[t], kSwTileN[t]) ? rounds : sw_per_cu(kSwTileM[t], kSwTileN[t]);
       // co-resident workgroups share the CU: full rate only with all of them there
       double cost = (per * kStepCost[t] + kFixed[t]) * (rounds / together) * (1.0 + 0.75 * (together - 1));
       if (splits > 1) {
-        const double bytes = (double)wgs * kTileM[t] * kTileN[t] * 4 * 2;
+        const double bytes = (double)wgs * kSwTileM[t] * kSwTileN[t] * 4 * 2;
         cost += 12.0 + bytes / 2.0e6;  // a second launch; about 4 TB/s against 0.5 us a step
       }
       if (cost < least) {
@@ -211,7 +214,7 @@ SwShape sw_shape(int form, int64_t M, int N, int steps) {
 }
 
 size_t sw_partials(const SwShape& s) {
-  return s.splits > 1 ? up256((size_t)s.splits * s.tiles_m * s.tiles_n * kTileM[s.tile] * kTileN[s.tile] * 4) : 0;
+  return s.splits > 1 ? up256((size_t)s.splits * s.tiles_m * s.tiles_n * kSwTileM[s.tile] * kSwTileN[s.tile] * 4) : 0;
 }
 
 int check_swiglu(const attnres_swiglu_desc* d) {
@@ -219,7 +222,7 @@ int check_swiglu(const attnres_swiglu_desc* d) {
   if (!known(d->dtype)) return api_fail(ATTNRES_EINVAL, "unknown dtype %d", d->dtype);
   if (d->n_tok < 0) return api_fail(ATTNRES_EINVAL, "n_tok=%lld < 0", (long long)d->n_tok);
   if (d->dim < 1 || d->hidden < 1) return api_fail(ATTNRES_EINVAL, "dim=%d, hidden=%d must be >= 1", d->dim, d->hidden);
-  if (d->n_tok > INT32_MAX / 2 || d->dim > (1 << 20) || d->hidden > (1 << 20) ||
+  if (d->n_tok > (1 << 22) || d->dim > (1 << 20) || d->hidden > (1 << 20) ||
       (int64_t)2 * round_up(d->hidden, 32) * round_up(d->dim, 8) * es_of(d->dtype) >= (int64_t)1 << 32)
     return api_fail(ATTNRES_EUNSUPPORTED, "n_tok=%lld, dim=%d, hidden=%d: outside the kernels' 32-bit offsets",
                     (long long)d->n_tok, d->dim, d->hidden);
@@ -244,14 +247,14 @@ SwShape dw_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
 size_t packed_x(const attnres_swiglu_desc* d, const SwLayout& l) {
   return l.x_ok ? 0 : up256((size_t)d->n_tok * l.Dp * l.es);
 }
-size_t packed_w(const attnres_swiglu_desc* d, const SwLayout& l) {
-  return l.w_ok ? 0 : up256((size_t)2 * d->hidden * l.Dp * l.es);
+size_t packed_w(const attnres_swiglu_desc* d, const SwLayout& l, bool dx) {
+  return (dx ? l.w_ok_dx : l.w_ok) ? 0 : up256((size_t)2 * (dx ? l.Fp : d->hidden) * l.Dp * l.es);
 }
 
-// an operand as the products read it: where it is, or copied to `to`
-hipError_t sw_operand(const attnres_swiglu_desc* d, const SwLayout& l, bool weight, char* to, hipStream_t st,
+// an operand as a product reads it: where it is, or copied to `to`
+hipError_t sw_operand(const attnres_swiglu_desc* d, const SwLayout& l, int form, bool weight, char* to, hipStream_t st,
                       const void** at, int64_t* stride) {
-  const bool ok = weight ? l.w_ok : l.x_ok;
+  const bool ok = !weight ? l.x_ok : form == kDx ? l.w_ok_dx : l.w_ok;
   *at = weight ? d->weight : d->x;
   *stride = weight ? d->weight_row_stride : d->x_row_stride;
   if (ok) return hipSuccess;
@@ -259,7 +262,9 @@ hipError_t sw_operand(const attnres_swiglu_desc* d, const SwLayout& l, bool weig
   k.from = *at;
   k.from_stride = *stride;
   k.to = to;
-  k.rows = weight ? (int64_t)2 * d->hidden : d->n_tok;
+  k.blocks = weight ? 2 : 1;
+  k.rows = weight ? d->hidden : d->n_tok;
+  k.to_rows = weight && form == kDx ? l.Fp : k.rows;
   k.to_stride = l.Dp;
   k.cols = d->dim;
   *at = to;
@@ -276,21 +281,24 @@ void set_shape(const SwShape& s, SwGemmParams* g) {
 
 }  // namespace
 
-extern "C" int64_t attnres_swiglu_saved_row_stride(const attnres_swiglu_desc* d) {
-  return d && known(d->dtype) && d->hidden >= 1 && d->hidden <= (1 << 20) ? sw_layout(d).Fp : 0;
+extern "C" size_t attnres_swiglu_saved_size(const attnres_swiglu_desc* d) {
+  if (check_swiglu(d) || d->n_tok == 0) return 0;
+  const SwLayout l = sw_layout(d);
+  const size_t low = d->dtype == ATTNRES_DTYPE_F32 ? 0 : 2 * (d->dtype == ATTNRES_DTYPE_BF16 ? 4 : 8);  // bits a pair
+  return (size_t)d->n_tok * l.Fp * 2 * l.es + (size_t)d->n_tok * l.Fp * low / 8;
 }
 
 extern "C" size_t attnres_swiglu_forward_workspace_size(const attnres_swiglu_desc* d) {
   if (check_swiglu(d) || d->n_tok == 0) return 0;
   const SwLayout l = sw_layout(d);
-  return packed_x(d, l) + packed_w(d, l) + sw_partials(fwd_shape(d, l));
+  return packed_x(d, l) + packed_w(d, l, false) + sw_partials(fwd_shape(d, l));
 }
 
 extern "C" size_t attnres_swiglu_backward_workspace_size(const attnres_swiglu_desc* d, int32_t want_dx, int32_t want_dw) {
   if (check_swiglu(d) || d->n_tok == 0) return 0;
   const SwLayout l = sw_layout(d);
   const size_t a = want_dx ? sw_partials(dx_shape(d, l)) : 0, b = want_dw ? sw_partials(dw_shape(d, l)) : 0;
-  return up256((size_t)d->n_tok * 2 * l.Fp * l.es) + (want_dw ? packed_x(d, l) : 0) + (want_dx ? packed_w(d, l) : 0) +
+  return up256((size_t)d->n_tok * 2 * l.Fp * l.es) + (want_dw ? packed_x(d, l) : 0) + (want_dx ? packed_w(d, l, true) : 0) +
          (a > b ? a : b);
 }
 
@@ -302,25 +310,25 @@ extern "C" int attnres_swiglu_forward(const attnres_swiglu_desc* d, void* h, voi
   if (saved && !aligned(saved, 16)) return api_fail(ATTNRES_EINVAL, "saved is not aligned to 16 bytes");
   const SwLayout l = sw_layout(d);
   const SwShape s = fwd_shape(d, l);
-  const size_t px = packed_x(d, l), pw = packed_w(d, l), need = px + pw + sw_partials(s);
+  const size_t px = packed_x(d, l), pw = packed_w(d, l, false), need = px + pw + sw_partials(s);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
   if (!s.steps) return api_fail(ATTNRES_EUNSUPPORTED, "too many tiles");
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
   SwGemmParams g{};
-  hipError_t err = sw_operand(d, l, false, ws, st, &g.q, &g.q_stride);
-  if (err == hipSuccess) err = sw_operand(d, l, true, ws + px, st, &g.p, &g.p_stride);
+  hipError_t err = sw_operand(d, l, kFwd, false, ws, st, &g.q, &g.q_stride);
+  if (err == hipSuccess) err = sw_operand(d, l, kFwd, true, ws + px, st, &g.p, &g.p_stride);
   g.M = (int)d->n_tok;
   g.N = g.F = g.n_out = d->hidden;
   g.Fp = l.Fp;
   g.K = l.Dp;
+  g.n_tok = d->n_tok;
   set_shape(s, &g);
   g.out = h;
   g.out_stride = d->hidden;
   g.out_vec = d->hidden % l.per == 0 && aligned(h, 16);
   g.saved = saved;
-  g.saved_stride = l.Fp;
   g.partials = (float*)(ws + px + pw);
   if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kFwd, s.tile, g, st);
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu forward launch failed: %s", hipGetErrorString(err));
@@ -350,7 +358,7 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
     return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
   char* ws = (char*)workspace;
   const size_t pd = up256((size_t)d->n_tok * 2 * l.Fp * l.es), px = dweight ? packed_x(d, l) : 0,
-               pw = dx ? packed_w(d, l) : 0;
+               pw = dx ? packed_w(d, l, true) : 0;
   SwGradParams e{};
   e.dh = grad_h;
   e.dh_stride = grad_row_stride;
@@ -363,11 +371,11 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
   err = launch_swiglu_grad(d->dtype, e, st);
   if (dx && err == hipSuccess) {
     SwGemmParams g{};
-    err = sw_operand(d, l, true, ws + pd + px, st, &g.p, &g.p_stride);
+    err = sw_operand(d, l, kDx, true, ws + pd + px, st, &g.p, &g.p_stride);
     g.q = ws;
-    g.q_stride = 2 * l.Fp;
+    g.n_tok = d->n_tok;
     g.M = (int)d->n_tok;
-    g.N = l.w_ok ? d->dim : l.Dp;
+    g.N = l.Dp;
     g.K = 2 * l.Fp;
     g.F = d->hidden;
     g.Fp = l.Fp;
@@ -381,11 +389,11 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
   }
   if (dweight && err == hipSuccess) {
     SwGemmParams g{};
-    err = sw_operand(d, l, false, ws + pd, st, &g.p, &g.p_stride);
+    err = sw_operand(d, l, kDw, false, ws + pd, st, &g.p, &g.p_stride);
     g.q = ws;
-    g.q_stride = 2 * l.Fp;
+    g.n_tok = d->n_tok;
     g.M = 2 * l.Fp;
-    g.N = l.x_ok ? d->dim : l.Dp;
+    g.N = l.Dp;
     g.K = (int)d->n_tok;
     g.F = d->hidden;
     g.Fp = l.Fp;

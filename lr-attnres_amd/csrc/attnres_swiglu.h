@@ -10,9 +10,9 @@
 //
 // Tile.  Four waves, 2 x 2, each with a quarter of the BM x BN tile as 32 x 32 MFMA
 // tiles.  P is the MFMA's row operand, so that a lane holds for one m (lane % 32)
-// groups of 4 consecutive n.  k runs in steps of 64 bytes through kStages stages of
-// LDS, filled by loads that write LDS directly (16 bytes a lane; no registers), three
-// steps ahead; a wave reads the fragments of the next half step while the matrix
+// groups of 4 consecutive n.  k runs in steps of 64 bytes through the stages of
+// LDS, filled by loads that write LDS directly (16 bytes a lane; no registers), two or
+// three steps ahead; a wave reads the fragments of the next half step while the matrix
 // cores work on this one.  One barrier a step: behind it the next stage has landed
 // (each wave waited for its own loads) and nobody reads the oldest one any more.
 //
@@ -37,46 +37,52 @@ namespace attnres {
 
 enum SwForm { kFwd = 0, kDx = 1, kDw = 2 };
 
-constexpr int kSwStages = 4;
 constexpr int kSwStepBytes = 64;  // of k, per row: 32 16-bit values, 16 fp32
+constexpr int kSwRows = 32;       // rows of the product that are stored together: a half's are padded to them
+constexpr int kSwTiles = 4;
+constexpr int kSwTileM[kSwTiles] = {256, 128, 128, 64}, kSwTileN[kSwTiles] = {256, 256, 128, 128};
+// stages of LDS, and the workgroups that a CU's 160 KB then hold
+constexpr int sw_stages(int bm, int bn) { return bm + bn == 384 ? 3 : 4; }
+constexpr int sw_per_cu(int bm, int bn) { return 160 * 1024 / (sw_stages(bm, bn) * (bm + bn) * kSwStepBytes); }
 
 struct SwGemmParams {
   const void* p;            // fwd / dx: W; dw: x
-  const void* q;            // fwd: x; dx / dw: [du dz], rows of 2 Fp
+  const void* q;            // fwd: x; dx / dw: [du dz], in blocks
   int64_t p_stride, q_stride;
   int32_t M, N;             // rows / columns of the product (fwd: N = hidden; else in whole chunks)
   int32_t n_out;            // columns of the output
   int32_t K;                // fwd: dim, dx: 2 Fp, dw: tokens
-  int32_t F, Fp;            // hidden, and rounded up to a whole number of steps
+  int32_t F, Fp;            // hidden, and rounded up to kSwRows
   int32_t tiles_m, tiles_n;
   int32_t splits, steps;    // k steps of a split
   void* out;                // [M, N] (dw: rows of the padded halves are left out)
   int64_t out_stride;
   int32_t out_vec;          // whole 16-byte stores to out
-  void* saved;              // fwd: u and z, [2, M, saved_stride], or null
-  int64_t saved_stride;
+  void* saved;              // fwd: u and z (SwPlanes), or null
+  int64_t n_tok;
   float* partials;          // splits > 1: [splits, tiles, BM * BN] in the kernel's own order
 };
 
 hipError_t launch_swiglu_gemm(int dtype, int form, int tile, const SwGemmParams& p, hipStream_t st);
 
-// [du dz] of the backward, rows of 2 Fp with zeros behind each half's F columns
+// [du dz] of the backward, in blocks, with zeros behind each half's F columns
 struct SwGradParams {
   const void* dh;           // [n, F], rows of dh_stride
-  const void* saved;        // u and z [2, n, Fp]
-  void* d;                  // [n, 2 Fp]
+  const void* saved;        // u and z (SwPlanes)
+  void* d;                  // [2 Fp / step blocks, n, step]
   int64_t n, dh_stride;
   int32_t F, Fp;
   int32_t vec;              // whole 16-byte loads of dh
 };
 hipError_t launch_swiglu_grad(int dtype, const SwGradParams& p, hipStream_t st);
 
-// rows x cols values to rows of to_stride, zeros behind the columns
+// blocks of `rows` rows of cols values to blocks of `to_rows` rows of to_stride, zeros
+// behind the columns and the rows
 struct SwPackParams {
   const void* from;
   void* to;
-  int64_t rows, from_stride, to_stride;
-  int32_t cols;
+  int64_t rows, to_rows, from_stride, to_stride;
+  int32_t blocks, cols;
 };
 hipError_t launch_swiglu_pack(int dtype, const SwPackParams& p, hipStream_t st);
 hipError_t launch_swiglu_clear(int dtype, void* to, int64_t values, hipStream_t st);
@@ -108,6 +114,27 @@ __device__ __forceinline__ void sw_mfma(const u32x4& a, const u32x4& b, sw_f16& 
 #pragma unroll
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
   }
+}
+
+// What the forward keeps of u and z, and [du dz] of the backward, is the kernels' own
+// and stands in blocks of one k step: [blocks, n, step] values.  A product's tile of
+// [du dz] is then one run of memory (as rows of 2 Fp values it was 256 pieces of 64
+// bytes, a page or more apart), and both sides of the activation's gradient are.
+// u and z are kept to 16 + kLow bits of their fp32 value, in two planes: rounded to the
+// dtype they would add two roundings to the one that [du dz] itself needs (an error of
+// 1.7 times the result's own rounding in dx and dweight; so it is 1.4 times).
+template <class DT> struct SwPlanes {
+  static constexpr int kLow = DT::kCode == 1 ? 4 : DT::kCode == 2 ? 8 : 0;
+  static constexpr int kLowBlock = SwElem<DT>::kStep * 2 * kLow / 8;  // bytes of a block's row of low bits
+};
+struct SwPlaneAddress {
+  char *u, *z, *low;
+};
+template <class DT>
+__host__ __device__ inline SwPlaneAddress sw_planes(const void* saved, int64_t n, int Fp) {
+  const int64_t plane = n * Fp * SwElem<DT>::kSize;
+  char* at = (char*)saved;
+  return {at, at + plane, at + 2 * plane};
 }
 
 // 16 bytes a lane from global memory straight to LDS: lane l's to lds + 16 l.  No

@@ -21,29 +21,54 @@ constexpr int kThreads = 256;
 
 // du = dh silu(z), dz = dh u silu'(z), silu'(z) = s + z s (1 - s), s = 1 / (1 + exp(-z)).
 // Both products of the backward read [du dz], each of them several times; it is
-// rounded to the dtype as they take it.  Bound by memory (10 bytes a hidden value
-// in 16 bits).
+// rounded to the dtype as they take it.  Bound by memory (11 bytes a hidden value
+// in bf16).  A workgroup takes 16 tokens of four neighbouring blocks, so that every
+// array is read and written in whole lines.
 template <class DT>
 __global__ __launch_bounds__(kThreads) void swiglu_grad_kernel(SwGradParams p) {
   using S = typename DT::S;
-  constexpr int V = 16 / (int)sizeof(S);
-  const int64_t chunks = p.Fp / V;
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (at >= p.n * chunks) return;
-  const int64_t t = at / chunks;
-  const int f = (int)(at - t * chunks) * V;
-  S* du = (S*)p.d + t * 2 * p.Fp + f;
-  float g[V], u[V], z[V], a[V], b[V];
+  constexpr int V = 16 / (int)sizeof(S), kStep = SwElem<DT>::kStep, L = SwPlanes<DT>::kLow;
+  const int blocks = p.Fp / kStep, across = (blocks + 3) / 4;
+  const int64_t group = (int64_t)blockIdx.x / across;
+  const int b = (int)(blockIdx.x - group * across) * 4 + threadIdx.x / 64;
+  const int64_t t = group * 16 + threadIdx.x % 64 / 4;
+  const int c = threadIdx.x % 4;
+  if (b >= blocks || t >= p.n) return;
+  const int f = b * kStep + c * V;
+  const int64_t at = ((int64_t)b * p.n + t) * kStep + c * V;
+  const SwPlaneAddress from = sw_planes<DT>(p.saved, p.n, p.Fp);
   const S* dh = (const S*)p.dh + t * p.dh_stride + f;
-  if (f < p.F) {
-    if (p.vec && f + V <= p.F) {
-      load_vec<DT, V, true>(dh, g);
-    } else {
+  float g[V], u[V], z[V], a[V], d[V];
+  if (f < p.F && p.vec && f + V <= p.F) {
+    load_vec<DT, V, true>(dh, g);
+  } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) g[e] = f + e < p.F ? DT::load1(dh + e) : 0.f;
+    for (int e = 0; e < V; ++e) g[e] = f + e < p.F ? DT::load1(dh + e) : 0.f;
+  }
+  if constexpr (L == 0) {
+    load_vec<DT, V, true>((const S*)from.u + at, u);
+    load_vec<DT, V, true>((const S*)from.z + at, z);
+  } else {
+    const u32x4 uh = __builtin_nontemporal_load((const u32x4*)((const S*)from.u + at));
+    const u32x4 zh = __builtin_nontemporal_load((const u32x4*)((const S*)from.z + at));
+    uint32_t low[V];  // u's low bits at L, z's above them
+    if constexpr (L == 4) {
+      const u32x2 w = __builtin_nontemporal_load((const u32x2*)(from.low + at));
+#pragma unroll
+      for (int e = 0; e < V; ++e) low[e] = w[e / 4] >> (8 * (e % 4));
+    } else {
+      const u32x4 w = __builtin_nontemporal_load((const u32x4*)(from.low + at * 2));
+#pragma unroll
+      for (int e = 0; e < V; ++e) low[e] = w[e / 2] >> (16 * (e % 2));
     }
-    load_vec<DT, V, true>((const S*)p.saved + t * p.Fp + f, u);
-    load_vec<DT, V, true>((const S*)p.saved + (p.n + t) * p.Fp + f, z);
+    constexpr uint32_t kMask = (1u << L) - 1;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const uint32_t uw = e % 2 ? uh[e / 2] & 0xffff0000u : uh[e / 2] << 16;
+      const uint32_t zw = e % 2 ? zh[e / 2] & 0xffff0000u : zh[e / 2] << 16;
+      u[e] = __uint_as_float(uw | (low[e] & kMask) << (16 - L));
+      z[e] = __uint_as_float(zw | (low[e] >> L & kMask) << (16 - L));
+    }
   }
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -52,10 +77,10 @@ __global__ __launch_bounds__(kThreads) void swiglu_grad_kernel(SwGradParams p) {
     else s = __builtin_amdgcn_rcpf(1.f + __expf(-z[e]));
     const float act = z[e] * s;
     a[e] = f + e < p.F ? g[e] * act : 0.f;
-    b[e] = f + e < p.F ? g[e] * u[e] * (s + act * (1.f - s)) : 0.f;
+    d[e] = f + e < p.F ? g[e] * u[e] * (s + act * (1.f - s)) : 0.f;
   }
-  store_vec<DT, V>(du, a);
-  store_vec<DT, V>(du + p.Fp, b);
+  store_vec<DT, V>((S*)p.d + at, a);
+  store_vec<DT, V>((S*)p.d + (int64_t)p.Fp * p.n + at, d);
 }
 
 // Small against the products that follow (a value copied once, multiplied by a
@@ -66,8 +91,10 @@ __global__ __launch_bounds__(kThreads) void swiglu_pack_kernel(SwPackParams p) {
   const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t r = at / p.to_stride;
   const int c = (int)(at - r * p.to_stride);
-  if (r >= p.rows) return;
-  ((S*)p.to)[at] = c < p.cols ? ((const S*)p.from)[r * p.from_stride + c] : (S)0;
+  if (r >= p.to_rows * p.blocks) return;
+  const int64_t block = r / p.to_rows, row = r - block * p.to_rows;
+  const bool in = c < p.cols && row < p.rows;
+  ((S*)p.to)[at] = in ? ((const S*)p.from)[(block * p.rows + row) * p.from_stride + c] : (S)0;
 }
 
 template <class DT>
@@ -85,15 +112,15 @@ bool grid_of(int64_t n, dim3* grid) {
 
 template <class DT>
 hipError_t run_grad(const SwGradParams& p, hipStream_t st) {
-  dim3 grid;
-  if (!grid_of(p.n * (p.Fp / (16 / (int)sizeof(typename DT::S))), &grid)) return hipErrorInvalidValue;
-  swiglu_grad_kernel<DT><<<grid, dim3(kThreads), 0, st>>>(p);
+  const int64_t grid = (p.n + 15) / 16 * ((p.Fp / SwElem<DT>::kStep + 3) / 4);
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  swiglu_grad_kernel<DT><<<dim3((unsigned)grid), dim3(kThreads), 0, st>>>(p);
   return hipGetLastError();
 }
 template <class DT>
 hipError_t run_pack(const SwPackParams& p, hipStream_t st) {
   dim3 grid;
-  if (!grid_of(p.rows * p.to_stride, &grid)) return hipErrorInvalidValue;
+  if (!grid_of(p.to_rows * p.blocks * p.to_stride, &grid)) return hipErrorInvalidValue;
   swiglu_pack_kernel<DT><<<grid, dim3(kThreads), 0, st>>>(p);
   return hipGetLastError();
 }

@@ -33,43 +33,149 @@ __device__ __forceinline__ void sw_tile(const SwGemmParams& p, int b, int n, int
   *tile = t;
 }
 
-// A wave's 32 x COLS values (m = lane % 32; v[j][4 i + e]: n = 32 j + 8 i + 4 (lane / 32)
-// + e) to rows of memory through the wave's own LDS, 16 bytes a lane.  `row` gives
-// the address of row m of the wave's columns or null.
-template <class DT, int COLS, class Row>
-__device__ __forceinline__ void sw_store_rows(char* lds, int lane, const float (&v)[COLS / 32][16], int n0, int n_end,
-                                              bool vec, Row row) {
-  using S = typename DT::S;
-  constexpr int kSize = sizeof(S), kPitch = COLS * kSize + 16, kChunks = COLS * kSize / 16, kPer = 16 / kSize;
-  char* mine = lds + (lane & 31) * kPitch;
+// A wave's 32 x COLS values go to memory through its own LDS: lane l holds for row m =
+// l % 32 groups of four columns, 32 j + 8 i + 4 (l / 32) + 0..3, and takes back 16
+// bytes of a row, so that memory sees whole 64-byte pieces.  Rows of PITCH bytes (16
+// more than they hold: the rows of a read then start in different banks).
+constexpr int sw_pitch(int row_bytes) { return row_bytes + 16; }
+
+template <class DT, int G>
+__device__ __forceinline__ void sw_put(char* lds, int lane, const float (&v)[G][16]) {
+  constexpr int kSize = sizeof(typename DT::S);
+  char* at = lds + (lane & 31) * sw_pitch(G * 32 * kSize) + 4 * (lane >> 5) * kSize;
 #pragma unroll
-  for (int j = 0; j < COLS / 32; ++j)
+  for (int j = 0; j < G; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      char* at = mine + (j * 32 + 8 * i + 4 * (lane >> 5)) * kSize;
-      if constexpr (kSize == 2) *(u32x2*)at = u32x2{pack2<DT>(v[j][4 * i], v[j][4 * i + 1]), pack2<DT>(v[j][4 * i + 2], v[j][4 * i + 3])};
-      else *(sw_f4*)at = sw_f4{v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3]};
+      const float* x = &v[j][4 * i];
+      if constexpr (kSize == 2) *(u32x2*)(at + (j * 32 + 8 * i) * 2) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+      else *(sw_f4*)(at + (j * 32 + 8 * i) * 4) = sw_f4{x[0], x[1], x[2], x[3]};
     }
-  __builtin_amdgcn_wave_barrier();
+}
+
+// Rows of the output: chunk c of row m to row(m) + 16 c bytes, columns n0.. below n_end
+template <int ROW_BYTES, int SIZE, class Row>
+__device__ __forceinline__ void sw_take_rows(const char* lds, int lane, bool whole, int n0, int n_end, bool vec, Row row) {
+  constexpr int kChunks = ROW_BYTES / 16, kPer = 16 / SIZE, kIters = 32 * kChunks / kWave;
+  u32x4 x[kIters];
 #pragma unroll
-  for (int i = 0; i < 32 * kChunks / kWave; ++i) {
-    const int q = i * kWave + lane, m = q / kChunks, c = q % kChunks;
-    const u32x4 x = *(const u32x4*)(lds + m * kPitch + c * 16);
-    S* dst = (S*)row(m);
-    const int n = n0 + c * kPer;
+  for (int i = 0; i < kIters; ++i) {
+    const int q = i * kWave + lane;
+    x[i] = *(const u32x4*)(lds + q / kChunks * sw_pitch(ROW_BYTES) + q % kChunks * 16);
+  }
+  if (whole) {  // (the whole tile: no row or column is left out)
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      const int q = i * kWave + lane;
+      *(u32x4*)(row(q / kChunks) + q % kChunks * 16) = x[i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kIters; ++i) {
+    const int q = i * kWave + lane, c = q % kChunks, n = n0 + c * kPer;
+    char* dst = row(q / kChunks);
     if (!dst || n >= n_end) continue;
     if (vec && n + kPer <= n_end) {
-      *(u32x4*)(dst + c * kPer) = x;
+      *(u32x4*)(dst + c * 16) = x[i];
     } else {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         if (n + e >= n_end) break;
-        if constexpr (kSize == 2) dst[c * kPer + e] = (S)(x[e / 2] >> (16 * (e & 1)));
-        else dst[c * kPer + e] = __uint_as_float(x[e]);
+        if constexpr (SIZE == 2) ((uint16_t*)dst)[c * kPer + e] = (uint16_t)(x[i][e / 2] >> (16 * (e & 1)));
+        else ((uint32_t*)dst)[c * kPer + e] = x[i][e];
       }
     }
   }
-  __builtin_amdgcn_wave_barrier();
+}
+
+// Rows of a plane in blocks (SwPlanes): G groups of 32 columns, BLOCK bytes of a row a block
+template <int ROW_BYTES, int BLOCK>
+__device__ __forceinline__ void sw_take_blocks(const char* lds, int lane, char* plane, int block0, int blocks, int64_t n,
+                                               int m0, int M) {
+  constexpr int kPer = BLOCK / 16, kBlocks = ROW_BYTES / BLOCK;  // chunks of a block's row, blocks
+  constexpr int kIters = 32 * kPer * kBlocks / kWave;
+#pragma unroll
+  for (int i = 0; i < kIters; ++i) {
+    const int q = i * kWave + lane, b = q / (32 * kPer), m = q / kPer % 32, c = q % kPer;
+    const u32x4 x = *(const u32x4*)(lds + m * sw_pitch(ROW_BYTES) + b * BLOCK + c * 16);
+    if (block0 + b < blocks && m0 + m < M) *(u32x4*)(plane + ((int64_t)(block0 + b) * n + m0 + m) * BLOCK + c * 16) = x;
+  }
+}
+
+// fp32 bits rounded to 16 + L of them, nearest; a NaN stays one
+template <int L>
+__device__ __forceinline__ uint32_t sw_round_bits(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return x != x ? b | 0x400000u : b + (1u << (15 - L));
+}
+
+// u and z of a wave's 32 rows to the planes that the backward reads
+template <class DT, int H>
+__device__ __forceinline__ void sw_save(const SwGemmParams& p, char* lds, int lane, int m0, int n0, const float (&v)[2 * H][16]) {
+  using P = SwPlanes<DT>;
+  constexpr int kSize = sizeof(typename DT::S), kRow = H * 32 * kSize;
+  constexpr int kStep = SwElem<DT>::kStep;
+  const SwPlaneAddress at = sw_planes<DT>(p.saved, p.n_tok, p.Fp);
+  const int blocks = p.Fp / kStep, block0 = n0 / kStep;
+  if constexpr (kSize == 4) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float x[H][16];
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[j][i] = v[half * H + j][i];
+      sw_put<DT, H>(lds, lane, x);
+      __builtin_amdgcn_wave_barrier();
+      sw_take_blocks<kRow, kSwStepBytes>(lds, lane, half ? at.z : at.u, block0, blocks, p.n_tok, m0, p.M);
+      __builtin_amdgcn_wave_barrier();
+    }
+  } else {
+    constexpr int L = P::kLow, kLowRow = H * 32 * L / 4;  // bytes of the low bits of a row's pairs
+    char* zu = lds + 32 * sw_pitch(kRow);
+    char* lo = zu + 32 * sw_pitch(kRow);
+    const int m = lane & 31, q = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < H; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t u[4], z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u[e] = sw_round_bits<L>(v[j][4 * i + e]);
+          z[e] = sw_round_bits<L>(v[H + j][4 * i + e]);
+        }
+        const int col = j * 32 + 8 * i + 4 * q;
+        *(u32x2*)(lds + m * sw_pitch(kRow) + col * 2) = u32x2{hi_pair(u[0], u[1]), hi_pair(u[2], u[3])};
+        *(u32x2*)(zu + m * sw_pitch(kRow) + col * 2) = u32x2{hi_pair(z[0], z[1]), hi_pair(z[2], z[3])};
+        if constexpr (L == 4) {  // a byte a pair: u's bits low
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w |= ((u[e] >> 12 & 15u) | (z[e] >> 8 & 0xf0u)) << (8 * e);
+          *(uint32_t*)(lo + m * sw_pitch(kLowRow) + col) = w;
+        } else {  // two bytes a pair
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = (u[e] >> 8 & 0xffu) | (z[e] & 0xff00u);
+          *(u32x2*)(lo + m * sw_pitch(kLowRow) + col * 2) = u32x2{w[0] | w[1] << 16, w[2] | w[3] << 16};
+        }
+      }
+    __builtin_amdgcn_wave_barrier();
+    sw_take_blocks<kRow, kSwStepBytes>(lds, lane, at.u, block0, blocks, p.n_tok, m0, p.M);
+    sw_take_blocks<kRow, kSwStepBytes>(zu, lane, at.z, block0, blocks, p.n_tok, m0, p.M);
+    sw_take_blocks<kLowRow, P::kLowBlock>(lo, lane, at.low, block0, blocks, p.n_tok, m0, p.M);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// LDS bytes of a wave in sw_finish, COLS columns of the product
+template <class DT, int FORM, int COLS>
+constexpr int sw_finish_lds() {
+  constexpr int kSize = sizeof(typename DT::S), H = FORM == kFwd ? COLS / 2 : COLS;
+  int n = 32 * sw_pitch(H * kSize);
+  if (FORM == kFwd && kSize == 2) n = 2 * n + 32 * sw_pitch(H * SwPlanes<DT>::kLow / 4);
+  return n;
 }
 
 // What becomes of a wave's 32 rows m0.. x COLS columns of the product (fwd: COLS is
@@ -77,58 +183,50 @@ __device__ __forceinline__ void sw_store_rows(char* lds, int lane, const float (
 template <class DT, int FORM, int COLS>
 __device__ __forceinline__ void sw_finish(const SwGemmParams& p, char* lds, int lane, int m0, int n0,
                                           float (&v)[COLS / 32][16]) {
-  using S = typename DT::S;
+  constexpr int kSize = sizeof(typename DT::S);
   if constexpr (FORM == kFwd) {
     constexpr int H = COLS / 64;  // 32-column groups of u
-    if (p.saved) {
-      const int n_end = (p.n_out + 7) / 8 * 8;  // (whole vectors: the rows are padded)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float x[H][16];
-#pragma unroll
-        for (int j = 0; j < H; ++j)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[j][i] = v[half * H + j][i];
-        sw_store_rows<DT, H * 32>(lds, lane, x, n0, n_end, true, [&](int m) -> void* {
-          return m0 + m < p.M ? (S*)p.saved + ((int64_t)half * p.M + m0 + m) * p.saved_stride + n0 : nullptr;
-        });
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+    if (p.saved) sw_save<DT, H>(p, lds, lane, m0, n0, v);
     float h[H][16];
 #pragma unroll
     for (int j = 0; j < H; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) h[j][i] = v[j][i] * sw_silu<DT>(v[H + j][i]);
-    sw_store_rows<DT, H * 32>(lds, lane, h, n0, p.n_out, p.out_vec, [&](int m) -> void* {
-      return m0 + m < p.M ? (S*)p.out + (int64_t)(m0 + m) * p.out_stride + n0 : nullptr;
+    sw_put<DT, H>(lds, lane, h);
+    __builtin_amdgcn_wave_barrier();
+    const bool whole = m0 + 32 <= p.M && n0 + H * 32 <= p.n_out && p.out_vec;
+    char* out = (char*)p.out + ((int64_t)m0 * p.out_stride + n0) * kSize;
+    sw_take_rows<H * 32 * kSize, kSize>(lds, lane, whole, n0, p.n_out, p.out_vec, [&](int m) -> char* {
+      return whole || m0 + m < p.M ? out + (int64_t)m * p.out_stride * kSize : nullptr;
     });
   } else {
-    sw_store_rows<DT, COLS>(lds, lane, v, n0, p.n_out, p.out_vec, [&](int m) -> void* {
-      int r = m0 + m;
-      if constexpr (FORM == kDw) {  // rows of the padded halves
-        const int half = r >= p.Fp, f = r - half * p.Fp;
-        if (half * p.Fp + f >= 2 * p.Fp || f >= p.F) return nullptr;
-        r = half * p.F + f;
-      } else {
-        if (r >= p.M) return nullptr;
-      }
-      return (S*)p.out + (int64_t)r * p.out_stride + n0;
+    sw_put<DT, COLS / 32>(lds, lane, v);
+    __builtin_amdgcn_wave_barrier();
+    // dw: rows of the padded halves
+    const int half = FORM == kDw && m0 >= p.Fp, f0 = m0 - half * p.Fp, r0 = half * p.F + f0;
+    const int rows = FORM == kDw ? (half < 2 && f0 < p.Fp ? p.F - f0 : 0) : p.M - m0;
+    const bool whole = rows >= 32 && n0 + COLS <= p.n_out && p.out_vec;
+    char* out = (char*)p.out + ((int64_t)r0 * p.out_stride + n0) * kSize;
+    sw_take_rows<COLS * kSize, kSize>(lds, lane, whole, n0, p.n_out, p.out_vec, [&](int m) -> char* {
+      return whole || m < rows ? out + (int64_t)m * p.out_stride * kSize : nullptr;
     });
   }
+  __builtin_amdgcn_wave_barrier();
 }
 
 template <class DT, int FORM, int BM, int BN, bool SPLIT>
-__global__ __launch_bounds__(256, BM * BN >= 256 * 256 ? 1 : 2) void swiglu_gemm_kernel(SwGemmParams p) {
+__global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gemm_kernel(SwGemmParams p) {
   using E = SwElem<DT>;
   using OpP = SwOperand<DT, BN, FORM != kFwd>;
   using OpQ = SwOperand<DT, BM, FORM == kDw>;
   constexpr int NP = BN / 64, NQ = BM / 64;  // 32 x 32 tiles of a wave
   constexpr int kStage = OpP::kBytes + OpQ::kBytes;
+  constexpr int kStages = sw_stages(BM, BN), kAhead = kStages - 1;  // steps loaded ahead
   constexpr int kLoads = OpP::kLoads + OpQ::kLoads;
+  constexpr int kFirst = kLoads / 2;  // of a step's loads, issued in the first half step
   constexpr int kCols = FORM == kFwd ? BN / 2 : BN;  // output columns of a tile
   constexpr int es = E::kSize;
-  __shared__ __align__(1024) char lds[kSwStages * kStage];
+  __shared__ __align__(1024) char lds[kStages * kStage];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave & 1, wn = wave >> 1;
@@ -160,10 +258,12 @@ __global__ __launch_bounds__(256, BM * BN >= 256 * 256 ? 1 : 2) void swiglu_gemm
     int r, c;
     OpQ::place(i, tid, &r, &c);
     if constexpr (FORM != kDw) {
-      oq.off[i] = (uint32_t)((int64_t)(min(m0 + r, p.M - 1) - m0) * p.q_stride * es) + c * 16;
+      // (dx: rows of a block are kSwStepBytes apart)
+      oq.off[i] = (uint32_t)((min(m0 + r, p.M - 1) - m0) * (FORM == kDx ? kSwStepBytes : p.q_stride * es)) + c * 16;
       oq.kr[i] = c * E::kPer;
     } else {
-      oq.off[i] = (uint32_t)((int64_t)r * p.q_stride * es) + (min(m0 + c * E::kPer, p.M - E::kPer) - m0) * es;
+      const int block = min(c / 4, (p.M - m0) / E::kStep - 1);
+      oq.off[i] = (uint32_t)((block * p.n_tok + r) * kSwStepBytes) + c % 4 * 16;
       oq.kr[i] = r;
     }
   }
@@ -171,40 +271,46 @@ __global__ __launch_bounds__(256, BM * BN >= 256 * 256 ? 1 : 2) void swiglu_gemm
   oq.place_reads(wm * (BM / 2), lane, OpP::kBytes);
   const uint32_t lds0 = lds_address(lds) + wave * 1024;
 
-  // loads of step s (counted within the split) into its stage
-  auto load = [&](int s) {
-    const int k0 = (first + s) * E::kStep;
-    const char *bp, *bq;
-    int left;  // k's of this step that exist
-    if constexpr (FORM == kFwd) {
-      bp = (const char*)p.p + (int64_t)k0 * es;
-      bq = (const char*)p.q + ((int64_t)m0 * p.q_stride + k0) * es;
-      left = p.K - k0;
-    } else if constexpr (FORM == kDx) {
-      const int half = k0 >= p.Fp, f = k0 - half * p.Fp;
-      bp = (const char*)p.p + ((int64_t)(half * p.F + f) * p.p_stride + n0) * es;
-      bq = (const char*)p.q + ((int64_t)m0 * p.q_stride + k0) * es;
-      left = p.F - f;
-    } else {
-      bp = (const char*)p.p + ((int64_t)k0 * p.p_stride + n0) * es;
-      bq = (const char*)p.q + ((int64_t)k0 * p.q_stride + m0) * es;
-      left = p.K - k0;
-    }
-    const uint32_t to = lds0 + (s & (kSwStages - 1)) * kStage;
+  // (kept in a register: read from memory in the loop, it would make every wait for
+  // LDS a wait for everything)
+  const char* zeros = (const char*)&sw_zeros;
+  asm volatile("" : "+s"(zeros));
+
+  // Loads of the next step into its stage, piece by piece so that the matrix cores
+  // work between them.
+  const int k0 = first * E::kStep;
+  const char* bp = (const char*)p.p + (FORM == kFwd ? (int64_t)k0 : (int64_t)k0 * p.p_stride + n0) * es;
+  const char* bq = (const char*)p.q + (FORM == kFwd  ? ((int64_t)m0 * p.q_stride + k0) * es
+                                       : FORM == kDx ? ((int64_t)(k0 / E::kStep) * p.n_tok + m0) * kSwStepBytes
+                                                     : ((int64_t)(m0 / E::kStep) * p.n_tok + k0) * kSwStepBytes);
+  const int64_t ahead_p = FORM == kFwd ? kSwStepBytes : (int64_t)E::kStep * p.p_stride * es;
+  const int64_t ahead_q = FORM == kFwd  ? kSwStepBytes
+                          : FORM == kDx ? p.n_tok * kSwStepBytes
+                                        : (int64_t)E::kStep * kSwStepBytes;
+  auto behind = [](uint32_t stage) { return stage == (kStages - 1) * kStage ? 0u : stage + kStage; };
+  uint32_t to = 0;  // the step's stage, in bytes
+  auto next_step = [&]() {
+    bp += ahead_p;
+    bq += ahead_q;
+    to = behind(to);
+  };
+  auto load_piece = [&](int i) {  // of a whole step
+    if (i < OpP::kLoads) sw_dma(bp, op.off[i % OpP::kLoads], lds0 + to + i * 4096);
+    else sw_dma(bq, oq.off[(i - OpP::kLoads) % OpQ::kLoads], lds0 + to + OpP::kBytes + (i - OpP::kLoads) * 4096);
+  };
+  auto load = [&](int s) {  // step s of the split, k possibly ending in it
+    const int left = p.K - (first + s) * E::kStep;
     if (left >= E::kStep) {
 #pragma unroll
-      for (int i = 0; i < OpP::kLoads; ++i) sw_dma(bp, op.off[i], to + i * 4096);
-#pragma unroll
-      for (int i = 0; i < OpQ::kLoads; ++i) sw_dma(bq, oq.off[i], to + OpP::kBytes + i * 4096);
+      for (int i = 0; i < kLoads; ++i) load_piece(i);
     } else {
-      const char* z = (const char*)&sw_zeros;
 #pragma unroll
-      for (int i = 0; i < OpP::kLoads; ++i) sw_dma64(op.kr[i] < left ? bp + op.off[i] : z, to + i * 4096);
+      for (int i = 0; i < OpP::kLoads; ++i) sw_dma64(op.kr[i] < left ? bp + op.off[i] : zeros, lds0 + to + i * 4096);
 #pragma unroll
       for (int i = 0; i < OpQ::kLoads; ++i)
-        // (dx: the gradients' columns behind the end are there, and zero)
-        sw_dma64(FORM == kDx || oq.kr[i] < left ? bq + oq.off[i] : z, to + OpP::kBytes + i * 4096);
+        sw_dma64(oq.kr[i] < left ? bq + oq.off[i] : zeros, lds0 + to + OpP::kBytes + i * 4096);
     }
+    next_step();
   };
 
   sw_f16 acc[NP][NQ];
@@ -216,41 +322,56 @@ __global__ __launch_bounds__(256, BM * BN >= 256 * 256 ? 1 : 2) void swiglu_gemm
       for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
 
   u32x4 fp[2][NP], fq[2][NQ];
-  auto read = [&](int buf, uint32_t stage, int kk) {
-#pragma unroll
-    for (int j = 0; j < NP; ++j) fp[buf][j] = op.read(lds, stage, kk, j);
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) fq[buf][j] = oq.read(lds, stage, kk, j);
+  auto read_one = [&](int buf, uint32_t stage, int kk, int j) {
+    if (j < NP) fp[buf][j % NP] = op.read(lds, stage, kk, j % NP);
+    else fq[buf][(j - NP) % NQ] = oq.read(lds, stage, kk, (j - NP) % NQ);
   };
-  auto multiply = [&](int buf) {
+  // The products of one half step, with what the next ones need issued evenly between
+  // them: the fragments' reads, then loads l0.. l1 of a step.
+  auto half_step = [&](int buf, uint32_t stage, int kk, int l0, int l1) {
+    constexpr int kTiles = NP * NQ, kReads = NP + NQ;
 #pragma unroll
-    for (int a = 0; a < NP; ++a)
+    for (int t = 0; t < kTiles; ++t) {
+      sw_mfma<DT>(fp[buf][t / NQ], fq[buf][t % NQ], acc[t / NQ][t % NQ]);
+      const int ops = kReads + l1 - l0;
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) sw_mfma<DT>(fp[buf][a], fq[buf][b], acc[a][b]);
+      for (int e = 0; e < kReads + kLoads; ++e) {
+        if (e >= ops || e * kTiles / ops != t) continue;
+        if (e < kReads) read_one(buf ^ 1, stage, kk, e);
+        else load_piece(l0 + e - kReads);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
-
   // the loads of the next `ahead` steps may still be under way
   auto wait = [&](int ahead) {
-    if (ahead >= 2) sw_wait_barrier<2 * kLoads>();
-    else if (ahead == 1) sw_wait_barrier<kLoads>();
+    if (ahead >= 2 && kAhead > 2) sw_wait_barrier<(kAhead > 2 ? 2 : 0) * kLoads>();
+    else if (ahead >= 1) sw_wait_barrier<kLoads>();
     else sw_wait_barrier<0>();
   };
 
 #pragma unroll
-  for (int s = 0; s < kSwStages - 1; ++s)
+  for (int s = 0; s < kAhead; ++s)
     if (s < nk) load(s);
   wait(nk - 1);
-  read(0, 0, 0);
-  for (int s = 0; s < nk; ++s) {
-    const uint32_t stage = (s & (kSwStages - 1)) * kStage;
-    read(1, stage, 1);
-    if (s + kSwStages - 1 < nk) load(s + kSwStages - 1);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < NP + NQ; ++j) read_one(0, 0, 0, j);
+  const int whole = (int)min((int64_t)nk, (int64_t)p.K / E::kStep - first);  // steps in which k does not end
+  int s = 0;
+  uint32_t stage = 0;
+  for (; s + kAhead < whole; ++s) {
+    half_step(0, stage, 1, 0, kFirst);
+    stage = behind(stage);
+    sw_wait_barrier<(kAhead - 2) * kLoads + kFirst>();
+    half_step(1, stage, 0, kFirst, kLoads);
+    next_step();
+  }
+  for (; s < nk; ++s) {
+    if (s + kAhead < nk) load(s + kAhead);
+    half_step(0, stage, 1, 0, 0);
+    stage = behind(stage);
     wait(nk - 2 - s);
-    if (s + 1 < nk) read(0, ((s + 1) & (kSwStages - 1)) * kStage, 0);
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
+    half_step(1, stage, 0, 0, 0);  // (behind the last step: read, not used)
   }
 
   if constexpr (SPLIT) {
@@ -265,8 +386,9 @@ __global__ __launch_bounds__(256, BM * BN >= 256 * 256 ? 1 : 2) void swiglu_gemm
               sw_f4{acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
   } else {
     sw_wait_barrier<0>();  // the stages are free
-    constexpr int kPitch = kCols / 2 * es + 16;
-    char* mine = lds + wave * (32 * kPitch);
+    constexpr int kMine = sw_finish_lds<DT, FORM, NP * 32>();
+    static_assert(4 * kMine <= kStages * kStage, "LDS");
+    char* mine = lds + wave * kMine;
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       float v[NP][16];
@@ -289,9 +411,8 @@ __global__ __launch_bounds__(256) void swiglu_reduce_kernel(SwGemmParams p) {
   // columns of a wave: all of them where u and z belong together, else one group of 32
   constexpr int G = FORM == kFwd ? NP : 1;
   constexpr int kParts = NP / G;
-  constexpr int kStaged = FORM == kFwd ? NP * 16 : 32;
-  constexpr int kPitch = kStaged * (int)sizeof(typename DT::S) + 16;
-  __shared__ __align__(16) char lds[4 * 32 * kPitch];
+  constexpr int kMine = sw_finish_lds<DT, FORM, G * 32>();
+  __shared__ __align__(16) char lds[4 * kMine];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int tiles = p.tiles_m * p.tiles_n;
   const int w = blockIdx.x * 4 + wave;
@@ -318,7 +439,7 @@ __global__ __launch_bounds__(256) void swiglu_reduce_kernel(SwGemmParams p) {
       }
   }
   const int wm = tw & 1, wn = tw >> 1;
-  sw_finish<DT, FORM, G * 32>(p, lds + wave * 32 * kPitch, lane, tm * BM + wm * (BM / 2) + 32 * b,
+  sw_finish<DT, FORM, G * 32>(p, lds + wave * kMine, lane, tm * BM + wm * (BM / 2) + 32 * b,
                               tn * kCols + wn * (kCols / 2) + part * 32, v);
 }
 
@@ -340,7 +461,8 @@ hipError_t sw_run(const SwGemmParams& p, hipStream_t st) {
 template <class DT, int FORM>
 hipError_t sw_tile_pick(int tile, const SwGemmParams& p, hipStream_t st) {
   if (tile == 0) return sw_run<DT, FORM, 256, 256>(p, st);
-  if (tile == 1) return sw_run<DT, FORM, 128, 128>(p, st);
+  if (tile == 1) return sw_run<DT, FORM, 128, 256>(p, st);
+  if (tile == 2) return sw_run<DT, FORM, 128, 128>(p, st);
   return sw_run<DT, FORM, 64, 128>(p, st);
 }
 

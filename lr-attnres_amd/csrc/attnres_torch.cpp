@@ -50,7 +50,7 @@ struct Lib {
   X(attnres_phase2_forward) X(attnres_phase2_backward) X(attnres_phase2_backward_workspace_size)                   \
   X(attnres_accum_read_forward) X(attnres_accum_read_backward) X(attnres_block_accum_forward)                      \
   X(attnres_block_accum_backward) X(attnres_qkv_rotary_forward) X(attnres_qkv_rotary_backward)                     \
-  X(attnres_swiglu_saved_row_stride) X(attnres_swiglu_forward_workspace_size)                                      \
+  X(attnres_swiglu_saved_size) X(attnres_swiglu_forward_workspace_size)                                      \
   X(attnres_swiglu_backward_workspace_size) X(attnres_swiglu_forward) X(attnres_swiglu_backward)
   ATTNRES_FNS(ATTNRES_FN)
 } lib;

@@ -169,7 +169,7 @@ struct SwigluFn : torch::autograd::Function<SwigluFn> {
     auto shape = x.sizes().vec();
     shape.back() = d.hidden;
     Tensor h = at::empty(shape, opt), ws;
-    if (save) *saved = at::empty({2, d.n_tok, lib.attnres_swiglu_saved_row_stride(&d)}, opt);
+    if (save) *saved = bytes(lib.attnres_swiglu_saved_size(&d), x.device());
     const size_t n = lib.attnres_swiglu_forward_workspace_size(&d);
     if (n) ws = bytes(n, x.device());
     check(lib.attnres_swiglu_forward(&d, h.data_ptr(), ptr(*saved), ptr(ws), n, stream_of(x.device())), "swiglu forward");
