@@ -1989,9 +1989,9 @@ def _swiglu_op(x: Tensor, weight: Tensor, save: bool) -> tuple[Tensor, Tensor]:
 @_swiglu_op.register_fake
 def _swiglu_fake(x, weight, save):
     n, F_ = x.size(0), weight.size(0) // 2
-    # attnres_swiglu_saved_size: hidden columns in groups of 32, bytes of a pair (u, z)
-    pair = {torch.float32: 8, torch.bfloat16: 5, torch.float16: 6}[x.dtype]
-    size = n * ((F_ + 31) // 32 * 32) * pair if save else 0
+    # attnres_swiglu_saved_size: hidden columns in whole k steps, bytes of a pair (u, z)
+    step, pair = {torch.float32: (16, 8), torch.bfloat16: (32, 5), torch.float16: (32, 6)}[x.dtype]
+    size = n * ((F_ + step - 1) // step * step) * pair if save else 0
     return x.new_empty((n, F_)), x.new_empty((size,), dtype=torch.uint8)
 
 

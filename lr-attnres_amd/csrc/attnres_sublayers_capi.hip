@@ -1,6 +1,5 @@
 // C ABI of the sublayer kernels: argument checks, kernel selection and launch
 // geometry.  Declared in include/attnres_sublayers.h.
-#include <stdlib.h>
 #include <string.h>
 
 #include "../../include/attnres_sublayers.h"
@@ -148,7 +147,7 @@ constexpr int kCus = 256;
 
 struct SwLayout {
   int es, per, step;   // bytes of a value, values of a chunk and of a k step
-  int Fp;              // hidden, in whole steps and rows of a store
+  int Fp;              // hidden, in whole steps
   int Dp;              // dim, in whole chunks
   bool x_ok, w_ok;     // the products can read the operand as it is
   bool w_ok_dx;        // and dx the weight: its halves fill k steps
@@ -162,7 +161,7 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
   l.es = es_of(d->dtype);
   l.per = 16 / l.es;
   l.step = kSwStepBytes / l.es;
-  l.Fp = round_up(d->hidden, kSwRows);
+  l.Fp = round_up(d->hidden, l.step);
   l.Dp = round_up(d->dim, l.per);
   // direct loads of 16 bytes; a tile's rows within 32-bit offsets of its first one
   const int64_t far = ((int64_t)1 << 32) / (256 * l.es) - d->dim;
@@ -174,39 +173,49 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
   return l;
 }
 
-// Tile and splits of a product with `steps` k steps: the least time in a simple
-// model, in units of a 256 x 256 tile's step.  A launch runs in rounds of as many
-// workgroups as the CUs hold; a split's sums are written and read once more.
+// Tile and splits of a product with `steps` k steps: the least time in a model of a
+// launch, in us.  The CUs take workgroups in rounds, as many together as LDS holds;
+// together they share the matrix cores.  A split product's sums are written and read
+// once more, by a second launch.  The constants are fitted to 700 launches (15 shapes
+// of 64 to 16384 tokens, every tile, 1 to 64 splits, fp32 and bf16); there the model's
+// choice is 1% slower than the best one in the mean and 11% at most.  The large tile
+// moves the least data a product, the small one fills the CUs: forward of 2000 tokens,
+// dim 1024, hidden 4096, bf16: 39 us with 256 x 256, 62 with 64 x 128; of 512 tokens,
+// dim 1024, hidden 1024: 29 and 8.5.
 struct SwShape {
   int tile, tiles_m, tiles_n, splits, steps;
 };
 
-SwShape sw_shape(int form, int64_t M, int N, int steps) {
-  // a step's and a tile's fixed cost, and the workgroups of a CU
-  constexpr double kStepCost[kSwTiles] = {1.0, 0.70, 0.40, 0.28}, kFixed[kSwTiles] = {12.0, 7.0, 6.0, 4.0};
-  static const int force = getenv("SW_TILE") ? atoi(getenv("SW_TILE")) : -1;
+struct SwCosts {
+  double step[kSwTiles];      // a k step of one workgroup
+  double together[kSwTiles];  // of g workgroups on a CU: g * together times that, if more
+  double fixed[kSwTiles];     // a workgroup's begin and end
+  double launch, bytes_us;    // a split's second launch, and its traffic
+};
+constexpr SwCosts kCost16 = {{0.589, 0.481, 0.232, 0.205}, {1.0, 0.935, 1.0, 0.73}, {5.77, 3.5, 3.26, 2.55}, 3.95, 8.7e6};
+constexpr SwCosts kCost32 = {{3.905, 2.052, 1.062, 0.59}, {1.0, 0.981, 0.968, 0.906}, {3.69, 0.82, 0.59, 0.0}, 5.32, 7.8e6};
+
+SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {
+  const SwCosts& k = dtype == ATTNRES_DTYPE_F32 ? kCost32 : kCost16;
   SwShape best{};
   double least = 1e300;
   for (int t = 0; t < kSwTiles; ++t) {
-    if (force >= 0 && t != force) continue;
     const int cols = form == kFwd ? kSwTileN[t] / 2 : kSwTileN[t];
-    const int tm = (int)((M + kSwTileM[t] - 1) / kSwTileM[t]), tn = (N + cols - 1) / cols;
-    for (int splits = 1; splits <= 64; ++splits) {
+    const int64_t tm = (M + kSwTileM[t] - 1) / kSwTileM[t], tn = (N + cols - 1) / cols;
+    const int together = sw_per_cu(kSwTileM[t], kSwTileN[t]);
+    for (int splits = 1; splits <= 64 && splits <= steps; ++splits) {
       const int per = (steps + splits - 1) / splits;
-      if (splits > 1 && (per < 4 || (steps + per - 1) / per != splits)) continue;
-      const int64_t wgs = (int64_t)tm * tn * splits;
-      if (wgs > (1 << 24)) continue;
-      const double rounds = (double)((wgs + kCus - 1) / kCus);  // tiles that one CU works on
-      const double together = rounds < sw_per_cu(kSwTileM[t], kSwTileN[t]) ? rounds : sw_per_cu(kSwTileM[t], kSwTileN[t]);
-      // co-resident workgroups share the CU: full rate only with all of them there
-      double cost = (per * kStepCost[t] + kFixed[t]) * (rounds / together) * (1.0 + 0.75 * (together - 1));
-      if (splits > 1) {
-        const double bytes = (double)wgs * kSwTileM[t] * kSwTileN[t] * 4 * 2;
-        cost += 12.0 + bytes / 2.0e6;  // a second launch; about 4 TB/s against 0.5 us a step
-      }
+      if ((steps + per - 1) / per != splits) continue;
+      const int64_t wgs = tm * tn * splits;
+      if (wgs > (1 << 24)) break;
+      const int64_t rounds = (wgs + kCus - 1) / kCus;  // workgroups that one CU works on
+      auto group = [&](int g) { return per * k.step[t] * (g * k.together[t] > 1.0 ? g * k.together[t] : 1.0) + k.fixed[t]; };
+      double cost = (double)(rounds / together) * group(together);
+      if (rounds % together) cost += group((int)(rounds % together));
+      if (splits > 1) cost += k.launch + (double)wgs * kSwTileM[t] * kSwTileN[t] * 8 / k.bytes_us;
       if (cost < least) {
         least = cost;
-        best = SwShape{t, tm, tn, splits, per};
+        best = SwShape{t, (int)tm, (int)tn, splits, per};
       }
     }
   }
@@ -235,13 +244,13 @@ int check_swiglu(const attnres_swiglu_desc* d) {
 }
 
 SwShape fwd_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
-  return sw_shape(kFwd, d->n_tok, d->hidden, (d->dim + l.step - 1) / l.step);
+  return sw_shape(kFwd, d->dtype, d->n_tok, d->hidden, (d->dim + l.step - 1) / l.step);
 }
 SwShape dx_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
-  return sw_shape(kDx, d->n_tok, d->dim, 2 * l.Fp / l.step);
+  return sw_shape(kDx, d->dtype, d->n_tok, d->dim, 2 * l.Fp / l.step);
 }
 SwShape dw_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
-  return sw_shape(kDw, 2 * l.Fp, d->dim, (int)((d->n_tok + l.step - 1) / l.step));
+  return sw_shape(kDw, d->dtype, 2 * l.Fp, d->dim, (int)((d->n_tok + l.step - 1) / l.step));
 }
 
 size_t packed_x(const attnres_swiglu_desc* d, const SwLayout& l) {
@@ -291,7 +300,7 @@ extern "C" size_t attnres_swiglu_saved_size(const attnres_swiglu_desc* d) {
 extern "C" size_t attnres_swiglu_forward_workspace_size(const attnres_swiglu_desc* d) {
   if (check_swiglu(d) || d->n_tok == 0) return 0;
   const SwLayout l = sw_layout(d);
-  return packed_x(d, l) + packed_w(d, l, false) + sw_partials(fwd_shape(d, l));
+  return packed_x(d, l) + packed_w(d, l, false) + (d->n_tok <= kSwFew ? 0 : sw_partials(fwd_shape(d, l)));
 }
 
 extern "C" size_t attnres_swiglu_backward_workspace_size(const attnres_swiglu_desc* d, int32_t want_dx, int32_t want_dw) {
@@ -309,7 +318,8 @@ extern "C" int attnres_swiglu_forward(const attnres_swiglu_desc* d, void* h, voi
   if (!h) return api_fail(ATTNRES_EINVAL, "h is NULL");
   if (saved && !aligned(saved, 16)) return api_fail(ATTNRES_EINVAL, "saved is not aligned to 16 bytes");
   const SwLayout l = sw_layout(d);
-  const SwShape s = fwd_shape(d, l);
+  const bool few = d->n_tok <= kSwFew;
+  const SwShape s = few ? SwShape{0, 0, 0, 1, 1} : fwd_shape(d, l);
   const size_t px = packed_x(d, l), pw = packed_w(d, l, false), need = px + pw + sw_partials(s);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
@@ -330,7 +340,7 @@ extern "C" int attnres_swiglu_forward(const attnres_swiglu_desc* d, void* h, voi
   g.out_vec = d->hidden % l.per == 0 && aligned(h, 16);
   g.saved = saved;
   g.partials = (float*)(ws + px + pw);
-  if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kFwd, s.tile, g, st);
+  if (err == hipSuccess) err = few ? launch_swiglu_few(d->dtype, g, st) : launch_swiglu_gemm(d->dtype, kFwd, s.tile, g, st);
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu forward launch failed: %s", hipGetErrorString(err));
   return ATTNRES_OK;
 }

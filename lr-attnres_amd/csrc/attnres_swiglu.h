@@ -38,7 +38,6 @@ namespace attnres {
 enum SwForm { kFwd = 0, kDx = 1, kDw = 2 };
 
 constexpr int kSwStepBytes = 64;  // of k, per row: 32 16-bit values, 16 fp32
-constexpr int kSwRows = 32;       // rows of the product that are stored together: a half's are padded to them
 constexpr int kSwTiles = 4;
 constexpr int kSwTileM[kSwTiles] = {256, 128, 128, 64}, kSwTileN[kSwTiles] = {256, 256, 128, 128};
 // stages of LDS, and the workgroups that a CU's 160 KB then hold
@@ -52,7 +51,7 @@ struct SwGemmParams {
   int32_t M, N;             // rows / columns of the product (fwd: N = hidden; else in whole chunks)
   int32_t n_out;            // columns of the output
   int32_t K;                // fwd: dim, dx: 2 Fp, dw: tokens
-  int32_t F, Fp;            // hidden, and rounded up to kSwRows
+  int32_t F, Fp;            // hidden, and rounded up to a whole number of steps
   int32_t tiles_m, tiles_n;
   int32_t splits, steps;    // k steps of a split
   void* out;                // [M, N] (dw: rows of the padded halves are left out)
@@ -64,6 +63,8 @@ struct SwGemmParams {
 };
 
 hipError_t launch_swiglu_gemm(int dtype, int form, int tile, const SwGemmParams& p, hipStream_t st);
+constexpr int kSwFew = 48;  // rows at most
+hipError_t launch_swiglu_few(int dtype, const SwGemmParams& p, hipStream_t st);  // the forward
 
 // [du dz] of the backward, in blocks, with zeros behind each half's F columns
 struct SwGradParams {
@@ -135,6 +136,30 @@ __host__ __device__ inline SwPlaneAddress sw_planes(const void* saved, int64_t n
   const int64_t plane = n * Fp * SwElem<DT>::kSize;
   char* at = (char*)saved;
   return {at, at + plane, at + 2 * plane};
+}
+
+// fp32 bits to be cut to 16 + L of them, rounded to nearest.  (A NaN stays one: those of
+// 16-bit operands, and the hardware's own, have no bits that the addition could carry.)
+template <int L>
+__device__ __forceinline__ uint32_t sw_round_bits(float x) {
+  return __float_as_uint(x) + (1u << (15 - L));
+}
+// byte 1 of each of four words
+__device__ __forceinline__ uint32_t sw_bytes1(const uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0501u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010c0cu);
+  return a | b;
+}
+// and the low bits of four pairs (u, z) of a row, from column col on: u's below z's
+template <int L>
+__device__ __forceinline__ void sw_store_low(char* row, int64_t col, const uint32_t (&u)[4], const uint32_t (&z)[4]) {
+  if constexpr (L == 4) {  // a byte a pair
+    *(uint32_t*)(row + col) = (sw_bytes1(u) >> 4 & 0x0f0f0f0fu) | (sw_bytes1(z) & 0xf0f0f0f0u);
+  } else {  // two bytes a pair
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_perm(z[e], u[e], 0x0c0c0501u);
+    *(u32x2*)(row + col * 2) = u32x2{lo_pair(w[0], w[1]), lo_pair(w[2], w[3])};
+  }
 }
 
 // 16 bytes a lane from global memory straight to LDS: lane l's to lds + 16 l.  No

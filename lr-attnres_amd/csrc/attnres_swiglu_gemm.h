@@ -94,20 +94,29 @@ template <int ROW_BYTES, int BLOCK>
 __device__ __forceinline__ void sw_take_blocks(const char* lds, int lane, char* plane, int block0, int blocks, int64_t n,
                                                int m0, int M) {
   constexpr int kPer = BLOCK / 16, kBlocks = ROW_BYTES / BLOCK;  // chunks of a block's row, blocks
-  constexpr int kIters = 32 * kPer * kBlocks / kWave;
+  constexpr int kRows = kWave / kPer, kIters = 32 / kRows;       // rows that a wave stores at a time
+  const int r = lane / kPer, c = lane % kPer;
+  const char* from = lds + r * sw_pitch(ROW_BYTES) + c * 16;
+  u32x4 x[kBlocks][kIters];
 #pragma unroll
-  for (int i = 0; i < kIters; ++i) {
-    const int q = i * kWave + lane, b = q / (32 * kPer), m = q / kPer % 32, c = q % kPer;
-    const u32x4 x = *(const u32x4*)(lds + m * sw_pitch(ROW_BYTES) + b * BLOCK + c * 16);
-    if (block0 + b < blocks && m0 + m < M) *(u32x4*)(plane + ((int64_t)(block0 + b) * n + m0 + m) * BLOCK + c * 16) = x;
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) x[b][i] = *(const u32x4*)(from + i * kRows * sw_pitch(ROW_BYTES) + b * BLOCK);
+  char* to = plane + ((int64_t)block0 * n + m0 + r) * BLOCK + c * 16;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    if (block0 + b < blocks) {
+      if (m0 + 32 <= M) {
+#pragma unroll
+        for (int i = 0; i < kIters; ++i) *(u32x4*)(to + i * kRows * BLOCK) = x[b][i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kIters; ++i)
+          if (m0 + r + i * kRows < M) *(u32x4*)(to + i * kRows * BLOCK) = x[b][i];
+      }
+    }
+    to += n * BLOCK;
   }
-}
-
-// fp32 bits rounded to 16 + L of them, nearest; a NaN stays one
-template <int L>
-__device__ __forceinline__ uint32_t sw_round_bits(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return x != x ? b | 0x400000u : b + (1u << (15 - L));
 }
 
 // u and z of a wave's 32 rows to the planes that the backward reads
@@ -149,17 +158,7 @@ __device__ __forceinline__ void sw_save(const SwGemmParams& p, char* lds, int la
         const int col = j * 32 + 8 * i + 4 * q;
         *(u32x2*)(lds + m * sw_pitch(kRow) + col * 2) = u32x2{hi_pair(u[0], u[1]), hi_pair(u[2], u[3])};
         *(u32x2*)(zu + m * sw_pitch(kRow) + col * 2) = u32x2{hi_pair(z[0], z[1]), hi_pair(z[2], z[3])};
-        if constexpr (L == 4) {  // a byte a pair: u's bits low
-          uint32_t w = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w |= ((u[e] >> 12 & 15u) | (z[e] >> 8 & 0xf0u)) << (8 * e);
-          *(uint32_t*)(lo + m * sw_pitch(kLowRow) + col) = w;
-        } else {  // two bytes a pair
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = (u[e] >> 8 & 0xffu) | (z[e] & 0xff00u);
-          *(u32x2*)(lo + m * sw_pitch(kLowRow) + col * 2) = u32x2{w[0] | w[1] << 16, w[2] | w[3] << 16};
-        }
+        sw_store_low<L>(lo + m * sw_pitch(kLowRow), col, u, z);
       }
     __builtin_amdgcn_wave_barrier();
     sw_take_blocks<kRow, kSwStepBytes>(lds, lane, at.u, block0, blocks, p.n_tok, m0, p.M);
@@ -202,13 +201,16 @@ __device__ __forceinline__ void sw_finish(const SwGemmParams& p, char* lds, int 
   } else {
     sw_put<DT, COLS / 32>(lds, lane, v);
     __builtin_amdgcn_wave_barrier();
-    // dw: rows of the padded halves
-    const int half = FORM == kDw && m0 >= p.Fp, f0 = m0 - half * p.Fp, r0 = half * p.F + f0;
-    const int rows = FORM == kDw ? (half < 2 && f0 < p.Fp ? p.F - f0 : 0) : p.M - m0;
-    const bool whole = rows >= 32 && n0 + COLS <= p.n_out && p.out_vec;
-    char* out = (char*)p.out + ((int64_t)r0 * p.out_stride + n0) * kSize;
+    // dw: rows of the padded halves, these (perhaps) in both
+    const int half = FORM == kDw && m0 >= p.Fp, skip = half * (p.Fp - p.F);
+    const int end = FORM == kDw ? half * p.Fp + p.F : p.M;  // of the rows that begin here
+    const bool whole = m0 + 32 <= end && n0 + COLS <= p.n_out && p.out_vec;
+    char* out = (char*)p.out + ((int64_t)(m0 - skip) * p.out_stride + n0) * kSize;
     sw_take_rows<COLS * kSize, kSize>(lds, lane, whole, n0, p.n_out, p.out_vec, [&](int m) -> char* {
-      return whole || m < rows ? out + (int64_t)m * p.out_stride * kSize : nullptr;
+      char* row = out + (int64_t)m * p.out_stride * kSize;
+      if (whole || m0 + m < end) return row;
+      if (FORM == kDw && !half && m0 + m >= p.Fp && m0 + m < p.Fp + p.F) return row - (int64_t)(p.Fp - p.F) * p.out_stride * kSize;
+      return nullptr;
     });
   }
   __builtin_amdgcn_wave_barrier();
