@@ -42,7 +42,7 @@ __device__ __forceinline__ int64_t rot_position(const QkvRotaryParams& p, int64_
 
 // DT: values, TT: tables.  A lane holds CHUNKS vectors of a head, LANES * VEC apart.
 template <class DT, class TT, int VEC, int LANES, int CHUNKS, bool BWD>
-__global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryParams p, int groups) {
+__global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryParams p, int groups, int iters) {
   using S = typename DT::S;
   using TS = typename TT::S;
   constexpr int kHeads = kWave / LANES;  // heads of a group
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryP
   const int n_rot = p.q_heads + p.kv_heads, n_all = BWD ? n_rot + p.kv_heads : n_rot;
   const int Dh = p.head_dim;
   const int col = (lane & (LANES - 1)) * VEC;
-  const int head0 = part * (kIters * kHeads) + lane / LANES;
+  const int head0 = part * (iters * kHeads) + lane / LANES;
   bool in[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) in[c] = col + c * LANES * VEC < Dh;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryP
   Raw<DT, VEC> x[kIters][CHUNKS], g[kIters][CHUNKS];
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
-    const int h = head0 + i * kHeads;
+    const int h = i < iters ? head0 + i * kHeads : n_all;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int at = col + c * LANES * VEC;
@@ -98,6 +98,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryP
   }
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
+    if (i >= iters) break;
     const int h = head0 + i * kHeads;
     float v[CHUNKS][VEC];
     float ss = 0.f;
@@ -233,11 +234,12 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_general(QkvRotary
 template <class DT, class TT, bool BWD, int VEC, int LANES, int CHUNKS>
 hipError_t run(const QkvRotaryParams& p, hipStream_t st) {
   const int n_all = p.q_heads + p.kv_heads * (BWD ? 2 : 1);
-  const int per_wave = kIters * (kWave / LANES);
-  const int groups = (n_all + per_wave - 1) / per_wave;
+  // head groups shared evenly by as few waves as hold them (36 heads of 64: 3 + 2 groups, not 4 + 1)
+  const int all = (n_all + kWave / LANES - 1) / (kWave / LANES);
+  const int groups = (all + kIters - 1) / kIters, iters = (all + groups - 1) / groups;
   const int64_t grid = (p.n_tok * groups + kRotWaves - 1) / kRotWaves;
   if (grid > INT32_MAX) return hipErrorInvalidValue;
-  qkv_rotary_kernel<DT, TT, VEC, LANES, CHUNKS, BWD><<<dim3((unsigned)grid), dim3(kRotWaves * kWave), 0, st>>>(p, groups);
+  qkv_rotary_kernel<DT, TT, VEC, LANES, CHUNKS, BWD><<<dim3((unsigned)grid), dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters);
   return hipGetLastError();
 }
 

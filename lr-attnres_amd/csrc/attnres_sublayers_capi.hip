@@ -260,25 +260,28 @@ size_t packed_w(const attnres_swiglu_desc* d, const SwLayout& l, bool dx) {
   return (dx ? l.w_ok_dx : l.w_ok) ? 0 : up256((size_t)2 * (dx ? l.Fp : d->hidden) * l.Dp * l.es);
 }
 
-// an operand as a product reads it: where it is, or copied to `to`
-hipError_t sw_operand(const attnres_swiglu_desc* d, const SwLayout& l, int form, bool weight, char* to, hipStream_t st,
-                      const void** at, int64_t* stride) {
-  const bool ok = !weight ? l.x_ok : form == kDx ? l.w_ok_dx : l.w_ok;
-  *at = weight ? d->weight : d->x;
-  *stride = weight ? d->weight_row_stride : d->x_row_stride;
-  if (ok) return hipSuccess;
+// the operands as the products read them: where they are, or (one launch) copied
+struct SwOperands {
+  const void *x, *w;
+  int64_t x_stride, w_stride;
+};
+hipError_t sw_operands(const attnres_swiglu_desc* d, const SwLayout& l, bool dx, char* x_to, char* w_to, hipStream_t st,
+                       SwOperands* o) {
+  *o = SwOperands{d->x, d->weight, d->x_row_stride, d->weight_row_stride};
   SwPackParams k{};
-  k.from = *at;
-  k.from_stride = *stride;
-  k.to = to;
-  k.blocks = weight ? 2 : 1;
-  k.rows = weight ? d->hidden : d->n_tok;
-  k.to_rows = weight && form == kDx ? l.Fp : k.rows;
-  k.to_stride = l.Dp;
   k.cols = d->dim;
-  *at = to;
-  *stride = l.Dp;
-  return launch_swiglu_pack(d->dtype, k, st);
+  k.to_stride = l.Dp;
+  if (x_to) {
+    k.part[k.parts++] = SwPack{d->x, x_to, d->n_tok, d->n_tok, d->x_row_stride, 1};
+    o->x = x_to;
+    o->x_stride = l.Dp;
+  }
+  if (w_to) {
+    k.part[k.parts++] = SwPack{d->weight, w_to, d->hidden, dx ? l.Fp : d->hidden, d->weight_row_stride, 2};
+    o->w = w_to;
+    o->w_stride = l.Dp;
+  }
+  return k.parts ? launch_swiglu_pack(d->dtype, k, st) : hipSuccess;
 }
 
 void set_shape(const SwShape& s, SwGemmParams* g) {
@@ -327,8 +330,12 @@ extern "C" int attnres_swiglu_forward(const attnres_swiglu_desc* d, void* h, voi
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
   SwGemmParams g{};
-  hipError_t err = sw_operand(d, l, kFwd, false, ws, st, &g.q, &g.q_stride);
-  if (err == hipSuccess) err = sw_operand(d, l, kFwd, true, ws + px, st, &g.p, &g.p_stride);
+  SwOperands o;
+  hipError_t err = sw_operands(d, l, false, px ? ws : nullptr, pw ? ws + px : nullptr, st, &o);
+  g.q = o.x;
+  g.q_stride = o.x_stride;
+  g.p = o.w;
+  g.p_stride = o.w_stride;
   g.M = (int)d->n_tok;
   g.N = g.F = g.n_out = d->hidden;
   g.Fp = l.Fp;
@@ -378,10 +385,13 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
   e.F = d->hidden;
   e.Fp = l.Fp;
   e.vec = aligned(grad_h, 16) && grad_row_stride % l.per == 0;
-  err = launch_swiglu_grad(d->dtype, e, st);
+  SwOperands o;
+  err = sw_operands(d, l, true, px ? ws + pd : nullptr, pw ? ws + pd + px : nullptr, st, &o);
+  if (err == hipSuccess) err = launch_swiglu_grad(d->dtype, e, st);
   if (dx && err == hipSuccess) {
     SwGemmParams g{};
-    err = sw_operand(d, l, kDx, true, ws + pd + px, st, &g.p, &g.p_stride);
+    g.p = o.w;
+    g.p_stride = o.w_stride;
     g.q = ws;
     g.n_tok = d->n_tok;
     g.M = (int)d->n_tok;
@@ -395,11 +405,12 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
     g.n_out = d->dim;
     g.out_vec = d->dim % l.per == 0 && aligned(dx, 16);
     g.partials = (float*)(ws + pd + px + pw);
-    if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kDx, sx.tile, g, st);
+    err = launch_swiglu_gemm(d->dtype, kDx, sx.tile, g, st);
   }
   if (dweight && err == hipSuccess) {
     SwGemmParams g{};
-    err = sw_operand(d, l, kDw, false, ws + pd, st, &g.p, &g.p_stride);
+    g.p = o.x;
+    g.p_stride = o.x_stride;
     g.q = ws;
     g.n_tok = d->n_tok;
     g.M = 2 * l.Fp;
@@ -413,7 +424,7 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
     g.n_out = d->dim;
     g.out_vec = d->dim % l.per == 0 && aligned(dweight, 16);
     g.partials = (float*)(ws + pd + px + pw);
-    if (err == hipSuccess) err = launch_swiglu_gemm(d->dtype, kDw, sw.tile, g, st);
+    err = launch_swiglu_gemm(d->dtype, kDw, sw.tile, g, st);
   }
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu backward launch failed: %s", hipGetErrorString(err));
   return ATTNRES_OK;

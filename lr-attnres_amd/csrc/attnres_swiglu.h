@@ -77,13 +77,17 @@ struct SwGradParams {
 };
 hipError_t launch_swiglu_grad(int dtype, const SwGradParams& p, hipStream_t st);
 
-// blocks of `rows` rows of cols values to blocks of `to_rows` rows of to_stride, zeros
-// behind the columns and the rows
-struct SwPackParams {
+// Copies of operands: blocks of `rows` rows of cols values to blocks of `to_rows` rows of
+// to_stride (whole chunks), zeros behind the columns and the rows.  One or two at once.
+struct SwPack {
   const void* from;
   void* to;
-  int64_t rows, to_rows, from_stride, to_stride;
-  int32_t blocks, cols;
+  int64_t rows, to_rows, from_stride;
+  int32_t blocks;
+};
+struct SwPackParams {
+  SwPack part[2];
+  int32_t parts, cols, to_stride;
 };
 hipError_t launch_swiglu_pack(int dtype, const SwPackParams& p, hipStream_t st);
 hipError_t launch_swiglu_clear(int dtype, void* to, int64_t values, hipStream_t st);

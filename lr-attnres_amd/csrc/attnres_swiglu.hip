@@ -83,18 +83,33 @@ __global__ __launch_bounds__(kThreads) void swiglu_grad_kernel(SwGradParams p) {
   store_vec<DT, V>((S*)p.d + (int64_t)p.Fp * p.n + at, d);
 }
 
-// Small against the products that follow (a value copied once, multiplied by a
-// whole row); single values, since a row may start anywhere.
+// Small against the products that follow (a value copied once, multiplied by a whole
+// row).  A thread writes a chunk of 16 bytes; it reads single values, since a row may
+// start anywhere.
 template <class DT>
-__global__ __launch_bounds__(kThreads) void swiglu_pack_kernel(SwPackParams p) {
+__global__ __launch_bounds__(kThreads) void swiglu_pack_kernel(SwPackParams p, int64_t first) {
   using S = typename DT::S;
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t r = at / p.to_stride;
-  const int c = (int)(at - r * p.to_stride);
-  if (r >= p.to_rows * p.blocks) return;
-  const int64_t block = r / p.to_rows, row = r - block * p.to_rows;
-  const bool in = c < p.cols && row < p.rows;
-  ((S*)p.to)[at] = in ? ((const S*)p.from)[(block * p.rows + row) * p.from_stride + c] : (S)0;
+  constexpr int V = 16 / (int)sizeof(S);
+  int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;  // chunk
+  const bool second = at >= first;
+  const SwPack& k = p.part[second];
+  if (second) at -= first;
+  const int chunks = p.to_stride / V;
+  const int64_t r = at / chunks;
+  const int c = (int)(at - r * chunks) * V;
+  if (r >= k.to_rows * k.blocks || (second && p.parts < 2)) return;
+  const int64_t block = r / k.to_rows, row = r - block * k.to_rows;
+  const S* from = (const S*)k.from + (block * k.rows + row) * k.from_stride + c;
+  u32x4 v = {0, 0, 0, 0};
+  if (row < k.rows) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (c + e >= p.cols) break;
+      if constexpr (V == 8) v[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
+      else v[e] = __float_as_uint(from[e]);
+    }
+  }
+  *(u32x4*)((S*)k.to + r * p.to_stride + c) = v;
 }
 
 template <class DT>
@@ -119,9 +134,11 @@ hipError_t run_grad(const SwGradParams& p, hipStream_t st) {
 }
 template <class DT>
 hipError_t run_pack(const SwPackParams& p, hipStream_t st) {
+  int64_t n[2] = {0, 0};
+  for (int i = 0; i < p.parts; ++i) n[i] = p.part[i].to_rows * p.part[i].blocks * (p.to_stride / (16 / (int)sizeof(typename DT::S)));
   dim3 grid;
-  if (!grid_of(p.to_rows * p.blocks * p.to_stride, &grid)) return hipErrorInvalidValue;
-  swiglu_pack_kernel<DT><<<grid, dim3(kThreads), 0, st>>>(p);
+  if (!grid_of(n[0] + n[1], &grid)) return hipErrorInvalidValue;
+  swiglu_pack_kernel<DT><<<grid, dim3(kThreads), 0, st>>>(p, n[0]);
   return hipGetLastError();
 }
 template <class DT>
