@@ -17,7 +17,7 @@ extern "C" {
 
 /*
  * The heads of one projection [batch, tokens, (q_heads + 2 kv_heads) head_dim]:
- * queries, keys, values (model.py:478-506).  With qk_norm each query and key head
+ * queries, keys, values (model.py:430-569).  With qk_norm each query and key head
  * is rms-normed (model.py:28-31); then each is rotated, interleaved pairs, by row
  * p of sin and cos (model.py:291-313): out[2i] = cos x[2i] - sin x[2i+1], out[2i+1]
  * = sin x[2i] + cos x[2i+1].  fp32 throughout, one rounding to the dtype.  Token

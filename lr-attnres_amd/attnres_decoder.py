@@ -32,7 +32,13 @@ adds both to the partial block and, at a block end, forms the block source in
 one pass (``fuse_block_accumulation``; bit-identical too); a sublayer that does
 not end a block also merges the grown block into the next site's read in that
 pass (``lrid_block_accumulate_read``, ``fuse_accumulate_read``; bit-identical,
-gradients included).  Module and parameter names match the reference's, so a
+gradients included).  ``fuse_qkv_rotary`` and ``fuse_swiglu`` (off unless
+asked for) run the sublayers' own work around their library products on HIP
+kernels too: the heads of the fused query / key / value projection in one pass
+(``qkv_norm_rotary``: qk-norm and rotation, one rounding where the eager chain
+rounds six times) and the MLP up to its output projection as one product with
+the activation behind it (``swiglu_projection``); results differ from the
+eager sublayers by those roundings.  Module and parameter names match the reference's, so a
 reference state dict for this configuration loads with ``load_state_dict``.
 
 The read functions are looked up on ``ops`` (default: the HIP-backed
@@ -109,6 +115,8 @@ class DecoderConfig:
     fold_block_summary: bool = True
     fuse_block_accumulation: bool = True
     fuse_accumulate_read: bool = True
+    fuse_qkv_rotary: bool = False
+    fuse_swiglu: bool = False
 
     def __post_init__(self):
         if self.norm_pos not in {"before", "after", "both"}:
@@ -246,6 +254,8 @@ class MultiHeadAttention(nn.Module):
         self.head_dim = config.n_embd // config.n_head
         self.qk_norm = config.qk_norm
         self.keyed = config.use_attnres
+        self.fused_heads = config.fuse_qkv_rotary
+        self.ops = ops
         self.rope = RotaryEmbedding(config)
         self.c_attn = nn.Linear(config.n_embd, 3 * config.n_embd, bias=False)
         if self.keyed:
@@ -255,15 +265,19 @@ class MultiHeadAttention(nn.Module):
 
     def forward(self, x: Tensor):
         B, T, C = x.shape
-        q, k, v = self.c_attn(x).split(C, dim=2)
-        q = q.view(B, T, self.n_head, self.head_dim).transpose(1, 2)
-        k = k.view(B, T, self.n_head, self.head_dim).transpose(1, 2)
-        v = v.view(B, T, self.n_head, self.head_dim).transpose(1, 2)
-        if self.qk_norm:
-            q = norm(q)
-            k = norm(k)
-        q = self.rope.rotate(q)
-        k = self.rope.rotate(k)
+        if self.fused_heads:
+            q, k, v = self.ops.qkv_norm_rotary(self.c_attn(x), self.n_head, self.rope.sin, self.rope.cos,
+                                               qk_norm=self.qk_norm)
+        else:
+            q, k, v = self.c_attn(x).split(C, dim=2)
+            q = q.view(B, T, self.n_head, self.head_dim).transpose(1, 2)
+            k = k.view(B, T, self.n_head, self.head_dim).transpose(1, 2)
+            v = v.view(B, T, self.n_head, self.head_dim).transpose(1, 2)
+            if self.qk_norm:
+                q = norm(q)
+                k = norm(k)
+            q = self.rope.rotate(q)
+            k = self.rope.rotate(k)
         y = _attend(q, k, v).transpose(1, 2).contiguous().view(B, T, C)
         if self.keyed:
             return self.c_proj(y)
@@ -277,6 +291,8 @@ class MLP(nn.Module):
         super().__init__()
         hidden = config.hidden_dim
         self.keyed = config.use_attnres
+        self.fused_gate = config.fuse_swiglu
+        self.ops = ops
         self.fc1 = nn.Linear(config.n_embd, 2 * hidden, bias=False)
         if self.keyed:
             self.fc2 = KeyedOutputProjection(config, hidden, config.n_embd, ops)
@@ -284,8 +300,11 @@ class MLP(nn.Module):
             self.fc2 = nn.Linear(hidden, config.n_embd, bias=False)
 
     def forward(self, x: Tensor):
-        up, gate = self.fc1(x).chunk(2, dim=-1)
-        h = F.silu(gate) * up
+        if self.fused_gate:
+            h = self.ops.swiglu_projection(x, self.fc1.weight)
+        else:
+            up, gate = self.fc1(x).chunk(2, dim=-1)
+            h = F.silu(gate) * up
         if self.keyed:
             return self.fc2(h)
         return self.fc2(h), None
@@ -334,7 +353,8 @@ class Decoder(nn.Module):
     def __init__(self, config: DecoderConfig, ops=None):
         super().__init__()
         self.config = config
-        self.ops = ops if ops is not None else (_default_ops() if config.use_attnres else None)
+        needs_ops = config.use_attnres or config.fuse_qkv_rotary or config.fuse_swiglu
+        self.ops = ops if ops is not None else (_default_ops() if needs_ops else None)
         self.block_ends = block_ends(config.n_layer, config.attnres_num_blocks) if config.use_attnres else None
         modules = dict(
             wte=nn.Embedding(config.vocab_size, config.n_embd),

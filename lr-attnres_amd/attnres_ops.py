@@ -1912,7 +1912,7 @@ def qkv_norm_rotary(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, posit
     """Attention's heads from a fused query / key / value projection, in one HIP pass each way.
 
     Not in the reference's op module: the reference's attention does this as a split, three transposes, ``norm`` of the
-    query and key heads and ``rope.rotate`` of both (model.py:478-506, 28-31, 291-313), about a dozen passes over them.
+    query and key heads and ``rope.rotate`` of both (model.py:430-569, 28-31, 291-313), about a dozen passes over them.
 
     ``qkv`` [B, T, (num_heads + 2 num_kv_heads) Dh]: query, key and value heads (``num_kv_heads``: as many as query heads
     unless given).  Query and key heads are rms-normed over Dh (``qk_norm``; torch's default eps) and rotated by interleaved

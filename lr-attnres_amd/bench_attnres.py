@@ -78,6 +78,10 @@ def parse_args(argv=None):
     p.add_argument("--fuse_block_accumulation", type=_bool, default=True)
     p.add_argument("--fuse_accumulate_read", type=_bool, default=True,
                    help="sublayers that do not end a block also form the next read")
+    p.add_argument("--fuse_qkv_rotary", type=_bool, default=False,
+                   help="attention's heads (qk-norm, rotation) from the fused projection in one pass, in both cases")
+    p.add_argument("--fuse_swiglu", type=_bool, default=False,
+                   help="the MLP's projections with their activation and product in one kernel, in both cases")
     p.add_argument("--dtype", choices=("fp32", "bf16", "fp16"), default="bf16")
     p.add_argument("--phase", choices=("forward", "train"), default="train")
     p.add_argument("--loss", choices=("hidden_mse", "lm"), default="lm")
@@ -115,7 +119,8 @@ def make_config(args, use_attnres, rank):
         attnres_fuse_read_norm=args.attnres_fuse_read_norm, lrid_rank=rank or 64,
         lrid_projection_rank=args.lrid_projection_rank if use_attnres else None, lrid_num_heads=1,
         lrid_use_logit_scale=True, fold_block_summary=args.fold_block_summary,
-        fuse_block_accumulation=args.fuse_block_accumulation, fuse_accumulate_read=args.fuse_accumulate_read)
+        fuse_block_accumulation=args.fuse_block_accumulation, fuse_accumulate_read=args.fuse_accumulate_read,
+        fuse_qkv_rotary=args.fuse_qkv_rotary, fuse_swiglu=args.fuse_swiglu)
 
 
 def training_loss(args, model, idx, targets):

@@ -1,5 +1,5 @@
 // Heads of a fused query / key / value projection: per-head rms-norm and rotary
-// positions in one pass, and its backward (MultiHeadAttention, model.py:478-506,
+// positions in one pass, and its backward (MultiHeadAttention, model.py:430-569,
 // with norm :28-31 and the rotation :291-313).
 //   n = x / sqrt(<x, x> / Dh + eps)        y = R(p) n   (pairs (2i, 2i+1) turned)
 //   g = R(p)^T dy                          dx = (g - n <g, n> / Dh) / rms

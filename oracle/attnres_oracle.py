@@ -519,6 +519,38 @@ def lrid_block_accumulate_ref(projected: Tensor, partial_value, partial_key, out
     return value, k
 
 
+def qkv_norm_rotary_ref(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, positions=None, num_kv_heads=None,
+                        qk_norm: bool = True):
+    """Attention's heads as the reference forms them (``model.py:430-569``): the
+    projection split into heads, query and key heads rms-normed (``:28-31``) and
+    rotated by interleaved pairs (``:291-313``), every op in the tensors' dtype.
+    ``positions`` and grouped key / value heads are not the reference's."""
+    B, T, C = qkv.shape
+    H, K = num_heads, num_heads if num_kv_heads is None else num_kv_heads
+    Dh = C // (H + 2 * K)
+    q, k, v = (t.reshape(B, T, -1, Dh).transpose(1, 2) for t in qkv.split([H * Dh, K * Dh, K * Dh], dim=2))
+    sin, cos = sin.reshape(-1, Dh // 2), cos.reshape(-1, Dh // 2)
+    if isinstance(positions, Tensor):
+        sin, cos = (t[positions.expand(B, T)].unsqueeze(1) for t in (sin, cos))
+    else:
+        start = positions or 0
+        sin, cos = (t[start:start + T][None, None] for t in (sin, cos))
+
+    def rotate(x):
+        even, odd = x[..., 0::2], x[..., 1::2]
+        return torch.stack([cos * even - sin * odd, sin * even + cos * odd], dim=-1).flatten(-2)
+    if qk_norm:
+        q, k = norm(q), norm(k)
+    return rotate(q), rotate(k), v
+
+
+def swiglu_projection_ref(x: Tensor, weight: Tensor) -> Tensor:
+    """The gated MLP up to its output projection (``model.py:572-589``):
+    ``silu(gate) * up`` with ``[up, gate]`` one linear layer's output."""
+    up, gate = F.linear(x, weight.to(x.dtype)).chunk(2, dim=-1)
+    return F.silu(gate) * up
+
+
 def softmax_weights_ref(values_or_keys, query: Tensor, num_heads: int, logit_scale: float, key_norm: bool,
                         base: bool, source_counts=None, source_logit_biases=None) -> Tensor:
     """fp32 softmax weights [S,B,T,H] of a read (what the kernels save).
@@ -570,5 +602,7 @@ __all__ = [
     "attention_residual_phase1_ref",
     "attention_residual_phase2_ref",
     "lrid_attention_residual_phase2_ref",
+    "qkv_norm_rotary_ref",
+    "swiglu_projection_ref",
     "softmax_weights_ref",
 ]
