@@ -8,19 +8,21 @@
 //   kDx   P = W^T, Q = [du dz], k over both halves of the hidden dimension
 //   kDw   P = x^T, Q = [du dz]^T, k over tokens
 //
-// Tile.  Four waves, 2 x 2, each with a quarter of the BM x BN tile as 32 x 32 MFMA
-// tiles.  P is the MFMA's row operand, so that a lane holds for one m (lane % 32)
-// groups of 4 consecutive n.  k runs in steps of 64 bytes through the stages of
-// LDS, filled by loads that write LDS directly (16 bytes a lane; no registers), two or
-// three steps ahead; a wave reads the fragments of the next half step while the matrix
-// cores work on this one.  One barrier a step: behind it the next stage has landed
-// (each wave waited for its own loads) and nobody reads the oldest one any more.
+// Tile.  Four waves, 2 x 2, each with a quarter of the BM x BN tile as 16 x 16 MFMA
+// tiles.  P is the MFMA's row operand, so that a lane holds for one m (lane % 16)
+// groups of 4 consecutive n.  k runs in steps of 64 bytes, one MFMA deep in 16 bits,
+// through the stages of LDS, filled by loads that write LDS directly (16 bytes a
+// lane; no registers) several steps ahead; a wave reads the fragments of the next
+// step while the matrix cores work on this one.  One barrier a step: behind it the
+// next stage has landed (each wave waited for its own loads) and nobody reads this
+// step's any more, so that the loads issued next go there.
 //
 // LDS layouts (a stage holds R rows of 64 bytes, or 32 / 16 rows of R values):
 //   k contiguous: the 16-byte chunks of row r are swapped by f(r) = (r / 2 % 4) ^ (r /
 //     8 % 2): the 8 (or 16) rows that a read serves at once then lie in all banks
 //   k strided, 16-bit: 32-byte units of row k are swapped by s(k) = 2 (k % 4) ^ (k / 2 %
-//     2) for the transposing reads (4 rows x 32 bytes per 16 lanes)
+//     2) ^ (k / 8 % 2) for the transposing reads (4 rows x 32 bytes per 16 lanes, rows 8
+//     apart in neighbouring 16s)
 //   k strided, fp32: rows as they are; a fragment's values are read one by one
 // The direct loads write LDS in lane order, so the swaps are made in the addresses
 // that the lanes read from.
@@ -100,24 +102,24 @@ template <class DT> struct SwElem {  // 16-byte fragments and their MFMA
   static constexpr int kStep = kSwStepBytes / kSize;     // k of a step
 };
 
-typedef float sw_f16 __attribute__((ext_vector_type(16)));
 typedef float sw_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 sw_bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 sw_h8 __attribute__((ext_vector_type(8)));
 typedef short sw_s4 __attribute__((ext_vector_type(4)));
 
-// acc += P-fragment x Q-fragment: lane l holds 16 bytes of row l % 32, the lower
-// half of the lanes the first 16 bytes of k, the upper the next.  fp32: four
-// products of 2 k each, the same permutation of k on both sides.
+// acc += P-fragment x Q-fragment, 16 x 16 values and 64 bytes of k: lane l holds 16 bytes
+// of row l % 16, the l / 16-th of them.  fp32: four products of 4 k each, the same
+// permutation of k on both sides.  Of the sums, lane l holds column l % 16 (of Q),
+// rows 4 (l / 16) + 0..3 (of P).
 template <class DT>
-__device__ __forceinline__ void sw_mfma(const u32x4& a, const u32x4& b, sw_f16& c) {
+__device__ __forceinline__ void sw_mfma(const u32x4& a, const u32x4& b, sw_f4& c) {
   if constexpr (DT::kCode == 1) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sw_bf8, a), __builtin_bit_cast(sw_bf8, b), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sw_bf8, a), __builtin_bit_cast(sw_bf8, b), c, 0, 0, 0);
   } else if constexpr (DT::kCode == 2) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(sw_h8, a), __builtin_bit_cast(sw_h8, b), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sw_h8, a), __builtin_bit_cast(sw_h8, b), c, 0, 0, 0);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
   }
 }
 
@@ -195,10 +197,11 @@ struct SwOperand {
   static constexpr int kUnitMask = R / 16 - 1;            // strided 16-bit: 32-byte units of a row
   uint32_t off[kLoads];   // byte offsets of this thread's chunks from the step's base
   int kr[kLoads];         // and their k: chunk * kPer (contiguous) or row (strided)
-  uint32_t rd[4];         // byte addresses of this lane's fragments
+  static constexpr int kReads = T ? R / 32 : 1;
+  uint32_t rd[kReads];    // byte addresses of this lane's fragments: strided, one for each 16 rows of a wave
 
   __device__ static int f_row(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
-  __device__ static int s_row(int k) { return ((2 * (k & 3)) ^ ((k >> 1) & 1)) & kUnitMask; }
+  __device__ static int s_row(int k) { return ((2 * (k & 3)) ^ ((k >> 1) & 1) ^ ((k >> 3) & 1)) & kUnitMask; }
 
   // row / first k and chunk of load i of a thread
   __device__ __forceinline__ static void place(int i, int tid, int* row, int* chunk) {
@@ -214,39 +217,34 @@ struct SwOperand {
     }
   }
 
-  // where this lane's fragments begin: rd by half step (contiguous), by 32-row group (strided)
+  // where this lane's fragments begin
   __device__ __forceinline__ void place_reads(int row0, int lane, uint32_t base) {
     if constexpr (!T) {
-      const int r = row0 + (lane & 31);
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) rd[kk] = base + r * 64 + (((2 * kk + (lane >> 5)) ^ f_row(r)) * 16);
+      const int r = row0 + (lane & 15);
+      rd[0] = base + r * 64 + ((lane >> 4) ^ f_row(r)) * 16;
     } else if constexpr (E::kSize == 2) {
-      const int g = lane >> 4, i = lane & 15;
-      const int k = (g >> 1) * 8 + (i >> 2);
+      const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int unit = (row0 + 32 * j) / 16 + (g & 1);
-        rd[j] = base + k * (R * 2) + ((unit ^ s_row(k)) & kUnitMask) * 32 + (i & 3) * 8;
-      }
+      for (int j = 0; j < kReads; ++j) rd[j] = base + k * (R * 2) + ((row0 / 16 + j) ^ s_row(k)) * 32 + (i & 3) * 8;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) rd[j] = base + (4 * (lane >> 5)) * (R * 4) + (row0 + 32 * j + (lane & 31)) * 4;
+      for (int j = 0; j < kReads; ++j) rd[j] = base + 4 * (lane >> 4) * (R * 4) + (row0 + 16 * j + (lane & 15)) * 4;
     }
   }
 
-  // the fragment of 32-row group j, half step kk, of the stage at `stage`
-  __device__ __forceinline__ u32x4 read(const char* lds, uint32_t stage, int kk, int j) const {
+  // the fragment of the wave's j-th 16 rows, of the stage at `stage`
+  __device__ __forceinline__ u32x4 read(const char* lds, uint32_t stage, int j) const {
     if constexpr (!T) {
-      return *(const u32x4*)(lds + stage + rd[kk] + j * 2048);
+      return *(const u32x4*)(lds + stage + rd[0] + j * 1024);
     } else if constexpr (E::kSize == 2) {
       typedef __attribute__((address_space(3))) sw_s4 lds_s4;
-      const char* at = lds + stage + rd[j] + kk * 16 * (R * 2);
+      const char* at = lds + stage + rd[j];
       const sw_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
       const sw_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 4 * (R * 2)));
       const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
       return u32x4{a.x, a.y, b.x, b.y};
     } else {
-      const char* at = lds + stage + rd[j] + kk * 8 * (R * 4);
+      const char* at = lds + stage + rd[j];
       u32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = *(const uint32_t*)(at + e * (R * 4));

@@ -2,6 +2,8 @@
 // split products.  Included by attnres_swiglu_{bf16,f16,f32}.hip.
 #pragma once
 
+#include <type_traits>
+
 #include "attnres_swiglu.h"
 
 namespace attnres {
@@ -33,23 +35,25 @@ __device__ __forceinline__ void sw_tile(const SwGemmParams& p, int b, int n, int
   *tile = t;
 }
 
-// A wave's 32 x COLS values go to memory through its own LDS: lane l holds for row m =
-// l % 32 groups of four columns, 32 j + 8 i + 4 (l / 32) + 0..3, and takes back 16
-// bytes of a row, so that memory sees whole 64-byte pieces.  Rows of PITCH bytes (16
+// A wave's 32 x COLS values go to memory through its own LDS: lane l holds in v[j][4 i + e]
+// row sw_row(l, i), column 32 j + sw_col(l, i) + e, and takes back 16 bytes of a row, so
+// that memory sees whole 64-byte pieces.  Rows of PITCH bytes (16
 // more than they hold: the rows of a read then start in different banks).
 constexpr int sw_pitch(int row_bytes) { return row_bytes + 16; }
+__device__ __forceinline__ int sw_row(int lane, int i) { return (lane & 15) + 16 * (i >> 1); }
+__device__ __forceinline__ int sw_col(int lane, int i) { return 4 * (lane >> 4) + 16 * (i & 1); }
 
 template <class DT, int G>
 __device__ __forceinline__ void sw_put(char* lds, int lane, const float (&v)[G][16]) {
   constexpr int kSize = sizeof(typename DT::S);
-  char* at = lds + (lane & 31) * sw_pitch(G * 32 * kSize) + 4 * (lane >> 5) * kSize;
 #pragma unroll
   for (int j = 0; j < G; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float* x = &v[j][4 * i];
-      if constexpr (kSize == 2) *(u32x2*)(at + (j * 32 + 8 * i) * 2) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
-      else *(sw_f4*)(at + (j * 32 + 8 * i) * 4) = sw_f4{x[0], x[1], x[2], x[3]};
+      char* at = lds + sw_row(lane, i) * sw_pitch(G * 32 * kSize) + (j * 32 + sw_col(lane, i)) * kSize;
+      if constexpr (kSize == 2) *(u32x2*)at = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+      else *(sw_f4*)at = sw_f4{x[0], x[1], x[2], x[3]};
     }
 }
 
@@ -144,7 +148,6 @@ __device__ __forceinline__ void sw_save(const SwGemmParams& p, char* lds, int la
     constexpr int L = P::kLow, kLowRow = H * 32 * L / 4;  // bytes of the low bits of a row's pairs
     char* zu = lds + 32 * sw_pitch(kRow);
     char* lo = zu + 32 * sw_pitch(kRow);
-    const int m = lane & 31, q = lane >> 5;
 #pragma unroll
     for (int j = 0; j < H; ++j)
 #pragma unroll
@@ -155,7 +158,7 @@ __device__ __forceinline__ void sw_save(const SwGemmParams& p, char* lds, int la
           u[e] = sw_round_bits<L>(v[j][4 * i + e]);
           z[e] = sw_round_bits<L>(v[H + j][4 * i + e]);
         }
-        const int col = j * 32 + 8 * i + 4 * q;
+        const int m = sw_row(lane, i), col = j * 32 + sw_col(lane, i);
         *(u32x2*)(lds + m * sw_pitch(kRow) + col * 2) = u32x2{hi_pair(u[0], u[1]), hi_pair(u[2], u[3])};
         *(u32x2*)(zu + m * sw_pitch(kRow) + col * 2) = u32x2{hi_pair(z[0], z[1]), hi_pair(z[2], z[3])};
         sw_store_low<L>(lo + m * sw_pitch(kLowRow), col, u, z);
@@ -221,11 +224,10 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
   using E = SwElem<DT>;
   using OpP = SwOperand<DT, BN, FORM != kFwd>;
   using OpQ = SwOperand<DT, BM, FORM == kDw>;
-  constexpr int NP = BN / 64, NQ = BM / 64;  // 32 x 32 tiles of a wave
+  constexpr int NP = BN / 32, NQ = BM / 32;  // 16 x 16 tiles of a wave
   constexpr int kStage = OpP::kBytes + OpQ::kBytes;
   constexpr int kStages = sw_stages(BM, BN), kAhead = kStages - 1;  // steps loaded ahead
   constexpr int kLoads = OpP::kLoads + OpQ::kLoads;
-  constexpr int kFirst = kLoads / 2;  // of a step's loads, issued in the first half step
   constexpr int kCols = FORM == kFwd ? BN / 2 : BN;  // output columns of a tile
   constexpr int es = E::kSize;
   __shared__ __align__(1024) char lds[kStages * kStage];
@@ -315,33 +317,41 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
     next_step();
   };
 
-  sw_f16 acc[NP][NQ];
+  sw_f4 acc[NP][NQ];
 #pragma unroll
   for (int a = 0; a < NP; ++a)
 #pragma unroll
-    for (int b = 0; b < NQ; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+    for (int b = 0; b < NQ; ++b) acc[a][b] = sw_f4{0.f, 0.f, 0.f, 0.f};
 
-  u32x4 fp[2][NP], fq[2][NQ];
-  auto read_one = [&](int buf, uint32_t stage, int kk, int j) {
-    if (j < NP) fp[buf][j % NP] = op.read(lds, stage, kk, j % NP);
-    else fq[buf][(j - NP) % NQ] = oq.read(lds, stage, kk, (j - NP) % NQ);
-  };
-  // The products of one half step, with what the next ones need issued evenly between
-  // them: the fragments' reads, then loads l0.. l1 of a step.
-  auto half_step = [&](int buf, uint32_t stage, int kk, int l0, int l1) {
-    constexpr int kTiles = NP * NQ, kReads = NP + NQ;
+  // A step's products in two halves, rows of P by rows of Q: fragments are read into the
+  // registers of those that are used up, half a step and more before they are needed.
+  //   half 0: rows 0.. H - 1 of P by all of Q, while the other rows of P are read (this
+  //           step's) and a later step's loads are issued
+  //   half 1: rows H.. by all of Q, column by column; behind each the next step's fragment
+  //           of Q takes its place, and early on the next step's first rows of P
+  constexpr int H = NP / 2, kHalf = H * NQ;
+  u32x4 fp[NP], fq[NQ];
+  auto half0 = [&](uint32_t stage, auto loads) {
+    constexpr int kOps = H + (decltype(loads)::value ? kLoads : 0);
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      sw_mfma<DT>(fp[buf][t / NQ], fq[buf][t % NQ], acc[t / NQ][t % NQ]);
-      const int ops = kReads + l1 - l0;
+    for (int t = 0; t < kHalf; ++t) {
+      sw_mfma<DT>(fp[t % H], fq[t / H], acc[t % H][t / H]);
 #pragma unroll
-      for (int e = 0; e < kReads + kLoads; ++e) {
-        if (e >= ops || e * kTiles / ops != t) continue;
-        if (e < kReads) read_one(buf ^ 1, stage, kk, e);
-        else load_piece(l0 + e - kReads);
+      for (int i = 0; i < (kOps + kHalf - 1) / kHalf; ++i) {
+        const int e = (t * kOps + kHalf - 1) / kHalf + i;  // op e goes behind product e kHalf / kOps
+        if (e >= ((t + 1) * kOps + kHalf - 1) / kHalf) continue;
+        if (e < H) fp[H + e % H] = op.read(lds, stage, H + e % H);
+        else load_piece(e - H);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto half1 = [&](uint32_t next) {
+#pragma unroll
+    for (int t = 0; t < kHalf; ++t) {
+      sw_mfma<DT>(fp[H + t % H], fq[t / H], acc[H + t % H][t / H]);
+      if (t < H) fp[t] = op.read(lds, next, t);
+      if (t % H == H - 1) fq[t / H] = oq.read(lds, next, t / H);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -357,48 +367,59 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
     if (s < nk) load(s);
   wait(nk - 1);
 #pragma unroll
-  for (int j = 0; j < NP + NQ; ++j) read_one(0, 0, 0, j);
+  for (int j = 0; j < H; ++j) fp[j] = op.read(lds, 0, j);
+#pragma unroll
+  for (int j = 0; j < NQ; ++j) fq[j] = oq.read(lds, 0, j);
+  // (no instruction: between the two loops the largest tile's sums stand in the
+  // accumulation registers, and so the compiler moves none of them around in either)
+  auto pin = [&]() {
+    if constexpr (NP * NQ == 64) {
+#pragma unroll
+      for (int a = 0; a < NP; ++a)
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) asm volatile("" : "+a"(acc[a][b]));
+    }
+  };
   const int whole = (int)min((int64_t)nk, (int64_t)p.K / E::kStep - first);  // steps in which k does not end
   int s = 0;
   uint32_t stage = 0;
   for (; s + kAhead < whole; ++s) {
-    half_step(0, stage, 1, 0, kFirst);
-    stage = behind(stage);
-    sw_wait_barrier<(kAhead - 2) * kLoads + kFirst>();
-    half_step(1, stage, 0, kFirst, kLoads);
+    half0(stage, std::true_type());
     next_step();
+    stage = behind(stage);
+    sw_wait_barrier<(kAhead - 1) * kLoads>();
+    half1(stage);
   }
+  pin();
   for (; s < nk; ++s) {
     if (s + kAhead < nk) load(s + kAhead);
-    half_step(0, stage, 1, 0, 0);
+    half0(stage, std::false_type());
     stage = behind(stage);
     wait(nk - 2 - s);
-    half_step(1, stage, 0, 0, 0);  // (behind the last step: read, not used)
+    half1(stage);  // (behind the last step: fragments read, not used)
   }
 
   if constexpr (SPLIT) {
     float* to = p.partials + ((int64_t)split * p.tiles_m * p.tiles_n + tile) * (BM * BN) + wave * (BM * BN / 4) + lane * 4;
 #pragma unroll
-    for (int b = 0; b < NQ; ++b)
+    for (int b = 0; b < NQ / 2; ++b)
 #pragma unroll
-      for (int a = 0; a < NP; ++a)
+      for (int a = 0; a < NP / 2; ++a)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(sw_f4*)(to + ((b * NP + a) * 4 + i) * 256) =
-              sw_f4{acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
+        for (int i = 0; i < 4; ++i) *(sw_f4*)(to + ((b * (NP / 2) + a) * 4 + i) * 256) = acc[2 * a + (i & 1)][2 * b + (i >> 1)];
   } else {
     sw_wait_barrier<0>();  // the stages are free
-    constexpr int kMine = sw_finish_lds<DT, FORM, NP * 32>();
+    constexpr int kMine = sw_finish_lds<DT, FORM, NP * 16>();
     static_assert(4 * kMine <= kStages * kStage, "LDS");
     char* mine = lds + wave * kMine;
 #pragma unroll
-    for (int b = 0; b < NQ; ++b) {
-      float v[NP][16];
+    for (int b = 0; b < NQ / 2; ++b) {
+      float v[NP / 2][16];
 #pragma unroll
-      for (int a = 0; a < NP; ++a)
+      for (int a = 0; a < NP / 2; ++a)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[a][i] = acc[a][b][i];
-      sw_finish<DT, FORM, NP * 32>(p, mine, lane, m0 + wm * (BM / 2) + 32 * b, n0 + wn * (kCols / 2), v);
+        for (int i = 0; i < 16; ++i) v[a][i] = acc[2 * a + (i >> 2 & 1)][2 * b + (i >> 3)][i & 3];
+      sw_finish<DT, FORM, NP * 16>(p, mine, lane, m0 + wm * (BM / 2) + 32 * b, n0 + wn * (kCols / 2), v);
       __builtin_amdgcn_sched_barrier(0);  // (the next rows' registers not before these are stored)
     }
   }
@@ -408,7 +429,7 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
 // wave per 32 rows of a wave's columns.
 template <class DT, int FORM, int BM, int BN>
 __global__ __launch_bounds__(256) void swiglu_reduce_kernel(SwGemmParams p) {
-  constexpr int NP = BN / 64, NQ = BM / 64;
+  constexpr int NP = BN / 64, NQ = BM / 64;  // 32 x 32 values
   constexpr int kCols = FORM == kFwd ? BN / 2 : BN;
   // columns of a wave: all of them where u and z belong together, else one group of 32
   constexpr int G = FORM == kFwd ? NP : 1;
