@@ -195,11 +195,12 @@ struct SwCosts {
 constexpr SwCosts kCost16 = {{0.589, 0.481, 0.232, 0.205}, {1.0, 0.935, 1.0, 0.73}, {5.77, 3.5, 3.26, 2.55}, 3.95, 8.7e6};
 constexpr SwCosts kCost32 = {{3.905, 2.052, 1.062, 0.59}, {1.0, 0.981, 0.968, 0.906}, {3.69, 0.82, 0.59, 0.0}, 5.32, 7.8e6};
 
-SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {
+SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {  // (forward: of two k steps each)
   const SwCosts& k = dtype == ATTNRES_DTYPE_F32 ? kCost32 : kCost16;
   SwShape best{};
   double least = 1e300;
   for (int t = 0; t < kSwTiles; ++t) {
+    if (form == kFwd && kSwTileM[t] + kSwTileN[t] == 384) continue;
     const int cols = form == kFwd ? kSwTileN[t] / 2 : kSwTileN[t];
     const int64_t tm = (M + kSwTileM[t] - 1) / kSwTileM[t], tn = (N + cols - 1) / cols;
     const int together = sw_per_cu(kSwTileM[t], kSwTileN[t]);
@@ -209,7 +210,7 @@ SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {
       const int64_t wgs = tm * tn * splits;
       if (wgs > (1 << 24)) break;
       const int64_t rounds = (wgs + kCus - 1) / kCus;  // workgroups that one CU works on
-      auto group = [&](int g) { return per * k.step[t] * (g * k.together[t] > 1.0 ? g * k.together[t] : 1.0) + k.fixed[t]; };
+      auto group = [&](int g) { return (form == kFwd ? 2 : 1) * per * k.step[t] * (g * k.together[t] > 1.0 ? g * k.together[t] : 1.0) + k.fixed[t]; };
       double cost = (double)(rounds / together) * group(together);
       if (rounds % together) cost += group((int)(rounds % together));
       if (splits > 1) cost += k.launch + (double)wgs * kSwTileM[t] * kSwTileN[t] * 8 / k.bytes_us;
@@ -244,7 +245,7 @@ int check_swiglu(const attnres_swiglu_desc* d) {
 }
 
 SwShape fwd_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
-  return sw_shape(kFwd, d->dtype, d->n_tok, d->hidden, (d->dim + l.step - 1) / l.step);
+  return sw_shape(kFwd, d->dtype, d->n_tok, d->hidden, (d->dim + 2 * l.step - 1) / (2 * l.step));
 }
 SwShape dx_shape(const attnres_swiglu_desc* d, const SwLayout& l) {
   return sw_shape(kDx, d->dtype, d->n_tok, d->dim, 2 * l.Fp / l.step);

@@ -18,14 +18,21 @@
 // step's any more, so that the loads issued next go there.
 //
 // LDS layouts (a stage holds R rows of 64 bytes, or 32 / 16 rows of R values):
-//   k contiguous: the 16-byte chunks of row r are swapped by f(r) = (r / 2 % 4) ^ (r /
-//     8 % 2): the 8 (or 16) rows that a read serves at once then lie in all banks
+//   k contiguous: the 16-byte chunks of row r are swapped by f(r) = 3 (r / 8 % 2), of rows of
+//     two steps by r / 2 % 8.  A read serves 16 lanes at once, lanes 0-3, 12-15 and 20-27
+//     first: rows 0-3 and 12-15 with one chunk, rows 4-11 with the next; so they lie in
+//     all banks (with r / 2 % 4 ^ r / 8 % 2 half of the cycles were conflicts)
 //   k strided, 16-bit: 32-byte units of row k are swapped by s(k) = 2 (k % 4) ^ (k / 2 %
 //     2) ^ (k / 8 % 2) for the transposing reads (4 rows x 32 bytes per 16 lanes, rows 8
 //     apart in neighbouring 16s)
 //   k strided, fp32: rows as they are; a fragment's values are read one by one
 // The direct loads write LDS in lane order, so the swaps are made in the addresses
 // that the lanes read from.
+//
+// Forward.  Both operands are rows of the caller's, and a step's 64 bytes of one are half a
+// line: loaded step by step, the L2 caches serve twice the requests for the same bytes
+// (33 million against 17 at 16384 tokens, dim 1024, hidden 4096) and become the limit.
+// There a stage holds two steps; there are two of them, and one barrier a stage.
 //
 // k beyond its end (dim not a whole number of steps, the last tokens, hidden columns
 // that fill no step) is loaded from a block of zeros, so that both operands vanish
@@ -42,9 +49,10 @@ enum SwForm { kFwd = 0, kDx = 1, kDw = 2 };
 constexpr int kSwStepBytes = 64;  // of k, per row: 32 16-bit values, 16 fp32
 constexpr int kSwTiles = 4;
 constexpr int kSwTileM[kSwTiles] = {256, 128, 128, 64}, kSwTileN[kSwTiles] = {256, 256, 128, 128};
-// stages of LDS, and the workgroups that a CU's 160 KB then hold
-constexpr int sw_stages(int bm, int bn) { return bm + bn == 384 ? 3 : 4; }
-constexpr int sw_per_cu(int bm, int bn) { return 160 * 1024 / (sw_stages(bm, bn) * (bm + bn) * kSwStepBytes); }
+// k steps of LDS (forward: two stages of two steps), and the workgroups that a CU's 160 KB
+// then hold
+constexpr int sw_steps(int bm, int bn) { return bm + bn == 384 ? 3 : 4; }
+constexpr int sw_per_cu(int bm, int bn) { return 160 * 1024 / (sw_steps(bm, bn) * (bm + bn) * kSwStepBytes); }
 
 struct SwGemmParams {
   const void* p;            // fwd / dx: W; dw: x
@@ -187,28 +195,33 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
 
-// One operand of R rows (values along m or n) in LDS.  T: k strided in memory.
-template <class DT, int R, bool T>
+// One operand of R rows (values along m or n) in LDS.  T: k strided in memory; KS: k steps
+// of a stage (k contiguous: 2 make whole 128-byte lines of a row).
+template <class DT, int R, bool T, int KS = 1>
 struct SwOperand {
   using E = SwElem<DT>;
-  static constexpr int kBytes = R * kSwStepBytes;         // of a stage
-  static constexpr int kLoads = R / 64;                   // direct loads of a thread per step
+  static_assert(KS == 1 || !T, "steps of a stage");
+  static constexpr int kBytes = R * kSwStepBytes * KS;    // of a stage
+  static constexpr int kLoads = R / 64 * KS;              // direct loads of a thread per stage
   static constexpr int kRowChunks = R / E::kPer;          // strided: chunks of a row of R values
   static constexpr int kUnitMask = R / 16 - 1;            // strided 16-bit: 32-byte units of a row
   uint32_t off[kLoads];   // byte offsets of this thread's chunks from the step's base
   int kr[kLoads];         // and their k: chunk * kPer (contiguous) or row (strided)
-  static constexpr int kReads = T ? R / 32 : 1;
-  uint32_t rd[kReads];    // byte addresses of this lane's fragments: strided, one for each 16 rows of a wave
+  static constexpr int kReads = T ? R / 32 : KS;
+  uint32_t rd[kReads];    // byte addresses of this lane's fragments: strided, one for each 16 rows of
+                          // a wave; contiguous, for each step of a stage
 
-  __device__ static int f_row(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+  __device__ static int f_row(int r) {
+    return KS == 2 ? (r >> 1) & 7 : ((r >> 3) & 1) * 3;
+  }
   __device__ static int s_row(int k) { return ((2 * (k & 3)) ^ ((k >> 1) & 1) ^ ((k >> 3) & 1)) & kUnitMask; }
 
   // row / first k and chunk of load i of a thread
   __device__ __forceinline__ static void place(int i, int tid, int* row, int* chunk) {
     const int q = i * 256 + tid;
     if constexpr (!T) {
-      *row = q >> 2;
-      *chunk = (q & 3) ^ f_row(*row);
+      *row = q / (4 * KS);
+      *chunk = q % (4 * KS) ^ f_row(*row);
     } else {
       *row = q / kRowChunks;
       const int c = q % kRowChunks;
@@ -221,7 +234,8 @@ struct SwOperand {
   __device__ __forceinline__ void place_reads(int row0, int lane, uint32_t base) {
     if constexpr (!T) {
       const int r = row0 + (lane & 15);
-      rd[0] = base + r * 64 + ((lane >> 4) ^ f_row(r)) * 16;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) rd[k] = base + r * (64 * KS) + ((4 * k + (lane >> 4)) ^ f_row(r)) * 16;
     } else if constexpr (E::kSize == 2) {
       const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
 #pragma unroll
@@ -232,10 +246,10 @@ struct SwOperand {
     }
   }
 
-  // the fragment of the wave's j-th 16 rows, of the stage at `stage`
-  __device__ __forceinline__ u32x4 read(const char* lds, uint32_t stage, int j) const {
+  // the fragment of the wave's j-th 16 rows, step ks of the stage at `stage`
+  __device__ __forceinline__ u32x4 read(const char* lds, uint32_t stage, int ks, int j) const {
     if constexpr (!T) {
-      return *(const u32x4*)(lds + stage + rd[0] + j * 1024);
+      return *(const u32x4*)(lds + stage + rd[ks] + j * (1024 * KS));
     } else if constexpr (E::kSize == 2) {
       typedef __attribute__((address_space(3))) sw_s4 lds_s4;
       const char* at = lds + stage + rd[j];

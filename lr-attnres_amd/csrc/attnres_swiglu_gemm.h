@@ -222,11 +222,13 @@ __device__ __forceinline__ void sw_finish(const SwGemmParams& p, char* lds, int 
 template <class DT, int FORM, int BM, int BN, bool SPLIT>
 __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gemm_kernel(SwGemmParams p) {
   using E = SwElem<DT>;
-  using OpP = SwOperand<DT, BN, FORM != kFwd>;
-  using OpQ = SwOperand<DT, BM, FORM == kDw>;
+  constexpr int KS = FORM == kFwd ? 2 : 1;  // k steps of a stage
+  constexpr int kStageK = E::kStep * KS;
+  using OpP = SwOperand<DT, BN, FORM != kFwd, KS>;
+  using OpQ = SwOperand<DT, BM, FORM == kDw, FORM == kFwd ? KS : 1>;
   constexpr int NP = BN / 32, NQ = BM / 32;  // 16 x 16 tiles of a wave
   constexpr int kStage = OpP::kBytes + OpQ::kBytes;
-  constexpr int kStages = sw_stages(BM, BN), kAhead = kStages - 1;  // steps loaded ahead
+  constexpr int kStages = sw_steps(BM, BN) / KS, kAhead = kStages - 1;  // stages loaded ahead
   constexpr int kLoads = OpP::kLoads + OpQ::kLoads;
   constexpr int kCols = FORM == kFwd ? BN / 2 : BN;  // output columns of a tile
   constexpr int es = E::kSize;
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
   int split, tm, tn, tile;
   sw_tile(p, blockIdx.x, gridDim.x, &split, &tm, &tn, &tile);
   const int m0 = tm * BM, n0 = tn * kCols;
-  const int all_steps = (p.K + E::kStep - 1) / E::kStep;
+  const int all_steps = (p.K + kStageK - 1) / kStageK;  // (stages)
   const int first = SPLIT ? split * p.steps : 0;
   const int nk = SPLIT ? min(p.steps, all_steps - first) : all_steps;
 
@@ -282,13 +284,13 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
 
   // Loads of the next step into its stage, piece by piece so that the matrix cores
   // work between them.
-  const int k0 = first * E::kStep;
+  const int k0 = first * kStageK;
   const char* bp = (const char*)p.p + (FORM == kFwd ? (int64_t)k0 : (int64_t)k0 * p.p_stride + n0) * es;
   const char* bq = (const char*)p.q + (FORM == kFwd  ? ((int64_t)m0 * p.q_stride + k0) * es
                                        : FORM == kDx ? ((int64_t)(k0 / E::kStep) * p.n_tok + m0) * kSwStepBytes
                                                      : ((int64_t)(m0 / E::kStep) * p.n_tok + k0) * kSwStepBytes);
-  const int64_t ahead_p = FORM == kFwd ? kSwStepBytes : (int64_t)E::kStep * p.p_stride * es;
-  const int64_t ahead_q = FORM == kFwd  ? kSwStepBytes
+  const int64_t ahead_p = FORM == kFwd ? kSwStepBytes * KS : (int64_t)E::kStep * p.p_stride * es;
+  const int64_t ahead_q = FORM == kFwd  ? kSwStepBytes * KS
                           : FORM == kDx ? p.n_tok * kSwStepBytes
                                         : (int64_t)E::kStep * kSwStepBytes;
   auto behind = [](uint32_t stage) { return stage == (kStages - 1) * kStage ? 0u : stage + kStage; };
@@ -303,8 +305,8 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
     else sw_dma(bq, oq.off[(i - OpP::kLoads) % OpQ::kLoads], lds0 + to + OpP::kBytes + (i - OpP::kLoads) * 4096);
   };
   auto load = [&](int s) {  // step s of the split, k possibly ending in it
-    const int left = p.K - (first + s) * E::kStep;
-    if (left >= E::kStep) {
+    const int left = p.K - (first + s) * kStageK;
+    if (left >= kStageK) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) load_piece(i);
     } else {
@@ -326,12 +328,16 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
   // A step's products in two halves, rows of P by rows of Q: fragments are read into the
   // registers of those that are used up, half a step and more before they are needed.
   //   half 0: rows 0.. H - 1 of P by all of Q, while the other rows of P are read (this
-  //           step's) and a later step's loads are issued
+  //           step's)
   //   half 1: rows H.. by all of Q, column by column; behind each the next step's fragment
   //           of Q takes its place, and early on the next step's first rows of P
+  // A later stage's loads are issued between the products of half 0, or (forward) of the
+  // half 1 behind the barrier that frees the stage.
   constexpr int H = NP / 2, kHalf = H * NQ;
+  using Yes = std::true_type;
+  using No = std::false_type;
   u32x4 fp[NP], fq[NQ];
-  auto half0 = [&](uint32_t stage, auto loads) {
+  auto half0 = [&](uint32_t stage, int ks, auto loads) {
     constexpr int kOps = H + (decltype(loads)::value ? kLoads : 0);
 #pragma unroll
     for (int t = 0; t < kHalf; ++t) {
@@ -340,36 +346,49 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
       for (int i = 0; i < (kOps + kHalf - 1) / kHalf; ++i) {
         const int e = (t * kOps + kHalf - 1) / kHalf + i;  // op e goes behind product e kHalf / kOps
         if (e >= ((t + 1) * kOps + kHalf - 1) / kHalf) continue;
-        if (e < H) fp[H + e % H] = op.read(lds, stage, H + e % H);
+        if (e < H) fp[H + e % H] = op.read(lds, stage, ks, H + e % H);
         else load_piece(e - H);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto half1 = [&](uint32_t next) {
+  auto half1 = [&](uint32_t next, int ks, auto loads) {  // next, ks: the next step's stage and place in it
 #pragma unroll
     for (int t = 0; t < kHalf; ++t) {
       sw_mfma<DT>(fp[H + t % H], fq[t / H], acc[H + t % H][t / H]);
-      if (t < H) fp[t] = op.read(lds, next, t);
-      if (t % H == H - 1) fq[t / H] = oq.read(lds, next, t / H);
+      if (t < H) fp[t] = op.read(lds, next, ks, t);
+      if (t % H == H - 1) fq[t / H] = oq.read(lds, next, ks, t / H);
+      if constexpr (decltype(loads)::value) {
+#pragma unroll
+        for (int i = 0; i < (kLoads + kHalf - 1) / kHalf; ++i) {
+          const int e = (t * kLoads + kHalf - 1) / kHalf + i;
+          if (e < ((t + 1) * kLoads + kHalf - 1) / kHalf) load_piece(e);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // the loads of the next `ahead` steps may still be under way
+  // the loads of the next `ahead` stages may still be under way
   auto wait = [&](int ahead) {
     if (ahead >= 2 && kAhead > 2) sw_wait_barrier<(kAhead > 2 ? 2 : 0) * kLoads>();
-    else if (ahead >= 1) sw_wait_barrier<kLoads>();
+    else if (ahead >= 1 && kAhead > 1) sw_wait_barrier<kLoads>();
     else sw_wait_barrier<0>();
   };
 
+  constexpr int kBegin = KS == 2 ? kStages : kAhead;  // stages loaded before the first product
 #pragma unroll
-  for (int s = 0; s < kAhead; ++s)
+  for (int s = 0; s < kBegin; ++s)
     if (s < nk) load(s);
-  wait(nk - 1);
+  if constexpr (KS == 2) {
+    if (nk > 1) sw_wait_barrier<kLoads>();
+    else sw_wait_barrier<0>();
+  } else {
+    wait(nk - 1);
+  }
 #pragma unroll
-  for (int j = 0; j < H; ++j) fp[j] = op.read(lds, 0, j);
+  for (int j = 0; j < H; ++j) fp[j] = op.read(lds, 0, 0, j);
 #pragma unroll
-  for (int j = 0; j < NQ; ++j) fq[j] = oq.read(lds, 0, j);
+  for (int j = 0; j < NQ; ++j) fq[j] = oq.read(lds, 0, 0, j);
   // (no instruction: between the two loops the largest tile's sums stand in the
   // accumulation registers, and so the compiler moves none of them around in either)
   auto pin = [&]() {
@@ -380,23 +399,45 @@ __global__ __launch_bounds__(256, sw_per_cu(BM, BN) < 2 ? 1 : 2) void swiglu_gem
         for (int b = 0; b < NQ; ++b) asm volatile("" : "+a"(acc[a][b]));
     }
   };
-  const int whole = (int)min((int64_t)nk, (int64_t)p.K / E::kStep - first);  // steps in which k does not end
+  const int whole = (int)min((int64_t)nk, (int64_t)p.K / kStageK - first);  // stages in which k does not end
   int s = 0;
   uint32_t stage = 0;
-  for (; s + kAhead < whole; ++s) {
-    half0(stage, std::true_type());
-    next_step();
-    stage = behind(stage);
-    sw_wait_barrier<(kAhead - 1) * kLoads>();
-    half1(stage);
-  }
-  pin();
-  for (; s < nk; ++s) {
-    if (s + kAhead < nk) load(s + kAhead);
-    half0(stage, std::false_type());
-    stage = behind(stage);
-    wait(nk - 2 - s);
-    half1(stage);  // (behind the last step: fragments read, not used)
+  if constexpr (KS == 2) {
+    for (; s + kStages < whole; ++s) {
+      half0(stage, 0, No());
+      half1(stage, 1, No());
+      half0(stage, 1, No());
+      stage = behind(stage);
+      sw_wait_barrier<0>();  // the next stage has landed, this one is free
+      half1(stage, 0, Yes());
+      next_step();
+    }
+    pin();
+    for (; s < nk; ++s) {
+      half0(stage, 0, No());
+      half1(stage, 1, No());
+      half0(stage, 1, No());
+      stage = behind(stage);
+      sw_wait_barrier<0>();
+      if (s + kStages < nk) load(s + kStages);
+      half1(stage, 0, No());  // (behind the last step: fragments read, not used)
+    }
+  } else {
+    for (; s + kAhead < whole; ++s) {
+      half0(stage, 0, Yes());
+      next_step();
+      stage = behind(stage);
+      sw_wait_barrier<(kAhead - 1) * kLoads>();
+      half1(stage, 0, No());
+    }
+    pin();
+    for (; s < nk; ++s) {
+      if (s + kAhead < nk) load(s + kAhead);
+      half0(stage, 0, No());
+      stage = behind(stage);
+      wait(nk - 2 - s);
+      half1(stage, 0, No());  // (behind the last step: fragments read, not used)
+    }
   }
 
   if constexpr (SPLIT) {
@@ -484,7 +525,11 @@ hipError_t sw_run(const SwGemmParams& p, hipStream_t st) {
 template <class DT, int FORM>
 hipError_t sw_tile_pick(int tile, const SwGemmParams& p, hipStream_t st) {
   if (tile == 0) return sw_run<DT, FORM, 256, 256>(p, st);
-  if (tile == 1) return sw_run<DT, FORM, 128, 256>(p, st);
+  if constexpr (FORM == kFwd) {
+    if (tile == 1) return hipErrorInvalidValue;  // (three steps of LDS hold no two stages of two)
+  } else {
+    if (tile == 1) return sw_run<DT, FORM, 128, 256>(p, st);
+  }
   if (tile == 2) return sw_run<DT, FORM, 128, 128>(p, st);
   return sw_run<DT, FORM, 64, 128>(p, st);
 }
