@@ -1223,6 +1223,8 @@ def swiglu_forward(x, weight, save: bool):
 def swiglu_backward(x, weight, saved, grad_h, want_dx: bool, want_dweight: bool):
     """(dx [n, D] or None, dweight [2 F, D] or None)"""
     lib, d = load(), swiglu_desc(x, weight)
+    if saved.data_ptr() % 16:  # (a saved-tensor hook may give it back anywhere)
+        saved = saved.clone()
     dx = x.new_empty((d.n_tok, d.dim)) if want_dx else None
     dw = x.new_empty((2 * d.hidden, d.dim)) if want_dweight else None
     n = lib.attnres_swiglu_backward_workspace_size(ctypes.byref(d), int(want_dx), int(want_dweight))

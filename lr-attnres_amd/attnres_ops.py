@@ -1917,7 +1917,7 @@ def qkv_norm_rotary(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, posit
     ``qkv`` [B, T, (num_heads + 2 num_kv_heads) Dh]: query, key and value heads (``num_kv_heads``: as many as query heads
     unless given).  Query and key heads are rms-normed over Dh (``qk_norm``; torch's default eps) and rotated by interleaved
     pairs, all in fp32 with one rounding to the dtype (the reference rounds the normed head, each product and each sum).
-    ``sin``, ``cos``: tables [..., rows, Dh / 2] (as ``RotaryEmbedding``'s buffers), fp32 or in ``qkv``'s dtype.
+    ``sin``, ``cos``: tables [rows, Dh / 2] (or [1, 1, rows, Dh / 2], as ``RotaryEmbedding``'s buffers), fp32 or in ``qkv``'s dtype.
     ``positions``: None (token t takes row t), an int (row ``positions`` + t), or an integer tensor [T] or [B, T] of rows;
     a row outside the tables gives NaN in that token's queries and keys (a tensor's values are not looked at on the host).
 
@@ -1945,8 +1945,8 @@ def qkv_norm_rotary(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, posit
     if Dh > _hip.QKV_ROTARY_MAX_HEAD_DIM:
         raise RuntimeError(f"{what}: head width {Dh} above {_hip.QKV_ROTARY_MAX_HEAD_DIM}")
     for name, t in (("sin", sin), ("cos", cos)):
-        if t.dim() < 2 or t.size(-1) != Dh // 2:
-            raise RuntimeError(f"{what}: {name} must be [..., rows, {Dh // 2}], got {tuple(t.shape)}")
+        if t.dim() < 2 or t.size(-1) != Dh // 2 or t.numel() != t.size(-2) * t.size(-1):
+            raise RuntimeError(f"{what}: {name} must be [rows, {Dh // 2}] (and leading ones), got {tuple(t.shape)}")
         if t.requires_grad:
             raise RuntimeError(f"{what}: {name} takes no gradient")
         if not t.is_floating_point():

@@ -192,8 +192,8 @@ struct SwCosts {
   double fixed[kSwTiles];     // a workgroup's begin and end
   double launch, bytes_us;    // a split's second launch, and its traffic
 };
-constexpr SwCosts kCost16 = {{0.589, 0.481, 0.232, 0.205}, {1.0, 0.935, 1.0, 0.73}, {5.77, 3.5, 3.26, 2.55}, 3.95, 8.7e6};
-constexpr SwCosts kCost32 = {{3.905, 2.052, 1.062, 0.59}, {1.0, 0.981, 0.968, 0.906}, {3.69, 0.82, 0.59, 0.0}, 5.32, 7.8e6};
+constexpr SwCosts kCost16 = {{0.638, 0.394, 0.239, 0.181}, {1.0, 0.961, 0.899, 0.778}, {6.45, 3.35, 2.63, 1.82}, 4.17, 9.5e6};
+constexpr SwCosts kCost32 = {{3.955, 2.036, 1.024, 0.557}, {1.0, 0.934, 0.971, 0.912}, {4.25, 0.92, 0.88, 0.2}, 5.31, 7.9e6};
 
 SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {  // (forward: of two k steps each)
   const SwCosts& k = dtype == ATTNRES_DTYPE_F32 ? kCost32 : kCost16;

@@ -73,7 +73,7 @@ struct SwGemmParams {
 };
 
 hipError_t launch_swiglu_gemm(int dtype, int form, int tile, const SwGemmParams& p, hipStream_t st);
-constexpr int kSwFew = 48;  // rows at most
+constexpr int kSwFew = 64;  // rows at most
 hipError_t launch_swiglu_few(int dtype, const SwGemmParams& p, hipStream_t st);  // the forward
 
 // [du dz] of the backward, in blocks, with zeros behind each half's F columns

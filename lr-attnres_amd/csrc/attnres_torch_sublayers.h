@@ -96,7 +96,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
 };
 
 bool rotary_table(const Tensor& t, const Tensor& qkv, int64_t half) {
-  return t.dim() >= 2 && t.size(-1) == half && t.numel() > 0 && t.is_contiguous() && !t.requires_grad() &&
+  return t.dim() >= 2 && t.size(-1) == half && t.numel() > 0 && t.numel() == t.size(-2) * half && t.is_contiguous() && !t.requires_grad() &&
          t.device() == qkv.device() && (t.scalar_type() == at::kFloat || t.scalar_type() == qkv.scalar_type());
 }
 

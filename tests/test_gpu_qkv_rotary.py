@@ -345,3 +345,45 @@ def test_compiled_matches_eager():
     (d,) = torch.autograd.grad(out, [x], grads)
     for a, b in zip((*[o.detach() for o in out], d), ref):
         assert torch.equal(a, b)
+
+
+def test_refused_calls_and_changed_values():
+    """Refusals that need GPU tensors, and writing into the values while their gradient is to come."""
+    B, T, Hq, K, Dh = 1, 4, 2, 1, 64
+    qkv, grads = _inputs(B, T, Hq, K, Dh, BF)
+    sin, cos = _tables(8, Dh)
+    bad = [dict(positions=5), dict(positions=-1), dict(positions=True), dict(positions=1.0),
+           dict(positions=torch.zeros(T, device="cuda")), dict(positions=torch.zeros(T + 1, device="cuda", dtype=torch.long)),
+           dict(positions=torch.zeros((T, B, 1), device="cuda", dtype=torch.long)),
+           dict(positions=torch.zeros(T, dtype=torch.long))]
+    for kw in bad:
+        with pytest.raises(RuntimeError):
+            ops.qkv_norm_rotary(qkv, Hq, sin, cos, num_kv_heads=K, **kw)
+    with pytest.raises(RuntimeError):
+        ops.qkv_norm_rotary(qkv, Hq, sin.cpu(), cos.cpu(), num_kv_heads=K)
+    x = qkv.clone().requires_grad_(True)
+    _, _, v = ops.qkv_norm_rotary(x, Hq, sin, cos, num_kv_heads=K)
+    with pytest.raises(RuntimeError):
+        v.add_(1.0)
+    # the projection changed in place between forward and backward is noticed
+    x = qkv.clone().requires_grad_(True)
+    y = x * 1.0
+    q, _, _ = ops.qkv_norm_rotary(y, Hq, sin, cos, num_kv_heads=K)
+    with torch.no_grad():
+        y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(q, x, grads[0])
+
+
+def test_general_route_gives_the_same(monkeypatch):
+    """The library ops that a traced call uses, run eagerly: the same results as the native call."""
+    B, T, Hq, K, Dh = 2, 9, 4, 2, 64
+    qkv, grads = _inputs(B, T, Hq, K, Dh, BF)
+    sin, cos = _tables(16, Dh)
+    at = torch.randint(0, 16, (B, T), device="cuda")
+    for kw in (dict(), dict(positions=3), dict(positions=at), dict(positions=at[0], qk_norm=False)):
+        ref = _call(qkv, Hq, K, sin, cos, grads, **kw)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_native", lambda *names: None)
+            got = _call(qkv, Hq, K, sin, cos, grads, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(ref, got))

@@ -310,3 +310,65 @@ def test_compiled_matches_eager():
     h = f(x, w)
     got = (h.detach(), *torch.autograd.grad(h, (x, w), dh))
     assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
+def test_general_route_gives_the_same(monkeypatch):
+    """The library ops that a traced call uses, run eagerly: the same results as the native call."""
+    for n, D, F in ((70, 64, 40), (5, 33, 17)):
+        x, w, dh = _values(n, D, F, BF)
+        ref = _run(x, w, dh)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_native", lambda *names: None)
+            got = _run(x, w, dh)
+            with torch.no_grad():
+                again = ops.swiglu_projection(x, w)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)):
+                moved = _run(x, w, dh)
+        assert all(torch.equal(a, b) for a, b in zip(ref, got)) and torch.equal(again, ref[0])
+        assert all(torch.equal(a, b) for a, b in zip(ref, moved))
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Two calls with workspaces of their own (copied operands, split sums) on two streams, several times over."""
+    args = [_values(300, 1000, 130, BF, seed=s) for s in (1, 2)] + [_values(90, 130, 77, F32, seed=s) for s in (3, 4)]
+    want = [_run(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for a, s in zip(args, streams):
+            with torch.cuda.stream(s):
+                got.append(_run(*a))
+        torch.cuda.synchronize()
+        for g, e in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(g, e))
+
+
+def test_two_captured_graphs_interleaved():
+    """Two graphs of calls with workspaces, replayed in turn and together with eager work, each from its own pool."""
+    sets = [[t.clone() for t in _values(200, 1000, 130, BF, seed=s)] for s in (5, 6)]
+    want = [_run(*a) for a in sets]
+    graphs, outs = [], []
+    for x, w, dh in sets:
+        x.requires_grad_(True), w.requires_grad_(True)
+
+        def step():
+            h = ops.swiglu_projection(x, w)
+            return (h, *torch.autograd.grad(h, (x, w), dh))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    for k in (0, 1, 1, 0, 1, 0):
+        for t in outs[k]:
+            t.detach().zero_()
+        graphs[k].replay()
+        eager = _run(*[t.detach() for t in sets[1 - k]])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[k], want[k]))
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[1 - k]))

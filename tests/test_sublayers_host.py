@@ -161,6 +161,7 @@ def test_python_refusals():
         (lambda: ops.qkv_norm_rotary(qkv, 2, sin[:, :3], cos), "sin must be"),
         (lambda: ops.qkv_norm_rotary(qkv, 2, sin, cos[0]), "cos must be"),
         (lambda: ops.qkv_norm_rotary(qkv, 2, sin, cos[:4]), "differ in shape"),
+        (lambda: ops.qkv_norm_rotary(qkv, 2, torch.zeros(2, 8, 4), torch.zeros(2, 8, 4)), "sin must be"),
         (lambda: ops.qkv_norm_rotary(qkv, 2, sin.clone().requires_grad_(True), cos), "no gradient"),
         (lambda: ops.qkv_norm_rotary(qkv, 2, sin.long(), cos.long()), "floating-point"),
         (lambda: ops.qkv_norm_rotary(qkv, 2, sin, cos), "ROCm GPU"),
