@@ -176,12 +176,12 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
 // Tile and splits of a product with `steps` k steps: the least time in a model of a
 // launch, in us.  The CUs take workgroups in rounds, as many together as LDS holds;
 // together they share the matrix cores.  A split product's sums are written and read
-// once more, by a second launch.  The constants are fitted to 700 launches (15 shapes
-// of 64 to 16384 tokens, every tile, 1 to 64 splits, fp32 and bf16); there the model's
-// choice is 1% slower than the best one in the mean and 11% at most.  The large tile
-// moves the least data a product, the small one fills the CUs: forward of 2000 tokens,
-// dim 1024, hidden 4096, bf16: 39 us with 256 x 256, 62 with 64 x 128; of 512 tokens,
-// dim 1024, hidden 1024: 29 and 8.5.
+// once more, by a second launch.  The constants are fitted to 1900 launches (24 shapes
+// of 60 to 16384 tokens, every tile, 1 to 64 splits, fp32 and bf16, all three products);
+// there the model's choice is 1.5% slower than the best one in the mean and 12% at most.
+// The large tile moves the least data a product, the small one fills the CUs: forward of
+// 2000 tokens, dim 1024, hidden 4096, bf16: 40 us with 256 x 256, 46 with 64 x 128; of
+// 512 tokens, dim 1024, hidden 1024: 29 and 9.
 struct SwShape {
   int tile, tiles_m, tiles_n, splits, steps;
 };
@@ -200,7 +200,7 @@ SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {  // (forwar
   SwShape best{};
   double least = 1e300;
   for (int t = 0; t < kSwTiles; ++t) {
-    if (form == kFwd && kSwTileM[t] + kSwTileN[t] == 384) continue;
+    if (!sw_has_tile(form, dtype, t)) continue;
     const int cols = form == kFwd ? kSwTileN[t] / 2 : kSwTileN[t];
     const int64_t tm = (M + kSwTileM[t] - 1) / kSwTileM[t], tn = (N + cols - 1) / cols;
     const int together = sw_per_cu(kSwTileM[t], kSwTileN[t]);

@@ -49,6 +49,12 @@ enum SwForm { kFwd = 0, kDx = 1, kDw = 2 };
 constexpr int kSwStepBytes = 64;  // of k, per row: 32 16-bit values, 16 fp32
 constexpr int kSwTiles = 4;
 constexpr int kSwTileM[kSwTiles] = {256, 128, 128, 64}, kSwTileN[kSwTiles] = {256, 256, 128, 128};
+// which of them a product has: a forward's two stages of two steps do not fit three steps
+// of LDS; in fp32, with a sixteenth of the matrix rate, smaller tiles are never slower
+// than the largest one
+constexpr bool sw_has_tile(int form, int dtype, int tile) {
+  return tile > 1 || (tile == 1 ? form != kFwd : dtype != F32::kCode);
+}
 // k steps of LDS (forward: two stages of two steps), and the workgroups that a CU's 160 KB
 // then hold
 constexpr int sw_steps(int bm, int bn) { return bm + bn == 384 ? 3 : 4; }

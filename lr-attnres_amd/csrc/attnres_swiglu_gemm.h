@@ -524,12 +524,13 @@ hipError_t sw_run(const SwGemmParams& p, hipStream_t st) {
 
 template <class DT, int FORM>
 hipError_t sw_tile_pick(int tile, const SwGemmParams& p, hipStream_t st) {
-  if (tile == 0) return sw_run<DT, FORM, 256, 256>(p, st);
-  if constexpr (FORM == kFwd) {
-    if (tile == 1) return hipErrorInvalidValue;  // (three steps of LDS hold no two stages of two)
-  } else {
+  if constexpr (sw_has_tile(FORM, DT::kCode, 0)) {
+    if (tile == 0) return sw_run<DT, FORM, 256, 256>(p, st);
+  }
+  if constexpr (sw_has_tile(FORM, DT::kCode, 1)) {
     if (tile == 1) return sw_run<DT, FORM, 128, 256>(p, st);
   }
+  if (tile < 2) return hipErrorInvalidValue;
   if (tile == 2) return sw_run<DT, FORM, 128, 128>(p, st);
   return sw_run<DT, FORM, 64, 128>(p, st);
 }

@@ -116,7 +116,7 @@ def test_head_widths(Dh, dtype, table):
     _check(2, 5, 3, 3, Dh, dtype, table)
 
 
-@pytest.mark.parametrize("Hq,K", [(1, 1), (2, 1), (5, 5), (8, 2), (12, 12), (16, 4), (33, 11), (7, 13)])
+@pytest.mark.parametrize("Hq,K", [(1, 1), (2, 1), (5, 5), (8, 2), (12, 12), (20, 4), (33, 11), (7, 13)])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_head_counts(Hq, K, dtype):
     _check(2, 7, Hq, K, 64, dtype)

@@ -99,6 +99,17 @@ def test_large(n, D, F, dtype):
     _check_exact(n, D, F, dtype)
 
 
+# together these take every tile of every product, whole and split over k, in 16 bits and in fp32
+TILES = [(65, 36, 49), (1758, 73, 2148), (1429, 1459, 814), (3568, 162, 1978), (6469, 2187, 485), (1363, 1750, 1904),
+         (4788, 1649, 46), (3729, 1840, 1258), (2202, 1913, 2240)]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("n,D,F", TILES)
+def test_every_tile_and_split(n, D, F, dtype):
+    _check_exact(n, D, F, dtype)
+
+
 def _strided(t, pad, offset=0):
     big = torch.full((t.size(0), t.size(1) + pad), float("nan"), device=t.device, dtype=t.dtype)
     big[:, offset:offset + t.size(1)] = t
