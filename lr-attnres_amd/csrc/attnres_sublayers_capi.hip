@@ -176,12 +176,16 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
 // Tile and splits of a product with `steps` k steps: the least time in a model of a
 // launch, in us.  The CUs take workgroups in rounds, as many together as LDS holds;
 // together they share the matrix cores.  A split product's sums are written and read
-// once more, by a second launch.  The constants are fitted to 1900 launches (24 shapes
-// of 60 to 16384 tokens, every tile, 1 to 64 splits, fp32 and bf16, all three products);
-// there the model's choice is 1.5% slower than the best one in the mean and 12% at most.
+// once more, by a second launch.  The constants are fitted to 1900 launches of these
+// products before their last speed-up (24 shapes of 60 to 16384 tokens, every tile, 1 to 64
+// splits, fp32 and bf16).  Measured again since, 1422 launches of 63 products (100 to 16384
+// tokens; dx and dw with the activation's gradient before them): the model's choice is 1.3%
+// slower than the best one in the mean, 17% at most (dx of 100 tokens, dim 512, hidden 1024:
+// 13.3 us, 11.4 with 8 splits) and 8% otherwise.
 // The large tile moves the least data a product, the small one fills the CUs: forward of
-// 2000 tokens, dim 1024, hidden 4096, bf16: 40 us with 256 x 256, 46 with 64 x 128; of
-// 512 tokens, dim 1024, hidden 1024: 29 and 9.
+// 2000 tokens, dim 1024, hidden 4096, bf16, with what the backward needs: 38 us with 256 x
+// 256, 39 with 128 x 128, 45 with 64 x 128; of 512 tokens, dim 1024, hidden 1024: 8.9 with
+// 64 x 128, 11.8 with 128 x 128.
 struct SwShape {
   int tile, tiles_m, tiles_n, splits, steps;
 };
