@@ -39,6 +39,19 @@ __device__ __forceinline__ void store_raw(typename DT::S* p, const Raw<DT, E>& r
   else *(uint32_t*)p = r.w[0];
 }
 
+// A launch dimension holds fewer than 2^32 threads; narrow heads of many tokens are more,
+// so workgroups continue in a second one.
+__device__ __forceinline__ int64_t rot_wave() {
+  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kRotWaves + threadIdx.x / kWave;
+}
+bool rot_grid(int64_t waves, dim3* grid) {
+  constexpr int64_t kMax = ((int64_t)1 << 32) / (kRotWaves * kWave) - 1;
+  const int64_t n = (waves + kRotWaves - 1) / kRotWaves, rows = (n + kMax - 1) / kMax;
+  if (rows > 65535) return false;
+  *grid = dim3((unsigned)((n + rows - 1) / rows), (unsigned)rows);
+  return true;
+}
+
 // row of the tables for token (b, t); -1: outside
 __device__ __forceinline__ int64_t rot_position(const QkvRotaryParams& p, int64_t b, int64_t t) {
   const int64_t at = p.pos ? p.pos[b * p.pos_b_stride + t * p.pos_t_stride] : p.start + t;
@@ -52,7 +65,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryP
   using TS = typename TT::S;
   constexpr int kHeads = kWave / LANES;  // heads of a group
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t wid = (int64_t)blockIdx.x * kRotWaves + threadIdx.x / kWave;
+  const int64_t wid = rot_wave();
   const int64_t tok = wid / groups;
   if (tok >= p.n_tok) return;
   const int part = (int)(wid - tok * groups);
@@ -179,7 +192,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_general(QkvRotary
   using TS = typename TT::S;
   const int lane = threadIdx.x & (kWave - 1);
   const int n_rot = p.q_heads + p.kv_heads, n_all = BWD ? n_rot + p.kv_heads : n_rot;
-  const int64_t wid = (int64_t)blockIdx.x * kRotWaves + threadIdx.x / kWave;
+  const int64_t wid = rot_wave();
   const int64_t tok = wid / n_all;
   if (tok >= p.n_tok) return;
   const int h = (int)(wid - tok * n_all);
@@ -242,18 +255,17 @@ hipError_t run(const QkvRotaryParams& p, hipStream_t st) {
   // head groups shared evenly by as few waves as hold them (36 heads of 64: 3 + 2 groups, not 4 + 1)
   const int all = (n_all + kWave / LANES - 1) / (kWave / LANES);
   const int groups = (all + kIters - 1) / kIters, iters = (all + groups - 1) / groups;
-  const int64_t grid = (p.n_tok * groups + kRotWaves - 1) / kRotWaves;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
-  qkv_rotary_kernel<DT, TT, VEC, LANES, CHUNKS, BWD><<<dim3((unsigned)grid), dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters);
+  dim3 grid;
+  if (!rot_grid(p.n_tok * groups, &grid)) return hipErrorInvalidValue;
+  qkv_rotary_kernel<DT, TT, VEC, LANES, CHUNKS, BWD><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters);
   return hipGetLastError();
 }
 
 template <class DT, class TT, bool BWD>
 hipError_t run_general(const QkvRotaryParams& p, hipStream_t st) {
-  const int64_t waves = p.n_tok * (p.q_heads + p.kv_heads * (BWD ? 2 : 1));
-  const int64_t grid = (waves + kRotWaves - 1) / kRotWaves;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
-  qkv_rotary_general<DT, TT, BWD><<<dim3((unsigned)grid), dim3(kRotWaves * kWave), 0, st>>>(p);
+  dim3 grid;
+  if (!rot_grid(p.n_tok * (p.q_heads + p.kv_heads * (BWD ? 2 : 1)), &grid)) return hipErrorInvalidValue;
+  qkv_rotary_general<DT, TT, BWD><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p);
   return hipGetLastError();
 }
 

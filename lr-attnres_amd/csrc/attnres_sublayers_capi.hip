@@ -212,7 +212,7 @@ SwShape sw_shape(int form, int dtype, int64_t M, int N, int steps) {  // (forwar
       const int per = (steps + splits - 1) / splits;
       if ((steps + per - 1) / per != splits) continue;
       const int64_t wgs = tm * tn * splits;
-      if (wgs > (1 << 24)) break;
+      if (wgs >= (1 << 24)) break;  // fewer than 2^32 threads
       const int64_t rounds = (wgs + kCus - 1) / kCus;  // workgroups that one CU works on
       auto group = [&](int g) { return (form == kFwd ? 2 : 1) * per * k.step[t] * (g * k.together[t] > 1.0 ? g * k.together[t] : 1.0) + k.fixed[t]; };
       double cost = (double)(rounds / together) * group(together);

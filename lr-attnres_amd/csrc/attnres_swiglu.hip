@@ -18,6 +18,7 @@ hipError_t launch_swiglu_gemm(int dtype, int form, int tile, const SwGemmParams&
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxGrid = (1 << 24) - 1;  // fewer than 2^32 threads
 
 // du = dh silu(z), dz = dh u silu'(z), silu'(z) = s + z s (1 - s), s = 1 / (1 + exp(-z)).
 // Both products of the backward read [du dz], each of them several times; it is
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_clear_kernel(typename DT::S* 
 
 bool grid_of(int64_t n, dim3* grid) {
   const int64_t g = (n + kThreads - 1) / kThreads;
-  if (g > INT32_MAX) return false;
+  if (g > kMaxGrid) return false;
   *grid = dim3((unsigned)g);
   return true;
 }
@@ -129,7 +130,7 @@ bool grid_of(int64_t n, dim3* grid) {
 template <class DT>
 hipError_t run_grad(const SwGradParams& p, hipStream_t st) {
   const int64_t grid = (p.n + 15) / 16 * ((p.Fp / SwElem<DT>::kStep + 3) / 4);
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (grid > kMaxGrid) return hipErrorInvalidValue;
   swiglu_grad_kernel<DT><<<dim3((unsigned)grid), dim3(kThreads), 0, st>>>(p);
   return hipGetLastError();
 }

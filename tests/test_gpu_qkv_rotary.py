@@ -387,3 +387,18 @@ def test_general_route_gives_the_same(monkeypatch):
             m.setattr(ops, "_native", lambda *names: None)
             got = _call(qkv, Hq, K, sin, cos, grads, **kw)
         assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
+@pytest.mark.parametrize("offset", [0, 1])  # vectors, single values
+def test_more_workgroups_than_one_launch_dimension_holds(offset):
+    # narrow heads of many tokens: above 2^32 threads; bit for bit as in halves
+    B, T, half = 1_060_000, 64, 530_000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    flat = torch.randn(B * T * 6 + offset, generator=g, device="cuda", dtype=BF)
+    qkv = flat[offset:].view(B, T, 6).requires_grad_(True)
+    grads = [torch.randn(B, 1, T, 2, generator=g, device="cuda", dtype=BF) for _ in range(3)]
+    sin, cos = _tables(T, 2)
+    whole = _call(qkv, 1, 1, sin, cos, grads)
+    for s in (slice(0, half), slice(half, B)):
+        part = _call(qkv[s], 1, 1, sin, cos, [x[s] for x in grads])
+        assert all(torch.equal(a[s], b) for a, b in zip(whole, part))
