@@ -2028,6 +2028,13 @@ def _swiglu_backward(ctx, grad_h, grad_saved):
 _swiglu_op.register_autograd(_swiglu_backward, setup_context=_swiglu_setup_context)
 
 
+def _autocast_operand(t: Tensor) -> Tensor:
+    """A linear layer's operand: under autocast in the autocast dtype, but for fp64 and whole numbers."""
+    if t.is_cuda and t.is_floating_point() and t.dtype != torch.float64 and torch.is_autocast_enabled("cuda"):
+        return t.to(torch.get_autocast_dtype("cuda"))
+    return t
+
+
 def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
     """A gated feed-forward block up to its output projection: ``(x @ W_up^T) * silu(x @ W_gate^T)``.
 
@@ -2037,7 +2044,8 @@ def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
     it by the weight and the input.
 
     ``x`` [..., D]; ``weight`` [2 F, D], rows ``[0, F)`` up and ``[F, 2 F)`` gate (``nn.Linear(D, 2 F, bias=False).weight``
-    with ``[up, gate] = fc1(x).chunk(2)``), taken in ``x``'s dtype.  Returns [..., F].  For the backward both projections
+    with ``[up, gate] = fc1(x).chunk(2)``), taken in ``x``'s dtype; under autocast both are taken in the autocast dtype, as
+    ``F.linear`` takes them.  Returns [..., F].  For the backward both projections
     are kept, in the 16-bit dtypes with 12 (bf16) or 16 (fp16) significant bits: 5 or 6 bytes for each of the [..., F].
     """
     what = "swiglu_projection"
@@ -2046,6 +2054,7 @@ def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
         out = nat.swiglu(x, weight)
         if out is not None:
             return out
+    x, weight = _autocast_operand(x), _autocast_operand(weight)
     if x.dim() < 1:
         raise RuntimeError(f"{what}: x must be [..., D]")
     if x.dtype not in _ALLOWED:

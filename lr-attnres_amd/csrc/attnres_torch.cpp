@@ -27,6 +27,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/autocast_mode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include "../../include/attnres_hip.h"

@@ -212,9 +212,22 @@ struct SwigluFn : torch::autograd::Function<SwigluFn> {
   }
 };
 
+// An operand as a linear layer takes it: under autocast in the autocast dtype (fp64 as it is).  The cast is
+// differentiable, and a weight's is kept by the autocast context as it keeps a linear layer's.
+Tensor autocast_operand(const Tensor& t) {
+  if (!at::autocast::is_autocast_enabled(at::kCUDA)) return t;
+  const auto to = at::autocast::get_autocast_dtype(at::kCUDA);
+  Tensor c = at::autocast::cached_cast(to, t, at::kCUDA);
+  // (a cast that was kept from a call without gradients has none to give)
+  if (at::GradMode::is_enabled() && t.requires_grad() && !c.requires_grad()) c = t.to(to);
+  return c;
+}
+
 py::object swiglu(const py::object& x_, const py::object& w_) {
   Tensor x, w;
   if (!plain_mode() || !unpack(x_.ptr(), &x) || !unpack(w_.ptr(), &w)) return py::none();
+  x = autocast_operand(x);
+  w = autocast_operand(w);
   if (x.dim() < 1 || x.numel() < 1 || dtype_code(x.scalar_type()) < 0 || w.scalar_type() != x.scalar_type() ||
       w.device() != x.device() || w.dim() != 2 || w.size(1) != x.size(-1) || w.size(0) < 2 || w.size(0) % 2)
     return py::none();
