@@ -38,7 +38,9 @@ kernels too: the heads of the fused query / key / value projection in one pass
 (``qkv_norm_rotary``: qk-norm and rotation, one rounding where the eager chain
 rounds six times) and the MLP up to its output projection as one product with
 the activation behind it (``swiglu_projection``); results differ from the
-eager sublayers by those roundings.  Module and parameter names match the reference's, so a
+eager sublayers by those roundings.  They stand for the modules that are built
+here: a sublayer whose ``fc1`` or ``rope`` was replaced, hooked or given a
+forward of its own runs the eager chain.  Module and parameter names match the reference's, so a
 reference state dict for this configuration loads with ``load_state_dict``.
 
 The read functions are looked up on ``ops`` (default: the HIP-backed
@@ -234,6 +236,21 @@ class SourceKeyProjection(nn.Module):
         return _norm_heads(key, self.heads) if self.key_norm else key
 
 
+def _plain_linear(m: nn.Module) -> bool:
+    """Whether calling ``m`` is ``x @ m.weight^T`` and nothing else, so that an operator may take the weight in its
+    place: an ``nn.Linear`` itself (not an adapter, a parametrization or a sharding wrapper in its place), without
+    bias, hooks or a forward of its own."""
+    return (type(m) is nn.Linear and m.bias is None and "forward" not in m.__dict__ and
+            not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks) and
+            not _any_global_hook())
+
+
+def _any_global_hook() -> bool:
+    g = nn.modules.module
+    return bool(g._global_forward_hooks or g._global_forward_pre_hooks or g._global_backward_hooks or
+                g._global_backward_pre_hooks)
+
+
 def _attend(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
     """Causal SDPA.  For 16-bit inputs on the GPU only the fused flash /
     memory-efficient kernels are allowed: the math path forms 16-bit batched
@@ -265,7 +282,8 @@ class MultiHeadAttention(nn.Module):
 
     def forward(self, x: Tensor):
         B, T, C = x.shape
-        if self.fused_heads:
+        # (a rotation of another kind is called as it is)
+        if self.fused_heads and type(self.rope) is RotaryEmbedding and "rotate" not in self.rope.__dict__:
             q, k, v = self.ops.qkv_norm_rotary(self.c_attn(x), self.n_head, self.rope.sin, self.rope.cos,
                                                qk_norm=self.qk_norm)
         else:
@@ -300,7 +318,7 @@ class MLP(nn.Module):
             self.fc2 = nn.Linear(hidden, config.n_embd, bias=False)
 
     def forward(self, x: Tensor):
-        if self.fused_gate:
+        if self.fused_gate and _plain_linear(self.fc1):
             h = self.ops.swiglu_projection(x, self.fc1.weight)
         else:
             up, gate = self.fc1(x).chunk(2, dim=-1)
