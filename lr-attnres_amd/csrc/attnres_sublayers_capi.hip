@@ -311,12 +311,31 @@ extern "C" size_t attnres_swiglu_forward_workspace_size(const attnres_swiglu_des
   return packed_x(d, l) + packed_w(d, l, false) + (d->n_tok <= kSwFew ? 0 : sw_partials(fwd_shape(d, l)));
 }
 
+namespace {
+
+// The backward's products (only those that are wanted: the search for one takes a microsecond, and a product that
+// nobody asked for refuses no call) and its workspace: [du dz], copied operands, one product's partial sums at a time.
+struct SwBackward {
+  SwShape dx, dw;
+  size_t d, x, w, need;
+};
+SwBackward sw_backward(const attnres_swiglu_desc* d, const SwLayout& l, bool want_dx, bool want_dw) {
+  SwBackward b{};
+  if (want_dx) b.dx = dx_shape(d, l);
+  if (want_dw) b.dw = dw_shape(d, l);
+  b.d = up256((size_t)d->n_tok * 2 * l.Fp * l.es);
+  b.x = want_dw ? packed_x(d, l) : 0;
+  b.w = want_dx ? packed_w(d, l, true) : 0;
+  const size_t dx = want_dx ? sw_partials(b.dx) : 0, dw = want_dw ? sw_partials(b.dw) : 0;
+  b.need = b.d + b.x + b.w + (dx > dw ? dx : dw);
+  return b;
+}
+
+}  // namespace
+
 extern "C" size_t attnres_swiglu_backward_workspace_size(const attnres_swiglu_desc* d, int32_t want_dx, int32_t want_dw) {
   if (check_swiglu(d) || d->n_tok == 0) return 0;
-  const SwLayout l = sw_layout(d);
-  const size_t a = want_dx ? sw_partials(dx_shape(d, l)) : 0, b = want_dw ? sw_partials(dw_shape(d, l)) : 0;
-  return up256((size_t)d->n_tok * 2 * l.Fp * l.es) + (want_dw ? packed_x(d, l) : 0) + (want_dx ? packed_w(d, l, true) : 0) +
-         (a > b ? a : b);
+  return sw_backward(d, sw_layout(d), want_dx != 0, want_dw != 0).need;
 }
 
 extern "C" int attnres_swiglu_forward(const attnres_swiglu_desc* d, void* h, void* saved, void* workspace,
@@ -373,14 +392,12 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
   if (!aligned(saved, 16)) return api_fail(ATTNRES_EINVAL, "saved is not aligned to 16 bytes");
   if (grad_row_stride < 0) return api_fail(ATTNRES_EINVAL, "grad_row_stride < 0");
   const SwLayout l = sw_layout(d);
-  const SwShape sx = dx_shape(d, l), sw = dw_shape(d, l);
-  if (!sx.steps || !sw.steps) return api_fail(ATTNRES_EUNSUPPORTED, "too many tiles");
-  const size_t need = attnres_swiglu_backward_workspace_size(d, dx != nullptr, dweight != nullptr);
-  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
-    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  const SwBackward b = sw_backward(d, l, dx != nullptr, dweight != nullptr);
+  if ((dx && !b.dx.steps) || (dweight && !b.dw.steps)) return api_fail(ATTNRES_EUNSUPPORTED, "too many tiles");
+  if (!workspace || workspace_bytes < b.need || !aligned(workspace, 256))
+    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", b.need, workspace ? workspace_bytes : (size_t)0);
   char* ws = (char*)workspace;
-  const size_t pd = up256((size_t)d->n_tok * 2 * l.Fp * l.es), px = dweight ? packed_x(d, l) : 0,
-               pw = dx ? packed_w(d, l, true) : 0;
+  float* const partials = (float*)(ws + b.d + b.x + b.w);
   SwGradParams e{};
   e.dh = grad_h;
   e.dh_stride = grad_row_stride;
@@ -391,7 +408,7 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
   e.Fp = l.Fp;
   e.vec = aligned(grad_h, 16) && grad_row_stride % l.per == 0;
   SwOperands o;
-  err = sw_operands(d, l, true, px ? ws + pd : nullptr, pw ? ws + pd + px : nullptr, st, &o);
+  err = sw_operands(d, l, true, b.x ? ws + b.d : nullptr, b.w ? ws + b.d + b.x : nullptr, st, &o);
   if (err == hipSuccess) err = launch_swiglu_grad(d->dtype, e, st);
   if (dx && err == hipSuccess) {
     SwGemmParams g{};
@@ -404,13 +421,13 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
     g.K = 2 * l.Fp;
     g.F = d->hidden;
     g.Fp = l.Fp;
-    set_shape(sx, &g);
+    set_shape(b.dx, &g);
     g.out = dx;
     g.out_stride = d->dim;
     g.n_out = d->dim;
     g.out_vec = d->dim % l.per == 0 && aligned(dx, 16);
-    g.partials = (float*)(ws + pd + px + pw);
-    err = launch_swiglu_gemm(d->dtype, kDx, sx.tile, g, st);
+    g.partials = partials;
+    err = launch_swiglu_gemm(d->dtype, kDx, b.dx.tile, g, st);
   }
   if (dweight && err == hipSuccess) {
     SwGemmParams g{};
@@ -423,13 +440,13 @@ extern "C" int attnres_swiglu_backward(const attnres_swiglu_desc* d, const void*
     g.K = (int)d->n_tok;
     g.F = d->hidden;
     g.Fp = l.Fp;
-    set_shape(sw, &g);
+    set_shape(b.dw, &g);
     g.out = dweight;
     g.out_stride = d->dim;
     g.n_out = d->dim;
     g.out_vec = d->dim % l.per == 0 && aligned(dweight, 16);
-    g.partials = (float*)(ws + pd + px + pw);
-    err = launch_swiglu_gemm(d->dtype, kDw, sw.tile, g, st);
+    g.partials = partials;
+    err = launch_swiglu_gemm(d->dtype, kDw, b.dw.tile, g, st);
   }
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "swiglu backward launch failed: %s", hipGetErrorString(err));
   return ATTNRES_OK;
