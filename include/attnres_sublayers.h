@@ -63,7 +63,10 @@ int attnres_qkv_rotary_backward(const attnres_qkv_rotary_desc* desc, const void*
  * Gated feed-forward projections (model.py:572-589): with weight [2 hidden, dim],
  * rows [0, hidden) up and [hidden, 2 hidden) gate, u = x up^T, z = x gate^T and
  *   h = u silu(z),  silu(z) = z / (1 + exp(-z)).
- * Products and activation in fp32, one rounding to the dtype.
+ * Products and activation in fp32.  h is rounded to the dtype once.  The backward
+ * forms the projections' gradient from u and z as the forward kept them (20 bits in
+ * bf16, 24 in fp16, all in fp32) and rounds it to the dtype, as the matrix cores take
+ * it, before the products that give dx and dweight, which are rounded once more.
  */
 typedef struct attnres_swiglu_desc {
   int32_t dtype;          /* ATTNRES_DTYPE_* */

@@ -2041,7 +2041,8 @@ def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
     Not in the reference's op module: the reference's MLP does this as a linear layer, a chunk, ``silu`` and a product
     (model.py:572-589).  Here the matrix-core kernel that forms both projections applies the activation and the product to
     the fp32 sums, with one rounding to the dtype; the backward forms the projections' gradient in one pass and multiplies
-    it by the weight and the input.
+    it by the weight and the input.  That gradient is rounded to the dtype, as the matrix cores take it, so that in 16 bits
+    dx and dweight carry two roundings.
 
     ``x`` [..., D]; ``weight`` [2 F, D], rows ``[0, F)`` up and ``[F, 2 F)`` gate (``nn.Linear(D, 2 F, bias=False).weight``
     with ``[up, gate] = fc1(x).chunk(2)``), taken in ``x``'s dtype; under autocast both are taken in the autocast dtype, as

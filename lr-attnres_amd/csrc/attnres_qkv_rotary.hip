@@ -17,8 +17,8 @@
 // head's sum of squares is log2(LANES) DPP or shuffle steps.
 //
 // Measured (bf16, one MI355X, 16384 tokens): 12 heads of 64, forward 23 us and backward 47-49
-// (4.4 and 4.1-4.3 TB/s of what each moves); 16 heads of 128, 55 and 99 us (4.9 and 5.4 TB/s; a
-// copy reaches 4.9).  With head groups given to waves in whole fours, the last wave of a token
+// (4.4 and 4.1-4.3 TB/s of what each moves); 16 heads of 128, 53 and 98 us (5.1 and 5.5 TB/s; a
+// non-temporal copy of 1 GiB reaches 6.5).  With head groups given to waves in whole fours, the last wave of a token
 // short of work, the backward of 12 heads of 64 took 50.
 #include "attnres_device.h"
 #include "attnres_launch.h"
@@ -185,7 +185,10 @@ __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_kernel(QkvRotaryP
 }
 
 // Any alignment and head width: one wave per head, its pairs in turn.  Two passes
-// over the row (the sums, then the pairs), the second from the caches.
+// over the row (the sums, then the pairs), the second from the caches.  Bound by its
+// accesses of single values: bf16, 16384 tokens, 4 heads of 512, 109 us forward and 241
+// backward (2.8 and 2.4 TB/s), 8 heads of 258, 163 and 314 (1.8), where the vector kernels take
+// 52 and 105 for 8 heads of 256.  Wider heads are not in use here, so they have no more.
 template <class DT, class TT, bool BWD>
 __global__ __launch_bounds__(kRotWaves* kWave) void qkv_rotary_general(QkvRotaryParams p) {
   using S = typename DT::S;

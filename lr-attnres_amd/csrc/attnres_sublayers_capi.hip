@@ -173,12 +173,14 @@ SwLayout sw_layout(const attnres_swiglu_desc* d) {
   return l;
 }
 
-// Tile and splits of a product with `steps` k steps: the least time in a model of a
-// launch, in us.  The CUs take workgroups in rounds, as many together as LDS holds;
+// Tile and splits of a product with `steps` k steps: the least cost in a model of a
+// launch.  The CUs take workgroups in rounds, as many together as LDS holds;
 // together they share the matrix cores.  A split product's sums are written and read
-// once more, by a second launch.  The constants are fitted to 1900 launches of these
+// once more, by a second launch.  The constants were fitted, in us, to 1900 launches of these
 // products before their last speed-up (24 shapes of 60 to 16384 tokens, every tile, 1 to 64
-// splits, fp32 and bf16).  Measured again since, 1422 launches of 63 products (100 to 16384
+// splits, fp32 and bf16).  They rank choices and are no times: the model has no term for what a
+// tile stores (16384 tokens, dim 1024, hidden 4096, bf16: 215 for a forward of 304 us) nor for the
+// single-value stores of odd widths.  Its choices, measured again since: 1422 launches of 63 products (100 to 16384
 // tokens; dx and dw with the activation's gradient before them): the model's choice is 1.3%
 // slower than the best one in the mean, 17% at most (dx of 100 tokens, dim 512, hidden 1024:
 // 13.3 us, 11.4 with 8 splits) and 8% otherwise.

@@ -40,7 +40,7 @@
 // life.  The clock falls to 1.55-1.8 GHz in these products, so power bounds dx and dw (in
 // the first milliseconds of such a load all three take up to a third longer).  The forward
 // is bound by what a tile does before and after its k steps (first loads 1.9 us, stores
-// 3.6, 7.7 with u and z) around 26 us of products.  Two workgroups of 128 x 256 on a CU
+// 3.6, 7.7 with u and z), in series with 26 us of products.  Two workgroups of 128 x 256 on a CU
 // took 340 us without u and z where 256 x 256 took 290.  On 32 x 32 MFMAs dx took 212 and
 // dw 218 where they then took 193 and 200.
 //

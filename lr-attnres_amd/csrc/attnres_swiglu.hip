@@ -22,7 +22,9 @@ constexpr int64_t kMaxGrid = (1 << 24) - 1;  // fewer than 2^32 threads
 
 // du = dh silu(z), dz = dh u silu'(z), silu'(z) = s + z s (1 - s), s = 1 / (1 + exp(-z)).
 // Both products of the backward read [du dz], each of them several times; it is
-// rounded to the dtype as they take it.  Bound by memory: 11 bytes a hidden value in
+// rounded to the dtype as they take it: in 16 bits dx and dweight are 1.4 times as far from the
+// 64-bit result (0.00235 of it by norm in bf16) as their own rounding (0.00166), and a chain that
+// rounds u, z, their activation and product too is at 0.0034.  Bound by memory: 11 bytes a hidden value in
 // bf16 (2 of dh, 5 of u and z, 4 of du and dz), 12 in fp16; 16384 tokens of hidden 4096, bf16, 738 MB:
 // 124-128 us, 5.8-6 TB/s.  A workgroup takes 16 tokens of four neighbouring blocks, so that every
 // array is read and written in whole lines.
