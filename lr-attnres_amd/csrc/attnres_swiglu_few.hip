@@ -21,20 +21,6 @@ namespace {
 
 constexpr int kCus = 256;
 
-typedef float few_f4 __attribute__((ext_vector_type(4)));
-
-template <class DT>
-__device__ __forceinline__ void few_mfma(const u32x4& a, const u32x4& b, few_f4& c) {
-  if constexpr (DT::kCode == 1) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sw_bf8, a), __builtin_bit_cast(sw_bf8, b), c, 0, 0, 0);
-  } else if constexpr (DT::kCode == 2) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sw_h8, a), __builtin_bit_cast(sw_h8, b), c, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-  }
-}
-
 // TT: tiles of 16 tokens; HT: MFMA tiles of 16 weight rows, for 8 HT hidden columns
 template <class DT, int TT, int HT>
 __global__ __launch_bounds__(256) void swiglu_few_kernel(SwGemmParams p) {
@@ -59,11 +45,11 @@ __global__ __launch_bounds__(256) void swiglu_few_kernel(SwGemmParams p) {
   const int steps = (p.K + E::kStep - 1) / E::kStep;
   const int per = (steps + 7) / 8 * 2;  // of a wave: whole pairs, 128 bytes of a row
   const int s0 = wave * per, s1 = min(s0 + per, steps);
-  few_f4 acc[TT][HT];
+  sw_f4 acc[TT][HT];
 #pragma unroll
   for (int t = 0; t < TT; ++t)
 #pragma unroll
-    for (int h = 0; h < HT; ++h) acc[t][h] = few_f4{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < HT; ++h) acc[t][h] = sw_f4{0.f, 0.f, 0.f, 0.f};
   for (int s = s0; s < s1; s += U) {
     u32x4 a[U][HT], b[U][TT];
 #pragma unroll
@@ -80,23 +66,23 @@ __global__ __launch_bounds__(256) void swiglu_few_kernel(SwGemmParams p) {
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int h = 0; h < HT; ++h) few_mfma<DT>(a[i][h], b[i][t], acc[t][h]);
+        for (int h = 0; h < HT; ++h) sw_mfma<DT>(a[i][h], b[i][t], acc[t][h]);
   }
   // lane: token r of a tile, rows 4 c .. 4 c + 3
 #pragma unroll
   for (int t = 0; t < TT; ++t)
 #pragma unroll
-    for (int h = 0; h < HT; ++h) *(few_f4*)&sums[wave][t][r][16 * h + 4 * c] = acc[t][h];
+    for (int h = 0; h < HT; ++h) *(sw_f4*)&sums[wave][t][r][16 * h + 4 * c] = acc[t][h];
   __syncthreads();
 
   // a thread: four hidden columns of one token
   const int tok = threadIdx.x / (2 * HT), q = threadIdx.x % (2 * HT), n0 = f0 + 4 * q;
   if (tok >= TT * 16 || tok >= p.M || n0 >= p.F) return;
-  few_f4 u = {0.f, 0.f, 0.f, 0.f}, z = u;
+  sw_f4 u = {0.f, 0.f, 0.f, 0.f}, z = u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    u += *(const few_f4*)&sums[i][tok >> 4][tok & 15][4 * q];
-    z += *(const few_f4*)&sums[i][tok >> 4][tok & 15][kHidden + 4 * q];
+    u += *(const sw_f4*)&sums[i][tok >> 4][tok & 15][4 * q];
+    z += *(const sw_f4*)&sums[i][tok >> 4][tok & 15][kHidden + 4 * q];
   }
   float h[4];
 #pragma unroll
@@ -118,8 +104,8 @@ __global__ __launch_bounds__(256) void swiglu_few_kernel(SwGemmParams p) {
   const SwPlaneAddress to = sw_planes<DT>(p.saved, p.n_tok, p.Fp);
   const int64_t at = ((int64_t)(n0 / E::kStep) * p.n_tok + tok) * E::kStep + n0 % E::kStep;
   if constexpr (P::kLow == 0) {
-    *(few_f4*)((float*)to.u + at) = u;
-    *(few_f4*)((float*)to.z + at) = z;
+    *(sw_f4*)((float*)to.u + at) = u;
+    *(sw_f4*)((float*)to.z + at) = z;
   } else {
     uint32_t uw[4], zw[4];
 #pragma unroll
