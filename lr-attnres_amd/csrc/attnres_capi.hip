@@ -61,16 +61,6 @@ inline void timer_end(hipStream_t st, bool began, hipError_t launch) {
   ++g_timer.n;
 }
 
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
 }  // namespace
 
 int attnres::api_fail(int code, const char* fmt, ...) {
@@ -84,6 +74,8 @@ int attnres::api_fail(int code, const char* fmt, ...) {
 }
 
 namespace {
+
+int (&fail)(int code, const char* fmt, ...) = attnres::api_fail;
 
 int elem_size(int dtype) { return dtype == ATTNRES_DTYPE_F32 ? 4 : 2; }
 
