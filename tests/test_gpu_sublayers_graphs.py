@@ -58,9 +58,9 @@ def test_replays_equal_the_eager_layer(attention):
     want = [step(layer, x, u) for x, u in zip(xs, ups)]
     # (the sample becomes the graphs' own input, which every call overwrites)
     graphed = torch.cuda.make_graphed_callables(layer, (rn().requires_grad_(True),), allow_unused_input=not attention)
-    for round in range(2):  # each graph replayed with eager work and the other inputs between
+    for turn in range(2):  # each graph replayed with eager work and the other inputs between
         for x, u, e in zip(xs, ups, want):
             got = step(graphed, x, u)
             torch.cuda.synchronize()
             same = [torch.equal(a, b) for a, b in zip(got, e)]
-            assert all(same), (round, same)
+            assert all(same), (turn, same)
