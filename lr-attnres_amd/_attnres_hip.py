@@ -31,6 +31,8 @@ PHASE_MAX_DIM = 4096
 SITE_LOGITS_MAX_QUERIES = 256
 SITE_LOGITS_MAX_RANK = 128
 QKV_ROTARY_MAX_HEAD_DIM = 1024
+CACHE_MAX_HEAD_DIM = 256
+CACHE_MAX_TOKENS = 1 << 30
 FLT_EPSILON = float(torch.finfo(torch.float32).eps)
 
 
@@ -242,6 +244,31 @@ class SwigluDesc(ctypes.Structure):
                 ("x_row_stride", c_int64), ("weight", c_void_p), ("weight_row_stride", c_int64)]
 
 
+class CacheDesc(ctypes.Structure):
+    """attnres_cache_desc (include/attnres_cache.h)."""
+    _fields_ = [("dtype", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32),
+                ("pages", c_int64), ("k", c_void_p), ("v", c_void_p), ("page_stride", c_int64),
+                ("head_stride", c_int64), ("slot_stride", c_int64), ("weights", c_void_p),
+                ("weight_page_stride", c_int64), ("weight_head_stride", c_int64), ("batch", c_int64),
+                ("block_table", c_void_p), ("table_stride", c_int64), ("table_pages", c_int64),
+                ("cached", c_void_p), ("fresh", c_void_p)]
+
+
+class CacheAppendDesc(ctypes.Structure):
+    """attnres_cache_append_desc (include/attnres_cache.h)."""
+    _fields_ = [("tokens", c_int64), ("q_heads", c_int32), ("qk_norm", c_int32), ("norm_eps", c_float),
+                ("table_dtype", c_int32), ("qkv", c_void_p), ("batch_stride", c_int64), ("token_stride", c_int64),
+                ("sin", c_void_p), ("cos", c_void_p), ("table_rows", c_int64), ("table_row_stride", c_int64),
+                ("positions", c_void_p)]
+
+
+class CacheAttendDesc(ctypes.Structure):
+    """attnres_cache_attend_desc (include/attnres_cache.h)."""
+    _fields_ = [("tokens", c_int64), ("q_heads", c_int32), ("scale", c_float), ("q", c_void_p),
+                ("q_batch_stride", c_int64), ("q_head_stride", c_int64), ("q_token_stride", c_int64),
+                ("decay", c_float)]
+
+
 def load() -> ctypes.CDLL:
     """Load the HIP library once; raise with a build hint if it is missing."""
     global _lib
@@ -357,6 +384,16 @@ def load() -> ctypes.CDLL:
                                             c_void_p, c_size_t, c_void_p]
     lib.attnres_kernel_timing.restype = c_int
     lib.attnres_kernel_timing.argtypes = [c_int]
+    lib.attnres_cache_append.restype = c_int
+    lib.attnres_cache_append.argtypes = [POINTER(CacheDesc), POINTER(CacheAppendDesc), c_void_p, c_void_p, c_void_p]
+    lib.attnres_cache_attend_workspace_size.restype = c_size_t
+    lib.attnres_cache_attend_workspace_size.argtypes = [POINTER(CacheDesc), POINTER(CacheAttendDesc)]
+    lib.attnres_cache_attend.restype = c_int
+    lib.attnres_cache_attend.argtypes = [POINTER(CacheDesc), POINTER(CacheAttendDesc), c_void_p, c_void_p, c_size_t,
+                                         c_void_p]
+    lib.attnres_cache_evict.restype = c_int
+    lib.attnres_cache_evict.argtypes = [POINTER(CacheDesc), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                        c_void_p]
     lib.attnres_test_phase2_block_layout.restype = c_int
     lib.attnres_test_phase2_block_layout.argtypes = [c_int]
     lib.attnres_kernel_times.restype = c_int
@@ -1233,3 +1270,68 @@ def swiglu_backward(x, weight, saved, grad_h, want_dx: bool, want_dweight: bool)
                                        _ptr(saved), _ptr(dx), _ptr(dw), _ptr(ws), n, _stream(x.device)),
            "swiglu backward")
     return dx, dw
+
+
+# ------------------------------------------------------------------ the paged key-value cache
+
+def cache_desc(k_pages, v_pages, weights, block_table, cached, fresh) -> CacheDesc:
+    """k_pages, v_pages [P, K, S, Dh] of the same strides and weights [P, K, S] or None, contiguous last dims; block_table
+    [B, M] with contiguous rows, cached and fresh [B] dense (or fresh None), all int32."""
+    d = CacheDesc()
+    d.dtype = DTYPE_CODE[k_pages.dtype]
+    d.pages, d.kv_heads, d.page_size, d.head_dim = k_pages.shape
+    d.k, d.v = k_pages.data_ptr(), v_pages.data_ptr()
+    # (a dimension of one is never stepped over: its stride may be anything)
+    d.page_stride, d.head_stride, d.slot_stride = (k_pages.stride(i) if k_pages.size(i) > 1 else 0 for i in range(3))
+    if weights is not None:
+        d.weights = weights.data_ptr()
+        d.weight_page_stride, d.weight_head_stride = (weights.stride(i) if weights.size(i) > 1 else 0 for i in range(2))
+    d.batch, d.table_pages = block_table.shape
+    d.block_table, d.table_stride = block_table.data_ptr(), block_table.stride(0) if block_table.size(0) > 1 else 0
+    d.cached, d.fresh = cached.data_ptr(), None if fresh is None else fresh.data_ptr()
+    return d
+
+
+def cache_append(qkv, sin, cos, k_pages, v_pages, weights, block_table, cached, fresh, positions, q_heads, qk_norm, heads):
+    """(q [B, q_heads, T, Dh], k [B, K, T, Dh] or None)"""
+    c = cache_desc(k_pages, v_pages, weights, block_table, cached, fresh)
+    B, T, _ = qkv.shape
+    d = CacheAppendDesc()
+    d.tokens, d.q_heads, d.qk_norm, d.norm_eps = T, q_heads, int(qk_norm), FLT_EPSILON
+    d.table_dtype = DTYPE_CODE[sin.dtype]
+    d.qkv = qkv.data_ptr()
+    d.batch_stride, d.token_stride = qkv.stride(0) if B > 1 else 0, qkv.stride(1) if T > 1 else 0
+    d.sin, d.cos = sin.data_ptr(), cos.data_ptr()
+    d.table_rows, d.table_row_stride = sin.size(0), sin.stride(0) if sin.size(0) > 1 else sin.size(1)
+    d.positions = None if positions is None else positions.data_ptr()
+    q = qkv.new_empty((B, q_heads, T, c.head_dim))
+    k = qkv.new_empty((B, c.kv_heads, T, c.head_dim)) if heads else None
+    _check(load().attnres_cache_append(ctypes.byref(c), ctypes.byref(d), _ptr(q), _ptr(k), _stream(qkv.device)),
+           "cache append")
+    return q, k
+
+
+def cache_attend(q, k_pages, v_pages, weights, block_table, cached, fresh, scale, decay):
+    """[B, T, H, Dh] from q [B, H, T, Dh] with a contiguous last dim"""
+    lib, c = load(), cache_desc(k_pages, v_pages, weights, block_table, cached, fresh)
+    B, H, T, Dh = q.shape
+    d = CacheAttendDesc()
+    d.tokens, d.q_heads, d.scale, d.decay = T, H, scale, decay
+    d.q = q.data_ptr()
+    d.q_batch_stride, d.q_head_stride, d.q_token_stride = (q.stride(i) if q.size(i) > 1 else 0 for i in range(3))
+    out = q.new_empty((B, T, H, Dh))
+    n = lib.attnres_cache_attend_workspace_size(ctypes.byref(c), ctypes.byref(d))
+    ws = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
+    _check(lib.attnres_cache_attend(ctypes.byref(c), ctypes.byref(d), _ptr(out), _ptr(ws), n, _stream(q.device)),
+           "cache attend")
+    return out
+
+
+def cache_evict(k_pages, v_pages, weights, block_table, cached, new_table, budget, recent):
+    """(kept [B, K, budget], left [B]), int32; new_table [B, M'] int32 with contiguous rows"""
+    c = cache_desc(k_pages, v_pages, weights, block_table, cached, None)
+    kept = torch.empty((c.batch, c.kv_heads, budget), dtype=torch.int32, device=k_pages.device)
+    left = torch.empty((c.batch,), dtype=torch.int32, device=k_pages.device)
+    _check(load().attnres_cache_evict(ctypes.byref(c), _ptr(new_table), new_table.stride(0), budget, recent, _ptr(kept),
+                                      _ptr(left), _stream(k_pages.device)), "cache evict")
+    return kept, left

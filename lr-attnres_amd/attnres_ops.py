@@ -341,7 +341,8 @@ _NATIVE = None
 _BOUND = {name: getattr(_hip, name) for name in (
     "forward", "backward", "phase1_forward", "phase1_backward_sites", "phase1_bank_forward", "phase1_bank_backward",
     "phase2_forward", "phase2_backward", "accum_read_forward", "accum_read_backward", "block_accum_forward",
-    "block_accum_backward", "qkv_rotary_forward", "qkv_rotary_backward", "swiglu_forward", "swiglu_backward")}
+    "block_accum_backward", "qkv_rotary_forward", "qkv_rotary_backward", "swiglu_forward", "swiglu_backward",
+    "cache_append", "cache_attend", "cache_evict")}
 
 
 def _native(fwd: str, bwd: str):
@@ -2071,3 +2072,254 @@ def swiglu_projection(x: Tensor, weight: Tensor) -> Tensor:
     save = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
     h, _ = _swiglu_op(rows, w, save)
     return h.view(*x.shape[:-1], w.size(0) // 2)
+
+
+# ------------------------------------------------------------------ the paged key-value cache
+
+@torch.library.custom_op("attnres_hip::cache_append", mutates_args=("k_pages", "v_pages", "weights"))
+def _cache_append_op(qkv: Tensor, sin: Tensor, cos: Tensor, k_pages: Tensor, v_pages: Tensor, weights: Optional[Tensor],
+                     block_table: Tensor, cached: Tensor, fresh: Optional[Tensor], positions: Optional[Tensor],
+                     q_heads: int, qk_norm: bool, heads: bool) -> tuple[Tensor, Tensor]:
+    with _device_ctx(qkv.device):
+        q, k = _hip.cache_append(qkv, sin, cos, k_pages, v_pages, weights, block_table, cached, fresh, positions, q_heads,
+                                 qk_norm, heads)
+    return q, k if k is not None else qkv.new_empty((0,))
+
+
+@_cache_append_op.register_fake
+def _cache_append_fake(qkv, sin, cos, k_pages, v_pages, weights, block_table, cached, fresh, positions, q_heads, qk_norm,
+                       heads):
+    B, T, _ = qkv.shape
+    K, Dh = k_pages.size(1), k_pages.size(3)
+    return qkv.new_empty((B, q_heads, T, Dh)), qkv.new_empty((B, K, T, Dh) if heads else (0,))
+
+
+@torch.library.custom_op("attnres_hip::cache_attend", mutates_args=("weights",))
+def _cache_attend_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, weights: Optional[Tensor], block_table: Tensor,
+                     cached: Tensor, fresh: Optional[Tensor], scale: float, decay: float) -> Tensor:
+    with _device_ctx(q.device):
+        return _hip.cache_attend(q, k_pages, v_pages, weights, block_table, cached, fresh, scale, decay)
+
+
+@_cache_attend_op.register_fake
+def _cache_attend_fake(q, k_pages, v_pages, weights, block_table, cached, fresh, scale, decay):
+    B, H, T, Dh = q.shape
+    return q.new_empty((B, T, H, Dh))
+
+
+@torch.library.custom_op("attnres_hip::cache_evict", mutates_args=("k_pages", "v_pages", "weights"))
+def _cache_evict_op(k_pages: Tensor, v_pages: Tensor, weights: Tensor, block_table: Tensor, cached: Tensor,
+                    new_table: Tensor, budget: int, recent: int) -> tuple[Tensor, Tensor]:
+    with _device_ctx(k_pages.device):
+        return _hip.cache_evict(k_pages, v_pages, weights, block_table, cached, new_table, budget, recent)
+
+
+@_cache_evict_op.register_fake
+def _cache_evict_fake(k_pages, v_pages, weights, block_table, cached, new_table, budget, recent):
+    B, K = block_table.size(0), k_pages.size(1)
+    return cached.new_empty((B, K, budget)), cached.new_empty((B,))
+
+
+def _int32(t: Tensor) -> Tensor:
+    """An integer tensor in int32; what it cannot hold becomes a value that no page, count or row has."""
+    if t.dtype == torch.int32:
+        return t
+    return (t.clamp(-1, 2 ** 31 - 1) if t.dtype == torch.int64 else t).to(torch.int32)
+
+
+def _cache_ints(what: str, name: str, t: Tensor, shape: tuple) -> Tensor:
+    if t.dtype not in _POSITION_TYPES:
+        raise RuntimeError(f"{what}: {name} must be integers, got {t.dtype}")
+    if t.shape != shape:
+        raise RuntimeError(f"{what}: {name} must be {list(shape)}, got {tuple(t.shape)}")
+    return _int32(t).contiguous()
+
+
+def _no_grad_needed(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
+
+
+def _cache_args(what: str, like: Tensor, k_pages: Tensor, v_pages: Tensor, weights: Optional[Tensor], block_table: Tensor,
+                cached: Tensor, fresh: Optional[Tensor], batch: int, writes: bool):
+    """Checks a cache; returns its integer tensors in int32."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise RuntimeError(f"{what}: k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] of one shape, got "
+                           f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    P, K, S, Dh = k_pages.shape
+    if K < 1 or S < 1 or Dh < 1:
+        raise RuntimeError(f"{what}: pages of shape {tuple(k_pages.shape)} hold no token")
+    if k_pages.dtype not in _ALLOWED:
+        raise RuntimeError(f"{what}: dtype {k_pages.dtype} is not supported (fp32, bf16, fp16)")
+    if v_pages.dtype != k_pages.dtype or like.dtype != k_pages.dtype:
+        raise RuntimeError(f"{what}: keys {k_pages.dtype}, values {v_pages.dtype} and {like.dtype} must be of one dtype")
+    if Dh > _hip.CACHE_MAX_HEAD_DIM:
+        raise RuntimeError(f"{what}: head width {Dh} above {_hip.CACHE_MAX_HEAD_DIM}")
+    if (Dh > 1 and k_pages.stride(3) != 1) or any(k_pages.stride(i) != v_pages.stride(i)
+                                                  for i in range(4) if k_pages.size(i) > 1):
+        raise RuntimeError(f"{what}: k_pages and v_pages must have the same strides and a contiguous last dimension, got "
+                           f"{k_pages.stride()} and {v_pages.stride()}")
+    if weights is not None:
+        if weights.shape != (P, K, S) or weights.dtype != torch.float32 or (S > 1 and weights.stride(2) != 1):
+            raise RuntimeError(f"{what}: weights must be fp32 [{P}, {K}, {S}] with a contiguous last dimension, got "
+                               f"{weights.dtype} {tuple(weights.shape)}")
+    for t in (*((k_pages, v_pages) if writes else ()), weights):
+        if t is not None and any(t.size(i) > 1 and t.stride(i) == 0 for i in range(t.dim())):
+            raise RuntimeError(f"{what}: pages that are written must not overlap themselves (stride 0)")
+    if block_table.dim() != 2 or block_table.size(0) != batch:
+        raise RuntimeError(f"{what}: block_table must be [{batch}, pages of a sequence], got {tuple(block_table.shape)}")
+    if block_table.dtype not in _POSITION_TYPES:
+        raise RuntimeError(f"{what}: block_table must be integers, got {block_table.dtype}")
+    if block_table.size(1) * S > _hip.CACHE_MAX_TOKENS:
+        raise RuntimeError(f"{what}: a block table of {block_table.size(1)} pages of {S} is above "
+                           f"{_hip.CACHE_MAX_TOKENS} tokens")
+    given = [t for t in (v_pages, weights, block_table, cached, fresh) if t is not None]
+    _check_gpu([like, k_pages, *given], what)
+    table = _int32(block_table)
+    if table.size(1) > 1 and table.stride(1) != 1:
+        table = table.contiguous()
+    return (table, _cache_ints(what, "cached", cached, (batch,)),
+            None if fresh is None else _cache_ints(what, "fresh", fresh, (batch,)))
+
+
+def qkv_norm_rotary_cached(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor, k_pages: Tensor, v_pages: Tensor,
+                           block_table: Tensor, cached: Tensor, fresh: Optional[Tensor] = None,
+                           positions: Optional[Tensor] = None, qk_norm: bool = True, weights: Optional[Tensor] = None,
+                           return_heads: bool = False):
+    """Attention's heads of new tokens from their fused projection, keys and values written into a paged cache, in one pass.
+
+    Not in the reference's op module: its attention norms and rotates the new tokens' heads and concatenates them to a cache
+    tensor (model.py:430-569).  The arithmetic is ``qkv_norm_rotary``'s.
+
+    ``qkv`` [B, T, (num_heads + 2 K) Dh].  ``k_pages``, ``v_pages`` [P, K, S, Dh]: pages of S tokens, of the same strides
+    (a layer's part of a larger tensor, or a permuted one); ``block_table`` [B, M]: the pages of each sequence, in order;
+    ``cached`` [B]: the tokens it has already.  Token t of sequence b goes to slot ``(cached[b] + t) % S`` of page
+    ``block_table[b, (cached[b] + t) // S]`` and is rotated by row ``positions[b] + t`` of ``sin`` and ``cos`` (``positions``
+    [B]; ``cached`` unless given: a cache that tokens were taken from has fewer than the sequence).  ``fresh`` [B]: how many of
+    the T tokens are the sequence's, in a padded batch; the others are not written and have zeros for queries and keys.
+    ``weights`` [P, K, S] (fp32): what each cached token received of attention so far, 0 for the new ones.
+
+    A token that has no slot, or whose page is not in [0, P), is not written; a row outside the tables gives NaN (the values
+    of device tensors are not looked at on the host).  A page that is written to belongs to one sequence.
+
+    Returns ``q`` [B, num_heads, T, Dh], dense; with ``return_heads`` also ``k`` [B, K, T, Dh], dense, and ``v`` [B, K, T, Dh],
+    a view of ``qkv``: what attention inside a prompt reads.  No backward.
+    """
+    what = "qkv_norm_rotary_cached"
+    H = int(num_heads)
+    nat = _native("cache_append", "cache_append")
+    if nat:
+        out = nat.cache_append(qkv, H, sin, cos, k_pages, v_pages, block_table, cached, fresh, positions, bool(qk_norm),
+                               weights, bool(return_heads))
+        if out is not None:
+            return out
+    _no_grad_needed(what, qkv, sin, cos, k_pages, v_pages, weights)
+    if qkv.dim() != 3:
+        raise RuntimeError(f"{what}: qkv must be [B, T, heads * head_dim], got {tuple(qkv.shape)}")
+    B, T, C = qkv.shape
+    table, cached, fresh = _cache_args(what, qkv, k_pages, v_pages, weights, block_table, cached, fresh, B, True)
+    K, Dh = k_pages.size(1), k_pages.size(3)
+    if H < 1 or Dh % 2 != 0 or C != (H + 2 * K) * Dh:
+        raise RuntimeError(f"{what}: {C} columns are not {H} + 2 * {K} heads of an even width {Dh}")
+    for name, t in (("sin", sin), ("cos", cos)):
+        if t.dim() < 2 or t.size(-1) != Dh // 2 or t.numel() != t.size(-2) * t.size(-1) or t.numel() < 1:
+            raise RuntimeError(f"{what}: {name} must be [rows, {Dh // 2}] (and leading ones), got {tuple(t.shape)}")
+        if not t.is_floating_point():
+            raise RuntimeError(f"{what}: {name} must be a floating-point table, got {t.dtype}")
+    if sin.shape != cos.shape:
+        raise RuntimeError(f"{what}: sin {tuple(sin.shape)} and cos {tuple(cos.shape)} differ in shape")
+    _check_gpu([qkv, sin, cos, *(() if positions is None else (positions,))], what)
+    rot = qkv.dtype if sin.dtype == cos.dtype == qkv.dtype else torch.float32
+    sin, cos = (t.to(rot).reshape(-1, Dh // 2).contiguous() for t in (sin, cos))
+    if positions is not None:
+        positions = _cache_ints(what, "positions", positions, (B,))
+    qkv = _last_dense(qkv)
+    q, k = _cache_append_op(qkv, sin, cos, k_pages, v_pages, weights, table, cached, fresh, positions, H, bool(qk_norm),
+                            bool(return_heads))
+    if not return_heads:
+        return q
+    return q, k, qkv[..., (H + K) * Dh:].view(B, T, K, Dh).transpose(1, 2)
+
+
+def cached_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor, cached: Tensor,
+                     fresh: Optional[Tensor] = None, scale: Optional[float] = None, weights: Optional[Tensor] = None,
+                     decay: float = 1.0) -> Tensor:
+    """Attention of the newest tokens over a paged key-value cache that holds them already.
+
+    Not in the reference's op module: its attention runs ``scaled_dot_product_attention`` over the concatenated cache
+    (model.py:430-569).
+
+    ``q`` [B, H, T, Dh]; the cache's arguments as ``qkv_norm_rotary_cached`` takes them, with the same ``cached`` and ``fresh``
+    (the counts before these T tokens; how many of them are the sequence's).  Query t of sequence b reads the tokens up to its
+    own, ``j < cached[b] + t + 1``, through key / value head ``h // (H // K)``: softmax of ``scale <q, k_j>`` (``Dh ** -0.5``
+    unless given), in fp32, one rounding to the dtype.  Made for one or a few tokens: each sixteen query rows of a key / value
+    head (heads of its group times tokens) read the cache once.
+
+    ``weights`` [P, K, S] (fp32, T = 1): becomes ``decay * weights`` plus the softmax weights of the head's queries, summed,
+    for every token that was read; with ``decay`` 0 what was there is not read.  ``evict_cached_tokens`` goes by it.
+
+    A query that its sequence does not have, or that sees no token (``cached[b] = -1`` of T = 1 is refused, as any negative
+    count), gives zeros; a page not in [0, P), a negative count or tokens beyond the table give NaN in that sequence.  Returns
+    [B, H, T, Dh], a view of a dense [B, T, H, Dh].  No backward.
+    """
+    what = "cached_attention"
+    nat = _native("cache_attend", "cache_attend")
+    if nat:
+        out = nat.cache_attend(q, k_pages, v_pages, block_table, cached, fresh, scale, weights, decay)
+        if out is not None:
+            return out
+    _no_grad_needed(what, q, k_pages, v_pages, weights)
+    if q.dim() != 4:
+        raise RuntimeError(f"{what}: q must be [B, heads, T, head_dim], got {tuple(q.shape)}")
+    B, H, T, Dh = q.shape
+    table, cached, fresh = _cache_args(what, q, k_pages, v_pages, weights, block_table, cached, fresh, B, False)
+    K = k_pages.size(1)
+    if Dh != k_pages.size(3) or H < 1 or H % K != 0:
+        raise RuntimeError(f"{what}: {H} query heads of {Dh} do not share {K} key / value heads of {k_pages.size(3)}")
+    if weights is not None and T > 1:
+        raise RuntimeError(f"{what}: weights are kept for a single new token, got {T}")
+    if not 0.0 <= decay <= 1.0:
+        raise RuntimeError(f"{what}: decay must be 0 .. 1, got {decay}")
+    scale = Dh ** -0.5 if scale is None else float(scale)
+    if not -3.4e38 < scale < 3.4e38:
+        raise RuntimeError(f"{what}: scale must be finite, got {scale}")
+    return _cache_attend_op(_last_dense(q), k_pages, v_pages, weights, table, cached, fresh, scale, float(decay)).transpose(1, 2)
+
+
+def evict_cached_tokens(k_pages: Tensor, v_pages: Tensor, weights: Tensor, block_table: Tensor, cached: Tensor,
+                        new_table: Tensor, budget: int, recent: int = 0):
+    """A paged cache brought back to ``budget`` tokens a sequence: of each key / value head the last ``recent`` tokens and, of
+    the others, those that received most attention.
+
+    Not in the reference.  The cache's arguments as ``cached_attention`` takes them, ``weights`` the sums it has added up.
+    A sequence of more than ``budget`` tokens keeps that many of them, each head its own: the last ``recent`` and the
+    ``budget - recent`` of the largest weights (equal ones: the earlier token; NaN: below every number).  They are copied in
+    their order, with keys, values and weights, into the pages ``new_table`` [B, M'] (``M' * S >= budget``).  Those pages hold
+    no token of any sequence of the call; only a sequence within its budget may name its own pages again, in their order, and is
+    then left as it is.  The old pages are not changed.
+
+    Returns ``kept`` [B, K, budget] (int32), the kept tokens' places in the old order, -1 behind the last, and ``left`` [B]
+    (int32), the tokens that each sequence has now: the next ``cached``.  Rotated keys keep their positions, so later calls
+    give ``qkv_norm_rotary_cached`` the sequence's own ``positions``.
+    """
+    what = "evict_cached_tokens"
+    budget, recent = int(budget), int(recent)
+    nat = _native("cache_evict", "cache_evict")
+    if nat:
+        out = nat.cache_evict(k_pages, v_pages, weights, block_table, cached, new_table, budget, recent)
+        if out is not None:
+            return out
+    _no_grad_needed(what, k_pages, v_pages, weights)
+    if weights is None:
+        raise RuntimeError(f"{what}: weights are what the choice goes by: None given")
+    B = block_table.size(0) if block_table.dim() == 2 else 0
+    table, cached, _ = _cache_args(what, k_pages, k_pages, v_pages, weights, block_table, cached, None, B, True)
+    if budget < 1 or not 0 <= recent <= budget:
+        raise RuntimeError(f"{what}: budget {budget} and recent {recent} must be budget >= 1 and 0 <= recent <= budget")
+    if new_table.dim() != 2 or new_table.size(0) != B or new_table.size(1) * k_pages.size(2) < budget:
+        raise RuntimeError(f"{what}: new_table must be [{B}, pages for {budget} tokens], got {tuple(new_table.shape)}")
+    if new_table.dtype not in _POSITION_TYPES:
+        raise RuntimeError(f"{what}: new_table must be integers, got {new_table.dtype}")
+    _check_gpu([k_pages, new_table], what)
+    new = _int32(new_table).contiguous()
+    return _cache_evict_op(k_pages, v_pages, weights, table, cached, new, budget, recent)

@@ -1,0 +1,87 @@
+// Internal interface of the paged cache's kernels (attnres_cache_*.hip) and their
+// C ABI (attnres_cache_capi.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace attnres {
+
+// records the message that attnres_last_error() returns and gives back `code`
+int api_fail(int code, const char* fmt, ...);
+
+struct CachePages {  // attnres_cache_desc
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, slot_stride;
+  float* w;
+  int64_t w_page_stride, w_head_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* cached;
+  const int32_t* fresh;
+  int32_t batch, kv_heads, head_dim, page_size, pages;
+  int32_t room;  // tokens that a row of the table has pages for
+};
+
+struct CacheAppendParams {
+  CachePages c;
+  const void* qkv;
+  int64_t b_stride, t_stride;
+  int64_t n_tok, tokens;  // batch * tokens
+  int32_t q_heads, qk_norm;
+  float eps;
+  const void* sin;
+  const void* cos;
+  int64_t table_rows, table_stride;
+  const int32_t* pos;
+  void* q;
+  void* k;  // or null
+};
+
+// vec, lanes: as launch_qkv_rotary's
+hipError_t launch_cache_append(int dtype, bool f32_table, const CacheAppendParams& p, int vec, int lanes, hipStream_t st);
+
+struct CacheAttendParams {
+  CachePages c;
+  const void* q;
+  int64_t q_b_stride, q_h_stride, q_t_stride;
+  int32_t tokens, q_heads;
+  float scale;  // of base-2 logarithms: the softmax's scale times log2(e)
+  float decay;
+  void* out;
+  float* lse;  // [batch, q_heads], with weights
+};
+
+hipError_t launch_cache_attend(int dtype, const CacheAttendParams& p, hipStream_t st);
+
+struct CacheEvictParams {
+  CachePages c;
+  const int32_t* new_table;
+  int64_t new_stride;
+  int32_t budget, recent;
+  int32_t* kept;
+  int32_t* left;
+  int32_t es;   // bytes of a value
+  int32_t vec;  // rows in whole vectors of 16 bytes
+};
+
+hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st);
+
+#ifdef __HIP__
+
+// tokens in the cache before the call: 0 .. room, or -1 for a count that the table has no room for
+__device__ __forceinline__ int cache_count(const CachePages& c, int b) {
+  const int n = c.cached[b];
+  return n >= 0 && n <= c.room ? n : -1;
+}
+
+// page of token j of sequence b, -1: outside the cache
+__device__ __forceinline__ int cache_page(const CachePages& c, int b, int j) {
+  const int page = c.table[b * c.table_stride + j / c.page_size];
+  return (unsigned)page < (unsigned)c.pages ? page : -1;
+}
+
+#endif
+
+}  // namespace attnres

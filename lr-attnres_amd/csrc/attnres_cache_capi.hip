@@ -1,0 +1,211 @@
+// C ABI of the paged cache's kernels: argument checks and kernel selection.
+// Declared in include/attnres_cache.h.
+#include <math.h>
+#include <string.h>
+
+#include "../../include/attnres_cache.h"
+#include "attnres_cache.h"
+
+using namespace attnres;
+
+namespace {
+
+int es_of(int dtype) { return dtype == ATTNRES_DTYPE_F32 ? 4 : 2; }
+bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+
+// the cache itself; what the calls write and read through it is checked by each
+int check_cache(const attnres_cache_desc* c) {
+  if (!c) return api_fail(ATTNRES_EINVAL, "cache is NULL");
+  if (c->dtype != ATTNRES_DTYPE_F32 && c->dtype != ATTNRES_DTYPE_BF16 && c->dtype != ATTNRES_DTYPE_F16)
+    return api_fail(ATTNRES_EINVAL, "unknown dtype %d", c->dtype);
+  if (c->kv_heads < 1 || c->kv_heads > (1 << 20)) return api_fail(ATTNRES_EINVAL, "kv_heads=%d must be >= 1", c->kv_heads);
+  if (c->head_dim < 1) return api_fail(ATTNRES_EINVAL, "head_dim=%d must be >= 1", c->head_dim);
+  if (c->head_dim > ATTNRES_CACHE_MAX_HEAD_DIM)
+    return api_fail(ATTNRES_EUNSUPPORTED, "head_dim=%d above %d", c->head_dim, ATTNRES_CACHE_MAX_HEAD_DIM);
+  if (c->page_size < 1) return api_fail(ATTNRES_EINVAL, "page_size=%d must be >= 1", c->page_size);
+  if (c->batch < 0 || c->batch > (1 << 20)) return api_fail(ATTNRES_EINVAL, "batch=%lld", (long long)c->batch);
+  if (c->pages < 0 || c->pages > INT32_MAX) return api_fail(ATTNRES_EINVAL, "pages=%lld", (long long)c->pages);
+  if (c->table_pages < 0) return api_fail(ATTNRES_EINVAL, "table_pages=%lld < 0", (long long)c->table_pages);
+  if (c->table_pages > ATTNRES_CACHE_MAX_TOKENS / c->page_size)
+    return api_fail(ATTNRES_EUNSUPPORTED, "table_pages=%lld of %d tokens: above %d tokens a sequence",
+                    (long long)c->table_pages, c->page_size, ATTNRES_CACHE_MAX_TOKENS);
+  if (c->batch == 0) return ATTNRES_OK;
+  if (!c->cached || (c->table_pages > 0 && !c->block_table)) return api_fail(ATTNRES_EINVAL, "block_table / cached is NULL");
+  if (c->table_stride < 0) return api_fail(ATTNRES_EINVAL, "table_stride < 0");
+  if (c->pages > 0 && (!c->k || !c->v)) return api_fail(ATTNRES_EINVAL, "k / v is NULL");
+  if (c->page_stride < 0 || c->head_stride < 0 || c->slot_stride < 0)
+    return api_fail(ATTNRES_EINVAL, "page, head and slot strides must be >= 0");
+  if (c->weights && (c->weight_page_stride < 0 || c->weight_head_stride < 0))
+    return api_fail(ATTNRES_EINVAL, "weight strides must be >= 0");
+  return ATTNRES_OK;
+}
+
+CachePages pages_of(const attnres_cache_desc* c) {
+  CachePages p{};
+  p.k = c->k;
+  p.v = c->v;
+  p.page_stride = c->page_stride;
+  p.head_stride = c->head_stride;
+  p.slot_stride = c->slot_stride;
+  p.w = c->weights;
+  p.w_page_stride = c->weight_page_stride;
+  p.w_head_stride = c->weight_head_stride;
+  p.table = c->block_table;
+  p.table_stride = c->table_stride;
+  p.cached = c->cached;
+  p.fresh = c->fresh;
+  p.batch = (int32_t)c->batch;
+  p.kv_heads = c->kv_heads;
+  p.head_dim = c->head_dim;
+  p.page_size = c->page_size;
+  p.pages = (int32_t)c->pages;
+  p.room = (int32_t)(c->table_pages * c->page_size);
+  return p;
+}
+
+// whether every row of the pages starts at a multiple of `per` values
+bool rows_at(const attnres_cache_desc* c, int per) {
+  const int bytes = per * es_of(c->dtype);
+  return c->head_dim % per == 0 && aligned(c->k, bytes) && aligned(c->v, bytes) && c->page_stride % per == 0 &&
+         c->head_stride % per == 0 && c->slot_stride % per == 0;
+}
+
+int check_append(const attnres_cache_desc* c, const attnres_cache_append_desc* d) {
+  if (int rc = check_cache(c)) return rc;
+  if (!d) return api_fail(ATTNRES_EINVAL, "desc is NULL");
+  if (d->table_dtype != ATTNRES_DTYPE_F32 && d->table_dtype != c->dtype)
+    return api_fail(ATTNRES_EINVAL, "table dtype %d is neither fp32 nor the cache's %d", d->table_dtype, c->dtype);
+  if (d->tokens < 0 || d->tokens > (int64_t)1 << 30)
+    return api_fail(ATTNRES_EINVAL, "tokens=%lld must be 0 .. 2^30", (long long)d->tokens);
+  if (d->q_heads < 1 || d->q_heads > (1 << 20)) return api_fail(ATTNRES_EINVAL, "q_heads=%d must be >= 1", d->q_heads);
+  if (c->head_dim % 2) return api_fail(ATTNRES_EINVAL, "head_dim=%d must be even", c->head_dim);
+  if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (c->batch * d->tokens > (int64_t)1 << 36) return api_fail(ATTNRES_EUNSUPPORTED, "too many tokens");
+  if (!d->qkv || !d->sin || !d->cos) return api_fail(ATTNRES_EINVAL, "qkv / sin / cos is NULL");
+  if (d->batch_stride < 0 || d->token_stride < 0)
+    return api_fail(ATTNRES_EINVAL, "batch_stride and token_stride must be >= 0");
+  if (d->table_rows < 1) return api_fail(ATTNRES_EINVAL, "table_rows=%lld < 1", (long long)d->table_rows);
+  if (d->table_row_stride < c->head_dim / 2)
+    return api_fail(ATTNRES_EINVAL, "table_row_stride=%lld below head_dim / 2 = %d", (long long)d->table_row_stride,
+                    c->head_dim / 2);
+  return ATTNRES_OK;
+}
+
+int check_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d) {
+  if (int rc = check_cache(c)) return rc;
+  if (!d) return api_fail(ATTNRES_EINVAL, "desc is NULL");
+  if (d->tokens < 0 || d->tokens > ATTNRES_CACHE_MAX_TOKENS)
+    return api_fail(ATTNRES_EINVAL, "tokens=%lld must be 0 .. 2^30", (long long)d->tokens);
+  if (d->q_heads < 1 || d->q_heads > (1 << 20) || d->q_heads % c->kv_heads)
+    return api_fail(ATTNRES_EINVAL, "q_heads=%d must be a multiple of kv_heads=%d", d->q_heads, c->kv_heads);
+  if (!isfinite(d->scale)) return api_fail(ATTNRES_EINVAL, "scale must be finite");
+  if (c->weights && d->tokens > 1) return api_fail(ATTNRES_EINVAL, "weights need a single new token, got %lld", (long long)d->tokens);
+  if (c->weights && !(d->decay >= 0.f && d->decay <= 1.f)) return api_fail(ATTNRES_EINVAL, "decay must be 0 .. 1");
+  if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (c->batch * d->tokens > (1 << 23) / d->q_heads)
+    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d: too many queries", (long long)c->batch,
+                    (long long)d->tokens, d->q_heads);
+  if (!d->q) return api_fail(ATTNRES_EINVAL, "q is NULL");
+  if (d->q_batch_stride < 0 || d->q_head_stride < 0 || d->q_token_stride < 0)
+    return api_fail(ATTNRES_EINVAL, "q strides must be >= 0");
+  return ATTNRES_OK;
+}
+
+}  // namespace
+
+extern "C" int attnres_cache_append(const attnres_cache_desc* c, const attnres_cache_append_desc* d, void* q, void* k,
+                                    void* stream) {
+  if (int rc = check_append(c, d)) return rc;
+  if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (!q) return api_fail(ATTNRES_EINVAL, "q is NULL");
+  CacheAppendParams p{};
+  p.c = pages_of(c);
+  p.qkv = d->qkv;
+  p.b_stride = d->batch_stride;
+  p.t_stride = d->token_stride;
+  p.n_tok = c->batch * d->tokens;
+  p.tokens = d->tokens;
+  p.q_heads = d->q_heads;
+  p.qk_norm = d->qk_norm != 0;
+  p.eps = d->norm_eps;
+  p.sin = d->sin;
+  p.cos = d->cos;
+  p.table_rows = d->table_rows;
+  p.table_stride = d->table_row_stride;
+  p.pos = d->positions;
+  p.q = q;
+  p.k = k;
+  // the widest vector that every row starts at a multiple of, and the lanes that cover a
+  // head with it; vec 1 is the general kernel
+  const int es = es_of(c->dtype), ts = es_of(d->table_dtype);
+  int vec = 1, lanes = 1;
+  for (int v = 16 / es; v >= 4 && vec == 1; v /= 2) {
+    if (!rows_at(c, v) || !aligned(d->qkv, v * es) || d->batch_stride % v || d->token_stride % v || !aligned(q, v * es) ||
+        !aligned(k, v * es) || !aligned(d->sin, v / 2 * ts) || !aligned(d->cos, v / 2 * ts) || d->table_row_stride % (v / 2))
+      continue;
+    for (int n = v == 8 ? 4 : 8; n <= (v == 8 ? 32 : 64); n *= 2)
+      if (vec == 1 && n * v >= c->head_dim) vec = v, lanes = n;
+  }
+  const hipError_t err = launch_cache_append(c->dtype, d->table_dtype == ATTNRES_DTYPE_F32, p, vec, lanes, (hipStream_t)stream);
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache append launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}
+
+extern "C" size_t attnres_cache_attend_workspace_size(const attnres_cache_desc* c, const attnres_cache_attend_desc* d) {
+  if (check_attend(c, d) || c->batch == 0 || d->tokens == 0) return 0;
+  return c->weights ? (size_t)c->batch * d->q_heads * 4 : 0;
+}
+
+extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d, void* out,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_attend(c, d)) return rc;
+  if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  if (!out) return api_fail(ATTNRES_EINVAL, "out is NULL");
+  const size_t need = attnres_cache_attend_workspace_size(c, d);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  CacheAttendParams p{};
+  p.c = pages_of(c);
+  p.q = d->q;
+  p.q_b_stride = d->q_batch_stride;
+  p.q_h_stride = d->q_head_stride;
+  p.q_t_stride = d->q_token_stride;
+  p.tokens = (int32_t)d->tokens;
+  p.q_heads = d->q_heads;
+  p.scale = (float)((double)d->scale * 1.4426950408889634);
+  p.decay = d->decay;
+  p.out = out;
+  p.lse = c->weights ? (float*)workspace : nullptr;
+  const hipError_t err = launch_cache_attend(c->dtype, p, (hipStream_t)stream);
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache attend launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}
+
+extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* new_table, int64_t new_stride,
+                                   int64_t budget, int64_t recent, int32_t* kept, int32_t* left, void* stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (budget < 1 || budget > ATTNRES_CACHE_MAX_TOKENS) return api_fail(ATTNRES_EINVAL, "budget=%lld must be 1 .. 2^30", (long long)budget);
+  if (recent < 0 || recent > budget)
+    return api_fail(ATTNRES_EINVAL, "recent=%lld must be 0 .. budget=%lld", (long long)recent, (long long)budget);
+  if (c->batch == 0) return ATTNRES_OK;
+  if (!new_table || !kept || !left) return api_fail(ATTNRES_EINVAL, "new_table / kept / left is NULL");
+  if (c->pages > 0 && !c->weights) return api_fail(ATTNRES_EINVAL, "weights is NULL");
+  if (new_stride < (budget + c->page_size - 1) / c->page_size && c->batch > 1)
+    return api_fail(ATTNRES_EINVAL, "new_stride=%lld below the pages of %lld tokens", (long long)new_stride, (long long)budget);
+  if (c->batch * c->kv_heads > (1 << 21) || c->batch * c->kv_heads * budget > (int64_t)1 << 28)
+    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, kv_heads=%d, budget=%lld: too many tokens", (long long)c->batch,
+                    c->kv_heads, (long long)budget);
+  CacheEvictParams p{};
+  p.c = pages_of(c);
+  p.new_table = new_table;
+  p.new_stride = new_stride;
+  p.budget = (int32_t)budget;
+  p.recent = (int32_t)recent;
+  p.kept = kept;
+  p.left = left;
+  p.es = es_of(c->dtype);
+  p.vec = rows_at(c, 16 / p.es);
+  const hipError_t err = launch_cache_evict(p, (hipStream_t)stream);
+  if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache evict launch failed: %s", hipGetErrorString(err));
+  return ATTNRES_OK;
+}

@@ -17,6 +17,7 @@
 // stream current then.
 #include <dlfcn.h>
 
+#include <cmath>
 #include <limits>
 #include <string>
 #include <vector>
@@ -30,6 +31,7 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
+#include "../../include/attnres_cache.h"
 #include "../../include/attnres_hip.h"
 #include "../../include/attnres_phase1_bank.h"
 #include "../../include/attnres_sublayers.h"
@@ -52,7 +54,8 @@ struct Lib {
   X(attnres_accum_read_forward) X(attnres_accum_read_backward) X(attnres_block_accum_forward)                      \
   X(attnres_block_accum_backward) X(attnres_qkv_rotary_forward) X(attnres_qkv_rotary_backward)                     \
   X(attnres_swiglu_saved_size) X(attnres_swiglu_forward_workspace_size)                                      \
-  X(attnres_swiglu_backward_workspace_size) X(attnres_swiglu_forward) X(attnres_swiglu_backward)
+  X(attnres_swiglu_backward_workspace_size) X(attnres_swiglu_forward) X(attnres_swiglu_backward)                   \
+  X(attnres_cache_append) X(attnres_cache_attend_workspace_size) X(attnres_cache_attend) X(attnres_cache_evict)
   ATTNRES_FNS(ATTNRES_FN)
 } lib;
 
@@ -1050,6 +1053,7 @@ py::object block_accum(const py::object& projected, const py::object& partial_va
 }
 
 #include "attnres_torch_sublayers.h"
+#include "attnres_torch_cache.h"
 
 }  // namespace
 
@@ -1063,4 +1067,7 @@ PYBIND11_MODULE(_attnres_torch, m) {
   m.def("block_accum", &block_accum);
   m.def("qkv_rotary", &qkv_rotary);
   m.def("swiglu", &swiglu);
+  m.def("cache_append", &cache_append);
+  m.def("cache_attend", &cache_attend);
+  m.def("cache_evict", &cache_evict);
 }
