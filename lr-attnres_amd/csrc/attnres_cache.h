@@ -42,18 +42,31 @@ struct CacheAppendParams {
 // vec, lanes: as launch_qkv_rotary's
 hipError_t launch_cache_append(int dtype, bool f32_table, const CacheAppendParams& p, int vec, int lanes, hipStream_t st);
 
+constexpr int kAttUnit = 128;  // tokens of a unit of attention's work
+
 struct CacheAttendParams {
   CachePages c;
   const void* q;
   int64_t q_b_stride, q_h_stride, q_t_stride;
   int32_t tokens, q_heads;
-  float scale;  // of base-2 logarithms: the softmax's scale times log2(e)
+  int32_t group, rows, blocks;  // query heads of a key / value head; with the new tokens; 16-row blocks of them
+  int32_t wgs;
+  int32_t tile;                 // 64 / 128 / 256: the head width it covers
+  int32_t vec, page16, whole, q_vec;  // aligned rows; pages of whole 16 tokens; head rows of whole 64 bytes; aligned queries
+  float scale;                  // of base-2 logarithms: the softmax's scale times log2(e)
   float decay;
   void* out;
-  float* lse;  // [batch, q_heads], with weights
+  float* part;     // [2 wgs][16][tile], pieces of rows
+  float* part_ml;  // [2 wgs][16][2], their maxima and sums
+  float* lse;      // [batch, q_heads], with weights
+  float* logits;   // [batch, q_heads, logit_stride], with weights
+  int64_t logit_stride;
 };
 
-hipError_t launch_cache_attend(int dtype, const CacheAttendParams& p, hipStream_t st);
+hipError_t launch_cache_attend_bf16(const CacheAttendParams& p, hipStream_t st);
+hipError_t launch_cache_attend_f16(const CacheAttendParams& p, hipStream_t st);
+hipError_t launch_cache_attend_f32(const CacheAttendParams& p, hipStream_t st);
+hipError_t launch_cache_weights(const CacheAttendParams& p, hipStream_t st);
 
 struct CacheEvictParams {
   CachePages c;

@@ -1,0 +1,692 @@
+// Attention of the newest tokens over the paged cache.
+//   p_j = softmax_j(scale <q, k_j>),   out = sum_j p_j v_j,   j < cached + t + 1
+//
+// Bound by memory: each key and value is read once for the (up to 16) query rows of its
+// head -- the heads of its group times the new tokens -- so 2 rows flops a byte in 16 bits.
+//
+// Products.  Query rows are columns of 16 x 16 matrix-core tiles: S^T = K Q^T with a tile's
+// tokens as rows, then O^T = V^T P^T.  Lane l holds column l % 16 of both, so a row's maximum,
+// sum and rescaling stay in its lanes, and the scores leave the first product in the very
+// lanes in which the second takes its weights: nothing goes through LDS.  A lane loads 16 bytes of
+// a key row as the product takes them, and of each of its tokens' value rows W consecutive
+// values, turned in registers (one byte permute a word) into the columns that the product
+// wants; output rows are d in the order (chunk, lane, value), put right when they are stored.
+// The idle 16 - rows columns cost matrix-core time that a memory-bound kernel does not miss.
+//
+// Rounding.  Scores, weights, sums and outputs are fp32; a weight goes into the 16-bit
+// product as the sum of two terms, rounded and the rest (one term alone would add an error
+// as large as the result's own rounding); fp16 weights are scaled by 2^14 so that small ones
+// keep their bits.
+//
+// Work.  A cache's units (kUnit tokens of one sequence's head and block of rows) are dealt
+// evenly to a fixed number of workgroups from the lengths on the device, whatever they are:
+// no length is known to the host, and a long sequence among short ones is shared by many.  A
+// workgroup that has a head's whole length writes its rows; pieces go to the workspace as
+// maximum, sum and unscaled output, joined by a second launch.
+#pragma once
+
+#include "attnres_cache.h"
+#include "attnres_device.h"
+#include "attnres_swiglu.h"
+
+namespace attnres {
+
+constexpr int kAttWaves = 4;
+constexpr int kAttRows = 16;  // query rows of a workgroup
+
+// The deal: `segs` segments (heads, blocks of rows) of each sequence, kUnit tokens a unit, unit x to
+// workgroup deal_of(x).
+struct Deal {
+  int total, per, more;  // units; of a workgroup; the first `more` have one more
+};
+
+// tokens that the queries of sequence b see together; 0: none has any, -1: counts that cannot be
+__device__ __forceinline__ int seq_len(const CacheAttendParams& p, int b) {
+  const int have = p.c.cached[b], fresh = p.c.fresh ? min(p.c.fresh[b], p.tokens) : p.tokens;
+  const int64_t n = (int64_t)have + fresh;
+  if (have < 0 || fresh < 0 || n > p.c.room || (fresh > 0 && p.c.pages == 0)) return -1;
+  return fresh > 0 ? (int)n : 0;
+}
+__device__ __forceinline__ int seq_units(const CacheAttendParams& p, int b) {
+  return b < p.c.batch ? (max(seq_len(p, b), 0) + kAttUnit - 1) / kAttUnit : 0;
+}
+
+__device__ __forceinline__ int wave_scan(int x) {  // inclusive
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int y = __shfl_up(x, o, kWave);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+__device__ __forceinline__ Deal deal(const CacheAttendParams& p, int segs, int wgs) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int sum = 0;
+  for (int b0 = 0; b0 < p.c.batch; b0 += kWave) sum += seq_units(p, b0 + lane);
+  for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+  Deal d;
+  d.total = __builtin_amdgcn_readfirstlane(sum) * segs;
+  d.per = d.total / wgs;
+  d.more = d.total - d.per * wgs;
+  return d;
+}
+__device__ __forceinline__ int deal_start(const Deal& d, int w) { return w * d.per + min(w, d.more); }
+__device__ __forceinline__ int deal_of(const Deal& d, int x) {
+  const int big = d.more * (d.per + 1);
+  return x < big ? x / (d.per + 1) : d.more + (x - big) / max(d.per, 1);
+}
+
+// The sequence that unit x is of, its first unit and how many a segment has.  Every x below the total is of one.
+__device__ __forceinline__ void find_unit(const CacheAttendParams& p, int segs, int x, int* b, int* start, int* units) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int before = 0;
+  for (int b0 = 0; b0 < p.c.batch; b0 += kWave) {
+    const int u = seq_units(p, b0 + lane);
+    const int upto = wave_scan(u) + before;
+    const int last = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (x < last * segs) {
+      const int i = __popcll(__ballot(upto * segs <= x));
+      *b = b0 + i;
+      *units = __builtin_amdgcn_readlane(u, i);
+      *start = (__builtin_amdgcn_readlane(upto, i) - *units) * segs;
+      return;
+    }
+    before = last;
+  }
+}
+// the first unit of sequence b
+__device__ __forceinline__ int units_before(const CacheAttendParams& p, int b, int segs) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int sum = 0;
+  for (int b0 = 0; b0 < b; b0 += kWave) sum += b0 + lane < b ? seq_units(p, b0 + lane) : 0;
+  for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+  return __builtin_amdgcn_readfirstlane(sum) * segs;
+}
+
+#ifdef ATTNRES_CACHE_ATTEND_KERNELS
+
+// A matrix product's result must not be read for some cycles.  The compiler counts them inside a block of
+// code but has been seen to miss them over a branch (a score tile whose zeroing branch came right before it
+// was read two instructions after its product, and wrong); where a branch may come between, this waits.
+__device__ __forceinline__ void att_settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+typedef _Float16 att_h4 __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(4))) int32_t att_const_i32;  // read by the scalar unit
+
+// HD: head width's tile (64, 128, 256); VEC: rows in aligned 16-byte vectors; PAGE16: pages of a multiple
+// of 16 tokens, so that 16 tokens lie in one and the scalar unit finds it.
+template <class DT, int HD, bool VEC, bool PAGE16>
+struct Att {
+  using S = typename DT::S;
+  static constexpr int kSize = sizeof(S);
+  static constexpr int kPer = 16 / kSize;                      // values of a key chunk
+  static constexpr int kKs = HD * kSize / 64;                  // key chunks of a lane
+  static constexpr bool k32 = kSize == 4;
+  static constexpr int kSub = k32 || HD == 256 ? 1 : 2;        // 16-token subtiles of a tile (one: half the registers)
+  static constexpr int kTok = 16 * kSub;
+  static constexpr int kW = k32 ? 4 : HD == 64 ? 4 : 8;        // values of a value chunk
+  static constexpr int kNi = HD / (16 * kW);
+  static constexpr int kWords = kW * kSize / 4;
+  static constexpr int kPitch = HD + 4;
+  static constexpr float kShift = DT::kCode == 2 ? 14.f : 0.f;
+
+  const CacheAttendParams& p;
+  int lane, wave, c, g;          // column (query row) and token group of the lane
+  int b, h, n, have;
+  int kcol[kKs], vcol[kNi];      // first value of each chunk, inside the row
+  uint32_t kofs[kKs], vofs[kNi]; // PAGE16: bytes from a subtile's first row (of a key), from its token `t`'s (of a value)
+  u32x4 q[kKs], k[kSub][kKs];
+  uint32_t v[kSub][4][kNi][kWords];
+  sw_f4 acc[kNi][kW];
+  float m, l;                    // of the lane's row: maximum (less kShift), the lane's part of the sum
+
+  struct Rows {
+    int64_t off[PAGE16 ? kSub : 1];  // of a subtile's first token, or of token `lane` of the tile; -1: no page
+  };
+
+  __device__ __forceinline__ Att(const CacheAttendParams& p_) : p(p_) {
+    lane = threadIdx.x & (kWave - 1);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    c = lane & 15;
+    g = lane >> 4;
+    const int Dh = p.c.head_dim;
+#pragma unroll
+    for (int i = 0; i < kKs; ++i) kcol[i] = (i * 4 + g) * kPer;
+#pragma unroll
+    for (int i = 0; i < kNi; ++i) vcol[i] = (i * 16 + c) * kW;
+    if constexpr (VEC) {  // lanes behind a row's end read inside it, and drop what they read
+      const uint32_t slot = (uint32_t)p.c.slot_stride;
+#pragma unroll
+      for (int i = 0; i < kNi; ++i) {
+        vcol[i] = min(vcol[i], Dh - kW);
+        vofs[i] = (g * 4 * slot + vcol[i]) * kSize;
+      }
+#pragma unroll
+      for (int i = 0; i < kKs; ++i) kofs[i] = (c * slot + min(kcol[i], Dh - kPer)) * kSize;
+    }
+  }
+
+  __device__ __forceinline__ Rows rows_of(int t0) const {
+    Rows r;
+    if constexpr (PAGE16) {
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) {
+        const int j = min(t0 + 16 * s, (n - 1) & ~15);
+        const int at = j / p.c.page_size;
+        const int page = ((att_const_i32*)(uintptr_t)p.c.table)[b * p.c.table_stride + at];
+        r.off[s] = (unsigned)page < (unsigned)p.c.pages
+                       ? page * p.c.page_stride + h * p.c.head_stride + (j - at * p.c.page_size) * p.c.slot_stride
+                       : -1;
+      }
+    } else {
+      const int j = min(t0 + (lane & (kTok - 1)), n - 1);
+      const int at = j / p.c.page_size;
+      const int page = p.c.table[b * p.c.table_stride + at];
+      r.off[0] = (unsigned)page < (unsigned)p.c.pages
+                     ? page * p.c.page_stride + h * p.c.head_stride + (j - at * p.c.page_size) * p.c.slot_stride
+                     : -1;
+    }
+    return r;
+  }
+
+  // E values at `at`, whole words
+  template <int E>
+  __device__ __forceinline__ void load_vec(const void* at, uint32_t* w) const {
+    if constexpr (E * kSize == 16) {
+      const u32x4 x = *(const u32x4*)at;
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const u32x2 x = *(const u32x2*)at;
+      w[0] = x.x, w[1] = x.y;
+    }
+  }
+  // values col .. col + E of a row that starts anywhere, zero behind its end
+  template <int E>
+  __device__ __forceinline__ void load_any(const S* row, int col, uint32_t* w) const {
+    const int Dh = p.c.head_dim;
+#pragma unroll
+    for (int e = 0; e < E; e += 4 / kSize) {
+      if constexpr (k32) {
+        w[e] = col + e < Dh ? __float_as_uint(row[col + e]) : 0;
+      } else {
+        const uint32_t lo = col + e < Dh ? row[col + e] : 0, hi = col + e + 1 < Dh ? row[col + e + 1] : 0;
+        w[e / 2] = lo | hi << 16;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load_k(const Rows& r) {
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      if constexpr (PAGE16) {
+        const char* row = (const char*)((const S*)p.c.k + max(r.off[s], (int64_t)0));
+#pragma unroll
+        for (int i = 0; i < kKs; ++i) k[s][i] = *(const u32x4*)(row + kofs[i]);
+      } else {
+        const S* row = (const S*)p.c.k + max(__shfl(r.off[0], 16 * s + c, kWave), (int64_t)0);
+#pragma unroll
+        for (int i = 0; i < kKs; ++i) {
+          uint32_t w[4];
+          if constexpr (VEC) load_vec<kPer>(row + min(kcol[i], p.c.head_dim - kPer), w);
+          else load_any<kPer>(row, kcol[i], w);
+          k[s][i] = u32x4{w[0], w[1], w[2], w[3]};
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load_v(const Rows& r) {
+#pragma unroll
+    for (int s = 0; s < kSub; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if constexpr (PAGE16) {
+          const char* row = (const char*)((const S*)p.c.v + max(r.off[s], (int64_t)0) + t * p.c.slot_stride);
+#pragma unroll
+          for (int i = 0; i < kNi; ++i) load_vec<kW>(row + vofs[i], v[s][t][i]);
+        } else {
+          const S* row = (const S*)p.c.v + max(__shfl(r.off[0], 16 * s + g * 4 + t, kWave), (int64_t)0);
+#pragma unroll
+          for (int i = 0; i < kNi; ++i) {
+            if constexpr (VEC) load_vec<kW>(row + vcol[i], v[s][t][i]);
+            else load_any<kW>(row, vcol[i], v[s][t][i]);
+          }
+        }
+      }
+  }
+
+  __device__ __forceinline__ bool no_page(const Rows& r, int s, int t) const {
+    return (PAGE16 ? r.off[PAGE16 ? s : 0] : __shfl(r.off[0], 16 * s + g * 4 + t, kWave)) < 0;
+  }
+
+  // a tile's weights as the second product takes them: fp32, or in two terms
+  struct Weights {
+    u32x4 hi, lo;
+    float e[kSub][4];
+  };
+  static __device__ __forceinline__ Weights split(const float (&e)[kSub][4]) {
+    Weights w;
+#pragma unroll
+    for (int s = 0; s < kSub; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; t += 2) {
+        w.e[s][t] = e[s][t], w.e[s][t + 1] = e[s][t + 1];
+        if constexpr (!k32) {
+          const uint32_t x = pack2<DT>(e[s][t], e[s][t + 1]);
+          w.hi[s * 2 + t / 2] = x;
+          w.lo[s * 2 + t / 2] = pack2<DT>(e[s][t] - bits_to_float<DT>(x & 0xffffu), e[s][t + 1] - bits_to_float<DT>(x >> 16));
+        }
+      }
+    return w;
+  }
+  // 16 tokens: a lane's four of each operand
+  static __device__ __forceinline__ sw_f4 mfma16(u32x2 a, u32x2 b, sw_f4 to) {
+    if constexpr (DT::kCode == 1)
+      return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(sw_s4, a), __builtin_bit_cast(sw_s4, b), to, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(att_h4, a), __builtin_bit_cast(att_h4, b), to, 0, 0, 0);
+  }
+  // a pair of values, 0 for one that is not finite
+  static __device__ __forceinline__ uint32_t finite(uint32_t w) {
+    constexpr uint32_t kExp = DT::kCode == 1 ? 0x7f80u : 0x7c00u;
+    return ((w & kExp) == kExp ? 0 : w & 0xffffu) | ((w >> 16 & kExp) == kExp ? 0 : w & 0xffff0000u);
+  }
+  // O^T += V^T P^T over a tile, value d of chunk i of the lanes' columns.  CARE: an infinite value times the second
+  // term, which may have the other sign, is left out.
+  template <bool CARE>
+  __device__ __forceinline__ sw_f4 weigh(const Weights& p, int i, int d, sw_f4 to) const {
+    if constexpr (k32) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        to = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[0][t][i][d]), p.e[0][t], to, 0, 0, 0);
+    } else {
+      u32x4 a;
+#pragma unroll
+      for (int s = 0; s < kSub; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; t += 2) {
+          const uint32_t x = v[s][t][i][d / 2], y = v[s][t + 1][i][d / 2];
+          a[s * 2 + t / 2] = d % 2 ? hi_pair(x, y) : lo_pair(x, y);
+        }
+      u32x4 a2 = a;
+      if constexpr (CARE) {
+#pragma unroll
+        for (int x = 0; x < 2 * kSub; ++x) a2[x] = finite(a[x]);
+      }
+      if constexpr (kSub == 2) {
+        sw_mfma<DT>(a, p.hi, to);
+        sw_mfma<DT>(a2, p.lo, to);
+      } else {
+        to = mfma16({a.x, a.y}, {p.hi.x, p.hi.y}, to);
+        to = mfma16({a2.x, a2.y}, {p.lo.x, p.lo.y}, to);
+      }
+    }
+    return to;
+  }
+
+  struct Row {       // the lane's
+    float* logits;   // of token 0, or null
+    int lim;         // tokens that it sees (one that is not there: whatever)
+    int t;           // its new token
+    int all;         // tokens that every row sees
+  };
+
+  // The tile of tokens t0 .., whose keys and values are on their way; CUT: some row does not see all of it; CARE: by
+  // itself, and so that a value that is not finite shows in the rows that see it and in no other.
+  template <bool CUT, bool CARE>
+  __device__ __forceinline__ void tile(int t0, bool more, const Row& row, Rows& now, Rows& next) {
+    Rows after;
+    if constexpr (!CARE) after = rows_of(min(t0 + 2 * kAttWaves * kTok, n - 1) / kTok * kTok);
+    // (before all of the products: no branch comes between them and what reads them)
+    if (VEC && !p.whole) {
+#pragma unroll
+      for (int s = 0; s < kSub; ++s)
+#pragma unroll
+        for (int i = 0; i < kKs; ++i)
+          if (kcol[i] >= p.c.head_dim) k[s][i] = u32x4{0, 0, 0, 0};
+    }
+    sw_f4 s4[kSub];
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      s4[s] = sw_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kKs; ++i) sw_mfma<DT>(k[s][i], q[i], s4[s]);
+    }
+    float x[kSub][4];
+#pragma unroll
+    for (int s = 0; s < kSub; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        x[s][t] = s4[s][t] * p.scale;
+        if (no_page(now, s, t)) x[s][t] = __builtin_nanf("");
+        if (CUT && t0 + 16 * s + g * 4 + t >= row.lim) x[s][t] = -INFINITY;
+      }
+    if (!CARE && more) load_k(next);
+    if (row.logits) {
+#pragma unroll
+      for (int s = 0; s < kSub; ++s)
+        *(sw_f4*)(row.logits + t0 + 16 * s + g * 4) = sw_f4{x[s][0], x[s][1], x[s][2], x[s][3]};
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int s = 0; s < kSub; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) top = fmaxf(top, x[s][t]);
+    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+    top = fmaxf(top, __shfl_xor(top, 32, kWave)) - kShift;
+    const float to = fmaxf(m, top), base = to == -INFINITY ? 0.f : to;
+    if (__any(to != m)) {
+      const float was = __builtin_amdgcn_exp2f(m - base);
+      l *= was;
+#pragma unroll
+      for (int i = 0; i < kNi; ++i)
+#pragma unroll
+        for (int d = 0; d < kW; ++d) acc[i][d] *= was;
+      m = to;
+    }
+    float e[kSub][4];
+#pragma unroll
+    for (int s = 0; s < kSub; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        e[s][t] = __builtin_amdgcn_exp2f(x[s][t] - base);
+        l += e[s][t];
+      }
+    const Weights w = split(e);
+    if constexpr (CUT) {  // what lies behind the last token may be anything
+#pragma unroll
+      for (int s = 0; s < kSub; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (t0 + 16 * s + g * 4 + t >= n) {
+#pragma unroll
+            for (int i = 0; i < kNi; ++i)
+#pragma unroll
+              for (int y = 0; y < kWords; ++y) v[s][t][i][y] = 0;
+          }
+    }
+    if constexpr (!CARE) {
+#pragma unroll
+      for (int i = 0; i < kNi; ++i)
+#pragma unroll
+        for (int d = 0; d < kW; ++d) acc[i][d] = weigh<false>(w, i, d, acc[i][d]);
+      if (more) load_v(next);
+      now = next;
+      next = after;
+    } else {
+      // (0 times such a value is NaN: each new token's rows take a product without the values behind it)
+      for (int tt = p.tokens - 1; tt >= 0; --tt) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (t0 + 16 * s + g * 4 + t > have + tt) {
+#pragma unroll
+              for (int i = 0; i < kNi; ++i)
+#pragma unroll
+                for (int y = 0; y < kWords; ++y) v[s][t][i][y] = 0;
+            }
+#pragma unroll
+        for (int i = 0; i < kNi; ++i)
+#pragma unroll
+          for (int d = 0; d < kW; ++d) {
+            const sw_f4 with = weigh<true>(w, i, d, acc[i][d]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[i][d][t] = row.t == tt ? with[t] : acc[i][d][t];
+          }
+        att_settle();
+      }
+    }
+  }
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kNi; ++i)
+#pragma unroll
+      for (int d = 0; d < kW; ++d) acc[i][d] = sw_f4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // tokens [first, end) of the head for rows [row0, row0 + rows); this wave's: tiles wave, wave + 4, ...
+  __device__ __forceinline__ void piece(int row0, int rows, int first, int end, float* logits) {
+    const int r = row0 + c, t_row = r / p.group;
+    const bool valid = c < rows;
+    const int hq = h * p.group + r - t_row * p.group;
+    const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
+#pragma unroll
+    for (int i = 0; i < kKs; ++i) {
+      q[i] = u32x4{0, 0, 0, 0};
+      uint32_t w[4];
+      if (valid && kcol[i] < p.c.head_dim) {
+        if constexpr (VEC) {
+          if (p.q_vec) {
+            q[i] = *(const u32x4*)(src + kcol[i]);
+            continue;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4 / kSize) {
+          const int col = kcol[i] + e, Dh = p.c.head_dim;
+          if constexpr (k32) {
+            w[e] = col < Dh ? __float_as_uint(src[col]) : 0;
+          } else {
+            const uint32_t lo = col < Dh ? src[col] : 0, hi = col + 1 < Dh ? src[col + 1] : 0;
+            w[e / 2] = lo | hi << 16;
+          }
+        }
+        q[i] = u32x4{w[0], w[1], w[2], w[3]};
+      }
+    }
+    clear();
+    const int lim = min(have + t_row + 1, n);  // of the lane's row (a row that is not there: whatever)
+    const int all = p.tokens > 1 ? have + 1 : n;  // tokens that every row sees
+    constexpr int kStep = kAttWaves * kTok;
+    const int t_first = first + wave * kTok;
+    if (t_first >= end) return;
+    Rows now = rows_of(t_first), next = rows_of(min(t_first + kStep, n - 1) / kTok * kTok);
+    load_k(now);
+    load_v(now);
+    int t0 = t_first;
+    const Row row{logits && valid ? logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row, all};
+    for (; t0 < end && t0 + kTok <= all; t0 += kStep) tile<false, false>(t0, t0 + kStep < end, row, now, next);
+    // tiles that a row does not see all of; never many
+    for (; t0 < end; t0 += kStep) tile<true, false>(t0, t0 + kStep < end, row, now, next);
+    att_settle();
+    float none = 0.f;
+#pragma unroll
+    for (int i = 0; i < kNi; ++i)
+#pragma unroll
+      for (int d = 0; d < kW; ++d)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) none = __builtin_fmaf(acc[i][d][t], 0.f, none);
+    if (__any(none != 0.f)) {  // NaN: something was not finite
+      clear();
+      for (t0 = t_first; t0 < end; t0 += kStep) {
+        now = rows_of(t0);
+        load_k(now);
+        load_v(now);
+        tile<true, true>(t0, false, row, now, now);
+      }
+    }
+    l += __shfl_xor(l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+  }
+};
+
+// What a part of a row's tokens weighs against the row's maximum; a part that saw nothing (or scores of -inf
+// alone) weighs nothing, whatever its values: 0 x NaN stays NaN.
+__device__ __forceinline__ float att_share(float m, float top) {
+  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+}
+
+template <class DT, int HD, bool VEC, bool PAGE16>
+__global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_attend_kernel(CacheAttendParams p) {
+  using A = Att<DT, HD, VEC, PAGE16>;
+  using S = typename DT::S;
+  __shared__ float so[kAttWaves][kAttRows][A::kPitch];
+  __shared__ float sm[kAttWaves][kAttRows], sl[kAttWaves][kAttRows];
+  A a(p);
+  const int Dh = p.c.head_dim, segs = p.c.kv_heads * p.blocks;
+  // neighbouring workgroups run on different XCDs; those of one XCD take neighbouring units
+  const int w = p.wgs % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (p.wgs / 8) + blockIdx.x / 8);
+  const Deal d = deal(p, segs, p.wgs);
+  int x = deal_start(d, w);
+  const int x1 = deal_start(d, w + 1);
+  int b_start = 0, b_end = 0, units = 1;
+  while (x < x1) {
+    if (x >= b_end) {
+      find_unit(p, segs, x, &a.b, &b_start, &units);
+      b_end = b_start + segs * units;
+      a.n = seq_len(p, a.b);
+      a.have = p.c.cached[a.b];
+    }
+    const int seg = (x - b_start) / units, u0 = x - b_start - seg * units, u1 = min(units, u0 + x1 - x);
+    x += u1 - u0;
+    a.h = seg / p.blocks;
+    const int row0 = (seg - a.h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
+    a.piece(row0, rows, u0 * kAttUnit, min(u1 * kAttUnit, a.n), p.logits);
+    if (a.c < rows) {
+      if (a.g == 0) sm[a.wave][a.c] = a.m, sl[a.wave][a.c] = a.l;
+#pragma unroll
+      for (int i = 0; i < A::kNi; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < A::kW; e += 4)
+            *(sw_f4*)&so[a.wave][a.c][(i * 16 + a.g * 4 + t) * A::kW + e] =
+                sw_f4{a.acc[i][e][t], a.acc[i][e + 1][t], a.acc[i][e + 2][t], a.acc[i][e + 3][t]};
+    }
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == units;
+    const int64_t slot = 2 * w + (u0 == 0 ? 1 : 0);
+    for (int at = threadIdx.x; at < rows * (HD / 4); at += kAttWaves * kWave) {
+      const int r = at / (HD / 4), col = at % (HD / 4) * 4;
+      float top = sm[0][r];
+#pragma unroll
+      for (int i = 1; i < kAttWaves; ++i) top = fmaxf(top, sm[i][r]);
+      float l = 0.f;
+      sw_f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kAttWaves; ++i) {
+        const float f = att_share(sm[i][r], top);
+        l += f * sl[i][r];
+        o += f * *(const sw_f4*)&so[i][r][col];
+      }
+      if (whole) {
+        const int t = (row0 + r) / p.group, hq = a.h * p.group + row0 + r - t * p.group;
+        const bool seen = !p.c.fresh || t < p.c.fresh[a.b];
+        S* out = (S*)p.out + ((a.b * (int64_t)p.tokens + t) * p.q_heads + hq) * Dh + col;
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < Dh) DT::store1(out + e, seen ? o[e] * inv : 0.f);
+        if (p.lse && col == 0) p.lse[a.b * p.q_heads + hq] = top + log2f(l);
+      } else {
+        *(sw_f4*)(p.part + (slot * kAttRows + r) * HD + col) = o;
+        if (col == 0) {
+          p.part_ml[(slot * kAttRows + r) * 2] = top;
+          p.part_ml[(slot * kAttRows + r) * 2 + 1] = l;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// A head's pieces joined; zeros for rows that see nothing, NaN for counts that cannot be.  One workgroup a
+// segment: threads take four columns of a row, and where there are fewer of them, a share of the pieces.
+template <class DT, int HD>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p) {
+  using S = typename DT::S;
+  __shared__ float sm[256], sl[256];
+  __shared__ sw_f4 so[256];
+  const int Dh = p.c.head_dim, segs = p.c.kv_heads * p.blocks;
+  const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs, h = seg / p.blocks;
+  const int row0 = (seg - h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
+  const int n = seq_len(p, b), units = seq_units(p, b);
+  int w0 = 0, w1 = -1;
+  if (units) {
+    const Deal d = deal(p, segs, p.wgs);
+    const int first = units_before(p, b, segs) + seg * units;
+    w0 = deal_of(d, first), w1 = deal_of(d, first + units - 1);
+    if (w0 == w1) return;  // one workgroup had all of it
+  }
+  const int items = rows * (HD / 4), shares = max(1, 256 / items);
+  for (int i0 = 0; i0 < items; i0 += 256) {
+    const int item = shares > 1 ? threadIdx.x % items : i0 + threadIdx.x, share = shares > 1 ? threadIdx.x / items : 0;
+    const int r = item / (HD / 4), col = item % (HD / 4) * 4;
+    const bool in = share < shares && item < items;
+    float top = -INFINITY, l = 0.f;
+    sw_f4 o = {0.f, 0.f, 0.f, 0.f};
+    if (in) {
+      for (int w = w0 + share; w <= w1; w += shares) {
+        const int64_t row = (2 * w + (w == w0 ? 1 : 0)) * (int64_t)kAttRows + r;
+        const float m = p.part_ml[row * 2], part = p.part_ml[row * 2 + 1];
+        const sw_f4 x = *(const sw_f4*)(p.part + row * HD + col);
+        const float to = fmaxf(top, m), f = att_share(top, to), g = att_share(m, to);
+        l = f * l + g * part;
+        o = f * o + g * x;
+        top = to;
+      }
+    }
+    if (shares > 1) {
+      sm[threadIdx.x] = top;
+      sl[threadIdx.x] = l;
+      so[threadIdx.x] = o;
+      __syncthreads();
+      if (share == 0 && in) {
+        float all = top;
+        for (int i = 1; i < shares; ++i) all = fmaxf(all, sm[i * items + item]);
+        const float f = att_share(top, all);
+        l *= f;
+        o *= f;
+        for (int i = 1; i < shares; ++i) {
+          const float g = att_share(sm[i * items + item], all);
+          l += g * sl[i * items + item];
+          o += g * so[i * items + item];
+        }
+        top = all;
+      }
+    }
+    if (in && share == 0) {
+      const int t = (row0 + r) / p.group, hq = h * p.group + row0 + r - t * p.group;
+      const bool seen = units && (!p.c.fresh || t < p.c.fresh[b]);
+      S* out = (S*)p.out + ((b * (int64_t)p.tokens + t) * p.q_heads + hq) * Dh + col;
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < Dh) DT::store1(out + e, n < 0 ? __builtin_nanf("") : seen ? o[e] * inv : 0.f);
+      if (p.lse && col == 0) p.lse[b * p.q_heads + hq] = top + log2f(l);
+    }
+  }
+}
+
+template <class DT, int HD>
+hipError_t run_attend(const CacheAttendParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.wgs), wg(kAttWaves * kWave);
+  if (p.vec && p.page16) cache_attend_kernel<DT, HD, true, true><<<grid, wg, 0, st>>>(p);
+  else if (p.vec) cache_attend_kernel<DT, HD, true, false><<<grid, wg, 0, st>>>(p);
+  else cache_attend_kernel<DT, HD, false, false><<<grid, wg, 0, st>>>(p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  cache_join_kernel<DT, HD><<<dim3((unsigned)(p.c.batch * p.c.kv_heads * p.blocks)), dim3(256), 0, st>>>(p);
+  return hipGetLastError();
+}
+
+template <class DT>
+hipError_t run_attend_type(const CacheAttendParams& p, hipStream_t st) {
+  if (p.tile == 64) return run_attend<DT, 64>(p, st);
+  if (p.tile == 128) return run_attend<DT, 128>(p, st);
+  return run_attend<DT, 256>(p, st);
+}
+
+#endif
+
+}  // namespace attnres

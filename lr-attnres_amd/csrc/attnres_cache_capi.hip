@@ -151,19 +151,61 @@ extern "C" int attnres_cache_append(const attnres_cache_desc* c, const attnres_c
   return ATTNRES_OK;
 }
 
+namespace {
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct AttendPlan {
+  int tile, rows, blocks, wgs;
+  int64_t logit_stride;
+  size_t part, part_ml, lse, logits, need;  // offsets in the workspace, and its size
+};
+
+int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d, AttendPlan* a) {
+  const int64_t rows = d->q_heads / c->kv_heads * d->tokens, blocks = (rows + 15) / 16;
+  const int64_t room = c->table_pages * c->page_size, units = (room + kAttUnit - 1) / kAttUnit;
+  const int64_t segs = c->batch * c->kv_heads * blocks;
+  if (rows > INT32_MAX || segs > (1 << 23) || segs * (units > 0 ? units : 1) > INT32_MAX / 2)
+    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d, %lld cached: too many tokens", (long long)c->batch,
+                    (long long)d->tokens, d->q_heads, (long long)room);
+  a->tile = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  a->rows = (int)rows;
+  a->blocks = (int)blocks;
+  const int64_t most = a->tile == 64 ? 1024 : a->tile == 128 ? 768 : 512;
+  const int64_t all = segs * units;
+  a->wgs = (int)(all < most ? (all > 0 ? all : 1) : most);
+  a->logit_stride = (room + 31) / 32 * 32;
+  size_t at = 0;
+  a->part = at;
+  at += up256((size_t)2 * a->wgs * 16 * a->tile * 4);
+  a->part_ml = at;
+  at += up256((size_t)2 * a->wgs * 16 * 2 * 4);
+  a->lse = at;
+  if (c->weights) at += up256((size_t)c->batch * d->q_heads * 4);
+  a->logits = at;
+  if (c->weights) at += up256((size_t)c->batch * d->q_heads * a->logit_stride * 4);
+  a->need = at;
+  return ATTNRES_OK;
+}
+
+}  // namespace
+
 extern "C" size_t attnres_cache_attend_workspace_size(const attnres_cache_desc* c, const attnres_cache_attend_desc* d) {
-  if (check_attend(c, d) || c->batch == 0 || d->tokens == 0) return 0;
-  return c->weights ? (size_t)c->batch * d->q_heads * 4 : 0;
+  AttendPlan a;
+  if (check_attend(c, d) || c->batch == 0 || d->tokens == 0 || plan_attend(c, d, &a)) return 0;
+  return a.need;
 }
 
 extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d, void* out,
                                     void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_attend(c, d)) return rc;
   if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
+  AttendPlan a;
+  if (int rc = plan_attend(c, d, &a)) return rc;
   if (!out) return api_fail(ATTNRES_EINVAL, "out is NULL");
-  const size_t need = attnres_cache_attend_workspace_size(c, d);
-  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
-    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  if (!workspace || workspace_bytes < a.need || !aligned(workspace, 256))
+    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", a.need, workspace ? workspace_bytes : (size_t)0);
+  const int es = es_of(c->dtype), per = 16 / es;
   CacheAttendParams p{};
   p.c = pages_of(c);
   p.q = d->q;
@@ -172,11 +214,32 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   p.q_t_stride = d->q_token_stride;
   p.tokens = (int32_t)d->tokens;
   p.q_heads = d->q_heads;
+  p.group = d->q_heads / c->kv_heads;
+  p.rows = a.rows;
+  p.blocks = a.blocks;
+  p.wgs = a.wgs;
+  p.tile = a.tile;
+  p.vec = rows_at(c, per);
+  // (a subtile's rows within 32-bit offsets of its first one)
+  p.page16 = c->page_size % 16 == 0 && c->slot_stride < (1 << 25);
+  p.whole = c->head_dim == a.tile;
+  p.q_vec = aligned(d->q, 16) && d->q_batch_stride % per == 0 && d->q_head_stride % per == 0 && d->q_token_stride % per == 0;
   p.scale = (float)((double)d->scale * 1.4426950408889634);
   p.decay = d->decay;
   p.out = out;
-  p.lse = c->weights ? (float*)workspace : nullptr;
-  const hipError_t err = launch_cache_attend(c->dtype, p, (hipStream_t)stream);
+  char* ws = (char*)workspace;
+  p.part = (float*)(ws + a.part);
+  p.part_ml = (float*)(ws + a.part_ml);
+  if (c->weights) {
+    p.lse = (float*)(ws + a.lse);
+    p.logits = (float*)(ws + a.logits);
+    p.logit_stride = a.logit_stride;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  hipError_t err = c->dtype == ATTNRES_DTYPE_F32    ? launch_cache_attend_f32(p, st)
+                   : c->dtype == ATTNRES_DTYPE_BF16 ? launch_cache_attend_bf16(p, st)
+                                                    : launch_cache_attend_f16(p, st);
+  if (err == hipSuccess && c->weights) err = launch_cache_weights(p, st);
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache attend launch failed: %s", hipGetErrorString(err));
   return ATTNRES_OK;
 }

@@ -57,7 +57,8 @@ def attend_ref(c, q, cached, fresh, scale, k=None, v=None):
     """(out, bound, p): out [B, H, T, Dh] in 64 bits; bound, how far a kernel may be from it; p[b][h]: [T][n] weights.
 
     bound: half a step of the dtype of the result, and of sum p |v| the share
-      2 d + n u + 2^-17 (16 bits: p in two terms of at least 9 bits, each off by half a step of it),
+      2 d + (n + 16) u + 2^-16 (16 bits: p in two terms, the second the rest of the first, 2^-8 of it at most, and off by
+      2^-8 of itself),
       d = (Dh + 8) u scale sum |q k| + 8 u |s|: the fp32 sum of a score, its scaling and the exponential.
     """
     B, H, T, Dh = q.shape
@@ -80,7 +81,7 @@ def attend_ref(c, q, cached, fresh, scale, k=None, v=None):
                 out[b, h, t] = (p[:, None] * vh).sum(0)
                 mag = (kh * x).abs().sum(-1) * abs(scale)
                 d = float(((Dh + 8) * U * mag + 8 * U * s.abs()).max())
-                share = 2 * d + (n + 16) * U + (0.0 if q.dtype == torch.float32 else 2.0 ** -17)
+                share = 2 * d + (n + 16) * U + (0.0 if q.dtype == torch.float32 else 2.0 ** -16)
                 bound[b, h, t] = HALF_STEP[q.dtype] * out[b, h, t].abs() * (1 + share) + share * (p[:, None] * vh.abs()).sum(0)
                 ps[b, h, t] = (p, share)
     return out, bound, ps
