@@ -31,7 +31,7 @@ SOURCES = ["attnres_capi.hip", "attnres_lr.hip", "attnres_lr_fast_fwd.hip", "att
            "attnres_sublayers_capi.hip", "attnres_qkv_rotary.hip", "attnres_swiglu.hip", "attnres_swiglu_few.hip", "attnres_swiglu_bf16.hip",
            "attnres_swiglu_f16.hip", "attnres_swiglu_f32.hip",
            "attnres_cache_capi.hip", "attnres_cache_append.hip", "attnres_cache_attend_bf16.hip", "attnres_cache_attend_f16.hip",
-           "attnres_cache_attend_f32.hip", "attnres_cache_weights.hip", "attnres_cache_evict.hip"]
+           "attnres_cache_attend_f32.hip", "attnres_cache_evict.hip"]
 
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

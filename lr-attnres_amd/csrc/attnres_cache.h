@@ -10,6 +10,18 @@ namespace attnres {
 // records the message that attnres_last_error() returns and gives back `code`
 int api_fail(int code, const char* fmt, ...);
 
+// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by a product: with 2^s < d <= 2^(s+1) and mul = ceil(2^(32+s) / d), mul * d
+// exceeds 2^(32+s) by less than d <= 2^(s+1), so that n * mul / 2^(32+s) exceeds n / d by less than 1 / d.
+struct FastDiv {
+  uint32_t mul, shift;  // mul 0: d is 1
+};
+inline FastDiv fast_div(int32_t d) {
+  if (d <= 1) return FastDiv{0, 0};
+  uint32_t s = 0;
+  while (((int64_t)2 << s) < d) ++s;
+  return FastDiv{(uint32_t)((((uint64_t)1 << (32 + s)) + d - 1) / d), s};
+}
+
 struct CachePages {  // attnres_cache_desc
   void* k;
   void* v;
@@ -22,6 +34,8 @@ struct CachePages {  // attnres_cache_desc
   const int32_t* fresh;
   int32_t batch, kv_heads, head_dim, page_size, pages;
   int32_t room;  // tokens that a row of the table has pages for
+  FastDiv by_page;  // page_size
+  uint32_t page_bytes, slot_bytes;  // the strides, where a page lies within 32 bits
 };
 
 struct CacheAppendParams {
@@ -42,7 +56,7 @@ struct CacheAppendParams {
 // vec, lanes: as launch_qkv_rotary's
 hipError_t launch_cache_append(int dtype, bool f32_table, const CacheAppendParams& p, int vec, int lanes, hipStream_t st);
 
-constexpr int kAttUnit = 128;  // tokens of a unit of attention's work
+constexpr int kAttUnit = 256;  // tokens of a unit of attention's work
 
 struct CacheAttendParams {
   CachePages c;
@@ -50,15 +64,19 @@ struct CacheAttendParams {
   int64_t q_b_stride, q_h_stride, q_t_stride;
   int32_t tokens, q_heads;
   int32_t group, rows, blocks;  // query heads of a key / value head; with the new tokens; 16-row blocks of them
-  int32_t wgs;
+  int32_t wgs;                  // of a split cache
+  int32_t weight_wgs;           // that add the weights up, 0: none are kept
+  FastDiv by_group, by_blocks, by_segs, by_wgs, by_weight_wgs;  // segments: kv_heads * blocks
+  int32_t direct;               // a workgroup takes a whole segment
   int32_t tile;                 // 64 / 128 / 256: the head width it covers
   int32_t vec, page16, whole, q_vec;  // aligned rows; pages of whole 16 tokens; head rows of whole 64 bytes; aligned queries
-  float scale;                  // of base-2 logarithms: the softmax's scale times log2(e)
+  int32_t negate;               // the queries
+  float scale;                  // of base-2 logarithms: the softmax's scale times log2(e), > 0
   float decay;
   void* out;
   float* part;     // [2 wgs][16][tile], pieces of rows
   float* part_ml;  // [2 wgs][16][2], their maxima and sums
-  float* lse;      // [batch, q_heads], with weights
+  float* row_ml;   // [batch, q_heads][2], with weights: of rows that one workgroup had
   float* logits;   // [batch, q_heads, logit_stride], with weights
   int64_t logit_stride;
 };
@@ -66,7 +84,6 @@ struct CacheAttendParams {
 hipError_t launch_cache_attend_bf16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f32(const CacheAttendParams& p, hipStream_t st);
-hipError_t launch_cache_weights(const CacheAttendParams& p, hipStream_t st);
 
 struct CacheEvictParams {
   CachePages c;
@@ -83,6 +100,10 @@ hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st);
 
 #ifdef __HIP__
 
+__device__ __forceinline__ int div_by(int n, const FastDiv& d) {
+  return d.mul ? (int)(__umulhi((uint32_t)n, d.mul) >> d.shift) : n;
+}
+
 // tokens in the cache before the call: 0 .. room, or -1 for a count that the table has no room for
 __device__ __forceinline__ int cache_count(const CachePages& c, int b) {
   const int n = c.cached[b];
@@ -91,7 +112,7 @@ __device__ __forceinline__ int cache_count(const CachePages& c, int b) {
 
 // page of token j of sequence b, -1: outside the cache
 __device__ __forceinline__ int cache_page(const CachePages& c, int b, int j) {
-  const int page = c.table[b * c.table_stride + j / c.page_size];
+  const int page = c.table[b * c.table_stride + div_by(j, c.by_page)];
   return (unsigned)page < (unsigned)c.pages ? page : -1;
 }
 

@@ -60,10 +60,11 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheApp
   const int head0 = part * (iters * kHeads) + lane / LANES;
 
   const S* src = (const S*)p.qkv + b * p.b_stride + t * p.t_stride;
+  const bool real = !p.c.fresh || t < p.c.fresh[b];  // (what is behind a sequence's tokens is not read)
   Raw<DT, VEC> x[kIters];
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
-    const int h = i < iters ? head0 + i * kHeads : n_all;
+    const int h = i < iters && real ? head0 + i * kHeads : n_all;
     if (h < n_all && in) load_raw<DT, VEC, true>(src + (int64_t)h * Dh + col, x[i]);
     else x[i] = {};
   }

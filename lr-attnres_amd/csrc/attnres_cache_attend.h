@@ -31,8 +31,8 @@
 
 namespace attnres {
 
-constexpr int kAttWaves = 4;
 constexpr int kAttRows = 16;  // query rows of a workgroup
+constexpr int kAttWaves = 4;
 
 // The deal: `segs` segments (heads, blocks of rows) of each sequence, kUnit tokens a unit, unit x to
 // workgroup deal_of(x).
@@ -61,14 +61,14 @@ __device__ __forceinline__ int wave_scan(int x) {  // inclusive
   return x;
 }
 
-__device__ __forceinline__ Deal deal(const CacheAttendParams& p, int segs, int wgs) {
+__device__ __forceinline__ Deal deal(const CacheAttendParams& p, int segs, int wgs, const FastDiv& by_wgs) {
   const int lane = threadIdx.x & (kWave - 1);
   int sum = 0;
   for (int b0 = 0; b0 < p.c.batch; b0 += kWave) sum += seq_units(p, b0 + lane);
   for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
   Deal d;
   d.total = __builtin_amdgcn_readfirstlane(sum) * segs;
-  d.per = d.total / wgs;
+  d.per = div_by(d.total, by_wgs);
   d.more = d.total - d.per * wgs;
   return d;
 }
@@ -135,19 +135,24 @@ struct Att {
   static constexpr int kWords = kW * kSize / 4;
   static constexpr int kPitch = HD + 4;
   static constexpr float kShift = DT::kCode == 2 ? 14.f : 0.f;
+  static constexpr int kStep = kAttWaves * kTok;               // tokens of a workgroup's round
 
   const CacheAttendParams& p;
   int lane, wave, c, g;          // column (query row) and token group of the lane
   int b, h, n, have;
   int kcol[kKs], vcol[kNi];      // first value of each chunk, inside the row
-  uint32_t kofs[kKs], vofs[kNi]; // PAGE16: bytes from a subtile's first row (of a key), from its token `t`'s (of a value)
+  uint32_t kofs[kKs], vofs[4][kNi]; // PAGE16: bytes from a subtile's first row
+  const S *kh, *vh;              // of the head, page 0
+  att_const_i32* table;          // of the sequence
   u32x4 q[kKs], k[kSub][kKs];
   uint32_t v[kSub][4][kNi][kWords];
   sw_f4 acc[kNi][kW];
-  float m, l;                    // of the lane's row: maximum (less kShift), the lane's part of the sum
+  float m, l;                    // of the lane's row: maximum of <q, k>, the lane's part of the sum
 
   struct Rows {
-    int64_t off[PAGE16 ? kSub : 1];  // of a subtile's first token, or of token `lane` of the tile; -1: no page
+    int64_t off[PAGE16 ? kSub : 1];  // PAGE16: bytes from the head's page 0 to a subtile's first token; else values to token
+                                     // `lane` of the tile, -1: no page
+    bool there[PAGE16 ? kSub : 1];   // PAGE16: whether it has a page (one that has none reads page 0)
   };
 
   __device__ __forceinline__ Att(const CacheAttendParams& p_) : p(p_) {
@@ -165,31 +170,30 @@ struct Att {
 #pragma unroll
       for (int i = 0; i < kNi; ++i) {
         vcol[i] = min(vcol[i], Dh - kW);
-        vofs[i] = (g * 4 * slot + vcol[i]) * kSize;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vofs[t][i] = ((g * 4 + t) * slot + vcol[i]) * kSize;
       }
 #pragma unroll
       for (int i = 0; i < kKs; ++i) kofs[i] = (c * slot + min(kcol[i], Dh - kPer)) * kSize;
     }
   }
 
-  __device__ __forceinline__ Rows rows_of(int t0) const {
+  __device__ __forceinline__ Rows rows_of(int t0) const {  // t0 < n
     Rows r;
     if constexpr (PAGE16) {
 #pragma unroll
       for (int s = 0; s < kSub; ++s) {
-        const int j = min(t0 + 16 * s, (n - 1) & ~15);
-        const int at = j / p.c.page_size;
-        const int page = ((att_const_i32*)(uintptr_t)p.c.table)[b * p.c.table_stride + at];
-        r.off[s] = (unsigned)page < (unsigned)p.c.pages
-                       ? page * p.c.page_stride + h * p.c.head_stride + (j - at * p.c.page_size) * p.c.slot_stride
-                       : -1;
+        const uint32_t j = min((uint32_t)(t0 + 16 * s), (uint32_t)(n - 1) & ~15u);
+        const uint32_t at = __umulhi(j, p.c.by_page.mul) >> p.c.by_page.shift, slot = j - at * p.c.page_size;
+        const uint32_t page = (uint32_t)table[at];
+        r.there[s] = page < (uint32_t)p.c.pages;
+        r.off[s] = (int64_t)((uint64_t)(r.there[s] ? page : 0) * p.c.page_bytes + slot * p.c.slot_bytes);
       }
     } else {
-      const int j = min(t0 + (lane & (kTok - 1)), n - 1);
-      const int at = j / p.c.page_size;
-      const int page = p.c.table[b * p.c.table_stride + at];
+      const int j = min(t0 + (lane & (kTok - 1)), n - 1), at = div_by(j, p.c.by_page);
+      const int page = table[at];
       r.off[0] = (unsigned)page < (unsigned)p.c.pages
-                     ? page * p.c.page_stride + h * p.c.head_stride + (j - at * p.c.page_size) * p.c.slot_stride
+                     ? page * p.c.page_stride + (j - at * p.c.page_size) * p.c.slot_stride
                      : -1;
     }
     return r;
@@ -221,15 +225,22 @@ struct Att {
     }
   }
 
+  // An offset in 32 bits where it is used, for loads from a scalar base: widened outside a loop it would cost 64-bit
+  // additions for each load.
+  static __device__ __forceinline__ uint32_t here(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  }
+
   __device__ __forceinline__ void load_k(const Rows& r) {
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
       if constexpr (PAGE16) {
-        const char* row = (const char*)((const S*)p.c.k + max(r.off[s], (int64_t)0));
+        const char* row = (const char*)kh + r.off[s];
 #pragma unroll
-        for (int i = 0; i < kKs; ++i) k[s][i] = *(const u32x4*)(row + kofs[i]);
+        for (int i = 0; i < kKs; ++i) k[s][i] = *(const u32x4*)(row + here(kofs[i]));
       } else {
-        const S* row = (const S*)p.c.k + max(__shfl(r.off[0], 16 * s + c, kWave), (int64_t)0);
+        const S* row = kh + max(__shfl(r.off[0], 16 * s + c, kWave), (int64_t)0);
 #pragma unroll
         for (int i = 0; i < kKs; ++i) {
           uint32_t w[4];
@@ -247,11 +258,11 @@ struct Att {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         if constexpr (PAGE16) {
-          const char* row = (const char*)((const S*)p.c.v + max(r.off[s], (int64_t)0) + t * p.c.slot_stride);
+          const char* row = (const char*)vh + r.off[s];
 #pragma unroll
-          for (int i = 0; i < kNi; ++i) load_vec<kW>(row + vofs[i], v[s][t][i]);
+          for (int i = 0; i < kNi; ++i) load_vec<kW>(row + here(vofs[t][i]), v[s][t][i]);
         } else {
-          const S* row = (const S*)p.c.v + max(__shfl(r.off[0], 16 * s + g * 4 + t, kWave), (int64_t)0);
+          const S* row = vh + max(__shfl(r.off[0], 16 * s + g * 4 + t, kWave), (int64_t)0);
 #pragma unroll
           for (int i = 0; i < kNi; ++i) {
             if constexpr (VEC) load_vec<kW>(row + vcol[i], v[s][t][i]);
@@ -259,10 +270,6 @@ struct Att {
           }
         }
       }
-  }
-
-  __device__ __forceinline__ bool no_page(const Rows& r, int s, int t) const {
-    return (PAGE16 ? r.off[PAGE16 ? s : 0] : __shfl(r.off[0], 16 * s + g * 4 + t, kWave)) < 0;
   }
 
   // a tile's weights as the second product takes them: fp32, or in two terms
@@ -330,19 +337,32 @@ struct Att {
     return to;
   }
 
+  // over the four lanes of a column
+  template <class F>
+  static __device__ __forceinline__ float across(float x, F f) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  }
+
+  // a maximum as the exponents' base; of no score at all: 0, so that -inf less it stays -inf
+  __device__ __forceinline__ float base_of(float top) const { return top == -INFINITY ? 0.f : top * p.scale - kShift; }
+
   struct Row {       // the lane's
     float* logits;   // of token 0, or null
     int lim;         // tokens that it sees (one that is not there: whatever)
     int t;           // its new token
-    int all;         // tokens that every row sees
   };
 
-  // The tile of tokens t0 .., whose keys and values are on their way; CUT: some row does not see all of it; CARE: by
-  // itself, and so that a value that is not finite shows in the rows that see it and in no other.
-  template <bool CUT, bool CARE>
-  __device__ __forceinline__ void tile(int t0, bool more, const Row& row, Rows& now, Rows& next) {
+  // The tile of tokens t0 .., whose keys and values are on their way.  AHEAD: all rows see all of it, and the next
+  // tile's are loaded where its registers become free (in every turn of the loop: a load under a condition would make
+  // each wait one for all loads).  CARE: a value that is not finite shows in the rows that see it and in no other.
+  template <bool AHEAD, bool CARE>
+  __device__ __forceinline__ void tile(int t0, const Row& row, Rows& now, Rows& next) {
+    constexpr bool CUT = !AHEAD;
     Rows after;
-    if constexpr (!CARE) after = rows_of(min(t0 + 2 * kAttWaves * kTok, n - 1) / kTok * kTok);
+    if constexpr (AHEAD) after = rows_of(min(t0 + 2 * kStep, (n - 1) & -kTok));
     // (before all of the products: no branch comes between them and what reads them)
     if (VEC && !p.whole) {
 #pragma unroll
@@ -358,31 +378,30 @@ struct Att {
 #pragma unroll
       for (int i = 0; i < kKs; ++i) sw_mfma<DT>(k[s][i], q[i], s4[s]);
     }
-    float x[kSub][4];
+    float scale[kSub];  // NaN where there is no page: the row shows it
 #pragma unroll
-    for (int s = 0; s < kSub; ++s)
+    for (int s = 0; s < kSub; ++s) {
+      scale[s] = PAGE16 && !now.there[PAGE16 ? s : 0] ? __builtin_nanf("") : p.scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        x[s][t] = s4[s][t] * p.scale;
-        if (no_page(now, s, t)) x[s][t] = __builtin_nanf("");
-        if (CUT && t0 + 16 * s + g * 4 + t >= row.lim) x[s][t] = -INFINITY;
+        if (!PAGE16 && __shfl(now.off[0], 16 * s + g * 4 + t, kWave) < 0) s4[s][t] = __builtin_nanf("");
+        if (CUT && t0 + 16 * s + g * 4 + t >= row.lim) s4[s][t] = -INFINITY;
       }
-    if (!CARE && more) load_k(next);
+    }
+    if constexpr (AHEAD) load_k(next);
     if (row.logits) {
 #pragma unroll
-      for (int s = 0; s < kSub; ++s)
-        *(sw_f4*)(row.logits + t0 + 16 * s + g * 4) = sw_f4{x[s][0], x[s][1], x[s][2], x[s][3]};
+      for (int s = 0; s < kSub; ++s) *(sw_f4*)(row.logits + t0 + 16 * s + g * 4) = s4[s] * scale[s];
     }
-    float top = x[0][0];
+    float top = s4[0][0];
 #pragma unroll
     for (int s = 0; s < kSub; ++s)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) top = fmaxf(top, x[s][t]);
-    top = fmaxf(top, __shfl_xor(top, 16, kWave));
-    top = fmaxf(top, __shfl_xor(top, 32, kWave)) - kShift;
-    const float to = fmaxf(m, top), base = to == -INFINITY ? 0.f : to;
+      for (int t = 0; t < 4; ++t) top = fmaxf(top, s4[s][t]);
+    top = across(top, [](float a, float b) { return fmaxf(a, b); });
+    const float to = fmaxf(m, top);
     if (__any(to != m)) {
-      const float was = __builtin_amdgcn_exp2f(m - base);
+      const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base_of(m) - base_of(to));
       l *= was;
 #pragma unroll
       for (int i = 0; i < kNi; ++i)
@@ -390,12 +409,13 @@ struct Att {
         for (int d = 0; d < kW; ++d) acc[i][d] *= was;
       m = to;
     }
+    const float base = base_of(to);
     float e[kSub][4];
 #pragma unroll
     for (int s = 0; s < kSub; ++s)
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        e[s][t] = __builtin_amdgcn_exp2f(x[s][t] - base);
+        e[s][t] = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[s][t], scale[s], -base));
         l += e[s][t];
       }
     const Weights w = split(e);
@@ -416,9 +436,11 @@ struct Att {
       for (int i = 0; i < kNi; ++i)
 #pragma unroll
         for (int d = 0; d < kW; ++d) acc[i][d] = weigh<false>(w, i, d, acc[i][d]);
-      if (more) load_v(next);
-      now = next;
-      next = after;
+      if constexpr (AHEAD) {
+        load_v(next);
+        now = next;
+        next = after;
+      }
     } else {
       // (0 times such a value is NaN: each new token's rows take a product without the values behind it)
       for (int tt = p.tokens - 1; tt >= 0; --tt) {
@@ -456,9 +478,12 @@ struct Att {
 
   // tokens [first, end) of the head for rows [row0, row0 + rows); this wave's: tiles wave, wave + 4, ...
   __device__ __forceinline__ void piece(int row0, int rows, int first, int end, float* logits) {
-    const int r = row0 + c, t_row = r / p.group;
+    const int r = row0 + c, t_row = div_by(r, p.by_group);
     const bool valid = c < rows;
     const int hq = h * p.group + r - t_row * p.group;
+    table = (att_const_i32*)(uintptr_t)(p.c.table + b * p.c.table_stride);
+    kh = (const S*)p.c.k + h * p.c.head_stride;
+    vh = (const S*)p.c.v + h * p.c.head_stride;
     const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
 #pragma unroll
     for (int i = 0; i < kKs; ++i) {
@@ -484,20 +509,31 @@ struct Att {
         q[i] = u32x4{w[0], w[1], w[2], w[3]};
       }
     }
+    if (p.negate) {
+#pragma unroll
+      for (int i = 0; i < kKs; ++i) q[i] ^= k32 ? 0x80000000u : 0x80008000u;
+    }
     clear();
     const int lim = min(have + t_row + 1, n);  // of the lane's row (a row that is not there: whatever)
     const int all = p.tokens > 1 ? have + 1 : n;  // tokens that every row sees
-    constexpr int kStep = kAttWaves * kTok;
     const int t_first = first + wave * kTok;
     if (t_first >= end) return;
-    Rows now = rows_of(t_first), next = rows_of(min(t_first + kStep, n - 1) / kTok * kTok);
+    Rows now = rows_of(t_first), next;
     load_k(now);
     load_v(now);
+    next = rows_of(min(t_first + kStep, (n - 1) & -kTok));
     int t0 = t_first;
-    const Row row{logits && valid ? logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row, all};
-    for (; t0 < end && t0 + kTok <= all; t0 += kStep) tile<false, false>(t0, t0 + kStep < end, row, now, next);
-    // tiles that a row does not see all of; never many
-    for (; t0 < end; t0 += kStep) tile<true, false>(t0, t0 + kStep < end, row, now, next);
+    const Row row{logits && valid ? logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row};
+    for (; t0 + kStep < end && t0 + kTok <= all; t0 += kStep) tile<true, false>(t0, row, now, next);
+    // the last tile, and those that a row does not see all of: never many
+    for (;;) {
+      tile<false, false>(t0, row, now, next);
+      t0 += kStep;
+      if (t0 >= end) break;
+      now = rows_of(t0);
+      load_k(now);
+      load_v(now);
+    }
     att_settle();
     float none = 0.f;
 #pragma unroll
@@ -512,11 +548,10 @@ struct Att {
         now = rows_of(t0);
         load_k(now);
         load_v(now);
-        tile<true, true>(t0, false, row, now, now);
+        tile<false, true>(t0, row, now, now);
       }
     }
-    l += __shfl_xor(l, 16, kWave);
-    l += __shfl_xor(l, 32, kWave);
+    l = across(l, [](float a, float b) { return a + b; });
   }
 };
 
@@ -524,6 +559,26 @@ struct Att {
 // alone) weighs nothing, whatever its values: 0 x NaN stays NaN.
 __device__ __forceinline__ float att_share(float m, float top) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// Columns col .. col + 3 of query row `row` of key / value head h: zeros where it saw nothing, NaN for counts that cannot be
+template <class DT>
+__device__ __forceinline__ void att_row_out(const CacheAttendParams& p, int b, int h, int row, int col, int n, float l,
+                                            sw_f4 o) {
+  const int t = div_by(row, p.by_group), hq = h * p.group + row - t * p.group, Dh = p.c.head_dim;
+  const bool seen = n > 0 && (!p.c.fresh || t < p.c.fresh[b]);
+  typename DT::S* out = (typename DT::S*)p.out + ((b * (int64_t)p.tokens + t) * p.q_heads + hq) * Dh + col;
+  const float inv = 1.f / l;
+  float x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = n < 0 ? __builtin_nanf("") : seen ? o[e] * inv : 0.f;
+  if (Dh % 4 == 0) {
+    if (col < Dh) store_vec<DT, 4>(out, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < Dh) DT::store1(out + e, x[e]);
+  }
 }
 
 template <class DT, int HD, bool VEC, bool PAGE16>
@@ -535,11 +590,20 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
   A a(p);
   const int Dh = p.c.head_dim, segs = p.c.kv_heads * p.blocks;
   // neighbouring workgroups run on different XCDs; those of one XCD take neighbouring units
-  const int w = p.wgs % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (p.wgs / 8) + blockIdx.x / 8);
-  const Deal d = deal(p, segs, p.wgs);
-  int x = deal_start(d, w);
-  const int x1 = deal_start(d, w + 1);
-  int b_start = 0, b_end = 0, units = 1;
+  const int grid = gridDim.x;
+  const int w = grid % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8);
+  int x = 0, x1 = 1, b_start = 0, b_end = 0, units = 1;
+  if (p.direct) {  // segment w
+    a.b = div_by(w, p.by_segs);
+    b_start = a.b * segs - w;
+    b_end = 1;
+    a.n = seq_len(p, a.b);
+    a.have = p.c.cached[a.b];
+  } else {
+    const Deal d = deal(p, segs, p.wgs, p.by_wgs);
+    x = deal_start(d, w);
+    x1 = deal_start(d, w + 1);
+  }
   while (x < x1) {
     if (x >= b_end) {
       find_unit(p, segs, x, &a.b, &b_start, &units);
@@ -549,11 +613,12 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
     }
     const int seg = (x - b_start) / units, u0 = x - b_start - seg * units, u1 = min(units, u0 + x1 - x);
     x += u1 - u0;
-    a.h = seg / p.blocks;
+    a.h = div_by(seg, p.by_blocks);
     const int row0 = (seg - a.h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
-    a.piece(row0, rows, u0 * kAttUnit, min(u1 * kAttUnit, a.n), p.logits);
-    if (a.c < rows) {
-      if (a.g == 0) sm[a.wave][a.c] = a.m, sl[a.wave][a.c] = a.l;
+    const bool whole = u0 == 0 && u1 == units;
+    if (a.n > 0) a.piece(row0, rows, u0 * kAttUnit, p.direct ? a.n : min(u1 * kAttUnit, a.n), p.logits);
+    if (a.n > 0 && a.c < rows) {
+      if (a.g == 0) sm[a.wave][a.c] = a.m == -INFINITY ? a.m : a.base_of(a.m), sl[a.wave][a.c] = a.l;
 #pragma unroll
       for (int i = 0; i < A::kNi; ++i)
 #pragma unroll
@@ -564,30 +629,28 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
                 sw_f4{a.acc[i][e][t], a.acc[i][e + 1][t], a.acc[i][e + 2][t], a.acc[i][e + 3][t]};
     }
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == units;
     const int64_t slot = 2 * w + (u0 == 0 ? 1 : 0);
     for (int at = threadIdx.x; at < rows * (HD / 4); at += kAttWaves * kWave) {
       const int r = at / (HD / 4), col = at % (HD / 4) * 4;
-      float top = sm[0][r];
-#pragma unroll
-      for (int i = 1; i < kAttWaves; ++i) top = fmaxf(top, sm[i][r]);
-      float l = 0.f;
+      float top = -INFINITY, l = 0.f;
       sw_f4 o = {0.f, 0.f, 0.f, 0.f};
+      if (a.n > 0) {
 #pragma unroll
-      for (int i = 0; i < kAttWaves; ++i) {
-        const float f = att_share(sm[i][r], top);
-        l += f * sl[i][r];
-        o += f * *(const sw_f4*)&so[i][r][col];
+        for (int i = 0; i < kAttWaves; ++i) top = fmaxf(top, sm[i][r]);
+#pragma unroll
+        for (int i = 0; i < kAttWaves; ++i) {
+          const float f = att_share(sm[i][r], top);
+          l += f * sl[i][r];
+          o += f * *(const sw_f4*)&so[i][r][col];
+        }
       }
       if (whole) {
-        const int t = (row0 + r) / p.group, hq = a.h * p.group + row0 + r - t * p.group;
-        const bool seen = !p.c.fresh || t < p.c.fresh[a.b];
-        S* out = (S*)p.out + ((a.b * (int64_t)p.tokens + t) * p.q_heads + hq) * Dh + col;
-        const float inv = 1.f / l;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < Dh) DT::store1(out + e, seen ? o[e] * inv : 0.f);
-        if (p.lse && col == 0) p.lse[a.b * p.q_heads + hq] = top + log2f(l);
+        att_row_out<DT>(p, a.b, a.h, row0 + r, col, a.n, l, o);
+        if (p.row_ml && col == 0) {
+          float* ml = p.row_ml + (a.b * (int64_t)p.q_heads + a.h * p.group + row0 + r) * 2;
+          ml[0] = top;
+          ml[1] = l;
+        }
       } else {
         *(sw_f4*)(p.part + (slot * kAttRows + r) * HD + col) = o;
         if (col == 0) {
@@ -600,83 +663,146 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
   }
 }
 
-// A head's pieces joined; zeros for rows that see nothing, NaN for counts that cannot be.  One workgroup a
-// segment: threads take four columns of a row, and where there are fewer of them, a share of the pieces.
+// The workgroups that have a segment of sequence b: w0 .. w1, none if it has no units.
+struct Pieces {
+  int w0, w1;
+};
+__device__ __forceinline__ Pieces pieces_of(const CacheAttendParams& p, int b, int seg) {
+  const int segs = p.c.kv_heads * p.blocks, units = seq_units(p, b);
+  if (!units) return Pieces{0, -1};
+  if (p.direct) return Pieces{0, 0};
+  const Deal d = deal(p, segs, p.wgs, p.by_wgs);
+  const int first = units_before(p, b, segs) + seg * units;
+  return Pieces{deal_of(d, first), deal_of(d, first + units - 1)};
+}
+__device__ __forceinline__ int64_t piece_row(const Pieces& s, int w, int row) {
+  return (2 * w + (w == s.w0 ? 1 : 0)) * (int64_t)kAttRows + row % kAttRows;
+}
+
+// A head's pieces joined; zeros for rows that see nothing, NaN for counts that cannot be.  A workgroup for each
+// row: its threads take four columns each, and a share of the pieces.
 template <class DT, int HD>
-__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p) {
-  using S = typename DT::S;
+__device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
   __shared__ float sm[256], sl[256];
   __shared__ sw_f4 so[256];
-  const int Dh = p.c.head_dim, segs = p.c.kv_heads * p.blocks;
-  const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs, h = seg / p.blocks;
-  const int row0 = (seg - h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
-  const int n = seq_len(p, b), units = seq_units(p, b);
-  int w0 = 0, w1 = -1;
-  if (units) {
-    const Deal d = deal(p, segs, p.wgs);
-    const int first = units_before(p, b, segs) + seg * units;
-    w0 = deal_of(d, first), w1 = deal_of(d, first + units - 1);
-    if (w0 == w1) return;  // one workgroup had all of it
-  }
-  const int items = rows * (HD / 4), shares = max(1, 256 / items);
-  for (int i0 = 0; i0 < items; i0 += 256) {
-    const int item = shares > 1 ? threadIdx.x % items : i0 + threadIdx.x, share = shares > 1 ? threadIdx.x / items : 0;
-    const int r = item / (HD / 4), col = item % (HD / 4) * 4;
-    const bool in = share < shares && item < items;
-    float top = -INFINITY, l = 0.f;
-    sw_f4 o = {0.f, 0.f, 0.f, 0.f};
-    if (in) {
-      for (int w = w0 + share; w <= w1; w += shares) {
-        const int64_t row = (2 * w + (w == w0 ? 1 : 0)) * (int64_t)kAttRows + r;
-        const float m = p.part_ml[row * 2], part = p.part_ml[row * 2 + 1];
-        const sw_f4 x = *(const sw_f4*)(p.part + row * HD + col);
-        const float to = fmaxf(top, m), f = att_share(top, to), g = att_share(m, to);
-        l = f * l + g * part;
-        o = f * o + g * x;
-        top = to;
-      }
-    }
-    if (shares > 1) {
-      sm[threadIdx.x] = top;
-      sl[threadIdx.x] = l;
-      so[threadIdx.x] = o;
-      __syncthreads();
-      if (share == 0 && in) {
-        float all = top;
-        for (int i = 1; i < shares; ++i) all = fmaxf(all, sm[i * items + item]);
-        const float f = att_share(top, all);
-        l *= f;
-        o *= f;
-        for (int i = 1; i < shares; ++i) {
-          const float g = att_share(sm[i * items + item], all);
-          l += g * sl[i * items + item];
-          o += g * so[i * items + item];
-        }
-        top = all;
-      }
-    }
-    if (in && share == 0) {
-      const int t = (row0 + r) / p.group, hq = h * p.group + row0 + r - t * p.group;
-      const bool seen = units && (!p.c.fresh || t < p.c.fresh[b]);
-      S* out = (S*)p.out + ((b * (int64_t)p.tokens + t) * p.q_heads + hq) * Dh + col;
-      const float inv = 1.f / l;
+  const int row = at % p.rows, bh = at / p.rows, b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads;
+  const Pieces s = pieces_of(p, b, h * p.blocks + row / kAttRows);
+  if (s.w0 == s.w1) return;  // one workgroup had all of it
+  constexpr int kItems = HD / 4, kShares = 256 / kItems, kBatch = 4;
+  const int item = threadIdx.x % kItems, share = threadIdx.x / kItems, col = item * 4;
+  float top = -INFINITY, l = 0.f;
+  sw_f4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int w = s.w0 + share; w <= s.w1; w += kShares * kBatch) {
+    float m[kBatch], part[kBatch];
+    sw_f4 x[kBatch];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < Dh) DT::store1(out + e, n < 0 ? __builtin_nanf("") : seen ? o[e] * inv : 0.f);
-      if (p.lse && col == 0) p.lse[b * p.q_heads + hq] = top + log2f(l);
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t r = piece_row(s, min(w + i * kShares, s.w1), row);
+      m[i] = p.part_ml[r * 2];
+      part[i] = p.part_ml[r * 2 + 1];
+      x[i] = *(const sw_f4*)(p.part + r * HD + col);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (w + i * kShares > s.w1) break;
+      const float to = fmaxf(top, m[i]), f = att_share(top, to), g = att_share(m[i], to);
+      l = f * l + g * part[i];
+      o = f * o + g * x[i];
+      top = to;
     }
   }
+  sm[threadIdx.x] = top;
+  sl[threadIdx.x] = l;
+  so[threadIdx.x] = o;
+  __syncthreads();
+  if (share) return;
+  float all = top;
+#pragma unroll
+  for (int i = 1; i < kShares; ++i) all = fmaxf(all, sm[i * kItems + item]);
+  float f = att_share(top, all);
+  l *= f;
+  o *= f;
+#pragma unroll
+  for (int i = 1; i < kShares; ++i) {
+    f = att_share(sm[i * kItems + item], all);
+    l += f * sl[i * kItems + item];
+    o += f * so[i * kItems + item];
+  }
+  att_row_out<DT>(p, b, h, row, col, seq_len(p, b), l, o);
+}
+
+// What each cached token received: with the scores x as attention left them (base-2 logarithms),
+//   w_j <- decay w_j + sum over the head's queries of 2^(x_j - lse).
+// Bound by memory: a group's scores read, the weights read and written, 4 bytes each.  Tokens are dealt
+// to workgroups as attention's units are; a row's lse comes from its pieces again, beside the join, which would
+// otherwise have to end first.
+__device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) {
+  __shared__ float lse[256];  // of the head's rows, 256 of them at a time
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, segs = p.c.kv_heads;
+  const Deal d = deal(p, segs, p.weight_wgs, p.by_weight_wgs);
+  const int x1 = deal_start(d, at + 1);
+  int b = 0, b_start = 0, b_end = 0, units = 1, n = 0;
+  for (int x = deal_start(d, at); x < x1; ++x) {
+    if (x >= b_end) {
+      find_unit(p, segs, x, &b, &b_start, &units);
+      b_end = b_start + segs * units;
+      n = seq_len(p, b);
+    }
+    const int h = (x - b_start) / units, j = (x - b_start - h * units) * kAttUnit + threadIdx.x;
+    float sum = 0.f;
+    for (int g0 = 0; g0 < p.group; g0 += 256) {
+      const int rows = min(256, p.group - g0);
+      __syncthreads();
+      for (int r = wave; r < rows; r += 256 / kWave) {
+        const int row = g0 + r;
+        const Pieces s = pieces_of(p, b, h * p.blocks + row / kAttRows);
+        float top = -INFINITY, l = 0.f;
+        if (s.w0 == s.w1) {
+          top = p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2];
+          l = lane ? 0.f : p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2 + 1];
+        }
+        for (int w = s.w0 + lane; w <= s.w1 && s.w0 != s.w1; w += kWave) {
+          const int64_t i = piece_row(s, w, row);
+          const float m = p.part_ml[i * 2], to = fmaxf(top, m);
+          l = att_share(top, to) * l + att_share(m, to) * p.part_ml[i * 2 + 1];
+          top = to;
+        }
+        float all = top;
+        for (int o = 1; o < kWave; o <<= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
+        l = wave_sum(att_share(top, all) * l);
+        if (lane == 0) lse[r] = all + log2f(l);
+      }
+      __syncthreads();
+      if (j < n)
+        for (int r = 0; r < rows; ++r)
+          sum += __builtin_amdgcn_exp2f(p.logits[(b * (int64_t)p.q_heads + h * p.group + g0 + r) * p.logit_stride + j] - lse[r]);
+    }
+    if (j >= n) continue;
+    const int page = cache_page(p.c, b, j);
+    if (page < 0) continue;
+    float* w = p.c.w + page * p.c.w_page_stride + h * p.c.w_head_stride + (j - div_by(j, p.c.by_page) * p.c.page_size);
+    *w = p.decay == 0.f ? sum : p.decay * *w + sum;
+  }
+}
+
+// joins: workgroups that join rows; the others behind them add weights up
+template <class DT, int HD>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p, int joins) {
+  if ((int)blockIdx.x < joins) join_row<DT, HD>(p, blockIdx.x);
+  else add_weights(p, blockIdx.x - joins);
 }
 
 template <class DT, int HD>
 hipError_t run_attend(const CacheAttendParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.wgs), wg(kAttWaves * kWave);
+  const int64_t segs = (int64_t)p.c.batch * p.c.kv_heads * p.blocks;
+  const dim3 grid((unsigned)(p.direct ? segs : p.wgs)), wg(kAttWaves * kWave);
   if (p.vec && p.page16) cache_attend_kernel<DT, HD, true, true><<<grid, wg, 0, st>>>(p);
   else if (p.vec) cache_attend_kernel<DT, HD, true, false><<<grid, wg, 0, st>>>(p);
   else cache_attend_kernel<DT, HD, false, false><<<grid, wg, 0, st>>>(p);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  cache_join_kernel<DT, HD><<<dim3((unsigned)(p.c.batch * p.c.kv_heads * p.blocks)), dim3(256), 0, st>>>(p);
+  const hipError_t err = hipGetLastError();
+  const int joins = p.direct ? 0 : p.c.batch * p.c.kv_heads * p.rows;
+  if (err != hipSuccess || joins + p.weight_wgs == 0) return err;
+  cache_join_kernel<DT, HD><<<dim3((unsigned)(joins + p.weight_wgs)), dim3(256), 0, st>>>(p, joins);
   return hipGetLastError();
 }
 

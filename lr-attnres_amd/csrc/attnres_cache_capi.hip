@@ -1,5 +1,6 @@
 // C ABI of the paged cache's kernels: argument checks and kernel selection.
 // Declared in include/attnres_cache.h.
+#include <float.h>
 #include <math.h>
 #include <string.h>
 
@@ -9,6 +10,8 @@
 using namespace attnres;
 
 namespace {
+
+constexpr int kCus = 256;
 
 int es_of(int dtype) { return dtype == ATTNRES_DTYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
@@ -60,6 +63,9 @@ CachePages pages_of(const attnres_cache_desc* c) {
   p.page_size = c->page_size;
   p.pages = (int32_t)c->pages;
   p.room = (int32_t)(c->table_pages * c->page_size);
+  p.by_page = fast_div(c->page_size);
+  p.page_bytes = (uint32_t)(c->page_stride * es_of(c->dtype));
+  p.slot_bytes = (uint32_t)(c->slot_stride * es_of(c->dtype));
   return p;
 }
 
@@ -156,9 +162,9 @@ namespace {
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct AttendPlan {
-  int tile, rows, blocks, wgs;
+  int tile, rows, blocks, wgs, direct, page16;
   int64_t logit_stride;
-  size_t part, part_ml, lse, logits, need;  // offsets in the workspace, and its size
+  size_t part, part_ml, row_ml, logits, need;  // offsets in the workspace, and its size
 };
 
 int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d, AttendPlan* a) {
@@ -168,20 +174,37 @@ int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d,
   if (rows > INT32_MAX || segs > (1 << 23) || segs * (units > 0 ? units : 1) > INT32_MAX / 2)
     return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d, %lld cached: too many tokens", (long long)c->batch,
                     (long long)d->tokens, d->q_heads, (long long)room);
+  // (pages, and tokens inside one, within 32-bit offsets of each other)
+  constexpr int64_t kFar = (int64_t)1 << 32;
+  a->page16 = c->page_size % 16 == 0 && c->page_stride < kFar / es_of(c->dtype) &&
+              c->slot_stride < kFar / es_of(c->dtype) / c->page_size;
   a->tile = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
   a->rows = (int)rows;
   a->blocks = (int)blocks;
-  const int64_t most = a->tile == 64 ? 1024 : a->tile == 128 ? 768 : 512;
+  // One workgroup a CU takes all that a CU can have in flight (2, 3 or 4, or twice the waves: the same to 3%).
   const int64_t all = segs * units;
-  a->wgs = (int)(all < most ? (all > 0 ? all : 1) : most);
+  a->wgs = (int)(all < kCus ? (all > 0 ? all : 1) : kCus);
+  // A CU reads at most 48 bytes a ns, and a round of its waves' tiles takes 650 ns (1100 with tokens looked up one by
+  // one); all CUs read 5500; joining takes 6 us.  A segment that is read in one piece, if it fills its table, ends the
+  // call at best after its rounds, all of them (half full) after segs * room_bytes / 2 / 5500.  Where that is later by
+  // less than the join, a workgroup takes a whole segment and writes its rows.  (us, whole / split: 16 x 12 heads of up to 2048 x
+  // 64 bf16 15.4 / 14 + 4; 12 heads of 300 5.6 / 6.8 + 4; 32 segments of up to 4096 25 / 9.4 + 4; 64 of up to 8192 x 128 fp16 100 / 48
+  // + 5; 15 heads of up to 700 x 40 fp32 15.5 / 10.3 + 4.)  Lengths are on the device alone, so longer tables are split though they
+  // may be nearly empty, and one long sequence among short ones is shared.
+  const int es = es_of(c->dtype);
+  const double room_bytes = 2.0 * room * c->head_dim * es, rounds = (double)room / (es == 4 || a->tile == 256 ? 64 : 128);
+  const double round_ns = a->page16 ? 650 : 1100;
+  const double piece_ns = rounds * round_ns > room_bytes / 48 ? rounds * round_ns : room_bytes / 48;
+  a->direct = room_bytes <= 1 << 20 && piece_ns - segs * room_bytes / 11000.0 <= 6000;
+  if (a->direct) a->wgs = 0;
   a->logit_stride = (room + 31) / 32 * 32;
   size_t at = 0;
   a->part = at;
   at += up256((size_t)2 * a->wgs * 16 * a->tile * 4);
   a->part_ml = at;
   at += up256((size_t)2 * a->wgs * 16 * 2 * 4);
-  a->lse = at;
-  if (c->weights) at += up256((size_t)c->batch * d->q_heads * 4);
+  a->row_ml = at;
+  if (c->weights) at += up256((size_t)c->batch * d->q_heads * 2 * 4);
   a->logits = at;
   if (c->weights) at += up256((size_t)c->batch * d->q_heads * a->logit_stride * 4);
   a->need = at;
@@ -203,7 +226,7 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   AttendPlan a;
   if (int rc = plan_attend(c, d, &a)) return rc;
   if (!out) return api_fail(ATTNRES_EINVAL, "out is NULL");
-  if (!workspace || workspace_bytes < a.need || !aligned(workspace, 256))
+  if (a.need && (!workspace || workspace_bytes < a.need || !aligned(workspace, 256)))
     return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", a.need, workspace ? workspace_bytes : (size_t)0);
   const int es = es_of(c->dtype), per = 16 / es;
   CacheAttendParams p{};
@@ -218,20 +241,33 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   p.rows = a.rows;
   p.blocks = a.blocks;
   p.wgs = a.wgs;
+  p.direct = a.direct;
+  p.by_group = fast_div(p.group);
+  p.by_blocks = fast_div(a.blocks);
+  p.by_segs = fast_div(c->kv_heads * a.blocks);
+  p.by_wgs = fast_div(a.wgs);
+  if (c->weights) {
+    const int64_t units = c->batch * c->kv_heads * ((p.c.room + kAttUnit - 1) / kAttUnit);
+    p.weight_wgs = (int32_t)(units < 16 * kCus ? units : 16 * kCus);
+    p.by_weight_wgs = fast_div(p.weight_wgs);
+  }
   p.tile = a.tile;
   p.vec = rows_at(c, per);
-  // (a subtile's rows within 32-bit offsets of its first one)
-  p.page16 = c->page_size % 16 == 0 && c->slot_stride < (1 << 25);
+  p.page16 = a.page16;
   p.whole = c->head_dim == a.tile;
   p.q_vec = aligned(d->q, 16) && d->q_batch_stride % per == 0 && d->q_head_stride % per == 0 && d->q_token_stride % per == 0;
-  p.scale = (float)((double)d->scale * 1.4426950408889634);
+  // (the kernels take the maximum before they scale: a negative scale goes into the queries' sign, and 0 is as good as
+  // the smallest number, which masked scores of -inf times it stay -inf with)
+  p.negate = d->scale < 0;
+  p.scale = (float)(fabs((double)d->scale) * 1.4426950408889634);
+  if (!(p.scale >= FLT_MIN)) p.scale = FLT_MIN;
   p.decay = d->decay;
   p.out = out;
   char* ws = (char*)workspace;
   p.part = (float*)(ws + a.part);
   p.part_ml = (float*)(ws + a.part_ml);
   if (c->weights) {
-    p.lse = (float*)(ws + a.lse);
+    p.row_ml = (float*)(ws + a.row_ml);
     p.logits = (float*)(ws + a.logits);
     p.logit_stride = a.logit_stride;
   }
@@ -239,7 +275,6 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   hipError_t err = c->dtype == ATTNRES_DTYPE_F32    ? launch_cache_attend_f32(p, st)
                    : c->dtype == ATTNRES_DTYPE_BF16 ? launch_cache_attend_bf16(p, st)
                                                     : launch_cache_attend_f16(p, st);
-  if (err == hipSuccess && c->weights) err = launch_cache_weights(p, st);
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache attend launch failed: %s", hipGetErrorString(err));
   return ATTNRES_OK;
 }
