@@ -122,7 +122,11 @@ int attnres_cache_attend(const attnres_cache_desc* cache, const attnres_cache_at
  * page lies outside the cache has the lowest weight and is not copied.
  */
 int attnres_cache_evict(const attnres_cache_desc* cache, const int32_t* new_table, int64_t new_stride, int64_t budget,
-                        int64_t recent, int32_t* kept, int32_t* left, void* stream);
+                        int64_t recent, int32_t* kept, int32_t* left, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Workspace bytes (host computation; aligned to 256); 0 for tables of few tokens. */
+size_t attnres_cache_evict_workspace_size(const attnres_cache_desc* cache, int64_t budget, int64_t recent);
 
 #ifdef __cplusplus
 }

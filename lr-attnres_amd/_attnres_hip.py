@@ -393,7 +393,9 @@ def load() -> ctypes.CDLL:
                                          c_void_p]
     lib.attnres_cache_evict.restype = c_int
     lib.attnres_cache_evict.argtypes = [POINTER(CacheDesc), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
-                                        c_void_p]
+                                        c_void_p, c_size_t, c_void_p]
+    lib.attnres_cache_evict_workspace_size.restype = c_size_t
+    lib.attnres_cache_evict_workspace_size.argtypes = [POINTER(CacheDesc), c_int64, c_int64]
     lib.attnres_test_phase2_block_layout.restype = c_int
     lib.attnres_test_phase2_block_layout.argtypes = [c_int]
     lib.attnres_kernel_times.restype = c_int
@@ -1332,6 +1334,8 @@ def cache_evict(k_pages, v_pages, weights, block_table, cached, new_table, budge
     c = cache_desc(k_pages, v_pages, weights, block_table, cached, None)
     kept = torch.empty((c.batch, c.kv_heads, budget), dtype=torch.int32, device=k_pages.device)
     left = torch.empty((c.batch,), dtype=torch.int32, device=k_pages.device)
+    n = load().attnres_cache_evict_workspace_size(ctypes.byref(c), budget, recent)
+    ws = torch.empty((n,), dtype=torch.uint8, device=k_pages.device) if n else None
     _check(load().attnres_cache_evict(ctypes.byref(c), _ptr(new_table), new_table.stride(0), budget, recent, _ptr(kept),
-                                      _ptr(left), _stream(k_pages.device)), "cache evict")
+                                      _ptr(left), _ptr(ws), n, _stream(k_pages.device)), "cache evict")
     return kept, left

@@ -56,7 +56,7 @@ struct CacheAppendParams {
 // vec, lanes: as launch_qkv_rotary's
 hipError_t launch_cache_append(int dtype, bool f32_table, const CacheAppendParams& p, int vec, int lanes, hipStream_t st);
 
-constexpr int kAttUnit = 256;  // tokens of a unit of attention's work
+constexpr int kAttUnit = 128;  // tokens of a unit of attention's work
 
 struct CacheAttendParams {
   CachePages c;
@@ -85,6 +85,8 @@ hipError_t launch_cache_attend_bf16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f32(const CacheAttendParams& p, hipStream_t st);
 
+constexpr int kEvictSlice = 8192;  // tokens whose keys a workgroup holds
+
 struct CacheEvictParams {
   CachePages c;
   const int32_t* new_table;
@@ -93,6 +95,8 @@ struct CacheEvictParams {
   int32_t* kept;
   int32_t* left;
   int32_t es;   // bytes of a value
+  int32_t slices;  // of a table
+  int32_t* hist;   // [heads][slices][6144], where there are several
   int32_t vec;  // rows in whole vectors of 16 bytes
 };
 

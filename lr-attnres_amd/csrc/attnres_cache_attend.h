@@ -40,34 +40,59 @@ struct Deal {
   int total, per, more;  // units; of a workgroup; the first `more` have one more
 };
 
-// tokens that the queries of sequence b see together; 0: none has any, -1: counts that cannot be
-__device__ __forceinline__ int seq_len(const CacheAttendParams& p, int b) {
-  const int have = p.c.cached[b], fresh = p.c.fresh ? min(p.c.fresh[b], p.tokens) : p.tokens;
+typedef const __attribute__((address_space(4))) int32_t att_const_i32;  // read by the scalar unit
+
+// tokens that a sequence's queries see together; 0: it has none, -1: counts that cannot be
+__device__ __forceinline__ int seen_of(const CacheAttendParams& p, int have, int fresh) {
   const int64_t n = (int64_t)have + fresh;
   if (have < 0 || fresh < 0 || n > p.c.room || (fresh > 0 && p.c.pages == 0)) return -1;
   return fresh > 0 ? (int)n : 0;
 }
-__device__ __forceinline__ int seq_units(const CacheAttendParams& p, int b) {
-  return b < p.c.batch ? (max(seq_len(p, b), 0) + kAttUnit - 1) / kAttUnit : 0;
+__device__ __forceinline__ int units_of(int n) { return (max(n, 0) + kAttUnit - 1) / kAttUnit; }
+
+struct Seq {
+  int have, n;
+};
+__device__ __forceinline__ Seq seq_of(const CacheAttendParams& p, int b) {  // b the same in all lanes
+  const int have = ((att_const_i32*)(uintptr_t)p.c.cached)[b];
+  const int fresh = p.c.fresh ? min(((att_const_i32*)(uintptr_t)p.c.fresh)[b], p.tokens) : p.tokens;
+  return Seq{have, seen_of(p, have, fresh)};
 }
 
-__device__ __forceinline__ int wave_scan(int x) {  // inclusive
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int y = __shfl_up(x, o, kWave);
-    if (lane >= o) x += y;
-  }
+// over the lanes up to and with this one, by moves inside rows of 16 lanes and broadcasts of a row's last
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // 1, 2, 4, 8 to the right
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 into rows 1 and 3's, of 0 and 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 into rows 2 and 3
   return x;
 }
 
-__device__ __forceinline__ Deal deal(const CacheAttendParams& p, int segs, int wgs, const FastDiv& by_wgs) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int sum = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += kWave) sum += seq_units(p, b0 + lane);
-  for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+// 64 sequences, one a lane: those from b0 on
+struct Chunk {
+  int b0, have, n, units, upto;  // upto: units of a segment of each sequence up to and with this one
+  __device__ __forceinline__ void load(const CacheAttendParams& p, int b0_, int before) {
+    const int b = b0_ + (int)(threadIdx.x & (kWave - 1));
+    b0 = b0_;
+    have = n = 0;
+    if (b < p.c.batch) {
+      have = p.c.cached[b];
+      n = seen_of(p, have, p.c.fresh ? min(p.c.fresh[b], p.tokens) : p.tokens);
+    }
+    units = units_of(n);
+    upto = wave_scan(units) + before;
+  }
+  __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, kWave - 1); }
+};
+
+// A cache's units among `wgs` workgroups.  Leaves the last 64 sequences in `c` (all of them, mostly).
+__device__ __forceinline__ Deal deal(const CacheAttendParams& p, int segs, int wgs, const FastDiv& by_wgs, Chunk& c) {
+  c.load(p, 0, 0);
+  for (int b0 = kWave; b0 < p.c.batch; b0 += kWave) c.load(p, b0, c.last());
   Deal d;
-  d.total = __builtin_amdgcn_readfirstlane(sum) * segs;
+  d.total = c.last() * segs;
   d.per = div_by(d.total, by_wgs);
   d.more = d.total - d.per * wgs;
   return d;
@@ -79,30 +104,18 @@ __device__ __forceinline__ int deal_of(const Deal& d, int x) {
 }
 
 // The sequence that unit x is of, its first unit and how many a segment has.  Every x below the total is of one.
-__device__ __forceinline__ void find_unit(const CacheAttendParams& p, int segs, int x, int* b, int* start, int* units) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int before = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += kWave) {
-    const int u = seq_units(p, b0 + lane);
-    const int upto = wave_scan(u) + before;
-    const int last = __builtin_amdgcn_readlane(upto, kWave - 1);
-    if (x < last * segs) {
-      const int i = __popcll(__ballot(upto * segs <= x));
-      *b = b0 + i;
-      *units = __builtin_amdgcn_readlane(u, i);
-      *start = (__builtin_amdgcn_readlane(upto, i) - *units) * segs;
-      return;
-    }
-    before = last;
+__device__ __forceinline__ void find_unit(const CacheAttendParams& p, int segs, int x, Chunk& c, int* b, Seq* q, int* start,
+                                          int* units) {
+  if (p.c.batch > kWave) {
+    c.load(p, 0, 0);
+    while (x >= c.last() * segs) c.load(p, c.b0 + kWave, c.last());
   }
-}
-// the first unit of sequence b
-__device__ __forceinline__ int units_before(const CacheAttendParams& p, int b, int segs) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int sum = 0;
-  for (int b0 = 0; b0 < b; b0 += kWave) sum += b0 + lane < b ? seq_units(p, b0 + lane) : 0;
-  for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-  return __builtin_amdgcn_readfirstlane(sum) * segs;
+  const int i = __popcll(__ballot(c.upto * segs <= x));
+  *b = c.b0 + i;
+  q->have = __builtin_amdgcn_readlane(c.have, i);
+  q->n = __builtin_amdgcn_readlane(c.n, i);
+  *units = __builtin_amdgcn_readlane(c.units, i);
+  *start = (__builtin_amdgcn_readlane(c.upto, i) - *units) * segs;
 }
 
 #ifdef ATTNRES_CACHE_ATTEND_KERNELS
@@ -117,7 +130,6 @@ __device__ __forceinline__ void att_settle() {
 }
 
 typedef _Float16 att_h4 __attribute__((ext_vector_type(4)));
-typedef const __attribute__((address_space(4))) int32_t att_const_i32;  // read by the scalar unit
 
 // HD: head width's tile (64, 128, 256); VEC: rows in aligned 16-byte vectors; PAGE16: pages of a multiple
 // of 16 tokens, so that 16 tokens lie in one and the scalar unit finds it.
@@ -178,19 +190,21 @@ struct Att {
     }
   }
 
-  __device__ __forceinline__ Rows rows_of(int t0) const {  // t0 < n
+  // of the tile at t0 < limit: the sequence's length, or the table's room before that is known (a page that is not
+  // there reads page 0, and the tile is not used)
+  __device__ __forceinline__ Rows rows_of(int t0, int limit) const {
     Rows r;
     if constexpr (PAGE16) {
 #pragma unroll
       for (int s = 0; s < kSub; ++s) {
-        const uint32_t j = min((uint32_t)(t0 + 16 * s), (uint32_t)(n - 1) & ~15u);
+        const uint32_t j = min((uint32_t)(t0 + 16 * s), (uint32_t)(limit - 1) & ~15u);
         const uint32_t at = __umulhi(j, p.c.by_page.mul) >> p.c.by_page.shift, slot = j - at * p.c.page_size;
         const uint32_t page = (uint32_t)table[at];
         r.there[s] = page < (uint32_t)p.c.pages;
         r.off[s] = (int64_t)((uint64_t)(r.there[s] ? page : 0) * p.c.page_bytes + slot * p.c.slot_bytes);
       }
     } else {
-      const int j = min(t0 + (lane & (kTok - 1)), n - 1), at = div_by(j, p.c.by_page);
+      const int j = min(t0 + (lane & (kTok - 1)), limit - 1), at = div_by(j, p.c.by_page);
       const int page = table[at];
       r.off[0] = (unsigned)page < (unsigned)p.c.pages
                      ? page * p.c.page_stride + (j - at * p.c.page_size) * p.c.slot_stride
@@ -277,6 +291,11 @@ struct Att {
     u32x4 hi, lo;
     float e[kSub][4];
   };
+  // two values in 16 bits; fp16 towards zero (one instruction): the second term takes what the first leaves
+  static __device__ __forceinline__ uint32_t terms(float a, float b) {
+    if constexpr (DT::kCode == 2) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    else return pack2<DT>(a, b);
+  }
   static __device__ __forceinline__ Weights split(const float (&e)[kSub][4]) {
     Weights w;
 #pragma unroll
@@ -285,9 +304,9 @@ struct Att {
       for (int t = 0; t < 4; t += 2) {
         w.e[s][t] = e[s][t], w.e[s][t + 1] = e[s][t + 1];
         if constexpr (!k32) {
-          const uint32_t x = pack2<DT>(e[s][t], e[s][t + 1]);
+          const uint32_t x = terms(e[s][t], e[s][t + 1]);
           w.hi[s * 2 + t / 2] = x;
-          w.lo[s * 2 + t / 2] = pack2<DT>(e[s][t] - bits_to_float<DT>(x & 0xffffu), e[s][t + 1] - bits_to_float<DT>(x >> 16));
+          w.lo[s * 2 + t / 2] = terms(e[s][t] - bits_to_float<DT>(x & 0xffffu), e[s][t + 1] - bits_to_float<DT>(x >> 16));
         }
       }
     return w;
@@ -362,7 +381,7 @@ struct Att {
   __device__ __forceinline__ void tile(int t0, const Row& row, Rows& now, Rows& next) {
     constexpr bool CUT = !AHEAD;
     Rows after;
-    if constexpr (AHEAD) after = rows_of(min(t0 + 2 * kStep, (n - 1) & -kTok));
+    if constexpr (AHEAD) after = rows_of(min(t0 + 2 * kStep, (n - 1) & -kTok), n);
     // (before all of the products: no branch comes between them and what reads them)
     if (VEC && !p.whole) {
 #pragma unroll
@@ -381,7 +400,7 @@ struct Att {
     float scale[kSub];  // NaN where there is no page: the row shows it
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
-      scale[s] = PAGE16 && !now.there[PAGE16 ? s : 0] ? __builtin_nanf("") : p.scale;
+      scale[s] = PAGE16 && !now.there[PAGE16 ? s : 0] && (!CUT || t0 + 16 * s < n) ? __builtin_nanf("") : p.scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         if (!PAGE16 && __shfl(now.off[0], 16 * s + g * 4 + t, kWave) < 0) s4[s][t] = __builtin_nanf("");
@@ -476,14 +495,24 @@ struct Att {
       for (int d = 0; d < kW; ++d) acc[i][d] = sw_f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // tokens [first, end) of the head for rows [row0, row0 + rows); this wave's: tiles wave, wave + 4, ...
-  __device__ __forceinline__ void piece(int row0, int rows, int first, int end, float* logits) {
+  // tokens [first, end) of the head for rows [row0, row0 + rows), of those that there are (all of them, where a workgroup
+  // takes a whole segment); this wave's: tiles wave, wave + 4, ...
+  __device__ __forceinline__ void piece(int row0, int rows, int first, int end, Seq seq) {
     const int r = row0 + c, t_row = div_by(r, p.by_group);
     const bool valid = c < rows;
     const int hq = h * p.group + r - t_row * p.group;
     table = (att_const_i32*)(uintptr_t)(p.c.table + b * p.c.table_stride);
     kh = (const S*)p.c.k + h * p.c.head_stride;
     vh = (const S*)p.c.v + h * p.c.head_stride;
+    // (the first tile's loads wait for the block table alone where the length is not known yet)
+    const int t_first = first + wave * kTok, limit = p.direct ? p.c.room : seq.n;
+    Rows now, next;
+    if (t_first < limit) {
+      now = rows_of(t_first, limit);
+      load_k(now);
+      load_v(now);
+      next = rows_of(min(t_first + kStep, (limit - 1) & -kTok), limit);
+    }
     const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
 #pragma unroll
     for (int i = 0; i < kKs; ++i) {
@@ -514,23 +543,21 @@ struct Att {
       for (int i = 0; i < kKs; ++i) q[i] ^= k32 ? 0x80000000u : 0x80008000u;
     }
     clear();
+    have = seq.have;
+    n = seq.n;
+    end = min(end, n);
+    if (t_first >= end) return;
     const int lim = min(have + t_row + 1, n);  // of the lane's row (a row that is not there: whatever)
     const int all = p.tokens > 1 ? have + 1 : n;  // tokens that every row sees
-    const int t_first = first + wave * kTok;
-    if (t_first >= end) return;
-    Rows now = rows_of(t_first), next;
-    load_k(now);
-    load_v(now);
-    next = rows_of(min(t_first + kStep, (n - 1) & -kTok));
     int t0 = t_first;
-    const Row row{logits && valid ? logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row};
+    const Row row{p.logits && valid ? p.logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row};
     for (; t0 + kStep < end && t0 + kTok <= all; t0 += kStep) tile<true, false>(t0, row, now, next);
     // the last tile, and those that a row does not see all of: never many
     for (;;) {
       tile<false, false>(t0, row, now, next);
       t0 += kStep;
       if (t0 >= end) break;
-      now = rows_of(t0);
+      now = rows_of(t0, n);
       load_k(now);
       load_v(now);
     }
@@ -545,7 +572,7 @@ struct Att {
     if (__any(none != 0.f)) {  // NaN: something was not finite
       clear();
       for (t0 = t_first; t0 < end; t0 += kStep) {
-        now = rows_of(t0);
+        now = rows_of(t0, n);
         load_k(now);
         load_v(now);
         tile<false, true>(t0, row, now, now);
@@ -593,30 +620,29 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
   const int grid = gridDim.x;
   const int w = grid % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8);
   int x = 0, x1 = 1, b_start = 0, b_end = 0, units = 1;
+  Chunk seqs;
+  Seq seq;
   if (p.direct) {  // segment w
     a.b = div_by(w, p.by_segs);
     b_start = a.b * segs - w;
     b_end = 1;
-    a.n = seq_len(p, a.b);
-    a.have = p.c.cached[a.b];
+    seq = seq_of(p, a.b);
   } else {
-    const Deal d = deal(p, segs, p.wgs, p.by_wgs);
+    const Deal d = deal(p, segs, p.wgs, p.by_wgs, seqs);
     x = deal_start(d, w);
     x1 = deal_start(d, w + 1);
   }
   while (x < x1) {
     if (x >= b_end) {
-      find_unit(p, segs, x, &a.b, &b_start, &units);
+      find_unit(p, segs, x, seqs, &a.b, &seq, &b_start, &units);
       b_end = b_start + segs * units;
-      a.n = seq_len(p, a.b);
-      a.have = p.c.cached[a.b];
     }
     const int seg = (x - b_start) / units, u0 = x - b_start - seg * units, u1 = min(units, u0 + x1 - x);
     x += u1 - u0;
     a.h = div_by(seg, p.by_blocks);
     const int row0 = (seg - a.h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
     const bool whole = u0 == 0 && u1 == units;
-    if (a.n > 0) a.piece(row0, rows, u0 * kAttUnit, p.direct ? a.n : min(u1 * kAttUnit, a.n), p.logits);
+    a.piece(row0, rows, u0 * kAttUnit, p.direct ? p.c.room : u1 * kAttUnit, seq);
     if (a.n > 0 && a.c < rows) {
       if (a.g == 0) sm[a.wave][a.c] = a.m == -INFINITY ? a.m : a.base_of(a.m), sl[a.wave][a.c] = a.l;
 #pragma unroll
@@ -667,12 +693,9 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
 struct Pieces {
   int w0, w1;
 };
-__device__ __forceinline__ Pieces pieces_of(const CacheAttendParams& p, int b, int seg) {
-  const int segs = p.c.kv_heads * p.blocks, units = seq_units(p, b);
-  if (!units) return Pieces{0, -1};
+// first: the segment's first unit
+__device__ __forceinline__ Pieces pieces_of(const CacheAttendParams& p, const Deal& d, int first, int units) {
   if (p.direct) return Pieces{0, 0};
-  const Deal d = deal(p, segs, p.wgs, p.by_wgs);
-  const int first = units_before(p, b, segs) + seg * units;
   return Pieces{deal_of(d, first), deal_of(d, first + units - 1)};
 }
 __device__ __forceinline__ int64_t piece_row(const Pieces& s, int w, int row) {
@@ -686,7 +709,18 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
   __shared__ float sm[256], sl[256];
   __shared__ sw_f4 so[256];
   const int row = at % p.rows, bh = at / p.rows, b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads;
-  const Pieces s = pieces_of(p, b, h * p.blocks + row / kAttRows);
+  const int segs = p.c.kv_heads * p.blocks;
+  Chunk seqs;
+  const Deal d = deal(p, segs, p.wgs, p.by_wgs, seqs);
+  if (p.c.batch > kWave) {
+    seqs.load(p, 0, 0);
+    while (b >= seqs.b0 + kWave) seqs.load(p, seqs.b0 + kWave, seqs.last());
+  }
+  const int n = __builtin_amdgcn_readlane(seqs.n, b - seqs.b0), units = units_of(n);
+  Pieces s{0, -1};
+  if (units)
+    s = pieces_of(p, d, (__builtin_amdgcn_readlane(seqs.upto, b - seqs.b0) - units) * segs +
+                            (h * p.blocks + row / kAttRows) * units, units);
   if (s.w0 == s.w1) return;  // one workgroup had all of it
   constexpr int kItems = HD / 4, kShares = 256 / kItems, kBatch = 4;
   const int item = threadIdx.x % kItems, share = threadIdx.x / kItems, col = item * 4;
@@ -728,7 +762,7 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
     l += f * sl[i * kItems + item];
     o += f * so[i * kItems + item];
   }
-  att_row_out<DT>(p, b, h, row, col, seq_len(p, b), l, o);
+  att_row_out<DT>(p, b, h, row, col, n, l, o);
 }
 
 // What each cached token received: with the scores x as attention left them (base-2 logarithms),
@@ -738,24 +772,33 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
 // otherwise have to end first.
 __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) {
   __shared__ float lse[256];  // of the head's rows, 256 of them at a time
+  __shared__ float half[kAttUnit];
+  static_assert(2 * kAttUnit == 256, "two threads a token");
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, segs = p.c.kv_heads;
-  const Deal d = deal(p, segs, p.weight_wgs, p.by_weight_wgs);
+  Chunk seqs;
+  Seq seq{0, 0};
+  const Deal d = deal(p, segs, p.weight_wgs, p.by_weight_wgs, seqs);
   const int x1 = deal_start(d, at + 1);
-  int b = 0, b_start = 0, b_end = 0, units = 1, n = 0;
+  Deal of;  // attention's
+  of.total = d.total * p.blocks;
+  of.per = p.direct ? 0 : div_by(of.total, p.by_wgs);
+  of.more = of.total - of.per * p.wgs;
+  int b = 0, b_start = 0, b_end = 0, units = 1;
   for (int x = deal_start(d, at); x < x1; ++x) {
     if (x >= b_end) {
-      find_unit(p, segs, x, &b, &b_start, &units);
+      find_unit(p, segs, x, seqs, &b, &seq, &b_start, &units);
       b_end = b_start + segs * units;
-      n = seq_len(p, b);
     }
-    const int h = (x - b_start) / units, j = (x - b_start - h * units) * kAttUnit + threadIdx.x;
+    const int n = seq.n;
+    const int h = (x - b_start) / units, j = (x - b_start - h * units) * kAttUnit + threadIdx.x % kAttUnit;
+    const int part = threadIdx.x / kAttUnit;  // of the rows
     float sum = 0.f;
     for (int g0 = 0; g0 < p.group; g0 += 256) {
       const int rows = min(256, p.group - g0);
       __syncthreads();
       for (int r = wave; r < rows; r += 256 / kWave) {
         const int row = g0 + r;
-        const Pieces s = pieces_of(p, b, h * p.blocks + row / kAttRows);
+        const Pieces s = pieces_of(p, of, b_start * p.blocks + (h * p.blocks + row / kAttRows) * units, units);
         float top = -INFINITY, l = 0.f;
         if (s.w0 == s.w1) {
           top = p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2];
@@ -774,10 +817,13 @@ __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) 
       }
       __syncthreads();
       if (j < n)
-        for (int r = 0; r < rows; ++r)
+        for (int r = part; r < rows; r += 2)
           sum += __builtin_amdgcn_exp2f(p.logits[(b * (int64_t)p.q_heads + h * p.group + g0 + r) * p.logit_stride + j] - lse[r]);
     }
-    if (j >= n) continue;
+    if (part) half[threadIdx.x - kAttUnit] = sum;
+    __syncthreads();
+    if (part || j >= n) continue;
+    sum += half[threadIdx.x];
     const int page = cache_page(p.c, b, j);
     if (page < 0) continue;
     float* w = p.c.w + page * p.c.w_page_stride + h * p.c.w_head_stride + (j - div_by(j, p.c.by_page) * p.c.page_size);

@@ -195,7 +195,7 @@ int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d,
   const double room_bytes = 2.0 * room * c->head_dim * es, rounds = (double)room / (es == 4 || a->tile == 256 ? 64 : 128);
   const double round_ns = a->page16 ? 650 : 1100;
   const double piece_ns = rounds * round_ns > room_bytes / 48 ? rounds * round_ns : room_bytes / 48;
-  a->direct = room_bytes <= 1 << 20 && piece_ns - segs * room_bytes / 11000.0 <= 6000;
+  a->direct = c->pages > 0 && room_bytes <= 1 << 20 && piece_ns - segs * room_bytes / 11000.0 <= 6000;
   if (a->direct) a->wgs = 0;
   a->logit_stride = (room + 31) / 32 * 32;
   size_t at = 0;
@@ -248,7 +248,7 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   p.by_wgs = fast_div(a.wgs);
   if (c->weights) {
     const int64_t units = c->batch * c->kv_heads * ((p.c.room + kAttUnit - 1) / kAttUnit);
-    p.weight_wgs = (int32_t)(units < 16 * kCus ? units : 16 * kCus);
+    p.weight_wgs = (int32_t)(units < 8 * kCus ? units : 8 * kCus);
     p.by_weight_wgs = fast_div(p.weight_wgs);
   }
   p.tile = a.tile;
@@ -279,20 +279,44 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   return ATTNRES_OK;
 }
 
-extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* new_table, int64_t new_stride,
-                                   int64_t budget, int64_t recent, int32_t* kept, int32_t* left, void* stream) {
+namespace {
+
+int check_evict(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
   if (int rc = check_cache(c)) return rc;
   if (budget < 1 || budget > ATTNRES_CACHE_MAX_TOKENS) return api_fail(ATTNRES_EINVAL, "budget=%lld must be 1 .. 2^30", (long long)budget);
   if (recent < 0 || recent > budget)
     return api_fail(ATTNRES_EINVAL, "recent=%lld must be 0 .. budget=%lld", (long long)recent, (long long)budget);
+  const int64_t heads = c->batch * c->kv_heads, slices = (c->table_pages * c->page_size + kEvictSlice - 1) / kEvictSlice;
+  if (heads > (1 << 21) || heads * budget >= (int64_t)1 << 31 || heads * slices > (1 << 21))
+    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, kv_heads=%d, budget=%lld, %lld pages of %d: too many tokens",
+                    (long long)c->batch, c->kv_heads, (long long)budget, (long long)c->table_pages, c->page_size);
+  return ATTNRES_OK;
+}
+
+int64_t evict_slices(const attnres_cache_desc* c) {
+  const int64_t n = (c->table_pages * c->page_size + kEvictSlice - 1) / kEvictSlice;
+  return n > 1 ? n : 1;
+}
+
+}  // namespace
+
+extern "C" size_t attnres_cache_evict_workspace_size(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
+  if (check_evict(c, budget, recent) || c->batch == 0) return 0;
+  return evict_slices(c) > 1 ? (size_t)c->batch * c->kv_heads * evict_slices(c) * 6144 * 4 : 0;
+}
+
+extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* new_table, int64_t new_stride,
+                                   int64_t budget, int64_t recent, int32_t* kept, int32_t* left, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (int rc = check_evict(c, budget, recent)) return rc;
   if (c->batch == 0) return ATTNRES_OK;
   if (!new_table || !kept || !left) return api_fail(ATTNRES_EINVAL, "new_table / kept / left is NULL");
   if (c->pages > 0 && !c->weights) return api_fail(ATTNRES_EINVAL, "weights is NULL");
   if (new_stride < (budget + c->page_size - 1) / c->page_size && c->batch > 1)
     return api_fail(ATTNRES_EINVAL, "new_stride=%lld below the pages of %lld tokens", (long long)new_stride, (long long)budget);
-  if (c->batch * c->kv_heads > (1 << 21) || c->batch * c->kv_heads * budget > (int64_t)1 << 28)
-    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, kv_heads=%d, budget=%lld: too many tokens", (long long)c->batch,
-                    c->kv_heads, (long long)budget);
+  const size_t need = attnres_cache_evict_workspace_size(c, budget, recent);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+    return api_fail(ATTNRES_EWORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace ? workspace_bytes : (size_t)0);
   CacheEvictParams p{};
   p.c = pages_of(c);
   p.new_table = new_table;
@@ -302,6 +326,8 @@ extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* n
   p.kept = kept;
   p.left = left;
   p.es = es_of(c->dtype);
+  p.slices = (int32_t)evict_slices(c);
+  p.hist = (int32_t*)workspace;
   p.vec = rows_at(c, 16 / p.es);
   const hipError_t err = launch_cache_evict(p, (hipStream_t)stream);
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache evict launch failed: %s", hipGetErrorString(err));

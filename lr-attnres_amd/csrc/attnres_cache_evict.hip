@@ -1,7 +1,7 @@
 // The paged cache reduced to a budget: per key / value head the most attended and the
 // last tokens, copied in their order to other pages.
 //
-// Choice (one workgroup a head).  Weights become keys whose unsigned order is theirs (a NaN
+// Choice (one workgroup a head and kEvictSlice tokens).  Weights become keys whose unsigned order is theirs (a NaN
 // below all), held in registers; the budget-th largest is found in three rounds of 12, 10 and 10
 // bits counted in LDS (twelve first: weights lie in few octaves, and lanes that count into one
 // place wait for each other), fewer where a round leaves nothing open.  What lies above it and, of
@@ -51,105 +51,219 @@ __device__ __forceinline__ int block_scan(int x, int* sums) {
   return x;
 }
 
-// R: keys that a thread holds; longer caches are read again, R * 1024 tokens at a time, in every round
-template <int R>
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(CacheEvictParams p) {
-  const CachePages& c = p.c;
-  const int b = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  constexpr int kWaves = kSelThreads / kWave, kBlock = R * kSelThreads;
-  constexpr int kBins = 4096, kMine = kBins / kSelThreads;
-  __shared__ int hist[kBins];
-  __shared__ int sums[2][kWaves];
-  __shared__ int s_digit, s_want, s_open;
-  __shared__ int s_above[R * kWaves], s_equal[R * kWaves];
-  int n = cache_count(c, b);
-  if (n < 0) n = 0;
-  const int budget = p.budget;
-  int32_t* kept = p.kept + (int64_t)blockIdx.x * budget;
-  if (h == 0 && tid == 0) p.left[b] = min(n, budget);
-  if (n <= budget) {
-    for (int i = tid; i < budget; i += kSelThreads) kept[i] = i < n ? i : -1;
-    return;
-  }
-  const int early = n - p.recent;  // the tokens to choose from
-  int want = budget - p.recent;    // and how many of them; want < early
-  for (int i = tid; i < p.recent; i += kSelThreads) kept[budget - p.recent + i] = early + i;
-  if (want == 0) return;
+constexpr int kBins = 4096;                         // of the first round, 1024 of the other two
+constexpr int kSlice = kEvictSlice, kR = kSlice / kSelThreads;  // tokens that a workgroup holds the keys of
+static_assert(kR * kSelThreads == kSlice, "whole keys a thread");
+constexpr int kWaves = kSelThreads / kWave;
 
-  uint32_t key[R];
-  auto load = [&](int j0) {
+__device__ __forceinline__ int round_bits(int round) { return round == 0 ? 12 : 10; }
+__device__ __forceinline__ int round_shift(int round) { return 20 - 10 * round; }
+
+// What the rounds so far have found: kept are the keys above prefix in the bits of mask, and `want` of those equal.
+struct Found {
+  uint32_t prefix, mask;
+  int want;
+  bool open;  // more are equal than wanted
+};
+
+struct SelectShared {
+  int sums[2][kWaves];
+  int digit, want, open;
+  int above[kR * kWaves], equal[kR * kWaves];
+};
+
+// The next digit of the want-th largest key, from the counts of its places: count(place) for any place of 2^bits.
+template <class F>
+__device__ __forceinline__ void next_digit(int round, Found& f, SelectShared& s, F count) {
+  const int bits = round_bits(round), mine = (1 << bits) / kSelThreads;
+  // from the largest place down
+  const int first = (1 << bits) - 1 - (int)threadIdx.x * mine;
+  int n[kBins / kSelThreads], sum = 0;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int j = j0 + i * kSelThreads + tid;
-      key[i] = j < early ? token_key(c, b, h, j) : 0;
-    }
-  };
-  load(0);
-  uint32_t prefix = 0, mask = 0;
-  for (int round = 0, bits = 12, shift = 20; round < 3; ++round, bits = 10, shift -= 10) {
-    for (int i = tid; i < 1 << bits; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int j0 = 0; j0 < early; j0 += kBlock) {
-      if (early > kBlock) load(j0);
-#pragma unroll
-      for (int i = 0; i < R; ++i)
-        if (j0 + i * kSelThreads + tid < early && (key[i] & mask) == prefix)
-          atomicAdd(&hist[(key[i] >> shift) & ((1 << bits) - 1)], 1);
-    }
-    __syncthreads();
-    // from the largest digit down: a thread's places, and what lies above them
-    const int mine = round == 0 ? kMine : 1, first = (1 << bits) - 1 - tid * mine;
-    int sum = 0;
-    for (int i = 0; i < mine; ++i) sum += hist[first - i];
-    int upto = block_scan(sum, sums[0]);
-    if (upto >= want && upto - sum < want) {
-      int left = want - (upto - sum), i = 0;
-      while (hist[first - i] < left) left -= hist[first - i++];
-      s_digit = first - i;
-      s_want = left;
-      s_open = hist[first - i] > left;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
-    mask |= ((1u << bits) - 1) << shift;
-    want = s_want;
-    if (!s_open) break;  // all that have these digits are kept
+  for (int i = 0; i < kBins / kSelThreads; ++i) {
+    n[i] = i < mine ? count(first - i) : 0;
+    sum += n[i];
   }
-  // kept: what lies above prefix, and of what equals it the first `want`
-  int above = 0, equal = 0;  // in the blocks before
-  for (int j0 = 0; j0 < early; j0 += kBlock) {
-    if (early > kBlock) load(j0);
-    __syncthreads();
+  const int upto = block_scan(sum, s.sums[0]);
+  if (upto >= f.want && upto - sum < f.want) {
+    int left = f.want - (upto - sum);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const bool in = j0 + i * kSelThreads + tid < early;
-      const uint64_t a = __ballot(in && (key[i] & mask) > prefix), e = __ballot(in && (key[i] & mask) == prefix);
-      if (lane == 0) {
-        s_above[i * kWaves + wave] = __popcll(a);
-        s_equal[i * kWaves + wave] = __popcll(e);
+    for (int i = 0; i < kBins / kSelThreads; ++i) {
+      if (left > 0 && left <= n[i]) {
+        s.digit = first - i;
+        s.want = left;
+        s.open = n[i] > left;
       }
+      left -= n[i];
     }
-    __syncthreads();
-    const int a0 = tid < R * kWaves ? s_above[tid] : 0, e0 = tid < R * kWaves ? s_equal[tid] : 0;
-    const int a1 = block_scan(a0, sums[0]), e1 = block_scan(e0, sums[1]);
-    if (tid < R * kWaves) {
-      s_above[tid] = above + a1 - a0;
-      s_equal[tid] = equal + e1 - e0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int j = j0 + i * kSelThreads + tid;
-      const bool is_above = j < early && (key[i] & mask) > prefix, is_equal = j < early && (key[i] & mask) == prefix;
-      const uint64_t below = (1ull << lane) - 1;
-      const int a = s_above[i * kWaves + wave] + __popcll(__ballot(is_above) & below);
-      const int e = s_equal[i * kWaves + wave] + __popcll(__ballot(is_equal) & below);
-      if (is_above || (is_equal && e < want)) kept[a + min(e, want)] = j;
-    }
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) above += sums[0][w], equal += sums[1][w];
   }
+  __syncthreads();
+  f.prefix |= (uint32_t)s.digit << round_shift(round);
+  f.mask |= ((1u << bits) - 1) << round_shift(round);
+  f.want = s.want;
+  f.open = s.open;
+}
+
+// The tokens j0 .. of a head: what is kept of them goes to its places, `above` and `equal` of the tokens before them
+// being above the found prefix and equal to it.
+__device__ __forceinline__ void place(const uint32_t (&key)[kR], int j0, int early, const Found& f, int above, int equal,
+                                      int32_t* kept, SelectShared& s) {
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+    const bool in = j0 + i * kSelThreads + tid < early;
+    const uint64_t a = __ballot(in && (key[i] & f.mask) > f.prefix), e = __ballot(in && (key[i] & f.mask) == f.prefix);
+    if (lane == 0) {
+      s.above[i * kWaves + wave] = __popcll(a);
+      s.equal[i * kWaves + wave] = __popcll(e);
+    }
+  }
+  __syncthreads();
+  const int a0 = tid < kR * kWaves ? s.above[tid] : 0, e0 = tid < kR * kWaves ? s.equal[tid] : 0;
+  const int a1 = block_scan(a0, s.sums[0]), e1 = block_scan(e0, s.sums[1]);
+  if (tid < kR * kWaves) {
+    s.above[tid] = above + a1 - a0;
+    s.equal[tid] = equal + e1 - e0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+    const int j = j0 + i * kSelThreads + tid;
+    const bool is_above = j < early && (key[i] & f.mask) > f.prefix, is_equal = j < early && (key[i] & f.mask) == f.prefix;
+    const uint64_t below = (1ull << lane) - 1;
+    const int a = s.above[i * kWaves + wave] + __popcll(__ballot(is_above) & below);
+    const int e = s.equal[i * kWaves + wave] + __popcll(__ballot(is_equal) & below);
+    if (is_above || (is_equal && e < f.want)) kept[a + min(e, f.want)] = j;
+  }
+}
+
+__device__ __forceinline__ void load_keys(const CachePages& c, int b, int h, int j0, int early, uint32_t (&key)[kR]) {
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+    const int j = j0 + i * kSelThreads + (int)threadIdx.x;
+    key[i] = j < early ? token_key(c, b, h, j) : 0;
+  }
+}
+
+__device__ __forceinline__ void count_keys(const uint32_t (&key)[kR], int j0, int early, int round, const Found& f, int* hist) {
+  const int bits = round_bits(round), shift = round_shift(round);
+  for (int i = threadIdx.x; i < 1 << bits; i += kSelThreads) hist[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kR; ++i)
+    if (j0 + i * kSelThreads + (int)threadIdx.x < early && (key[i] & f.mask) == f.prefix)
+      atomicAdd(&hist[(key[i] >> shift) & ((1 << bits) - 1)], 1);
+  __syncthreads();
+}
+
+// what needs no choice; false: `early` tokens to choose budget - recent of
+__device__ __forceinline__ bool no_choice(const CacheEvictParams& p, int n, int32_t* kept) {
+  if (n <= p.budget) {
+    for (int i = threadIdx.x; i < p.budget; i += kSelThreads) kept[i] = i < n ? i : -1;
+    return true;
+  }
+  for (int i = threadIdx.x; i < p.recent; i += kSelThreads) kept[p.budget - p.recent + i] = n - p.recent + i;
+  return p.budget == p.recent;
+}
+
+// tables of at most kSlice tokens
+__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(CacheEvictParams p) {
+  __shared__ int hist[kBins];
+  __shared__ SelectShared s;
+  const int b = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads, n = max(cache_count(p.c, b), 0);
+  int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
+  if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
+  if (no_choice(p, n, kept)) return;
+  const int early = n - p.recent;
+  uint32_t key[kR];
+  load_keys(p.c, b, h, 0, early, key);
+  Found f{0, 0, p.budget - p.recent, true};
+  for (int round = 0; round < 3 && f.open; ++round) {
+    count_keys(key, 0, early, round, f, hist);
+    next_digit(round, f, s, [&](int place) { return hist[place]; });
+    __syncthreads();
+  }
+  place(key, 0, early, f, 0, 0, kept, s);
+}
+
+// Longer tables: kSlice tokens a workgroup, a launch for each round's counts and one that places what is kept.  Every
+// workgroup finds the digits of the earlier rounds again, from the counts of all slices.
+// hist[head][slice]: 4096, 1024, 1024 places
+constexpr int kSlots = 6144;
+__device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 3072 + 1024 * round; }
+
+// above, equal: keys of the slices before this one
+__device__ __forceinline__ Found replay(const CacheEvictParams& p, int head, int slices, int slice, int rounds, int* above,
+                                        int* equal, SelectShared& s) {
+  Found f{0, 0, p.budget - p.recent, true};
+  const int32_t* all = p.hist + (int64_t)head * p.slices * kSlots;
+  int a = 0, e = 0;
+  for (int round = 0; round < rounds && f.open; ++round) {
+    const int32_t* at = all + round_at(round);
+    // (eight slices' loads at once)
+    auto over = [&](int place, int n) {
+      int sum = 0;
+      for (int i0 = 0; i0 < n; i0 += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int x = at[(int64_t)min(i0 + i, n - 1) * kSlots + place];
+          sum += i0 + i < n ? x : 0;
+        }
+      return sum;
+    };
+    next_digit(round, f, s, [&](int place) { return over(place, slices); });
+    const int digit = s.digit;
+#pragma unroll
+    for (int q = 0; q < kBins / kSelThreads; ++q) {
+      const int place = q * kSelThreads + (int)threadIdx.x;
+      if (place > digit && place < 1 << round_bits(round)) a += over(place, slice);
+    }
+    if (threadIdx.x == 0) e = over(digit, slice);
+    __syncthreads();
+  }
+  if (threadIdx.x < 2) (threadIdx.x ? s.want : s.digit) = 0;
+  __syncthreads();
+  if (a) atomicAdd(&s.digit, a);
+  if (e) atomicAdd(&s.want, e);
+  __syncthreads();
+  *above = s.digit;
+  *equal = s.want;
+  return f;
+}
+
+__global__ __launch_bounds__(kSelThreads) void evict_count_kernel(CacheEvictParams p, int round) {
+  __shared__ int hist[kBins];
+  __shared__ SelectShared s;
+  const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
+  const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
+  const int early = n - p.recent, j0 = slice * kSlice;
+  if (n <= p.budget || p.budget == p.recent || j0 >= early) return;
+  uint32_t key[kR];
+  load_keys(p.c, b, h, j0, early, key);
+  int above, equal;
+  const Found f = replay(p, head, (early + kSlice - 1) / kSlice, 0, round, &above, &equal, s);
+  if (!f.open) return;
+  count_keys(key, j0, early, round, f, hist);
+  int32_t* to = p.hist + ((int64_t)head * p.slices + slice) * kSlots + round_at(round);
+  for (int i = threadIdx.x; i < 1 << round_bits(round); i += kSelThreads) to[i] = hist[i];
+}
+
+__global__ __launch_bounds__(kSelThreads) void evict_place_kernel(CacheEvictParams p) {
+  __shared__ SelectShared s;
+  const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
+  const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
+  int32_t* kept = p.kept + (int64_t)head * p.budget;
+  if (slice == 0) {
+    if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
+    if (no_choice(p, n, kept)) return;
+  }
+  const int early = n - p.recent, j0 = slice * kSlice;
+  if (n <= p.budget || p.budget == p.recent || j0 >= early) return;
+  uint32_t key[kR];
+  load_keys(p.c, b, h, j0, early, key);
+  int above, equal;
+  const Found f = replay(p, head, (early + kSlice - 1) / kSlice, slice, 3, &above, &equal, s);
+  place(key, j0, early, f, above, equal, kept, s);
 }
 
 // lanes: of a row (its 16-byte vectors, or single values)
@@ -183,11 +297,13 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(CacheEvictParams p, int
 
 hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st) {
   const int64_t heads = (int64_t)p.c.batch * p.c.kv_heads;
-  // keys of the longest table in registers, where 64 a thread are enough
-  const dim3 sel((unsigned)heads), wg(kSelThreads);
-  if (p.c.room <= 4 * kSelThreads) evict_select_kernel<4><<<sel, wg, 0, st>>>(p);
-  else if (p.c.room <= 16 * kSelThreads) evict_select_kernel<16><<<sel, wg, 0, st>>>(p);
-  else evict_select_kernel<64><<<sel, wg, 0, st>>>(p);
+  const dim3 sel((unsigned)(heads * p.slices)), wg(kSelThreads);
+  if (p.slices == 1) {
+    evict_select_kernel<<<sel, wg, 0, st>>>(p);
+  } else {
+    for (int round = 0; round < 3; ++round) evict_count_kernel<<<sel, wg, 0, st>>>(p, round);
+    evict_place_kernel<<<sel, wg, 0, st>>>(p);
+  }
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   const int size = p.vec ? 16 : p.es, per = p.c.head_dim * p.es / size;

@@ -55,7 +55,8 @@ struct Lib {
   X(attnres_block_accum_backward) X(attnres_qkv_rotary_forward) X(attnres_qkv_rotary_backward)                     \
   X(attnres_swiglu_saved_size) X(attnres_swiglu_forward_workspace_size)                                      \
   X(attnres_swiglu_backward_workspace_size) X(attnres_swiglu_forward) X(attnres_swiglu_backward)                   \
-  X(attnres_cache_append) X(attnres_cache_attend_workspace_size) X(attnres_cache_attend) X(attnres_cache_evict)
+  X(attnres_cache_append) X(attnres_cache_attend_workspace_size) X(attnres_cache_attend) X(attnres_cache_evict)  \
+  X(attnres_cache_evict_workspace_size)
   ATTNRES_FNS(ATTNRES_FN)
 } lib;
 

@@ -167,8 +167,12 @@ py::object cache_evict(const py::object& k_, const py::object& v_, const py::obj
   c10::DeviceGuard guard(c.k.device());
   const auto opt = c.table.options();
   Tensor kept = at::empty({B, c.d.kv_heads, budget}, opt), left = at::empty({B}, opt);
+  const size_t bytes_needed = lib.attnres_cache_evict_workspace_size(&c.d, budget, recent);
+  Tensor ws;
+  if (bytes_needed) ws = bytes(bytes_needed, c.k.device());
   check(lib.attnres_cache_evict(&c.d, to.data_ptr<int32_t>(), B > 1 ? to.stride(0) : to.size(1), budget, recent,
-                                kept.data_ptr<int32_t>(), left.data_ptr<int32_t>(), stream_of(c.k.device())),
+                                kept.data_ptr<int32_t>(), left.data_ptr<int32_t>(), ptr(ws), bytes_needed,
+                                stream_of(c.k.device())),
         "cache evict");
   written(c.k);
   written(c.v);

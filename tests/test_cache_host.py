@@ -25,7 +25,7 @@ def test_library_exports_every_declared_symbol():
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
     names = sorted(set(re.findall(r"\b(attnres_[a-z0-9_]+)\s*\(", text)))
     assert names == sorted(["attnres_cache_append", "attnres_cache_attend_workspace_size", "attnres_cache_attend",
-                            "attnres_cache_evict"])
+                            "attnres_cache_evict", "attnres_cache_evict_workspace_size"])
     nm = subprocess.run(["nm", "-D", "--defined-only", H.LIB_PATH], capture_output=True, text=True).stdout
     for n in names:
         assert re.search(rf"\bT {n}\b", nm), n
@@ -127,8 +127,20 @@ def test_evict_refusals(kw, code, word):
     c = _cache(**{**dict(weights=0x5000), **kw})
     a = {**dict(new=0x6000, new_stride=2, budget=32, recent=8, kept=0x7000, left=0x8000), **kw}
     assert lib.attnres_cache_evict(ctypes.byref(c), a["new"], a["new_stride"], a["budget"], a["recent"], a["kept"], a["left"],
-                                   None) == code
+                                   None, 0, None) == code
     assert word in lib.attnres_last_error().decode()
+
+
+@needs_lib
+def test_evict_workspace():
+    lib = H.load()
+    short, long = _cache(weights=0x5000), _cache(weights=0x5000, table_pages=1 << 12, table_stride=1 << 12)
+    assert lib.attnres_cache_evict_workspace_size(ctypes.byref(short), 32, 8) == 0
+    n = lib.attnres_cache_evict_workspace_size(ctypes.byref(long), 32, 8)
+    assert n > 0
+    for ws, size in ((None, n), (0x100000, n - 1), (0x100010, n)):
+        assert lib.attnres_cache_evict(ctypes.byref(long), 0x6000, 2, 32, 8, 0x7000, 0x8000, ws, size, None) == -4
+        assert "workspace" in lib.attnres_last_error().decode()
 
 
 def test_no_cpu_path():
