@@ -42,7 +42,8 @@ struct CacheAppendParams {
   CachePages c;
   const void* qkv;
   int64_t b_stride, t_stride;
-  int64_t n_tok, tokens;  // batch * tokens
+  int32_t n_tok, tokens;  // batch * tokens; times the heads of a token below 2^31
+  FastDiv by_tokens;
   int32_t q_heads, qk_norm;
   float eps;
   const void* sin;
@@ -86,6 +87,7 @@ hipError_t launch_cache_attend_f16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f32(const CacheAttendParams& p, hipStream_t st);
 
 constexpr int kEvictSlice = 8192;  // tokens whose keys a workgroup holds
+constexpr int kEvictSlots = 6152;  // counts and state of a workgroup, 4 bytes each
 
 struct CacheEvictParams {
   CachePages c;
@@ -96,7 +98,7 @@ struct CacheEvictParams {
   int32_t* left;
   int32_t es;   // bytes of a value
   int32_t slices;  // of a table
-  int32_t* hist;   // [heads][slices][6144], where there are several
+  int32_t* hist;   // [heads][slices][kEvictSlots], where there are several
   int32_t vec;  // rows in whole vectors of 16 bytes
 };
 

@@ -9,7 +9,7 @@
 // the projection's loads do not wait for it.
 //
 // Layout.  As the projection's kernel: LANES lanes a head, VEC consecutive values (16
-// bytes) a lane, up to kIters head groups a wave.  A row of a page is as long as a head, so
+// bytes) a lane, up to kGroups head groups a wave.  A row of a page is as long as a head, so
 // stores are whole rows whatever the pages' order.
 #include "attnres_cache.h"
 #include "attnres_rotary.h"
@@ -18,6 +18,11 @@ namespace attnres {
 
 namespace {
 
+// Head groups of a wave, all loads of them in flight at once: 48 heads of 64 are one wave's (8 prompts of up to 2048: 40.7
+// us in two waves of three groups, 38.1 in one of six).
+constexpr int kGroups = 6;
+constexpr int kFewWaves = 4096;  // half of what the CUs hold
+
 struct Place {  // of one new token
   int64_t row;  // its elements in a page, head 0; -1: not written
   int64_t w;    // its weight's
@@ -25,15 +30,15 @@ struct Place {  // of one new token
   bool real;    // one of its sequence's
 };
 
-__device__ __forceinline__ Place place_of(const CacheAppendParams& p, int b, int64_t t) {
+__device__ __forceinline__ Place place_of(const CacheAppendParams& p, int b, int t) {
   Place r{-1, 0, -1, !p.c.fresh || t < p.c.fresh[b]};
   const int have = p.c.cached[b];
-  const int64_t j = have + t, at = (p.pos ? p.pos[b] : have) + t;
+  const int64_t j = (int64_t)have + t, at = (int64_t)(p.pos ? p.pos[b] : have) + t;
   if (at >= 0 && at < p.table_rows) r.at = at;
   if (r.real && have >= 0 && j < p.c.room) {
-    const int page = cache_page(p.c, b, (int)j);
-    const int slot = (int)j % p.c.page_size;
-    if (page >= 0) {
+    const int i = div_by((int)j, p.c.by_page), slot = (int)j - i * p.c.page_size;
+    const int page = p.c.table[b * p.c.table_stride + i];
+    if ((unsigned)page < (unsigned)p.c.pages) {
       r.row = page * p.c.page_stride + slot * p.c.slot_stride;
       r.w = page * p.c.w_page_stride + slot;
     }
@@ -42,17 +47,17 @@ __device__ __forceinline__ Place place_of(const CacheAppendParams& p, int b, int
 }
 
 template <class DT, class TT, int VEC, int LANES>
-__global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheAppendParams p, int groups, int iters) {
+__global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheAppendParams p, int groups, int iters,
+                                                                          FastDiv by_groups) {
   using S = typename DT::S;
   using TS = typename TT::S;
   constexpr int kHeads = kWave / LANES;  // heads of a group
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t wid = rot_wave();
-  const int64_t tok = wid / groups;
+  const int wid = (int)rot_wave();
+  const int tok = div_by(wid, by_groups);
   if (tok >= p.n_tok) return;
-  const int part = (int)(wid - tok * groups);
-  const int b = (int)(tok / p.tokens);
-  const int64_t t = tok - b * p.tokens;
+  const int part = wid - tok * groups;
+  const int b = div_by(tok, p.by_tokens), t = tok - b * p.tokens;
   const int n_rot = p.q_heads + p.c.kv_heads, n_all = n_rot + p.c.kv_heads;
   const int Dh = p.c.head_dim;
   const int col = (lane & (LANES - 1)) * VEC;
@@ -61,9 +66,9 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheApp
 
   const S* src = (const S*)p.qkv + b * p.b_stride + t * p.t_stride;
   const bool real = !p.c.fresh || t < p.c.fresh[b];  // (what is behind a sequence's tokens is not read)
-  Raw<DT, VEC> x[kIters];
+  Raw<DT, VEC> x[kGroups];
 #pragma unroll
-  for (int i = 0; i < kIters; ++i) {
+  for (int i = 0; i < kGroups; ++i) {
     const int h = i < iters && real ? head0 + i * kHeads : n_all;
     if (h < n_all && in) load_raw<DT, VEC, true>(src + (int64_t)h * Dh + col, x[i]);
     else x[i] = {};
@@ -78,7 +83,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheApp
     for (int e = 0; e < VEC / 2; ++e) sn[e] = cs[e] = __builtin_nanf("");
   }
 #pragma unroll
-  for (int i = 0; i < kIters; ++i) {
+  for (int i = 0; i < kGroups; ++i) {
     if (i >= iters) break;
     const int h = head0 + i * kHeads;
     float v[VEC], r[VEC];
@@ -120,12 +125,11 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_general(CacheAp
   using TS = typename TT::S;
   const int lane = threadIdx.x & (kWave - 1);
   const int n_rot = p.q_heads + p.c.kv_heads, n_all = n_rot + p.c.kv_heads;
-  const int64_t wid = rot_wave();
-  const int64_t tok = wid / n_all;
+  const int wid = (int)rot_wave();
+  const int tok = wid / n_all;
   if (tok >= p.n_tok) return;
-  const int h = (int)(wid - tok * n_all);
-  const int b = (int)(tok / p.tokens);
-  const int64_t t = tok - b * p.tokens;
+  const int h = wid - tok * n_all;
+  const int b = div_by(tok, p.by_tokens), t = tok - b * p.tokens;
   const int Dh = p.c.head_dim;
   const S* x = (const S*)p.qkv + b * p.b_stride + t * p.t_stride + (int64_t)h * Dh;
   const Place at = place_of(p, b, t);
@@ -170,11 +174,13 @@ template <class DT, class TT, int VEC, int LANES>
 hipError_t run(const CacheAppendParams& p, hipStream_t st) {
   const int n_all = p.q_heads + 2 * p.c.kv_heads;
   const int all = (n_all + kWave / LANES - 1) / (kWave / LANES);
-  // head groups shared evenly by as few waves as hold them
-  const int groups = (all + kIters - 1) / kIters, iters = (all + groups - 1) / groups;
+  // head groups shared evenly by as few waves as hold them; few tokens, whose launch is all latency, take a wave a
+  // group (16 tokens of 36 heads of 64: 7.3 us a call, 8.2 with five groups in turn)
+  const int most = (int64_t)p.n_tok * all <= kFewWaves ? 1 : kGroups;
+  const int groups = (all + most - 1) / most, iters = (all + groups - 1) / groups;
   dim3 grid;
-  if (!rot_grid(p.n_tok * groups, &grid)) return hipErrorInvalidValue;
-  cache_append_kernel<DT, TT, VEC, LANES><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters);
+  if (!rot_grid((int64_t)p.n_tok * groups, &grid)) return hipErrorInvalidValue;
+  cache_append_kernel<DT, TT, VEC, LANES><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters, fast_div(groups));
   return hipGetLastError();
 }
 
@@ -196,7 +202,7 @@ hipError_t pick(const CacheAppendParams& p, int vec, int lanes, hipStream_t st) 
   }
   if (vec != 1) return hipErrorInvalidValue;
   dim3 grid;
-  if (!rot_grid(p.n_tok * (p.q_heads + 2 * p.c.kv_heads), &grid)) return hipErrorInvalidValue;
+  if (!rot_grid((int64_t)p.n_tok * (p.q_heads + 2 * p.c.kv_heads), &grid)) return hipErrorInvalidValue;
   cache_append_general<DT, TT><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p);
   return hipGetLastError();
 }

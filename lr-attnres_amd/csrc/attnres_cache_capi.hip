@@ -86,7 +86,9 @@ int check_append(const attnres_cache_desc* c, const attnres_cache_append_desc* d
   if (d->q_heads < 1 || d->q_heads > (1 << 20)) return api_fail(ATTNRES_EINVAL, "q_heads=%d must be >= 1", d->q_heads);
   if (c->head_dim % 2) return api_fail(ATTNRES_EINVAL, "head_dim=%d must be even", c->head_dim);
   if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
-  if (c->batch * d->tokens > (int64_t)1 << 36) return api_fail(ATTNRES_EUNSUPPORTED, "too many tokens");
+  if (c->batch * d->tokens > INT32_MAX / ((int64_t)d->q_heads + 2 * c->kv_heads))
+    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, %d + 2 * %d heads: too many", (long long)c->batch,
+                    (long long)d->tokens, d->q_heads, c->kv_heads);
   if (!d->qkv || !d->sin || !d->cos) return api_fail(ATTNRES_EINVAL, "qkv / sin / cos is NULL");
   if (d->batch_stride < 0 || d->token_stride < 0)
     return api_fail(ATTNRES_EINVAL, "batch_stride and token_stride must be >= 0");
@@ -129,8 +131,9 @@ extern "C" int attnres_cache_append(const attnres_cache_desc* c, const attnres_c
   p.qkv = d->qkv;
   p.b_stride = d->batch_stride;
   p.t_stride = d->token_stride;
-  p.n_tok = c->batch * d->tokens;
-  p.tokens = d->tokens;
+  p.n_tok = (int32_t)(c->batch * d->tokens);
+  p.tokens = (int32_t)d->tokens;
+  p.by_tokens = fast_div(p.tokens);
   p.q_heads = d->q_heads;
   p.qk_norm = d->qk_norm != 0;
   p.eps = d->norm_eps;
@@ -302,7 +305,7 @@ int64_t evict_slices(const attnres_cache_desc* c) {
 
 extern "C" size_t attnres_cache_evict_workspace_size(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
   if (check_evict(c, budget, recent) || c->batch == 0) return 0;
-  return evict_slices(c) > 1 ? (size_t)c->batch * c->kv_heads * evict_slices(c) * 6144 * 4 : 0;
+  return evict_slices(c) > 1 ? (size_t)c->batch * c->kv_heads * evict_slices(c) * kEvictSlots * 4 : 0;
 }
 
 extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* new_table, int64_t new_stride,

@@ -186,20 +186,27 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(CacheEvictPar
   place(key, 0, early, f, 0, 0, kept, s);
 }
 
-// Longer tables: kSlice tokens a workgroup, a launch for each round's counts and one that places what is kept.  Every
-// workgroup finds the digits of the earlier rounds again, from the counts of all slices.
-// hist[head][slice]: 4096, 1024, 1024 places
-constexpr int kSlots = 6144;
+// Longer tables: kSlice tokens a workgroup, a launch for each round's counts and one that places what is kept.  Each
+// launch finds the digit of the round before it, from the counts of all of the head's slices, and each workgroup
+// keeps what it has found for its next launch.
+// hist[head][slice]: 4096, 1024, 1024 places, then prefix, mask, want, open, above, equal
+constexpr int kSlots = kEvictSlots, kState = 6144;
+static_assert(kSlots >= kState + 6, "places and state");
 __device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 3072 + 1024 * round; }
 
-// above, equal: keys of the slices before this one
-__device__ __forceinline__ Found replay(const CacheEvictParams& p, int head, int slices, int slice, int rounds, int* above,
-                                        int* equal, SelectShared& s) {
+// What the rounds before `round` have found; above, equal: keys of the slices before this one.
+__device__ __forceinline__ Found found_before(const CacheEvictParams& p, int head, int slices, int slice, int round, int* above,
+                                              int* equal, SelectShared& s) {
   Found f{0, 0, p.budget - p.recent, true};
-  const int32_t* all = p.hist + (int64_t)head * p.slices * kSlots;
   int a = 0, e = 0;
-  for (int round = 0; round < rounds && f.open; ++round) {
-    const int32_t* at = all + round_at(round);
+  int32_t* state = p.hist + ((int64_t)head * p.slices + slice) * kSlots + kState;
+  if (round > 1) {
+    f = Found{(uint32_t)state[0], (uint32_t)state[1], state[2], state[3] != 0};
+    a = state[4];
+    e = state[5];
+  }
+  if (round > 0 && f.open) {
+    const int32_t* at = p.hist + (int64_t)head * p.slices * kSlots + round_at(round - 1);
     // (eight slices' loads at once)
     auto over = [&](int place, int n) {
       int sum = 0;
@@ -211,23 +218,32 @@ __device__ __forceinline__ Found replay(const CacheEvictParams& p, int head, int
         }
       return sum;
     };
-    next_digit(round, f, s, [&](int place) { return over(place, slices); });
+    next_digit(round - 1, f, s, [&](int place) { return over(place, slices); });
     const int digit = s.digit;
+    int more = 0;
 #pragma unroll
     for (int q = 0; q < kBins / kSelThreads; ++q) {
       const int place = q * kSelThreads + (int)threadIdx.x;
-      if (place > digit && place < 1 << round_bits(round)) a += over(place, slice);
+      if (place > digit && place < 1 << round_bits(round - 1)) more += over(place, slice);
     }
-    if (threadIdx.x == 0) e = over(digit, slice);
     __syncthreads();
+    if (threadIdx.x == 0) s.digit = 0;
+    __syncthreads();
+    if (more) atomicAdd(&s.digit, more);
+    __syncthreads();
+    a += s.digit;
+    e = slice ? over(digit, slice) : 0;
   }
-  if (threadIdx.x < 2) (threadIdx.x ? s.want : s.digit) = 0;
-  __syncthreads();
-  if (a) atomicAdd(&s.digit, a);
-  if (e) atomicAdd(&s.want, e);
-  __syncthreads();
-  *above = s.digit;
-  *equal = s.want;
+  if (round < 3 && threadIdx.x == 0) {
+    state[0] = (int32_t)f.prefix;
+    state[1] = (int32_t)f.mask;
+    state[2] = f.want;
+    state[3] = f.open;
+    state[4] = a;
+    state[5] = e;
+  }
+  *above = a;
+  *equal = e;
   return f;
 }
 
@@ -241,7 +257,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_count_kernel(CacheEvictPara
   uint32_t key[kR];
   load_keys(p.c, b, h, j0, early, key);
   int above, equal;
-  const Found f = replay(p, head, (early + kSlice - 1) / kSlice, 0, round, &above, &equal, s);
+  const Found f = found_before(p, head, (early + kSlice - 1) / kSlice, slice, round, &above, &equal, s);
   if (!f.open) return;
   count_keys(key, j0, early, round, f, hist);
   int32_t* to = p.hist + ((int64_t)head * p.slices + slice) * kSlots + round_at(round);
@@ -262,7 +278,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_place_kernel(CacheEvictPara
   uint32_t key[kR];
   load_keys(p.c, b, h, j0, early, key);
   int above, equal;
-  const Found f = replay(p, head, (early + kSlice - 1) / kSlice, slice, 3, &above, &equal, s);
+  const Found f = found_before(p, head, (early + kSlice - 1) / kSlice, slice, 3, &above, &equal, s);
   place(key, j0, early, f, above, equal, kept, s);
 }
 
