@@ -21,9 +21,15 @@ head:
   partial block in with ``lrid_attention_residual_phase2[_torch]``
   (``model.py:1919-1942``, ``:1616-1643``).
 
+Generation (``generate``, or ``forward`` with a ``PagedCache``) runs the same
+schedule over the new tokens alone: the reads are independent per token, so
+attention's keys and values are all that is kept of earlier ones, in pages
+(``attnres_cache.py``) that ``qkv_norm_rotary_cached`` writes,
+``cached_attention`` reads and ``evict_cached_tokens`` reduces.
+
 What differs from the reference's module: only this path is built (one depth
-head, static queries, projection keys; no KV cache, no base AttnRes, no
-split-sublayer mode), and the live partial block is handed to phase 2 raw
+head, static queries, projection keys; no base AttnRes, no split-sublayer
+mode), and the live partial block is handed to phase 2 raw
 with ``partial_scale = count**-alpha`` instead of being multiplied out first
 (``fold_block_summary``; the result is bit-identical, the kernel applies the
 same rounding), and with pre-norm sublayers each sublayer's fused projection
@@ -58,6 +64,8 @@ from typing import Optional
 import torch
 from torch import Tensor, nn
 from torch.nn import functional as F
+
+from attnres_cache import PagedCache
 
 try:
     from torch.nn.attention import SDPBackend, sdpa_kernel
@@ -280,10 +288,34 @@ class MultiHeadAttention(nn.Module):
         else:
             self.c_proj = nn.Linear(config.n_embd, config.n_embd, bias=False)
 
-    def forward(self, x: Tensor):
+    def _plain_rope(self) -> bool:
+        return type(self.rope) is RotaryEmbedding and "rotate" not in self.rope.__dict__
+
+    def _forward_cached(self, x: Tensor, step: "CachedStep", layer: int) -> Tensor:
+        """Attention of new tokens over a cache that they join (``model.py:430-569``), [B, T, C] before the output projection."""
+        if not self._plain_rope():
+            raise NotImplementedError("a cache holds keys rotated by RotaryEmbedding's tables; this rope is another")
+        B, T, C = x.shape
+        c = step.cache
+        ops = self.ops if self.ops is not None else _default_ops()
+        k, v = c.k[layer], c.v[layer]
+        w = None if c.weights is None else c.weights[layer]
+        heads = ops.qkv_norm_rotary_cached(self.c_attn(x), self.n_head, self.rope.sin, self.rope.cos, k, v, step.table, c.cached,
+                                           fresh=step.fresh, positions=c.positions, qk_norm=self.qk_norm, weights=w,
+                                           return_heads=step.prompt)
+        if step.prompt:  # nothing is cached: attention inside the prompts alone, whose padding is behind them
+            y = _attend(*heads)
+        else:
+            y = ops.cached_attention(heads, k, v, step.table, c.cached, fresh=step.fresh, weights=w if T == 1 else None)
+        return y.transpose(1, 2).reshape(B, T, C)
+
+    def forward(self, x: Tensor, step: Optional["CachedStep"] = None, layer: int = 0):
+        if step is not None:
+            y = self._forward_cached(x, step, layer)
+            return self.c_proj(y) if self.keyed else (self.c_proj(y), None)
         B, T, C = x.shape
         # (a rotation of another kind is called as it is)
-        if self.fused_heads and type(self.rope) is RotaryEmbedding and "rotate" not in self.rope.__dict__:
+        if self.fused_heads and self._plain_rope():
             q, k, v = self.ops.qkv_norm_rotary(self.c_attn(x), self.n_head, self.rope.sin, self.rope.cos,
                                                qk_norm=self.qk_norm)
         else:
@@ -349,8 +381,10 @@ class Block(nn.Module):
             out = norm(out)
         return out, key
 
-    def attention(self, x: Tensor, x_is_normalized: bool = False):
-        return self._sublayer(self.attn, x, x_is_normalized)
+    def attention(self, x: Tensor, x_is_normalized: bool = False, step: Optional["CachedStep"] = None, layer: int = 0):
+        if step is None:
+            return self._sublayer(self.attn, x, x_is_normalized)
+        return self._sublayer(lambda h: self.attn(h, step, layer), x, x_is_normalized)
 
     def feed_forward(self, x: Tensor, x_is_normalized: bool = False):
         return self._sublayer(self.mlp, x, x_is_normalized)
@@ -359,6 +393,16 @@ class Block(nn.Module):
 def _default_ops():
     import attnres_ops
     return attnres_ops
+
+
+@dataclass
+class CachedStep:
+    """What a forward pass over new tokens has of the cache: the counts before it, and which tokens are the sequences'."""
+
+    cache: PagedCache
+    table: Tensor              # the pages that are in use
+    fresh: Optional[Tensor]    # [B] tokens of each sequence, None: all
+    prompt: bool               # nothing is cached yet, and the sequences have several tokens
 
 
 class Decoder(nn.Module):
@@ -413,25 +457,88 @@ class Decoder(nn.Module):
 
     # -- forward ------------------------------------------------------------
 
-    def forward(self, idx: Tensor, return_hidden: bool = False) -> Tensor:
+    def forward(self, idx: Tensor, return_hidden: bool = False, cache: Optional[PagedCache] = None, fresh=None) -> Tensor:
+        """With ``cache``, ``idx`` holds new tokens [B, T] of its sequences, which join it: row b's first ``fresh[b]`` (all
+        unless given; the rest is padding, whose outputs mean nothing).  No gradients."""
         _, T = idx.shape
         if T > self.config.block_size:
             raise ValueError(f"token length {T} exceeds block_size {self.config.block_size}")
+        step = None if cache is None else self._begin_step(idx, cache, fresh)
         x = self.transformer.wte(idx)
         if self.config.use_attnres:
-            x = self._forward_block_lrid(x)
+            x = self._forward_block_lrid(x, step)
         else:
-            x = self._forward_baseline(x)
-        if return_hidden:
-            return x
+            x = self._forward_baseline(x, step)
+        if step is not None:
+            cache.advance(T if fresh is None else fresh)
+        return x if return_hidden else self._logits(x)
+
+    def _logits(self, x: Tensor) -> Tensor:
         if self.config.weight_tying:
             return F.linear(x, self.transformer.wte.weight, None)
         return self.lm_head(x)
 
-    def _forward_baseline(self, x: Tensor) -> Tensor:
+    def new_cache(self, batch: int, max_tokens: Optional[int] = None, **kw) -> PagedCache:
+        """A cache for this model's layers, in its dtype and on its device."""
+        c, w = self.config, self.transformer.wte.weight
+        return PagedCache(c.n_layer, c.n_head, c.n_embd // c.n_head, batch, max_tokens or c.block_size, dtype=w.dtype,
+                          device=w.device, **kw)
+
+    def _begin_step(self, idx: Tensor, cache: PagedCache, fresh) -> CachedStep:
+        B, T = idx.shape
+        if B != cache.batch:
+            raise ValueError(f"{B} rows of tokens for a cache of {cache.batch} sequences")
+        new = [T] * B if fresh is None else list(fresh)
+        if len(new) != B or any(not 0 <= n <= T for n in new):
+            raise ValueError(f"fresh must be {B} counts of 0 .. {T}, got {fresh}")
+        far = max(p + n for p, n in zip(cache.next_positions, new))
+        if far > self.config.block_size:
+            raise ValueError(f"position {far - 1} is outside block_size {self.config.block_size}")
+        cache.reserve(new)
+        prompt = T > 1 and not any(cache.lengths)
+        counts = None if fresh is None else torch.tensor(new, dtype=torch.int32).to(idx.device)
+        return CachedStep(cache, cache.table[:, :cache.pages_in_use()], counts, prompt)
+
+    @torch.no_grad()
+    def generate(self, idx: Tensor, max_new_tokens: int, lengths=None, cache: Optional[PagedCache] = None,
+                 budget: Optional[int] = None, recent: int = 0, pick=None) -> Tensor:
+        """``max_new_tokens`` more tokens of each row of ``idx`` [B, T] (``lengths``: the tokens of each row, in a padded batch),
+        [B, max_new_tokens].  The reference's model generates with a key-value cache too (``model.py:2662-2709``).
+
+        ``pick`` takes logits [B, vocab] to the next tokens [B]; the largest logit's unless given.  With ``budget`` a sequence
+        that has a page's tokens more than that in the cache is brought back to it (``PagedCache.evict``, which keeps the last
+        ``recent``).
+        """
+        B, T = idx.shape
+        if lengths is not None and (len(lengths) != B or any(not 1 <= n <= T for n in lengths)):
+            raise ValueError(f"lengths must be {B} counts of 1 .. {T}, got {lengths}")
+        if cache is None:
+            most = min(self.config.block_size, T + max_new_tokens)
+            # (with a budget, pages for a second copy of what is kept while it moves)
+            extra = {} if budget is None else dict(weights=True, spare_tokens=budget)
+            cache = self.new_cache(B, most, **extra)
+        far = max(p + n for p, n in zip(cache.next_positions, lengths or [T] * B)) + max_new_tokens - 1
+        if far > self.config.block_size:
+            raise ValueError(f"position {far - 1} is outside block_size {self.config.block_size}")
+        out = idx.new_empty((B, max_new_tokens))
+        tokens, fresh = idx, lengths
+        for i in range(max_new_tokens):
+            h = self(tokens, return_hidden=True, cache=cache, fresh=fresh)
+            if fresh is None:
+                h = h[:, -1]
+            else:
+                h = h[torch.arange(B, device=h.device), torch.tensor([n - 1 for n in fresh], device=h.device)]
+            logits = self._logits(h)
+            out[:, i] = logits.argmax(-1) if pick is None else pick(logits)
+            tokens, fresh = out[:, i:i + 1], None
+            if budget is not None and max(cache.lengths) >= budget + cache.page_size:
+                cache.evict(self.ops if self.ops is not None else _default_ops(), budget, recent)
+        return out
+
+    def _forward_baseline(self, x: Tensor, step: Optional[CachedStep] = None) -> Tensor:
         """Plain residual stream ``x += sublayer(x)`` and a final norm (``model.py:704-733``, ``:2642-2643``)."""
-        for block in self.transformer.layers:
-            out, _ = block.attention(x)
+        for i, block in enumerate(self.transformer.layers):
+            out, _ = block.attention(x) if step is None else block.attention(x, step=step, layer=i)
             x = x + out
             out, _ = block.feed_forward(x)
             x = x + out
@@ -460,7 +567,7 @@ class Decoder(nn.Module):
             return 0.0
         return beta * math.log(float(count))
 
-    def _forward_block_lrid(self, x: Tensor) -> Tensor:
+    def _forward_block_lrid(self, x: Tensor, step: Optional[CachedStep] = None) -> Tensor:
         c = self.config
         ops = self.ops
         n_sites = 2 * c.n_layer
@@ -592,7 +699,10 @@ class Decoder(nn.Module):
 
         h = read(0)
         for layer_idx, block in enumerate(self.transformer.layers):
-            out, key = block.attention(h, x_is_normalized=fused_norm)
+            if step is None:
+                out, key = block.attention(h, x_is_normalized=fused_norm)
+            else:
+                out, key = block.attention(h, x_is_normalized=fused_norm, step=step, layer=layer_idx)
             site = 2 * layer_idx + 1
             h = add(out, key, site)
             if h is None:

@@ -579,6 +579,78 @@ def softmax_weights_ref(values_or_keys, query: Tensor, num_heads: int, logit_sca
     return F.softmax(logits.float(), dim=0)
 
 
+# ---------------------------------------------------------------- the paged key-value cache
+#
+# Not in the reference, whose attention concatenates to a cache tensor (model.py:430-569): the drop-in's own operators,
+# token by token.
+
+def _places(block_table, page_size, b, first, count):
+    """(page, slot) of tokens first .. first + count of sequence b"""
+    at = torch.arange(first, first + count)
+    return block_table[b].long()[at // page_size], at % page_size
+
+
+def qkv_norm_rotary_cached_ref(qkv, num_heads, sin, cos, k_pages, v_pages, block_table, cached, fresh=None, positions=None,
+                               qk_norm=True, weights=None, return_heads=False):
+    """Heads of the new tokens by ``qkv_norm_rotary_ref``, keys and values written into their pages."""
+    B, T, _ = qkv.shape
+    K = k_pages.size(1)
+    start = cached if positions is None else positions
+    at = start.long()[:, None] + torch.arange(T)
+    q, k, v = qkv_norm_rotary_ref(qkv, num_heads, sin, cos, positions=at.clamp(max=sin.numel() // sin.size(-1) - 1),
+                                  num_kv_heads=K, qk_norm=qk_norm)
+    q, k = q.clone(), k.clone()
+    for b in range(B):
+        n = T if fresh is None else int(fresh[b])
+        q[b, :, n:] = 0
+        k[b, :, n:] = 0
+        page, slot = _places(block_table, k_pages.size(2), b, int(cached[b]), n)
+        k_pages[page, :, slot] = k[b, :, :n].transpose(0, 1)
+        v_pages[page, :, slot] = v[b, :, :n].transpose(0, 1)
+        if weights is not None:
+            weights[page, :, slot] = 0
+    return (q, k, v) if return_heads else q
+
+
+def cached_attention_ref(q, k_pages, v_pages, block_table, cached, fresh=None, scale=None, weights=None, decay=1.0):
+    """Softmax attention of the newest tokens over their sequence's pages, fp32 with one rounding."""
+    B, H, T, Dh = q.shape
+    G = H // k_pages.size(1)
+    out = torch.zeros_like(q)
+    for b in range(B):
+        for t in range(T if fresh is None else int(fresh[b])):
+            n = int(cached[b]) + t + 1
+            page, slot = _places(block_table, k_pages.size(2), b, 0, n)
+            k, v = (p[page, :, slot].transpose(0, 1).float().repeat_interleave(G, 0) for p in (k_pages, v_pages))
+            s = (k * q[b, :, t, None].float()).sum(-1) * (Dh ** -0.5 if scale is None else scale)
+            p = F.softmax(s, dim=-1)
+            out[b, :, t] = (p[..., None] * v).sum(1).to(q.dtype)
+            if weights is not None:
+                got = p.view(-1, G, n).sum(1).transpose(0, 1)
+                weights[page, :, slot] = got + (decay * weights[page, :, slot] if decay else 0)
+    return out
+
+
+def evict_cached_tokens_ref(k_pages, v_pages, weights, block_table, cached, new_table, budget, recent=0):
+    """The last ``recent`` tokens and the most attended others of each head, moved in order into other pages."""
+    B, K, S = block_table.size(0), k_pages.size(1), k_pages.size(2)
+    kept = torch.full((B, K, budget), -1, dtype=torch.int32)
+    old = [t.clone() for t in (k_pages, v_pages, weights)]
+    for b in range(B):
+        n = int(cached[b])
+        page, slot = _places(block_table, S, b, 0, n)
+        for h in range(K):
+            w = old[2][page, h, slot].tolist()
+            early = range(n) if n <= budget else range(n - recent)
+            first = sorted(early, key=lambda j: (w[j] != w[j], -w[j] if w[j] == w[j] else 0.0, j))
+            keep = sorted(first[:budget if n <= budget else budget - recent]) + list(range(len(early), n))
+            kept[b, h, :len(keep)] = torch.tensor(keep, dtype=torch.int32)
+            to, at = _places(new_table, S, b, 0, len(keep))
+            for t, o in zip((k_pages, v_pages, weights), old):
+                t[to, h, at] = o[page[keep], h, slot[keep]]
+    return kept, torch.clamp(cached, max=budget)
+
+
 __all__ = [
     "norm",
     "stack_sources",
@@ -604,5 +676,8 @@ __all__ = [
     "lrid_attention_residual_phase2_ref",
     "qkv_norm_rotary_ref",
     "swiglu_projection_ref",
+    "qkv_norm_rotary_cached_ref",
+    "cached_attention_ref",
+    "evict_cached_tokens_ref",
     "softmax_weights_ref",
 ]
