@@ -70,7 +70,8 @@ struct CacheAttendParams {
   FastDiv by_group, by_blocks, by_segs, by_wgs, by_weight_wgs;  // segments: kv_heads * blocks
   int32_t direct;               // a workgroup takes a whole segment
   int32_t tile;                 // 64 / 128 / 256: the head width it covers
-  int32_t vec, page16, whole, q_vec;  // aligned rows; pages of whole 16 tokens; head rows of whole 64 bytes; aligned queries
+  int32_t vb;                   // bytes (16, 8, 4 or a value's) that every row starts and ends at a multiple of
+  int32_t page16, whole, q_vec; // pages of whole 16 tokens; heads as wide as the tile; queries in rows of 16 bytes
   int32_t negate;               // the queries
   float scale;                  // of base-2 logarithms: the softmax's scale times log2(e), > 0
   float decay;
@@ -86,7 +87,7 @@ hipError_t launch_cache_attend_bf16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f32(const CacheAttendParams& p, hipStream_t st);
 
-constexpr int kEvictSlice = 8192;  // tokens whose keys a workgroup holds
+constexpr int kEvictSlice = 8192;  // tokens whose keys a workgroup holds (twice as many where it has a whole head)
 constexpr int kEvictSlots = 6152;  // counts and state of a workgroup, 4 bytes each
 
 struct CacheEvictParams {
@@ -99,7 +100,7 @@ struct CacheEvictParams {
   int32_t es;   // bytes of a value
   int32_t slices;  // of a table
   int32_t* hist;   // [heads][slices][kEvictSlots], where there are several
-  int32_t vec;  // rows in whole vectors of 16 bytes
+  int32_t vb;      // bytes (16, 8, 4 or a value's) that every row starts and ends at a multiple of
 };
 
 hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st);

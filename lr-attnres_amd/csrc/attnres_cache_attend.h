@@ -131,15 +131,18 @@ __device__ __forceinline__ void att_settle() {
 
 typedef _Float16 att_h4 __attribute__((ext_vector_type(4)));
 
-// HD: head width's tile (64, 128, 256); VEC: rows in aligned 16-byte vectors; PAGE16: pages of a multiple
-// of 16 tokens, so that 16 tokens lie in one and the scalar unit finds it.
-template <class DT, int HD, bool VEC, bool PAGE16>
+// HD: head width's tile (64, 128, 256); VB: bytes that every row starts and ends at a multiple of, and that one load
+// takes (16, or 8, 4, 2); PAGE16 (VB 16): pages of a multiple of 16 tokens, so that 16 tokens lie in one and the
+// scalar unit finds it.
+template <class DT, int HD, int VB, bool PAGE16>
 struct Att {
   using S = typename DT::S;
   static constexpr int kSize = sizeof(S);
   static constexpr int kPer = 16 / kSize;                      // values of a key chunk
   static constexpr int kKs = HD * kSize / 64;                  // key chunks of a lane
   static constexpr bool k32 = kSize == 4;
+  static constexpr bool VEC = VB == 16;
+  static constexpr int kG = VB / kSize;                        // values of a load
   static constexpr int kSub = k32 || HD == 256 ? 1 : 2;        // 16-token subtiles of a tile (one: half the registers)
   static constexpr int kTok = 16 * kSub;
   static constexpr int kW = k32 ? 4 : HD == 64 ? 4 : 8;        // values of a value chunk
@@ -152,7 +155,7 @@ struct Att {
   const CacheAttendParams& p;
   int lane, wave, c, g;          // column (query row) and token group of the lane
   int b, h, n, have;
-  int kcol[kKs], vcol[kNi];      // first value of each chunk, inside the row
+  int kcol[kKs], vcol0;          // first value of each key chunk; of the first value chunk
   uint32_t kofs[kKs], vofs[4][kNi]; // PAGE16: bytes from a subtile's first row
   const S *kh, *vh;              // of the head, page 0
   att_const_i32* table;          // of the sequence
@@ -173,18 +176,15 @@ struct Att {
     c = lane & 15;
     g = lane >> 4;
     const int Dh = p.c.head_dim;
+    vcol0 = c * kW;
 #pragma unroll
     for (int i = 0; i < kKs; ++i) kcol[i] = (i * 4 + g) * kPer;
-#pragma unroll
-    for (int i = 0; i < kNi; ++i) vcol[i] = (i * 16 + c) * kW;
-    if constexpr (VEC) {  // lanes behind a row's end read inside it, and drop what they read
+    if constexpr (PAGE16) {  // lanes behind a row's end read inside it, and drop what they read
       const uint32_t slot = (uint32_t)p.c.slot_stride;
 #pragma unroll
-      for (int i = 0; i < kNi; ++i) {
-        vcol[i] = min(vcol[i], Dh - kW);
+      for (int i = 0; i < kNi; ++i)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) vofs[t][i] = ((g * 4 + t) * slot + vcol[i]) * kSize;
-      }
+        for (int t = 0; t < 4; ++t) vofs[t][i] = ((g * 4 + t) * slot + min(vcol0 + i * 16 * kW, Dh - kW)) * kSize;
 #pragma unroll
       for (int i = 0; i < kKs; ++i) kofs[i] = (c * slot + min(kcol[i], Dh - kPer)) * kSize;
     }
@@ -215,32 +215,45 @@ struct Att {
 
   // E values at `at`, whole words
   template <int E>
-  __device__ __forceinline__ void load_vec(const void* at, uint32_t* w) const {
+  static __device__ __forceinline__ void load_vec(const void* at, uint32_t* w) {
     if constexpr (E * kSize == 16) {
       const u32x4 x = *(const u32x4*)at;
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    } else {
+    } else if constexpr (E * kSize == 8) {
       const u32x2 x = *(const u32x2*)at;
       w[0] = x.x, w[1] = x.y;
+    } else {
+      w[0] = *(const uint32_t*)at;
     }
   }
-  // values col .. col + E of a row that starts anywhere, zero behind its end
-  template <int E>
+  // values col .. col + E of a row, G a load; what is behind its end is read inside it (and not used)
+  template <int E, int G>
   __device__ __forceinline__ void load_any(const S* row, int col, uint32_t* w) const {
+    const int last = p.c.head_dim - G;
+    if constexpr (G * kSize < 4) {
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        w[e / 2] = row[min(col + e, last)] | (uint32_t)row[min(col + e + 1, last)] << 16;
+    } else {
+      constexpr int kOne = G < E ? G : E;
+#pragma unroll
+      for (int e = 0; e < E; e += kOne) load_vec<kOne>(row + min(col + e, p.c.head_dim - kOne), w + e * kSize / 4);
+    }
+  }
+  // the words of a chunk of 16 bytes from value col on, 0 behind the row's end
+  __device__ __forceinline__ u32x4 inside(u32x4 w, int col) const {
     const int Dh = p.c.head_dim;
 #pragma unroll
-    for (int e = 0; e < E; e += 4 / kSize) {
-      if constexpr (k32) {
-        w[e] = col + e < Dh ? __float_as_uint(row[col + e]) : 0;
-      } else {
-        const uint32_t lo = col + e < Dh ? row[col + e] : 0, hi = col + e + 1 < Dh ? row[col + e + 1] : 0;
-        w[e / 2] = lo | hi << 16;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int at = col + i * 4 / kSize;
+      if constexpr (k32) w[i] = at < Dh ? w[i] : 0;
+      else w[i] = at + 1 < Dh ? w[i] : at < Dh ? w[i] & 0xffffu : 0;
     }
+    return w;
   }
 
-  // An offset in 32 bits where it is used, for loads from a scalar base: widened outside a loop it would cost 64-bit
-  // additions for each load.
+  // An offset as it is where it is used: one that is widened, added to or bounded outside the loop costs 64-bit
+  // additions, or a register for each load.
   static __device__ __forceinline__ uint32_t here(uint32_t x) {
     asm volatile("" : "+v"(x));
     return x;
@@ -258,8 +271,7 @@ struct Att {
 #pragma unroll
         for (int i = 0; i < kKs; ++i) {
           uint32_t w[4];
-          if constexpr (VEC) load_vec<kPer>(row + min(kcol[i], p.c.head_dim - kPer), w);
-          else load_any<kPer>(row, kcol[i], w);
+          load_any<kPer, kG>(row, (int)here(kcol[0]) + i * 4 * kPer, w);
           k[s][i] = u32x4{w[0], w[1], w[2], w[3]};
         }
       }
@@ -279,8 +291,7 @@ struct Att {
           const S* row = vh + max(__shfl(r.off[0], 16 * s + g * 4 + t, kWave), (int64_t)0);
 #pragma unroll
           for (int i = 0; i < kNi; ++i) {
-            if constexpr (VEC) load_vec<kW>(row + vcol[i], v[s][t][i]);
-            else load_any<kW>(row, vcol[i], v[s][t][i]);
+            load_any<kW, kG>(row, (int)here(vcol0) + i * 16 * kW, v[s][t][i]);
           }
         }
       }
@@ -383,12 +394,14 @@ struct Att {
     Rows after;
     if constexpr (AHEAD) after = rows_of(min(t0 + 2 * kStep, (n - 1) & -kTok), n);
     // (before all of the products: no branch comes between them and what reads them)
-    if (VEC && !p.whole) {
+    if (!p.whole) {
 #pragma unroll
       for (int s = 0; s < kSub; ++s)
 #pragma unroll
-        for (int i = 0; i < kKs; ++i)
-          if (kcol[i] >= p.c.head_dim) k[s][i] = u32x4{0, 0, 0, 0};
+        for (int i = 0; i < kKs; ++i) {
+          if constexpr (!VEC) k[s][i] = inside(k[s][i], (int)here(kcol[0]) + i * 4 * kPer);
+          else if (kcol[i] >= p.c.head_dim) k[s][i] = u32x4{0, 0, 0, 0};
+        }
     }
     sw_f4 s4[kSub];
 #pragma unroll
@@ -496,8 +509,8 @@ struct Att {
   }
 
   // tokens [first, end) of the head for rows [row0, row0 + rows), of those that there are (all of them, where a workgroup
-  // takes a whole segment); this wave's: tiles wave, wave + 4, ...
-  __device__ __forceinline__ void piece(int row0, int rows, int first, int end, Seq seq) {
+  // takes a whole segment); this wave's: tiles wave, wave + 4, ...  stage: 16 rows of LDS that nobody uses.
+  __device__ __forceinline__ void piece(int row0, int rows, int first, int end, Seq seq, void* stage) {
     const int r = row0 + c, t_row = div_by(r, p.by_group);
     const bool valid = c < rows;
     const int hq = h * p.group + r - t_row * p.group;
@@ -513,30 +526,27 @@ struct Att {
       load_v(now);
       next = rows_of(min(t_first + kStep, (limit - 1) & -kTok), limit);
     }
-    const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
+    if (VEC && p.q_vec) {
+      const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
 #pragma unroll
-    for (int i = 0; i < kKs; ++i) {
-      q[i] = u32x4{0, 0, 0, 0};
-      uint32_t w[4];
-      if (valid && kcol[i] < p.c.head_dim) {
-        if constexpr (VEC) {
-          if (p.q_vec) {
-            q[i] = *(const u32x4*)(src + kcol[i]);
-            continue;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < kPer; e += 4 / kSize) {
-          const int col = kcol[i] + e, Dh = p.c.head_dim;
-          if constexpr (k32) {
-            w[e] = col < Dh ? __float_as_uint(src[col]) : 0;
-          } else {
-            const uint32_t lo = col < Dh ? src[col] : 0, hi = col + 1 < Dh ? src[col + 1] : 0;
-            w[e / 2] = lo | hi << 16;
-          }
-        }
-        q[i] = u32x4{w[0], w[1], w[2], w[3]};
+      for (int i = 0; i < kKs; ++i) {
+        q[i] = u32x4{0, 0, 0, 0};
+        if (valid && kcol[i] < p.c.head_dim) q[i] = *(const u32x4*)(src + kcol[i]);
       }
+    } else {  // (by single values, in few registers)
+      S* const rows_q = (S*)stage;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < kAttRows * HD; i += kAttWaves * kWave) {
+        const int qr = row0 + i / HD, col = i % HD, t = div_by(qr, p.by_group);
+        rows_q[i] = i / HD < rows && col < p.c.head_dim
+                        ? ((const S*)p.q)[b * p.q_b_stride + (h * p.group + qr - t * p.group) * p.q_h_stride +
+                                          t * p.q_t_stride + col]
+                        : (S)0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kKs; ++i) q[i] = *(const u32x4*)(rows_q + c * HD + kcol[i]);
+      __syncthreads();
     }
     if (p.negate) {
 #pragma unroll
@@ -608,9 +618,9 @@ __device__ __forceinline__ void att_row_out(const CacheAttendParams& p, int b, i
   }
 }
 
-template <class DT, int HD, bool VEC, bool PAGE16>
+template <class DT, int HD, int VB, bool PAGE16>
 __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_attend_kernel(CacheAttendParams p) {
-  using A = Att<DT, HD, VEC, PAGE16>;
+  using A = Att<DT, HD, VB, PAGE16>;
   using S = typename DT::S;
   __shared__ float so[kAttWaves][kAttRows][A::kPitch];
   __shared__ float sm[kAttWaves][kAttRows], sl[kAttWaves][kAttRows];
@@ -642,7 +652,7 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
     a.h = div_by(seg, p.by_blocks);
     const int row0 = (seg - a.h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
     const bool whole = u0 == 0 && u1 == units;
-    a.piece(row0, rows, u0 * kAttUnit, p.direct ? p.c.room : u1 * kAttUnit, seq);
+    a.piece(row0, rows, u0 * kAttUnit, p.direct ? p.c.room : u1 * kAttUnit, seq, so);
     if (a.n > 0 && a.c < rows) {
       if (a.g == 0) sm[a.wave][a.c] = a.m == -INFINITY ? a.m : a.base_of(a.m), sl[a.wave][a.c] = a.l;
 #pragma unroll
@@ -842,9 +852,11 @@ template <class DT, int HD>
 hipError_t run_attend(const CacheAttendParams& p, hipStream_t st) {
   const int64_t segs = (int64_t)p.c.batch * p.c.kv_heads * p.blocks;
   const dim3 grid((unsigned)(p.direct ? segs : p.wgs)), wg(kAttWaves * kWave);
-  if (p.vec && p.page16) cache_attend_kernel<DT, HD, true, true><<<grid, wg, 0, st>>>(p);
-  else if (p.vec) cache_attend_kernel<DT, HD, true, false><<<grid, wg, 0, st>>>(p);
-  else cache_attend_kernel<DT, HD, false, false><<<grid, wg, 0, st>>>(p);
+  if (p.vb == 16 && p.page16) cache_attend_kernel<DT, HD, 16, true><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 16) cache_attend_kernel<DT, HD, 16, false><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 8) cache_attend_kernel<DT, HD, 8, false><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 4) cache_attend_kernel<DT, HD, 4, false><<<grid, wg, 0, st>>>(p);
+  else if constexpr (DT::kCode != 0) cache_attend_kernel<DT, HD, 2, false><<<grid, wg, 0, st>>>(p);
   const hipError_t err = hipGetLastError();
   const int joins = p.direct ? 0 : p.c.batch * p.c.kv_heads * p.rows;
   if (err != hipSuccess || joins + p.weight_wgs == 0) return err;

@@ -76,6 +76,14 @@ bool rows_at(const attnres_cache_desc* c, int per) {
          c->head_stride % per == 0 && c->slot_stride % per == 0;
 }
 
+// the widest of 16, 8, 4 bytes that every row of the pages starts and ends at a multiple of, or a value's
+int row_bytes(const attnres_cache_desc* c) {
+  const int es = es_of(c->dtype);
+  for (int b = 16; b > es; b /= 2)
+    if (rows_at(c, b / es)) return b;
+  return es;
+}
+
 int check_append(const attnres_cache_desc* c, const attnres_cache_append_desc* d) {
   if (int rc = check_cache(c)) return rc;
   if (!d) return api_fail(ATTNRES_EINVAL, "desc is NULL");
@@ -179,7 +187,7 @@ int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d,
                     (long long)d->tokens, d->q_heads, (long long)room);
   // (pages, and tokens inside one, within 32-bit offsets of each other)
   constexpr int64_t kFar = (int64_t)1 << 32;
-  a->page16 = c->page_size % 16 == 0 && c->page_stride < kFar / es_of(c->dtype) &&
+  a->page16 = row_bytes(c) == 16 && c->page_size % 16 == 0 && c->page_stride < kFar / es_of(c->dtype) &&
               c->slot_stride < kFar / es_of(c->dtype) / c->page_size;
   a->tile = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
   a->rows = (int)rows;
@@ -255,7 +263,7 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
     p.by_weight_wgs = fast_div(p.weight_wgs);
   }
   p.tile = a.tile;
-  p.vec = rows_at(c, per);
+  p.vb = row_bytes(c);
   p.page16 = a.page16;
   p.whole = c->head_dim == a.tile;
   p.q_vec = aligned(d->q, 16) && d->q_batch_stride % per == 0 && d->q_head_stride % per == 0 && d->q_token_stride % per == 0;
@@ -296,16 +304,18 @@ int check_evict(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
   return ATTNRES_OK;
 }
 
-int64_t evict_slices(const attnres_cache_desc* c) {
-  const int64_t n = (c->table_pages * c->page_size + kEvictSlice - 1) / kEvictSlice;
-  return n > 1 ? n : 1;
+// workgroups that choose a head's tokens: one, where it can hold all keys or there is nothing to choose
+int64_t evict_slices(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
+  const int64_t room = c->table_pages * c->page_size;
+  return room <= 2 * kEvictSlice || budget == recent ? 1 : (room + kEvictSlice - 1) / kEvictSlice;
 }
 
 }  // namespace
 
 extern "C" size_t attnres_cache_evict_workspace_size(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
   if (check_evict(c, budget, recent) || c->batch == 0) return 0;
-  return evict_slices(c) > 1 ? (size_t)c->batch * c->kv_heads * evict_slices(c) * kEvictSlots * 4 : 0;
+  const int64_t slices = evict_slices(c, budget, recent);
+  return slices > 1 ? (size_t)c->batch * c->kv_heads * slices * kEvictSlots * 4 : 0;
 }
 
 extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* new_table, int64_t new_stride,
@@ -329,9 +339,9 @@ extern "C" int attnres_cache_evict(const attnres_cache_desc* c, const int32_t* n
   p.kept = kept;
   p.left = left;
   p.es = es_of(c->dtype);
-  p.slices = (int32_t)evict_slices(c);
+  p.slices = (int32_t)evict_slices(c, budget, recent);
   p.hist = (int32_t*)workspace;
-  p.vec = rows_at(c, 16 / p.es);
+  p.vb = row_bytes(c);
   const hipError_t err = launch_cache_evict(p, (hipStream_t)stream);
   if (err != hipSuccess) return api_fail(ATTNRES_ELAUNCH, "cache evict launch failed: %s", hipGetErrorString(err));
   return ATTNRES_OK;

@@ -52,7 +52,7 @@ __device__ __forceinline__ int block_scan(int x, int* sums) {
 }
 
 constexpr int kBins = 4096;                         // of the first round, 1024 of the other two
-constexpr int kSlice = kEvictSlice, kR = kSlice / kSelThreads;  // tokens that a workgroup holds the keys of
+constexpr int kSlice = kEvictSlice, kR = kSlice / kSelThreads;  // tokens of a workgroup, keys a thread
 static_assert(kR * kSelThreads == kSlice, "whole keys a thread");
 constexpr int kWaves = kSelThreads / kWave;
 
@@ -66,15 +66,16 @@ struct Found {
   bool open;  // more are equal than wanted
 };
 
+template <int R>
 struct SelectShared {
   int sums[2][kWaves];
   int digit, want, open;
-  int above[kR * kWaves], equal[kR * kWaves];
+  int above[R * kWaves], equal[R * kWaves];
 };
 
 // The next digit of the want-th largest key, from the counts of its places: count(place) for any place of 2^bits.
-template <class F>
-__device__ __forceinline__ void next_digit(int round, Found& f, SelectShared& s, F count) {
+template <int R, class F>
+__device__ __forceinline__ void next_digit(int round, Found& f, SelectShared<R>& s, F count) {
   const int bits = round_bits(round), mine = (1 << bits) / kSelThreads;
   // from the largest place down
   const int first = (1 << bits) - 1 - (int)threadIdx.x * mine;
@@ -106,11 +107,12 @@ __device__ __forceinline__ void next_digit(int round, Found& f, SelectShared& s,
 
 // The tokens j0 .. of a head: what is kept of them goes to its places, `above` and `equal` of the tokens before them
 // being above the found prefix and equal to it.
-__device__ __forceinline__ void place(const uint32_t (&key)[kR], int j0, int early, const Found& f, int above, int equal,
-                                      int32_t* kept, SelectShared& s) {
+template <int R>
+__device__ __forceinline__ void place(const uint32_t (&key)[R], int j0, int early, const Found& f, int above, int equal,
+                                      int32_t* kept, SelectShared<R>& s) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
 #pragma unroll
-  for (int i = 0; i < kR; ++i) {
+  for (int i = 0; i < R; ++i) {
     const bool in = j0 + i * kSelThreads + tid < early;
     const uint64_t a = __ballot(in && (key[i] & f.mask) > f.prefix), e = __ballot(in && (key[i] & f.mask) == f.prefix);
     if (lane == 0) {
@@ -119,15 +121,15 @@ __device__ __forceinline__ void place(const uint32_t (&key)[kR], int j0, int ear
     }
   }
   __syncthreads();
-  const int a0 = tid < kR * kWaves ? s.above[tid] : 0, e0 = tid < kR * kWaves ? s.equal[tid] : 0;
+  const int a0 = tid < R * kWaves ? s.above[tid] : 0, e0 = tid < R * kWaves ? s.equal[tid] : 0;
   const int a1 = block_scan(a0, s.sums[0]), e1 = block_scan(e0, s.sums[1]);
-  if (tid < kR * kWaves) {
+  if (tid < R * kWaves) {
     s.above[tid] = above + a1 - a0;
     s.equal[tid] = equal + e1 - e0;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kR; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int j = j0 + i * kSelThreads + tid;
     const bool is_above = j < early && (key[i] & f.mask) > f.prefix, is_equal = j < early && (key[i] & f.mask) == f.prefix;
     const uint64_t below = (1ull << lane) - 1;
@@ -137,20 +139,22 @@ __device__ __forceinline__ void place(const uint32_t (&key)[kR], int j0, int ear
   }
 }
 
-__device__ __forceinline__ void load_keys(const CachePages& c, int b, int h, int j0, int early, uint32_t (&key)[kR]) {
+template <int R>
+__device__ __forceinline__ void load_keys(const CachePages& c, int b, int h, int j0, int early, uint32_t (&key)[R]) {
 #pragma unroll
-  for (int i = 0; i < kR; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int j = j0 + i * kSelThreads + (int)threadIdx.x;
     key[i] = j < early ? token_key(c, b, h, j) : 0;
   }
 }
 
-__device__ __forceinline__ void count_keys(const uint32_t (&key)[kR], int j0, int early, int round, const Found& f, int* hist) {
+template <int R>
+__device__ __forceinline__ void count_keys(const uint32_t (&key)[R], int j0, int early, int round, const Found& f, int* hist) {
   const int bits = round_bits(round), shift = round_shift(round);
   for (int i = threadIdx.x; i < 1 << bits; i += kSelThreads) hist[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kR; ++i)
+  for (int i = 0; i < R; ++i)
     if (j0 + i * kSelThreads + (int)threadIdx.x < early && (key[i] & f.mask) == f.prefix)
       atomicAdd(&hist[(key[i] >> shift) & ((1 << bits) - 1)], 1);
   __syncthreads();
@@ -166,16 +170,17 @@ __device__ __forceinline__ bool no_choice(const CacheEvictParams& p, int n, int3
   return p.budget == p.recent;
 }
 
-// tables of at most kSlice tokens
+// tables of at most R * 1024 tokens
+template <int R>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(CacheEvictParams p) {
   __shared__ int hist[kBins];
-  __shared__ SelectShared s;
+  __shared__ SelectShared<R> s;
   const int b = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
   if (no_choice(p, n, kept)) return;
   const int early = n - p.recent;
-  uint32_t key[kR];
+  uint32_t key[R];
   load_keys(p.c, b, h, 0, early, key);
   Found f{0, 0, p.budget - p.recent, true};
   for (int round = 0; round < 3 && f.open; ++round) {
@@ -196,7 +201,7 @@ __device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 307
 
 // What the rounds before `round` have found; above, equal: keys of the slices before this one.
 __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int head, int slices, int slice, int round, int* above,
-                                              int* equal, SelectShared& s) {
+                                              int* equal, SelectShared<kR>& s) {
   Found f{0, 0, p.budget - p.recent, true};
   int a = 0, e = 0;
   int32_t* state = p.hist + ((int64_t)head * p.slices + slice) * kSlots + kState;
@@ -249,7 +254,7 @@ __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int hea
 
 __global__ __launch_bounds__(kSelThreads) void evict_count_kernel(CacheEvictParams p, int round) {
   __shared__ int hist[kBins];
-  __shared__ SelectShared s;
+  __shared__ SelectShared<kR> s;
   const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
   const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   const int early = n - p.recent, j0 = slice * kSlice;
@@ -265,7 +270,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_count_kernel(CacheEvictPara
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_place_kernel(CacheEvictParams p) {
-  __shared__ SelectShared s;
+  __shared__ SelectShared<kR> s;
   const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
   const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   int32_t* kept = p.kept + (int64_t)head * p.budget;
@@ -315,19 +320,20 @@ hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st) {
   const int64_t heads = (int64_t)p.c.batch * p.c.kv_heads;
   const dim3 sel((unsigned)(heads * p.slices)), wg(kSelThreads);
   if (p.slices == 1) {
-    evict_select_kernel<<<sel, wg, 0, st>>>(p);
+    if (p.c.room <= kSlice) evict_select_kernel<kR><<<sel, wg, 0, st>>>(p);
+    else evict_select_kernel<2 * kR><<<sel, wg, 0, st>>>(p);
   } else {
     for (int round = 0; round < 3; ++round) evict_count_kernel<<<sel, wg, 0, st>>>(p, round);
     evict_place_kernel<<<sel, wg, 0, st>>>(p);
   }
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const int size = p.vec ? 16 : p.es, per = p.c.head_dim * p.es / size;
-  const int lanes = per < 64 ? per : 64;
+  const int per = p.c.head_dim * p.es / p.vb, lanes = per < 64 ? per : 64;
   const int64_t rows = heads * p.budget, blocks = (rows + 256 / lanes - 1) / (256 / lanes);
   const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
-  if (size == 16) evict_copy_kernel<u32x4><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
-  else if (size == 4) evict_copy_kernel<uint32_t><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
+  if (p.vb == 16) evict_copy_kernel<u32x4><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
+  else if (p.vb == 8) evict_copy_kernel<u32x2><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
+  else if (p.vb == 4) evict_copy_kernel<uint32_t><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
   else evict_copy_kernel<uint16_t><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
   return hipGetLastError();
 }

@@ -52,7 +52,7 @@ def run_and_check(c, new, cached, budget, recent, table=None, cached_as=None, ne
 
 
 @pytest.mark.parametrize("dtype,K,Dh,S", [("bf16", 2, 64, 16), ("fp16", 3, 40, 24), ("fp32", 1, 128, 64), ("bf16", 2, 17, 7),
-                                          ("fp32", 2, 5, 1), ("bf16", 1, 256, 128)])
+                                          ("fp32", 2, 5, 1), ("bf16", 1, 256, 128), ("bf16", 2, 62, 16), ("fp16", 1, 36, 32), ("fp32", 2, 6, 16)])
 @pytest.mark.parametrize("budget,recent", [(1, 0), (1, 1), (50, 0), (50, 13), (64, 64), (130, 32)])
 def test_choice_and_copies(dtype, K, Dh, S, budget, recent):
     cached = [0, 1, budget, budget + 1, 2 * budget + 5, 333]
@@ -68,7 +68,7 @@ def test_layouts(layout, dtype):
     run_and_check(c, new, cached, 70, 10)
 
 
-@pytest.mark.parametrize("cached,budget,recent", [([5000, 3000], 1024, 100), ([20000], 4000, 0), ([70000], 100, 50),
+@pytest.mark.parametrize("cached,budget,recent", [([5000, 3000], 1024, 100), ([20000], 4000, 0), ([70000], 100, 50), ([9000, 16384, 12000], 2500, 300), ([16000, 5], 300, 300), ([20000, 17000], 64, 64),
                                                   ([1024, 1025, 2048, 2049], 1024, 1023)])
 def test_long(cached, budget, recent):
     c, new = build(5, "bf16", 2, 8, 64, cached, budget, ties=len(cached) > 1)

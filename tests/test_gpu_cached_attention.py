@@ -42,7 +42,9 @@ def check(c, q, cached, fresh, pass_fresh=False, scale=None, **kw):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("H,K,Dh,S", [
     (1, 1, 64, 64), (12, 12, 64, 16), (8, 2, 128, 32), (16, 1, 64, 64), (20, 1, 96, 48), (6, 2, 256, 128), (3, 3, 40, 24),
-    (4, 4, 32, 1), (2, 1, 20, 5), (5, 5, 17, 7), (34, 2, 80, 20), (4, 2, 8, 256), (2, 2, 200, 100)])
+    (4, 4, 32, 1), (2, 1, 20, 5), (5, 5, 17, 7), (34, 2, 80, 20), (4, 2, 8, 256), (2, 2, 200, 100),
+    (4, 2, 148, 64), (2, 1, 134, 16), (3, 1, 62, 32), (2, 2, 36, 24), (8, 1, 196, 32), (2, 1, 129, 16), (6, 2, 100, 48),
+    (2, 2, 1, 16), (3, 1, 254, 20)])
 def test_lengths_and_shapes(dtype, H, K, Dh, S):
     cached = [0, 1, 30, 31, 32, 63, 64, 65, 127, 128, 129, 300]
     c, q, fresh = build(H * 131 + Dh, dtype, H, K, Dh, S, cached)
