@@ -66,7 +66,8 @@ struct CacheAttendParams {
   int32_t tokens, q_heads;
   int32_t group, rows, blocks;  // query heads of a key / value head; with the new tokens; 16-row blocks of them
   int32_t wgs;                  // of a split cache
-  int32_t weight_wgs;           // that add the weights up, 0: none are kept
+  int32_t weight_wgs;           // that add the weights up in a launch of their own
+  int32_t own_weights;          // the workgroup of a whole segment does it
   FastDiv by_group, by_blocks, by_segs, by_wgs, by_weight_wgs;  // segments: kv_heads * blocks
   int32_t direct;               // a workgroup takes a whole segment
   int32_t tile;                 // 64 / 128 / 256: the head width it covers

@@ -165,9 +165,13 @@ struct Att {
   float m, l;                    // of the lane's row: maximum of <q, k>, the lane's part of the sum
 
   struct Rows {
-    int64_t off[PAGE16 ? kSub : 1];  // PAGE16: bytes from the head's page 0 to a subtile's first token; else values to token
-                                     // `lane` of the tile, -1: no page
-    bool there[PAGE16 ? kSub : 1];   // PAGE16: whether it has a page (one that has none reads page 0)
+    // PAGE16: of each subtile, bytes from the head's page 0 to its first token, and whether it has a page (one that has
+    // none reads page 0)
+    int64_t off[kSub];
+    bool there[kSub];
+    // else, of token `lane` of the tile: its page as the table has it (not looked at before the tile's loads: that
+    // would wait for the table, and for all loads before it), and its slot
+    int page, slot;
   };
 
   __device__ __forceinline__ Att(const CacheAttendParams& p_) : p(p_) {
@@ -205,12 +209,14 @@ struct Att {
       }
     } else {
       const int j = min(t0 + (lane & (kTok - 1)), limit - 1), at = div_by(j, p.c.by_page);
-      const int page = table[at];
-      r.off[0] = (unsigned)page < (unsigned)p.c.pages
-                     ? page * p.c.page_stride + (j - at * p.c.page_size) * p.c.slot_stride
-                     : -1;
+      r.page = table[at];
+      r.slot = j - at * p.c.page_size;
     }
     return r;
+  }
+  // values from the head's page 0 to token `lane` of the tile; of page 0 for one that has no page
+  __device__ __forceinline__ int64_t token_off(const Rows& r) const {
+    return (unsigned)r.page < (unsigned)p.c.pages ? r.page * p.c.page_stride + r.slot * p.c.slot_stride : 0;
   }
 
   // E values at `at`, whole words
@@ -260,6 +266,7 @@ struct Att {
   }
 
   __device__ __forceinline__ void load_k(const Rows& r) {
+    const int64_t off = PAGE16 ? 0 : token_off(r);
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
       if constexpr (PAGE16) {
@@ -267,7 +274,7 @@ struct Att {
 #pragma unroll
         for (int i = 0; i < kKs; ++i) k[s][i] = *(const u32x4*)(row + here(kofs[i]));
       } else {
-        const S* row = kh + max(__shfl(r.off[0], 16 * s + c, kWave), (int64_t)0);
+        const S* row = kh + __shfl(off, 16 * s + c, kWave);
 #pragma unroll
         for (int i = 0; i < kKs; ++i) {
           uint32_t w[4];
@@ -279,6 +286,7 @@ struct Att {
   }
 
   __device__ __forceinline__ void load_v(const Rows& r) {
+    const int64_t off = PAGE16 ? 0 : token_off(r);
 #pragma unroll
     for (int s = 0; s < kSub; ++s)
 #pragma unroll
@@ -288,7 +296,7 @@ struct Att {
 #pragma unroll
           for (int i = 0; i < kNi; ++i) load_vec<kW>(row + here(vofs[t][i]), v[s][t][i]);
         } else {
-          const S* row = vh + max(__shfl(r.off[0], 16 * s + g * 4 + t, kWave), (int64_t)0);
+          const S* row = vh + __shfl(off, 16 * s + g * 4 + t, kWave);
 #pragma unroll
           for (int i = 0; i < kNi; ++i) {
             load_any<kW, kG>(row, (int)here(vcol0) + i * 16 * kW, v[s][t][i]);
@@ -413,10 +421,10 @@ struct Att {
     float scale[kSub];  // NaN where there is no page: the row shows it
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
-      scale[s] = PAGE16 && !now.there[PAGE16 ? s : 0] && (!CUT || t0 + 16 * s < n) ? __builtin_nanf("") : p.scale;
+      scale[s] = PAGE16 && !now.there[s] && (!CUT || t0 + 16 * s < n) ? __builtin_nanf("") : p.scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if (!PAGE16 && __shfl(now.off[0], 16 * s + g * 4 + t, kWave) < 0) s4[s][t] = __builtin_nanf("");
+        if (!PAGE16 && (unsigned)__shfl(now.page, 16 * s + g * 4 + t, kWave) >= (unsigned)p.c.pages) s4[s][t] = __builtin_nanf("");
         if (CUT && t0 + 16 * s + g * 4 + t >= row.lim) s4[s][t] = -INFINITY;
       }
     }
@@ -517,15 +525,7 @@ struct Att {
     table = (att_const_i32*)(uintptr_t)(p.c.table + b * p.c.table_stride);
     kh = (const S*)p.c.k + h * p.c.head_stride;
     vh = (const S*)p.c.v + h * p.c.head_stride;
-    // (the first tile's loads wait for the block table alone where the length is not known yet)
-    const int t_first = first + wave * kTok, limit = p.direct ? p.c.room : seq.n;
-    Rows now, next;
-    if (t_first < limit) {
-      now = rows_of(t_first, limit);
-      load_k(now);
-      load_v(now);
-      next = rows_of(min(t_first + kStep, (limit - 1) & -kTok), limit);
-    }
+    // (before the tiles' loads: a wait for what came last waits for all of them, in every turn of the loop)
     if (VEC && p.q_vec) {
       const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
 #pragma unroll
@@ -548,6 +548,17 @@ struct Att {
       for (int i = 0; i < kKs; ++i) q[i] = *(const u32x4*)(rows_q + c * HD + kcol[i]);
       __syncthreads();
     }
+    // (the first tile's loads wait for the block table alone where the length is not known yet)
+    const int t_first = first + wave * kTok, limit = p.direct ? p.c.room : seq.n;
+    if (t_first >= limit) {
+      clear();
+      n = seq.n;
+      return;
+    }
+    Rows now = rows_of(t_first, limit), next;
+    load_k(now);
+    load_v(now);
+    next = rows_of(min(t_first + kStep, (limit - 1) & -kTok), limit);
     if (p.negate) {
 #pragma unroll
       for (int i = 0; i < kKs; ++i) q[i] ^= k32 ? 0x80000000u : 0x80008000u;
@@ -618,12 +629,31 @@ __device__ __forceinline__ void att_row_out(const CacheAttendParams& p, int b, i
   }
 }
 
+// One token's weight: w_j <- decay w_j + got
+__device__ __forceinline__ void add_weight(const CacheAttendParams& p, int b, int h, int j, float got) {
+  const int at = div_by(j, p.c.by_page), page = p.c.table[b * p.c.table_stride + at];
+  if ((unsigned)page >= (unsigned)p.c.pages) return;
+  float* w = p.c.w + page * p.c.w_page_stride + h * p.c.w_head_stride + (j - at * p.c.page_size);
+  *w = p.decay == 0.f ? got : p.decay * *w + got;
+}
+
+// By the workgroup that has all of the head's queries and tokens, from the scores that it has stored.
+__device__ __forceinline__ void add_own_weights(const CacheAttendParams& p, int b, int h, int rows, int n, const float* lse) {
+  const float* x = p.logits + (b * (int64_t)p.q_heads + h * p.group) * p.logit_stride;
+  for (int j = threadIdx.x; j < n; j += kAttWaves * kWave) {
+    float sum = 0.f;
+    for (int r = 0; r < rows; ++r) sum += __builtin_amdgcn_exp2f(x[r * p.logit_stride + j] - lse[r]);
+    add_weight(p, b, h, j, sum);
+  }
+}
+
 template <class DT, int HD, int VB, bool PAGE16>
 __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_attend_kernel(CacheAttendParams p) {
   using A = Att<DT, HD, VB, PAGE16>;
   using S = typename DT::S;
   __shared__ float so[kAttWaves][kAttRows][A::kPitch];
   __shared__ float sm[kAttWaves][kAttRows], sl[kAttWaves][kAttRows];
+  __shared__ float lse[kAttRows];
   A a(p);
   const int Dh = p.c.head_dim, segs = p.c.kv_heads * p.blocks;
   // neighbouring workgroups run on different XCDs; those of one XCD take neighbouring units
@@ -682,7 +712,9 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
       }
       if (whole) {
         att_row_out<DT>(p, a.b, a.h, row0 + r, col, a.n, l, o);
-        if (p.row_ml && col == 0) {
+        if (p.own_weights) {
+          if (col == 0) lse[r] = top + log2f(l);
+        } else if (p.row_ml && col == 0) {
           float* ml = p.row_ml + (a.b * (int64_t)p.q_heads + a.h * p.group + row0 + r) * 2;
           ml[0] = top;
           ml[1] = l;
@@ -696,6 +728,7 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
       }
     }
     __syncthreads();
+    if (p.own_weights) add_own_weights(p, a.b, a.h, rows, a.n, lse);
   }
 }
 
@@ -833,11 +866,7 @@ __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) 
     if (part) half[threadIdx.x - kAttUnit] = sum;
     __syncthreads();
     if (part || j >= n) continue;
-    sum += half[threadIdx.x];
-    const int page = cache_page(p.c, b, j);
-    if (page < 0) continue;
-    float* w = p.c.w + page * p.c.w_page_stride + h * p.c.w_head_stride + (j - div_by(j, p.c.by_page) * p.c.page_size);
-    *w = p.decay == 0.f ? sum : p.decay * *w + sum;
+    add_weight(p, b, h, j, sum + half[threadIdx.x]);
   }
 }
 

@@ -257,7 +257,8 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   p.by_blocks = fast_div(a.blocks);
   p.by_segs = fast_div(c->kv_heads * a.blocks);
   p.by_wgs = fast_div(a.wgs);
-  if (c->weights) {
+  p.own_weights = c->weights && a.direct && a.blocks == 1;
+  if (c->weights && !p.own_weights) {
     const int64_t units = c->batch * c->kv_heads * ((p.c.room + kAttUnit - 1) / kAttUnit);
     p.weight_wgs = (int32_t)(units < 8 * kCus ? units : 8 * kCus);
     p.by_weight_wgs = fast_div(p.weight_wgs);

@@ -178,17 +178,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(CacheEvictPar
   const int b = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
-  if (no_choice(p, n, kept)) return;
-  const int early = n - p.recent;
-  uint32_t key[R];
-  load_keys(p.c, b, h, 0, early, key);
-  Found f{0, 0, p.budget - p.recent, true};
-  for (int round = 0; round < 3 && f.open; ++round) {
-    count_keys(key, 0, early, round, f, hist);
-    next_digit(round, f, s, [&](int place) { return hist[place]; });
-    __syncthreads();
+  if (!no_choice(p, n, kept)) {
+    const int early = n - p.recent;
+    uint32_t key[R];
+    load_keys(p.c, b, h, 0, early, key);
+    Found f{0, 0, p.budget - p.recent, true};
+    for (int round = 0; round < 3 && f.open; ++round) {
+      count_keys(key, 0, early, round, f, hist);
+      next_digit(round, f, s, [&](int place) { return hist[place]; });
+      __syncthreads();
+    }
+    place(key, 0, early, f, 0, 0, kept, s);
   }
-  place(key, 0, early, f, 0, 0, kept, s);
 }
 
 // Longer tables: kSlice tokens a workgroup, a launch for each round's counts and one that places what is kept.  Each
@@ -287,30 +288,35 @@ __global__ __launch_bounds__(kSelThreads) void evict_place_kernel(CacheEvictPara
   place(key, j0, early, f, above, equal, kept, s);
 }
 
-// lanes: of a row (its 16-byte vectors, or single values)
+// Row i of what a head keeps: its key, value and weight, from token j, by `lanes` threads of which this is `col`.
+template <class V>
+__device__ __forceinline__ void copy_row(const CacheEvictParams& p, int b, int h, int i, int j, int col, int lanes, int per) {
+  const CachePages& c = p.c;
+  const int at = div_by(j, c.by_page), at_to = div_by(i, c.by_page);
+  const int from = c.table[b * c.table_stride + at], to = p.new_table[b * p.new_stride + at_to];
+  if ((unsigned)from >= (unsigned)c.pages || (unsigned)to >= (unsigned)c.pages) return;
+  const int slot = j - at * c.page_size, slot_to = i - at_to * c.page_size;
+  if (from == to && slot == slot_to) return;
+  const int64_t src = (from * c.page_stride + h * c.head_stride + slot * c.slot_stride) * p.es;
+  const int64_t dst = (to * c.page_stride + h * c.head_stride + slot_to * c.slot_stride) * p.es;
+  for (int x = col; x < per; x += lanes) {
+    const V k = ((const V*)((const char*)c.k + src))[x], v = ((const V*)((const char*)c.v + src))[x];
+    ((V*)((char*)c.k + dst))[x] = k;
+    ((V*)((char*)c.v + dst))[x] = v;
+  }
+  if (col == 0)
+    c.w[to * c.w_page_stride + h * c.w_head_stride + slot_to] = c.w[from * c.w_page_stride + h * c.w_head_stride + slot];
+}
+
+// lanes: of a row (of its vectors V)
 template <class V>
 __global__ __launch_bounds__(256) void evict_copy_kernel(CacheEvictParams p, int lanes, int per, int64_t rows) {
-  const CachePages& c = p.c;
   const int here = 256 / lanes, col = threadIdx.x % lanes;
   if ((int)threadIdx.x / lanes >= here) return;
   for (int64_t row = (int64_t)blockIdx.x * here + threadIdx.x / lanes; row < rows; row += (int64_t)gridDim.x * here) {
     const int bh = (int)(row / p.budget), i = (int)(row - (int64_t)bh * p.budget);
-    const int b = bh / c.kv_heads, h = bh % c.kv_heads;
-    const int j = p.kept[row];
-    if (j < 0) continue;
-    const int from = cache_page(c, b, j), to = p.new_table[b * p.new_stride + i / c.page_size];
-    if (from < 0 || (unsigned)to >= (unsigned)c.pages) continue;
-    const int slot = j % c.page_size, slot_to = i % c.page_size;
-    if (from == to && slot == slot_to) continue;
-    const int64_t src = from * c.page_stride + h * c.head_stride + slot * c.slot_stride;
-    const int64_t dst = to * c.page_stride + h * c.head_stride + slot_to * c.slot_stride;
-    for (int x = col; x < per; x += lanes) {
-      const V k = ((const V*)((const char*)c.k + src * p.es))[x], v = ((const V*)((const char*)c.v + src * p.es))[x];
-      ((V*)((char*)c.k + dst * p.es))[x] = k;
-      ((V*)((char*)c.v + dst * p.es))[x] = v;
-    }
-    if (col == 0)
-      c.w[to * c.w_page_stride + h * c.w_head_stride + slot_to] = c.w[from * c.w_page_stride + h * c.w_head_stride + slot];
+    const int b = bh / p.c.kv_heads, h = bh % p.c.kv_heads, j = p.kept[row];
+    if (j >= 0) copy_row<V>(p, b, h, i, j, col, lanes, per);
   }
 }
 
