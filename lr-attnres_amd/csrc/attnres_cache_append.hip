@@ -46,7 +46,8 @@ __device__ __forceinline__ Place place_of(const CacheAppendParams& p, int b, int
   return r;
 }
 
-template <class DT, class TT, int VEC, int LANES>
+// A lane holds CHUNKS vectors of a head, LANES * VEC apart.
+template <class DT, class TT, int VEC, int LANES, int CHUNKS>
 __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheAppendParams p, int groups, int iters,
                                                                           FastDiv by_groups) {
   using S = typename DT::S;
@@ -60,65 +61,79 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheApp
   const int b = div_by(tok, p.by_tokens), t = tok - b * p.tokens;
   const int n_rot = p.q_heads + p.c.kv_heads, n_all = n_rot + p.c.kv_heads;
   const int Dh = p.c.head_dim;
-  const int col = (lane & (LANES - 1)) * VEC;
-  const bool in = col < Dh;
+  const int col0 = (lane & (LANES - 1)) * VEC;
   const int head0 = part * (iters * kHeads) + lane / LANES;
+  bool in[CHUNKS];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) in[c] = col0 + c * LANES * VEC < Dh;
 
   const S* src = (const S*)p.qkv + b * p.b_stride + t * p.t_stride;
   const bool real = !p.c.fresh || t < p.c.fresh[b];  // (what is behind a sequence's tokens is not read)
-  Raw<DT, VEC> x[kGroups];
+  Raw<DT, VEC> x[kGroups][CHUNKS];
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int h = i < iters && real ? head0 + i * kHeads : n_all;
-    if (h < n_all && in) load_raw<DT, VEC, true>(src + (int64_t)h * Dh + col, x[i]);
-    else x[i] = {};
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      if (h < n_all && in[c]) load_raw<DT, VEC, true>(src + (int64_t)h * Dh + col0 + c * LANES * VEC, x[i][c]);
+      else x[i][c] = {};
+    }
   }
   const Place at = place_of(p, b, t);
-  float sn[VEC / 2], cs[VEC / 2];
-  if (at.at >= 0 && in) {
-    load_vec<TT, VEC / 2>((const TS*)p.sin + at.at * p.table_stride + col / 2, sn);
-    load_vec<TT, VEC / 2>((const TS*)p.cos + at.at * p.table_stride + col / 2, cs);
-  } else {  // NaN outside the tables, so that the token shows it
+  float sn[CHUNKS][VEC / 2], cs[CHUNKS][VEC / 2];
 #pragma unroll
-    for (int e = 0; e < VEC / 2; ++e) sn[e] = cs[e] = __builtin_nanf("");
+  for (int c = 0; c < CHUNKS; ++c) {
+    if (at.at >= 0 && in[c]) {
+      const int64_t o = at.at * p.table_stride + (col0 + c * LANES * VEC) / 2;
+      load_vec<TT, VEC / 2>((const TS*)p.sin + o, sn[c]);
+      load_vec<TT, VEC / 2>((const TS*)p.cos + o, cs[c]);
+    } else {  // NaN outside the tables, so that the token shows it
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) sn[c][e] = cs[c][e] = __builtin_nanf("");
+    }
   }
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     if (i >= iters) break;
     const int h = head0 + i * kHeads;
-    float v[VEC], r[VEC];
-    unpack<DT, VEC>(x[i], v);
-    float inv = 1.f;
-    if (p.qk_norm) {
-      float ss = 0.f;
+    float v[CHUNKS][VEC];
+    float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) ss += v[e] * v[e];
-      inv = 1.f / sqrtf(group_sum(ss, LANES) / (float)Dh + p.eps);
-    }
+    for (int c = 0; c < CHUNKS; ++c) {
+      unpack<DT, VEC>(x[i][c], v[c]);
 #pragma unroll
-    for (int e = 0; e < VEC / 2; ++e) {
-      const float even = v[2 * e] * inv, odd = v[2 * e + 1] * inv;
-      r[2 * e] = at.real ? cs[e] * even - sn[e] * odd : 0.f;
-      r[2 * e + 1] = at.real ? sn[e] * even + cs[e] * odd : 0.f;
+      for (int e = 0; e < VEC; ++e) ss += v[c][e] * v[c][e];
     }
-    if (h >= n_all || !in) continue;
-    if (h < p.q_heads) {
-      store_vec<DT, VEC>((S*)p.q + ((b * (int64_t)p.q_heads + h) * p.tokens + t) * Dh + col, r);
-    } else if (h < n_rot) {
-      const int hh = h - p.q_heads;
-      if (p.k) store_vec<DT, VEC>((S*)p.k + ((b * (int64_t)p.c.kv_heads + hh) * p.tokens + t) * Dh + col, r);
-      if (at.row >= 0) {
-        store_vec<DT, VEC>((S*)p.c.k + at.row + hh * p.c.head_stride + col, r);
-        if (p.c.w && col == 0) p.c.w[at.w + hh * p.c.w_head_stride] = 0.f;
+    const float inv = p.qk_norm ? 1.f / sqrtf(group_sum(ss, LANES) / (float)Dh + p.eps) : 1.f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      float r[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) {
+        const float even = v[c][2 * e] * inv, odd = v[c][2 * e + 1] * inv;
+        r[2 * e] = at.real ? cs[c][e] * even - sn[c][e] * odd : 0.f;
+        r[2 * e + 1] = at.real ? sn[c][e] * even + cs[c][e] * odd : 0.f;
       }
-    } else if (at.row >= 0) {  // a value, bit for bit
-      store_raw<DT, VEC>((S*)p.c.v + at.row + (h - n_rot) * p.c.head_stride + col, x[i]);
+      if (h >= n_all || !in[c]) continue;
+      const int col = col0 + c * LANES * VEC;
+      if (h < p.q_heads) {
+        store_vec<DT, VEC>((S*)p.q + ((b * (int64_t)p.q_heads + h) * p.tokens + t) * Dh + col, r);
+      } else if (h < n_rot) {
+        const int hh = h - p.q_heads;
+        if (p.k) store_vec<DT, VEC>((S*)p.k + ((b * (int64_t)p.c.kv_heads + hh) * p.tokens + t) * Dh + col, r);
+        if (at.row >= 0) {
+          store_vec<DT, VEC>((S*)p.c.k + at.row + hh * p.c.head_stride + col, r);
+          if (p.c.w && col == 0) p.c.w[at.w + hh * p.c.w_head_stride] = 0.f;
+        }
+      } else if (at.row >= 0) {  // a value, bit for bit
+        store_raw<DT, VEC>((S*)p.c.v + at.row + (h - n_rot) * p.c.head_stride + col, x[i][c]);
+      }
     }
   }
 }
 
-// Any alignment and (even) head width: one wave per head, its pairs in turn, the sum and the pairs
-// in two passes over the row.
+// Any alignment: one wave per head, its pairs in turn, the sum and the pairs in two passes over the row.  Single
+// values: 49 x 180 tokens of 66 heads of 86, fp16, 269 us, where pairs in the vector kernel take 106 (and 88 columns, in eights, 48).
 template <class DT, class TT>
 __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_general(CacheAppendParams p) {
   using S = typename DT::S;
@@ -170,7 +185,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_general(CacheAp
   if (row && p.c.w && lane == 0) p.c.w[at.w + hh * p.c.w_head_stride] = 0.f;
 }
 
-template <class DT, class TT, int VEC, int LANES>
+template <class DT, class TT, int VEC, int LANES, int CHUNKS = 1>
 hipError_t run(const CacheAppendParams& p, hipStream_t st) {
   const int n_all = p.q_heads + 2 * p.c.kv_heads;
   const int all = (n_all + kWave / LANES - 1) / (kWave / LANES);
@@ -180,7 +195,7 @@ hipError_t run(const CacheAppendParams& p, hipStream_t st) {
   const int groups = (all + most - 1) / most, iters = (all + groups - 1) / groups;
   dim3 grid;
   if (!rot_grid((int64_t)p.n_tok * groups, &grid)) return hipErrorInvalidValue;
-  cache_append_kernel<DT, TT, VEC, LANES><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters, fast_div(groups));
+  cache_append_kernel<DT, TT, VEC, LANES, CHUNKS><<<grid, dim3(kRotWaves * kWave), 0, st>>>(p, groups, iters, fast_div(groups));
   return hipGetLastError();
 }
 
@@ -199,6 +214,11 @@ hipError_t pick(const CacheAppendParams& p, int vec, int lanes, hipStream_t st) 
     if (lanes == 16) return run<DT, TT, 4, 16>(p, st);
     if (lanes == 32) return run<DT, TT, 4, 32>(p, st);
     if (lanes == 64) return run<DT, TT, 4, 64>(p, st);
+  }
+  if (vec == 2) {
+    if (lanes == 32) return run<DT, TT, 2, 32>(p, st);
+    if (lanes == 64) return run<DT, TT, 2, 64>(p, st);
+    if (lanes == 128) return run<DT, TT, 2, 64, 2>(p, st);  // two vectors a lane
   }
   if (vec != 1) return hipErrorInvalidValue;
   dim3 grid;
