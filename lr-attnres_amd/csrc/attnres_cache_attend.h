@@ -155,6 +155,7 @@ struct Att {
   const CacheAttendParams& p;
   int lane, wave, c, g;          // column (query row) and token group of the lane
   int b, h, n, have;
+  int t_lo, t_hi;                // new tokens of the rows
   int kcol[kKs], vcol0;          // first value of each key chunk; of the first value chunk
   uint32_t kofs[kKs], vofs[4][kNi]; // PAGE16: bytes from a subtile's first row
   const S *kh, *vh;              // of the head, page 0
@@ -483,7 +484,7 @@ struct Att {
       }
     } else {
       // (0 times such a value is NaN: each new token's rows take a product without the values behind it)
-      for (int tt = p.tokens - 1; tt >= 0; --tt) {
+      for (int tt = t_hi; tt >= t_lo; --tt) {
 #pragma unroll
         for (int s = 0; s < kSub; ++s)
 #pragma unroll
@@ -566,10 +567,12 @@ struct Att {
     clear();
     have = seq.have;
     n = seq.n;
-    end = min(end, n);
+    t_lo = div_by(row0, p.by_group);
+    t_hi = div_by(row0 + rows - 1, p.by_group);
+    end = min(end, min(have + t_hi + 1, n));  // (behind it no row sees any)
     if (t_first >= end) return;
     const int lim = min(have + t_row + 1, n);  // of the lane's row (a row that is not there: whatever)
-    const int all = p.tokens > 1 ? have + 1 : n;  // tokens that every row sees
+    const int all = have + t_lo + 1;               // tokens that every row sees
     int t0 = t_first;
     const Row row{p.logits && valid ? p.logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row};
     for (; t0 + kStep < end && t0 + kTok <= all; t0 += kStep) tile<true, false>(t0, row, now, next);
