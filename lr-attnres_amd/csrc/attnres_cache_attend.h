@@ -59,17 +59,6 @@ __device__ __forceinline__ Seq seq_of(const CacheAttendParams& p, int b) {  // b
   return Seq{have, seen_of(p, have, fresh)};
 }
 
-// over the lanes up to and with this one, by moves inside rows of 16 lanes and broadcasts of a row's last
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // 1, 2, 4, 8 to the right
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 into rows 1 and 3's, of 0 and 2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 into rows 2 and 3
-  return x;
-}
-
 // 64 sequences, one a lane: those from b0 on
 struct Chunk {
   int b0, have, n, units, upto;  // upto: units of a segment of each sequence up to and with this one

@@ -16,48 +16,36 @@ namespace attnres {
 
 namespace {
 
-constexpr int kSelThreads = 1024;
-
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (!(w == w)) return 0;
   const uint32_t u = __float_as_uint(w + 0.f);  // -0 as 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ uint32_t token_key(const CachePages& c, int b, int h, int j) {
-  const int page = cache_page(c, b, j);
-  return page < 0 ? 0 : weight_key(c.w[page * c.w_page_stride + h * c.w_head_stride + j % c.page_size]);
-}
+// TH: threads of a workgroup, 1024 or 256.  Places of a round's counts: 2^12, 2^10, 2^10, or 2^11, 2^11, 2^10.
+constexpr int kBig = 1024, kFew = 256;
+constexpr int kSlice = kEvictSlice, kR = kSlice / kBig;  // tokens of a workgroup, keys a thread
+static_assert(kR * kBig == kSlice, "whole keys a thread");
+template <int TH>
+constexpr int kBins = TH == kBig ? 4096 : 2048;
 
-__device__ __forceinline__ int wave_scan(int x) {  // inclusive
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int y = __shfl_up(x, o, kWave);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
+template <int TH>
+__device__ __forceinline__ int round_bits(int round) { return TH == kBig ? (round == 0 ? 12 : 10) : round == 2 ? 10 : 11; }
+template <int TH>
+__device__ __forceinline__ int round_shift(int round) { return TH == kBig ? 20 - 10 * round : round == 0 ? 21 : round == 1 ? 10 : 0; }
 
 // x summed over the workgroup's threads up to and with this one; `sums`: one place a wave
+template <int TH>
 __device__ __forceinline__ int block_scan(int x, int* sums) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   x = wave_scan(x);
   if (lane == kWave - 1) sums[wave] = x;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSelThreads / kWave; ++w)
+  for (int w = 0; w < TH / kWave; ++w)
     if (w < wave) x += sums[w];
   return x;
 }
-
-constexpr int kBins = 4096;                         // of the first round, 1024 of the other two
-constexpr int kSlice = kEvictSlice, kR = kSlice / kSelThreads;  // tokens of a workgroup, keys a thread
-static_assert(kR * kSelThreads == kSlice, "whole keys a thread");
-constexpr int kWaves = kSelThreads / kWave;
-
-__device__ __forceinline__ int round_bits(int round) { return round == 0 ? 12 : 10; }
-__device__ __forceinline__ int round_shift(int round) { return 20 - 10 * round; }
 
 // What the rounds so far have found: kept are the keys above prefix in the bits of mask, and `want` of those equal.
 struct Found {
@@ -66,127 +54,153 @@ struct Found {
   bool open;  // more are equal than wanted
 };
 
-template <int R>
+template <int R, int TH>
 struct SelectShared {
-  int sums[2][kWaves];
-  int digit, want, open;
-  int above[R * kWaves], equal[R * kWaves];
+  int sums[2][TH / kWave];
+  int digit, want, open, before_above, before_equal;
+  int above[R * TH / kWave], equal[R * TH / kWave];
 };
 
-// The next digit of the want-th largest key, from the counts of its places: count(place) for any place of 2^bits.
-template <int R, class F>
-__device__ __forceinline__ void next_digit(int round, Found& f, SelectShared<R>& s, F count) {
-  const int bits = round_bits(round), mine = (1 << bits) / kSelThreads;
+// The next digit of the want-th largest key from the counts of its places, 2^bits of them: count(place, &n, &before),
+// `before` being those of n that lie in slices before this one.  In s.before_*: keys of theirs that are above
+// the digit and equal to it.
+template <bool SLICES, int R, int TH, class F>
+__device__ __forceinline__ void next_digit(int round, Found& f, SelectShared<R, TH>& s, F count) {
+  const int bits = round_bits<TH>(round), mine = (1 << bits) / TH;
   // from the largest place down
   const int first = (1 << bits) - 1 - (int)threadIdx.x * mine;
-  int n[kBins / kSelThreads], sum = 0;
+  int n[kBins<TH> / TH], before[kBins<TH> / TH], sum = 0, sum_before = 0;
 #pragma unroll
-  for (int i = 0; i < kBins / kSelThreads; ++i) {
-    n[i] = i < mine ? count(first - i) : 0;
+  for (int i = 0; i < kBins<TH> / TH; ++i) {
+    n[i] = before[i] = 0;
+    if (i < mine) count(first - i, &n[i], &before[i]);
     sum += n[i];
+    sum_before += before[i];
   }
-  const int upto = block_scan(sum, s.sums[0]);
-  if (upto >= f.want && upto - sum < f.want) {
-    int left = f.want - (upto - sum);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  int upto = wave_scan(sum), upto_before = SLICES ? wave_scan(sum_before) : 0;
+  if (lane == kWave - 1) s.sums[0][wave] = upto, s.sums[1][wave] = upto_before;
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kBins / kSelThreads; ++i) {
+  for (int w = 0; w < (TH / kWave); ++w)
+    if (w < wave) {
+      upto += s.sums[0][w];
+      if (SLICES) upto_before += s.sums[1][w];
+    }
+  if (upto >= f.want && upto - sum < f.want) {
+    int left = f.want - (upto - sum), above = upto_before - sum_before;
+#pragma unroll
+    for (int i = 0; i < kBins<TH> / TH; ++i) {
       if (left > 0 && left <= n[i]) {
         s.digit = first - i;
         s.want = left;
         s.open = n[i] > left;
+        s.before_above = above;
+        s.before_equal = before[i];
       }
       left -= n[i];
+      above += before[i];
     }
   }
   __syncthreads();
-  f.prefix |= (uint32_t)s.digit << round_shift(round);
-  f.mask |= ((1u << bits) - 1) << round_shift(round);
+  f.prefix |= (uint32_t)s.digit << round_shift<TH>(round);
+  f.mask |= ((1u << bits) - 1) << round_shift<TH>(round);
   f.want = s.want;
   f.open = s.open;
 }
 
 // The tokens j0 .. of a head: what is kept of them goes to its places, `above` and `equal` of the tokens before them
 // being above the found prefix and equal to it.
-template <int R>
+template <int R, int TH>
 __device__ __forceinline__ void place(const uint32_t (&key)[R], int j0, int early, const Found& f, int above, int equal,
-                                      int32_t* kept, SelectShared<R>& s) {
+                                      int32_t* kept, SelectShared<R, TH>& s) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const bool in = j0 + i * kSelThreads + tid < early;
+    const bool in = j0 + i * TH + tid < early;
     const uint64_t a = __ballot(in && (key[i] & f.mask) > f.prefix), e = __ballot(in && (key[i] & f.mask) == f.prefix);
     if (lane == 0) {
-      s.above[i * kWaves + wave] = __popcll(a);
-      s.equal[i * kWaves + wave] = __popcll(e);
+      s.above[i * (TH / kWave) + wave] = __popcll(a);
+      s.equal[i * (TH / kWave) + wave] = __popcll(e);
     }
   }
   __syncthreads();
-  const int a0 = tid < R * kWaves ? s.above[tid] : 0, e0 = tid < R * kWaves ? s.equal[tid] : 0;
-  const int a1 = block_scan(a0, s.sums[0]), e1 = block_scan(e0, s.sums[1]);
-  if (tid < R * kWaves) {
+  const int a0 = tid < R * TH / kWave ? s.above[tid] : 0, e0 = tid < R * TH / kWave ? s.equal[tid] : 0;
+  const int a1 = block_scan<TH>(a0, s.sums[0]), e1 = block_scan<TH>(e0, s.sums[1]);
+  if (tid < R * TH / kWave) {
     s.above[tid] = above + a1 - a0;
     s.equal[tid] = equal + e1 - e0;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int j = j0 + i * kSelThreads + tid;
+    const int j = j0 + i * TH + tid;
     const bool is_above = j < early && (key[i] & f.mask) > f.prefix, is_equal = j < early && (key[i] & f.mask) == f.prefix;
     const uint64_t below = (1ull << lane) - 1;
-    const int a = s.above[i * kWaves + wave] + __popcll(__ballot(is_above) & below);
-    const int e = s.equal[i * kWaves + wave] + __popcll(__ballot(is_equal) & below);
+    const int a = s.above[i * (TH / kWave) + wave] + __popcll(__ballot(is_above) & below);
+    const int e = s.equal[i * (TH / kWave) + wave] + __popcll(__ballot(is_equal) & below);
     if (is_above || (is_equal && e < f.want)) kept[a + min(e, f.want)] = j;
   }
 }
 
-template <int R>
-__device__ __forceinline__ void load_keys(const CachePages& c, int b, int h, int j0, int early, uint32_t (&key)[R]) {
+// The keys of a head's tokens j0 .., as far as the table goes: no load waits for the sequence's length.
+template <int R, int TH>
+__device__ __forceinline__ void load_keys(const CachePages& c, int b, int h, int j0, uint32_t (&key)[R]) {
+  int page[R], slot[R];
+  float w[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int j = j0 + i * kSelThreads + (int)threadIdx.x;
-    key[i] = j < early ? token_key(c, b, h, j) : 0;
+    const int j = j0 + i * TH + (int)threadIdx.x, at = div_by(j, c.by_page);
+    slot[i] = j - at * c.page_size;
+    page[i] = j < c.room ? c.table[b * c.table_stride + at] : -1;
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    w[i] = (unsigned)page[i] < (unsigned)c.pages ? c.w[page[i] * c.w_page_stride + h * c.w_head_stride + slot[i]] : __builtin_nanf("");
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = weight_key(w[i]);
 }
 
-template <int R>
+template <int R, int TH>
 __device__ __forceinline__ void count_keys(const uint32_t (&key)[R], int j0, int early, int round, const Found& f, int* hist) {
-  const int bits = round_bits(round), shift = round_shift(round);
-  for (int i = threadIdx.x; i < 1 << bits; i += kSelThreads) hist[i] = 0;
+  const int bits = round_bits<TH>(round), shift = round_shift<TH>(round);
+  for (int i = threadIdx.x; i < 1 << bits; i += TH) hist[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    if (j0 + i * kSelThreads + (int)threadIdx.x < early && (key[i] & f.mask) == f.prefix)
+    if (j0 + i * TH + (int)threadIdx.x < early && (key[i] & f.mask) == f.prefix)
       atomicAdd(&hist[(key[i] >> shift) & ((1 << bits) - 1)], 1);
   __syncthreads();
 }
 
 // what needs no choice; false: `early` tokens to choose budget - recent of
+template <int TH>
 __device__ __forceinline__ bool no_choice(const CacheEvictParams& p, int n, int32_t* kept) {
   if (n <= p.budget) {
-    for (int i = threadIdx.x; i < p.budget; i += kSelThreads) kept[i] = i < n ? i : -1;
+    for (int i = threadIdx.x; i < p.budget; i += TH) kept[i] = i < n ? i : -1;
     return true;
   }
-  for (int i = threadIdx.x; i < p.recent; i += kSelThreads) kept[p.budget - p.recent + i] = n - p.recent + i;
+  for (int i = threadIdx.x; i < p.recent; i += TH) kept[p.budget - p.recent + i] = n - p.recent + i;
   return p.budget == p.recent;
 }
 
-// tables of at most R * 1024 tokens
-template <int R>
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(CacheEvictParams p) {
-  __shared__ int hist[kBins];
-  __shared__ SelectShared<R> s;
-  const int b = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads, n = max(cache_count(p.c, b), 0);
+// tables of at most R * TH tokens
+template <int R, int TH>
+__global__ __launch_bounds__(TH) void evict_select_kernel(CacheEvictParams p) {
+  __shared__ int hist[kBins<TH>];
+  __shared__ SelectShared<R, TH> s;
+  const int b = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads;
+  uint32_t key[R];
+  load_keys<R, TH>(p.c, b, h, 0, key);
+  const int n = max(cache_count(p.c, b), 0);
   int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
-  if (!no_choice(p, n, kept)) {
+  if (!no_choice<TH>(p, n, kept)) {
     const int early = n - p.recent;
-    uint32_t key[R];
-    load_keys(p.c, b, h, 0, early, key);
     Found f{0, 0, p.budget - p.recent, true};
     for (int round = 0; round < 3 && f.open; ++round) {
-      count_keys(key, 0, early, round, f, hist);
-      next_digit(round, f, s, [&](int place) { return hist[place]; });
-      __syncthreads();
+      count_keys<R, TH>(key, 0, early, round, f, hist);
+      next_digit<false>(round, f, s, [&](int place, int* n, int*) { *n = hist[place]; });
     }
     place(key, 0, early, f, 0, 0, kept, s);
   }
@@ -202,7 +216,7 @@ __device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 307
 
 // What the rounds before `round` have found; above, equal: keys of the slices before this one.
 __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int head, int slices, int slice, int round, int* above,
-                                              int* equal, SelectShared<kR>& s) {
+                                              int* equal, SelectShared<kR, kBig>& s) {
   Found f{0, 0, p.budget - p.recent, true};
   int a = 0, e = 0;
   int32_t* state = p.hist + ((int64_t)head * p.slices + slice) * kSlots + kState;
@@ -213,32 +227,17 @@ __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int hea
   }
   if (round > 0 && f.open) {
     const int32_t* at = p.hist + (int64_t)head * p.slices * kSlots + round_at(round - 1);
-    // (eight slices' loads at once)
-    auto over = [&](int place, int n) {
-      int sum = 0;
-      for (int i0 = 0; i0 < n; i0 += 8)
+    next_digit<true>(round - 1, f, s, [&](int place, int* n, int* before) {
+      for (int i0 = 0; i0 < slices; i0 += 8)  // (eight slices' loads at once)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int x = at[(int64_t)min(i0 + i, n - 1) * kSlots + place];
-          sum += i0 + i < n ? x : 0;
+        for (int i = i0; i < i0 + 8; ++i) {
+          const int x = at[(int64_t)min(i, slices - 1) * kSlots + place];
+          *n += i < slices ? x : 0;
+          *before += i < slice ? x : 0;
         }
-      return sum;
-    };
-    next_digit(round - 1, f, s, [&](int place) { return over(place, slices); });
-    const int digit = s.digit;
-    int more = 0;
-#pragma unroll
-    for (int q = 0; q < kBins / kSelThreads; ++q) {
-      const int place = q * kSelThreads + (int)threadIdx.x;
-      if (place > digit && place < 1 << round_bits(round - 1)) more += over(place, slice);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) s.digit = 0;
-    __syncthreads();
-    if (more) atomicAdd(&s.digit, more);
-    __syncthreads();
-    a += s.digit;
-    e = slice ? over(digit, slice) : 0;
+    });
+    a += s.before_above;
+    e = s.before_equal;
   }
   if (round < 3 && threadIdx.x == 0) {
     state[0] = (int32_t)f.prefix;
@@ -253,36 +252,36 @@ __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int hea
   return f;
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_count_kernel(CacheEvictParams p, int round) {
-  __shared__ int hist[kBins];
-  __shared__ SelectShared<kR> s;
+__global__ __launch_bounds__(kBig) void evict_count_kernel(CacheEvictParams p, int round) {
+  __shared__ int hist[kBins<kBig>];
+  __shared__ SelectShared<kR, kBig> s;
   const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
   const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   const int early = n - p.recent, j0 = slice * kSlice;
   if (n <= p.budget || p.budget == p.recent || j0 >= early) return;
   uint32_t key[kR];
-  load_keys(p.c, b, h, j0, early, key);
+  load_keys<kR, kBig>(p.c, b, h, j0, key);
   int above, equal;
   const Found f = found_before(p, head, (early + kSlice - 1) / kSlice, slice, round, &above, &equal, s);
   if (!f.open) return;
-  count_keys(key, j0, early, round, f, hist);
+  count_keys<kR, kBig>(key, j0, early, round, f, hist);
   int32_t* to = p.hist + ((int64_t)head * p.slices + slice) * kSlots + round_at(round);
-  for (int i = threadIdx.x; i < 1 << round_bits(round); i += kSelThreads) to[i] = hist[i];
+  for (int i = threadIdx.x; i < 1 << round_bits<kBig>(round); i += kBig) to[i] = hist[i];
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_place_kernel(CacheEvictParams p) {
-  __shared__ SelectShared<kR> s;
+__global__ __launch_bounds__(kBig) void evict_place_kernel(CacheEvictParams p) {
+  __shared__ SelectShared<kR, kBig> s;
   const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
   const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   int32_t* kept = p.kept + (int64_t)head * p.budget;
   if (slice == 0) {
     if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
-    if (no_choice(p, n, kept)) return;
+    if (no_choice<kBig>(p, n, kept)) return;
   }
   const int early = n - p.recent, j0 = slice * kSlice;
   if (n <= p.budget || p.budget == p.recent || j0 >= early) return;
   uint32_t key[kR];
-  load_keys(p.c, b, h, j0, early, key);
+  load_keys<kR, kBig>(p.c, b, h, j0, key);
   int above, equal;
   const Found f = found_before(p, head, (early + kSlice - 1) / kSlice, slice, 3, &above, &equal, s);
   place(key, j0, early, f, above, equal, kept, s);
@@ -324,10 +323,11 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(CacheEvictParams p, int
 
 hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st) {
   const int64_t heads = (int64_t)p.c.batch * p.c.kv_heads;
-  const dim3 sel((unsigned)(heads * p.slices)), wg(kSelThreads);
+  const dim3 sel((unsigned)(heads * p.slices)), wg(kBig);
   if (p.slices == 1) {
-    if (p.c.room <= kSlice) evict_select_kernel<kR><<<sel, wg, 0, st>>>(p);
-    else evict_select_kernel<2 * kR><<<sel, wg, 0, st>>>(p);
+    if (p.c.room <= kR * kFew) evict_select_kernel<kR, kFew><<<sel, dim3(kFew), 0, st>>>(p);
+    else if (p.c.room <= kSlice) evict_select_kernel<kR, kBig><<<sel, wg, 0, st>>>(p);
+    else evict_select_kernel<2 * kR, kBig><<<sel, wg, 0, st>>>(p);
   } else {
     for (int round = 0; round < 3; ++round) evict_count_kernel<<<sel, wg, 0, st>>>(p, round);
     evict_place_kernel<<<sel, wg, 0, st>>>(p);
