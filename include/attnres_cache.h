@@ -16,6 +16,7 @@ extern "C" {
 
 #define ATTNRES_CACHE_MAX_HEAD_DIM 256
 #define ATTNRES_CACHE_MAX_TOKENS (1 << 30) /* of one sequence */
+#define ATTNRES_CACHE_MAX_SCALE 1e38f      /* (base-2 logarithms: log2(e) times it is finite) */
 
 /*
  * One layer's pages.  Token j of sequence b, head h lies at
@@ -88,13 +89,15 @@ int attnres_cache_append(const attnres_cache_desc* cache, const attnres_cache_ap
  * in fp32 (the products' operands in the dtype, p in two terms of it), one rounding to
  * the dtype.  With weights (tokens 1): each cached token's weight becomes decay * weight +
  * the sum of p_j over the key / value head's queries; with decay 0 the old one is not read.
- * A query that its sequence does not have (t >= fresh[b]), or that sees no token, gives
- * zeros; a page outside the cache or counts beyond the table give NaN in that sequence.
+ * Pages may be shared between sequences, but not with weights.
+ * A query that its sequence does not have (t >= fresh[b]) gives zeros; a page outside the
+ * cache gives NaN in that sequence, in every row that reads it, and a count that is
+ * negative or beyond the table's room gives NaN in all its rows.
  */
 typedef struct attnres_cache_attend_desc {
   int64_t tokens;         /* 0 is allowed */
   int32_t q_heads;        /* a multiple of kv_heads */
-  float scale;
+  float scale;            /* at most ATTNRES_CACHE_MAX_SCALE either way */
   const void* q;          /* [batch, q_heads, tokens, head_dim], last dimension contiguous */
   int64_t q_batch_stride; /* elements */
   int64_t q_head_stride;
@@ -102,8 +105,9 @@ typedef struct attnres_cache_attend_desc {
   float decay;            /* with weights */
 } attnres_cache_attend_desc;
 
-/* Workspace bytes (host computation; aligned to 256).  It grows with the table's room
- * only where weights are kept. */
+/* Workspace bytes (host computation; aligned to 256): pieces of at most 256 workgroups' rows
+ * and, with weights, 4 bytes for each query head and token that the table has room for (a
+ * table of the pages in use keeps it small). */
 size_t attnres_cache_attend_workspace_size(const attnres_cache_desc* cache, const attnres_cache_attend_desc* desc);
 
 /* out [batch, tokens, q_heads, head_dim], dense */
@@ -115,8 +119,8 @@ int attnres_cache_attend(const attnres_cache_desc* cache, const attnres_cache_at
  * the last `recent` and, of the others, those of the largest weights (a NaN is below
  * every number; equal ones: the earlier token).  What is kept is copied in its order,
  * keys, values and weights, to the first slots of the pages new_table[b * new_stride +
- * ...], which hold no token that the call reads; only a sequence within its budget may
- * keep its own pages, in the same order, and is then left as it is.  `fresh` is not used.
+ * ...], which are all different and hold no token that the call reads; only a sequence
+ * within its budget may keep its own pages, in the same order, and is then left as it is.  `fresh` is not used.
  * kept [batch, kv_heads, budget]: the tokens kept, ascending, -1 behind them; left
  * [batch]: their number.  Counts beyond the table's room are taken as 0.  A token whose
  * page lies outside the cache has the lowest weight and is not copied.

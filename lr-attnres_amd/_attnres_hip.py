@@ -33,6 +33,7 @@ SITE_LOGITS_MAX_RANK = 128
 QKV_ROTARY_MAX_HEAD_DIM = 1024
 CACHE_MAX_HEAD_DIM = 256
 CACHE_MAX_TOKENS = 1 << 30
+CACHE_MAX_SCALE = 1e38
 FLT_EPSILON = float(torch.finfo(torch.float32).eps)
 
 

@@ -488,7 +488,7 @@ class Decoder(nn.Module):
         B, T = idx.shape
         if B != cache.batch:
             raise ValueError(f"{B} rows of tokens for a cache of {cache.batch} sequences")
-        new = [T] * B if fresh is None else list(fresh)
+        new = [T] * B if fresh is None else [int(n) for n in fresh]
         if len(new) != B or any(not 0 <= n <= T for n in new):
             raise ValueError(f"fresh must be {B} counts of 0 .. {T}, got {fresh}")
         far = max(p + n for p, n in zip(cache.next_positions, new))
@@ -507,9 +507,11 @@ class Decoder(nn.Module):
 
         ``pick`` takes logits [B, vocab] to the next tokens [B]; the largest logit's unless given.  With ``budget`` a sequence
         that has a page's tokens more than that in the cache is brought back to it (``PagedCache.evict``, which keeps the last
-        ``recent``).
+        ``recent``).  What counts is the attention of the generated tokens; a prompt's own is not added up, so that one that
+        has to be cut at once keeps its beginning and its end.
         """
         B, T = idx.shape
+        lengths = None if lengths is None else [int(n) for n in lengths]
         if lengths is not None and (len(lengths) != B or any(not 1 <= n <= T for n in lengths)):
             raise ValueError(f"lengths must be {B} counts of 1 .. {T}, got {lengths}")
         if cache is None:
@@ -517,7 +519,7 @@ class Decoder(nn.Module):
             # (with a budget, pages for a second copy of what is kept while it moves)
             extra = {} if budget is None else dict(weights=True, spare_tokens=budget)
             cache = self.new_cache(B, most, **extra)
-        far = max(p + n for p, n in zip(cache.next_positions, lengths or [T] * B)) + max_new_tokens - 1
+        far = max(p + n for p, n in zip(cache.next_positions, [T] * B if lengths is None else lengths)) + max_new_tokens - 1
         if far > self.config.block_size:
             raise ValueError(f"position {far - 1} is outside block_size {self.config.block_size}")
         out = idx.new_empty((B, max_new_tokens))

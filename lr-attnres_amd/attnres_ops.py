@@ -2256,10 +2256,12 @@ def cached_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: T
     head (heads of its group times tokens) read the cache once.
 
     ``weights`` [P, K, S] (fp32, T = 1): becomes ``decay * weights`` plus the softmax weights of the head's queries, summed,
-    for every token that was read; with ``decay`` 0 what was there is not read.  ``evict_cached_tokens`` goes by it.
+    for every token that was read; with ``decay`` 0 what was there is not read.  ``evict_cached_tokens`` goes by it.  Pages may
+    be shared between sequences, but not with ``weights``, whose workspace has 4 bytes for each query head and token that the
+    table has room for: give it the columns in use.
 
-    A query that its sequence does not have, or that sees no token (``cached[b] = -1`` of T = 1 is refused, as any negative
-    count), gives zeros; a page not in [0, P), a negative count or tokens beyond the table give NaN in that sequence.  Returns
+    A query that its sequence does not have gives zeros; a page not in [0, P) gives NaN in that sequence, in every row that
+    reads it, and a negative count or more tokens than the table has room for give NaN in all its rows.  Returns
     [B, H, T, Dh], a view of a dense [B, T, H, Dh].  No backward.
     """
     what = "cached_attention"
@@ -2281,8 +2283,8 @@ def cached_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: T
     if not 0.0 <= decay <= 1.0:
         raise RuntimeError(f"{what}: decay must be 0 .. 1, got {decay}")
     scale = Dh ** -0.5 if scale is None else float(scale)
-    if not -3.4e38 < scale < 3.4e38:
-        raise RuntimeError(f"{what}: scale must be finite, got {scale}")
+    if not abs(scale) <= _hip.CACHE_MAX_SCALE:
+        raise RuntimeError(f"{what}: scale must be finite, of at most {_hip.CACHE_MAX_SCALE}, got {scale}")
     return _cache_attend_op(_last_dense(q), k_pages, v_pages, weights, table, cached, fresh, scale, float(decay)).transpose(1, 2)
 
 
@@ -2294,9 +2296,10 @@ def evict_cached_tokens(k_pages: Tensor, v_pages: Tensor, weights: Tensor, block
     Not in the reference.  The cache's arguments as ``cached_attention`` takes them, ``weights`` the sums it has added up.
     A sequence of more than ``budget`` tokens keeps that many of them, each head its own: the last ``recent`` and the
     ``budget - recent`` of the largest weights (equal ones: the earlier token; NaN: below every number).  They are copied in
-    their order, with keys, values and weights, into the pages ``new_table`` [B, M'] (``M' * S >= budget``).  Those pages hold
-    no token of any sequence of the call; only a sequence within its budget may name its own pages again, in their order, and is
-    then left as it is.  The old pages are not changed.
+    their order, with keys, values and weights, into the pages ``new_table`` [B, M'] (``M' * S >= budget``).  Those pages are
+    all different and hold no token of any sequence of the call; only a sequence within its budget may name its own pages again,
+    in their order, and is then left as it is.  The old pages are not changed.  A token whose page is not in [0, P) counts as
+    the least attended and is not copied, and a count that cannot be counts as 0.
 
     Returns ``kept`` [B, K, budget] (int32), the kept tokens' places in the old order, -1 behind the last, and ``left`` [B]
     (int32), the tokens that each sequence has now: the next ``cached``.  Rotated keys keep their positions, so later calls

@@ -114,7 +114,8 @@ int check_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d
     return api_fail(ATTNRES_EINVAL, "tokens=%lld must be 0 .. 2^30", (long long)d->tokens);
   if (d->q_heads < 1 || d->q_heads > (1 << 20) || d->q_heads % c->kv_heads)
     return api_fail(ATTNRES_EINVAL, "q_heads=%d must be a multiple of kv_heads=%d", d->q_heads, c->kv_heads);
-  if (!isfinite(d->scale)) return api_fail(ATTNRES_EINVAL, "scale must be finite");
+  if (!(fabsf(d->scale) <= ATTNRES_CACHE_MAX_SCALE))
+    return api_fail(ATTNRES_EINVAL, "scale must be finite, of at most %g", (double)ATTNRES_CACHE_MAX_SCALE);
   if (c->weights && d->tokens > 1) return api_fail(ATTNRES_EINVAL, "weights need a single new token, got %lld", (long long)d->tokens);
   if (c->weights && !(d->decay >= 0.f && d->decay <= 1.f)) return api_fail(ATTNRES_EINVAL, "decay must be 0 .. 1");
   if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;

@@ -137,7 +137,7 @@ py::object cache_attend(const py::object& q_, const py::object& k_, const py::ob
   } else {
     if (!PyFloat_CheckExact(scale_.ptr())) return py::none();
     d.scale = (float)PyFloat_AS_DOUBLE(scale_.ptr());
-    if (!std::isfinite(d.scale)) return py::none();
+    if (!(std::fabs(d.scale) <= ATTNRES_CACHE_MAX_SCALE)) return py::none();
   }
   d.tokens = T;
   d.q_heads = (int)H;

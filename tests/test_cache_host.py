@@ -88,7 +88,7 @@ def test_append_refusals(kw, code, word):
 @needs_lib
 @pytest.mark.parametrize("kw,code,word", CACHE_REFUSALS + [
     (dict(tokens=-1), -1, "tokens"), (dict(q_heads=3), -1, "q_heads"), (dict(q_heads=0), -1, "q_heads"),
-    (dict(scale=float("inf")), -1, "scale"), (dict(scale=float("nan")), -1, "scale"), (dict(q=0), -1, "NULL"),
+    (dict(scale=float("inf")), -1, "scale"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=-2e38), -1, "scale"), (dict(q=0), -1, "NULL"),
     (dict(q_token_stride=-1), -1, "stride"), (dict(weights=0x5000, tokens=2), -1, "single"),
     (dict(weights=0x5000, decay=1.5), -1, "decay"), (dict(weights=0x5000, decay=float("nan")), -1, "decay"),
     (dict(tokens=1 << 30), -2, "too many")])

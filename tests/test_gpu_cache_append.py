@@ -163,6 +163,53 @@ def test_agrees_with_the_uncached_operator():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Dh", [62, 86, 130, 198, 254])
+@pytest.mark.parametrize("T", [1, 7])
+def test_heads_of_pairs(dtype, Dh, T):
+    """Widths of 4 n + 2, of up to two pairs a lane."""
+    cached = [0, 15, 40]
+    c, qkv, sin, cos = build(Dh, dtype, 4, 2, Dh, 16, cached, T, weights=True, table="fp32" if T > 1 else dtype)
+    check(c, qkv, 4, sin, cos, cached, fresh=[T, T - 1, T], weights=True)
+
+
+def test_far_pages():
+    """Pages whose elements lie beyond 2^32 of the first."""
+    S, Dh = 16, 64
+    P = (1 << 32) // (S * Dh) + 64
+    c, qkv, sin, cos = build(61, "bf16", 2, 1, Dh, S, [20], 9)
+    k, v = (torch.empty((P, 1, S, Dh), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    far = torch.tensor([[P - 3, P - 40]], dtype=torch.int32, device=DEV)
+    q = ops.qkv_norm_rotary_cached(qkv, 2, sin, cos, c.k, c.v, c.table, c.cached)
+    assert torch.equal(ops.qkv_norm_rotary_cached(qkv, 2, sin, cos, k, v, far, c.cached), q)
+    for a, b in ((k, c.k), (v, c.v)):
+        assert torch.equal(a[P - 40, :, 4:13], b[int(c.table[0, 1]), :, 4:13])
+
+
+def test_a_pool_without_pages():
+    c, qkv, sin, cos = build(63, "bf16", 2, 1, 64, 16, [20, 3], 4)
+    q = ops.qkv_norm_rotary_cached(qkv, 2, sin, cos, c.k, c.v, c.table, c.cached)
+    assert torch.equal(ops.qkv_norm_rotary_cached(qkv, 2, sin, cos, c.k[:0], c.v[:0], c.table, c.cached), q)
+
+
+def test_two_streams():
+    """Two caches at once, each on a stream of its own."""
+    made = [build(s, "bf16", 4, 2, 64, 16, [0, 100, 30], 50) for s in (65, 66)]
+    want = []
+    for c, qkv, sin, cos in made:
+        want.append((ops.qkv_norm_rotary_cached(qkv, 4, sin, cos, c.k, c.v, c.table, c.cached), c.k.clone(), c.v.clone()))
+        c.k.fill_(0.125)
+        c.v.fill_(0.125)
+    torch.cuda.synchronize()
+    got = []
+    for s, (c, qkv, sin, cos) in zip([torch.cuda.Stream(), torch.cuda.Stream()], made):
+        with torch.cuda.stream(s):
+            got.append(ops.qkv_norm_rotary_cached(qkv, 4, sin, cos, c.k, c.v, c.table, c.cached))
+    torch.cuda.synchronize()
+    for q, (c, *_), (e, k, v) in zip(got, made, want):
+        assert torch.equal(q, e) and torch.equal(c.k, k) and torch.equal(c.v, v)
+
+
 def test_empty_calls():
     c, qkv, sin, cos = build(17, "bf16", 4, 2, 64, 16, [3, 3], 2)
     kept = c.k.clone()

@@ -75,6 +75,55 @@ def test_long(cached, budget, recent):
     run_and_check(c, new, cached, budget, recent)
 
 
+@pytest.mark.parametrize("room", [2048, 2064, 8192, 8208, 16384, 16400])
+def test_tables_up_to_and_above_what_a_workgroup_holds(room):
+    cached = [room, room - 1, 900]
+    c, new = build(room, "bf16", 1, 8, 16, cached, 700, ties=False, room=room)
+    run_and_check(c, new, cached, 700, 90)
+
+
+def test_far_pages():
+    """Rows from and to pages whose elements lie beyond 2^32 of the first."""
+    S, Dh = 16, 64
+    P = (1 << 32) // (S * Dh) + 64
+    c, new = build(23, "bf16", 1, Dh, S, [40], 20)
+    k, v = (torch.empty((P, 1, S, Dh), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    w = torch.zeros((P, 1, S), device=DEV)
+    far = torch.tensor([[P - 3, P - 40, P - 7]], dtype=torch.int32, device=DEV)
+    to = torch.tensor([[P - 50, P - 1]], dtype=torch.int32, device=DEV)
+    for a, b in ((k, c.k), (v, c.v), (w, c.w)):
+        a[far[0].long()] = b[c.table[0].long()]
+    want = ops.evict_cached_tokens(c.k, c.v, c.w, c.table, c.cached, new, 20, 4)
+    got = ops.evict_cached_tokens(k, v, w, far, c.cached, to, 20, 4)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for a, b in ((k, c.k), (v, c.v), (w, c.w)):
+        assert torch.equal(a[P - 50], b[int(new[0, 0])]) and torch.equal(a[P - 1, :, :4], b[int(new[0, 1]), :, :4])
+
+
+def test_a_pool_without_pages():
+    """Nothing to copy; the choice is by place alone."""
+    c, new = build(25, "bf16", 2, 64, 16, [40, 10], 20)
+    kept, left = ops.evict_cached_tokens(c.k[:0], c.v[:0], c.w[:0], c.table, c.cached, new, 20, 5)
+    assert left.tolist() == [20, 10]
+    assert kept[0, 1].tolist() == list(range(15)) + list(range(35, 40)) and kept[1, 0].tolist() == list(range(10)) + [-1] * 10
+
+
+def test_two_streams():
+    """Two caches at once, each on a stream of its own; of tables of one workgroup a head and of several."""
+    made = [build(s, "bf16", 2, 64, 16, [20000 if s == 27 else 3000, 700], 600) for s in (27, 28)]
+    before = [[t.clone() for t in (c.k, c.v, c.w)] for c, _ in made]
+    want = [ops.evict_cached_tokens(*t, c.table, c.cached, new, 600, 50) for t, (c, new) in zip(before, made)]
+    torch.cuda.synchronize()
+    got = []
+    for s, (c, new) in zip([torch.cuda.Stream(), torch.cuda.Stream()], made):
+        with torch.cuda.stream(s):
+            got.append(ops.evict_cached_tokens(c.k, c.v, c.w, c.table, c.cached, new, 600, 50))
+    torch.cuda.synchronize()
+    for a, b, t, (c, _) in zip(got, want, before, made):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        assert torch.equal(c.k, t[0]) and torch.equal(c.v, t[1]) and torch.equal(c.w, t[2])
+
+
 @pytest.mark.parametrize("values", [[0.0], [-0.0, 0.0], [NAN], [NAN, -INF, -1.0, 0.0], [INF, NAN, 3.0], [-INF],
                                     [1e-45, 0.0, -1e-45], [3.4e38, INF, -3.4e38], [1.0, 1.0000001]])
 def test_weights_of_all_kinds(values):

@@ -84,6 +84,32 @@ def test_several_new_tokens(dtype, T, H, K, Dh, S):
     check(c, q, cached, fresh)
 
 
+@pytest.mark.parametrize("dtype,T,H,K,Dh,S", [("bf16", 200, 4, 2, 64, 64), ("fp16", 150, 3, 1, 96, 20), ("fp32", 140, 2, 2, 32, 16)])
+def test_a_prompt_after_cached_tokens(dtype, T, H, K, Dh, S):
+    """Rows of far apart tokens, each block of them with its own last one."""
+    cached = [0, 90, 517]
+    fresh = [T, T - 1, T // 3]
+    c, q, _ = build(T, dtype, H, K, Dh, S, cached, T=T, fresh=fresh)
+    check(c, q, cached, fresh, pass_fresh=True)
+
+
+@pytest.mark.parametrize("T", [17, 40])
+def test_values_that_are_not_finite_in_a_prompt(T):
+    """Each row takes what its own token sees of them, in blocks of rows and tiles of tokens that do not end together."""
+    cached = [70]
+    c, q, fresh = build(T, "bf16", 2, 1, 64, 16, cached, T=T)
+    page, slot = c.where(0, 70 + T)
+    for bad in (0, 9, T - 2):
+        c.v[page[70 + bad], 0, slot[70 + bad], bad] = float("inf")
+    o = ops.cached_attention(q, c.k, c.v, c.table, c.cached)
+    e, bound, _ = attend_ref(c, q, cached, fresh, 64 ** -0.5)
+    for bad in (0, 9, T - 2):
+        assert bool((o[0, :, bad:, bad] == math.inf).all()) and bool(torch.isfinite(o[0, :, :bad, bad]).all())
+    fine = torch.isfinite(e)
+    assert torch.equal(torch.isfinite(o), fine)
+    assert_within(o[fine], e[fine], bound[fine], "finite")
+
+
 @pytest.mark.parametrize("T", [1, 4, 20])
 def test_padded_batch(T):
     cached = [0, 0, 50, 131, 7]
@@ -267,6 +293,16 @@ def test_graphs(weights):
             c.k[c.table[0, 0].long()] *= 0.5
 
 
+def test_a_pool_without_pages():
+    """Tokens have nowhere to be: NaN; a sequence without new ones has zeros."""
+    c, q, _ = build(57, "bf16", 4, 2, 64, 16, [5, 5], weights=True)
+    k, v, w = c.k[:0], c.v[:0], c.w[:0]
+    fresh = torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    for kw in ({}, dict(weights=w)):
+        o = ops.cached_attention(q, k, v, c.table, c.cached, fresh=fresh, **kw)
+        assert bool(o[0].isnan().all()) and not bool(o[1].any())
+
+
 def test_two_streams():
     made = [build(s, "bf16", 8, 2, 64, 16, [1000, 40, 3000]) for s in (41, 42)]
     want = [ops.cached_attention(q, c.k, c.v, c.table, c.cached) for c, q, _ in made]
@@ -333,6 +369,7 @@ def test_refusals():
     refused("decay", weights=c.w, decay=1.5)
     refused("decay", weights=c.w, decay=float("nan"))
     refused("scale", scale=float("inf"))
+    refused("scale", scale=-2e38)
     refused("weights must be", weights=c.w.half())
     refused("weights must be", weights=c.w[:, :1])
     refused("overlap", weights=c.w[:1].expand(c.w.size(0), -1, -1))
