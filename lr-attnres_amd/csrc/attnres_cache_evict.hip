@@ -252,10 +252,16 @@ __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int hea
   return f;
 }
 
+// A head's slices in neighbouring places, which one XCD has: its L2 then holds the counts that they all read.
+__device__ __forceinline__ int place_of_block() {
+  const int grid = gridDim.x;
+  return grid % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8);
+}
+
 __global__ __launch_bounds__(kBig) void evict_count_kernel(CacheEvictParams p, int round) {
   __shared__ int hist[kBins<kBig>];
   __shared__ SelectShared<kR, kBig> s;
-  const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
+  const int at = place_of_block(), head = at / p.slices, slice = at - head * p.slices;
   const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   const int early = n - p.recent, j0 = slice * kSlice;
   if (n <= p.budget || p.budget == p.recent || j0 >= early) return;
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(kBig) void evict_count_kernel(CacheEvictParams p, i
 
 __global__ __launch_bounds__(kBig) void evict_place_kernel(CacheEvictParams p) {
   __shared__ SelectShared<kR, kBig> s;
-  const int head = blockIdx.x / p.slices, slice = blockIdx.x - head * p.slices;
+  const int at = place_of_block(), head = at / p.slices, slice = at - head * p.slices;
   const int b = head / p.c.kv_heads, h = head - b * p.c.kv_heads, n = max(cache_count(p.c, b), 0);
   int32_t* kept = p.kept + (int64_t)head * p.budget;
   if (slice == 0) {
