@@ -89,7 +89,7 @@ hipError_t launch_cache_attend_f16(const CacheAttendParams& p, hipStream_t st);
 hipError_t launch_cache_attend_f32(const CacheAttendParams& p, hipStream_t st);
 
 constexpr int kEvictSlice = 8192;  // tokens whose keys a workgroup holds (twice as many where it has a whole head)
-constexpr int kEvictSlots = 6152;  // counts and state of a workgroup, 4 bytes each
+constexpr int kEvictSlots = 3080;  // counts and state of a workgroup, 4 bytes each
 
 struct CacheEvictParams {
   CachePages c;

@@ -2,7 +2,11 @@
 //   p_j = softmax_j(scale <q, k_j>),   out = sum_j p_j v_j,   j < cached + t + 1
 //
 // Bound by memory: each key and value is read once for the (up to 16) query rows of its
-// head -- the heads of its group times the new tokens -- so 2 rows flops a byte in 16 bits.
+// head -- the heads of its group times the new tokens -- so 2 rows flops a byte in 16 bits.  4 x 4 heads of
+// 128 over 32768 to 131072 tokens, bf16: 782 MB in 135 us (5.8 TB/s; 6.2 without the ramp of the first tiles).  Rows
+// above 16 read it again, from L2, at what a CU takes (48 bytes a ns): 128 rows of a head over 4096 tokens,
+// 32 heads of 64, 33 us where 16 rows take 17.  Two and four blocks of rows in one workgroup were no faster (36 and
+// 38): what is saved in loads is waited for in one wave's chain of products and exponentials.
 //
 // Products.  Query rows are columns of 16 x 16 matrix-core tiles: S^T = K Q^T with a tile's
 // tokens as rows, then O^T = V^T P^T.  Lane l holds column l % 16 of both, so a row's maximum,
@@ -18,11 +22,12 @@
 // as large as the result's own rounding); fp16 weights are scaled by 2^14 so that small ones
 // keep their bits.
 //
-// Work.  A cache's units (kUnit tokens of one sequence's head and block of rows) are dealt
+// Work.  A cache's units (kAttUnit tokens of one sequence's head and block of rows) are dealt
 // evenly to a fixed number of workgroups from the lengths on the device, whatever they are:
 // no length is known to the host, and a long sequence among short ones is shared by many.  A
 // workgroup that has a head's whole length writes its rows; pieces go to the workspace as
-// maximum, sum and unscaled output, joined by a second launch.
+// maximum, sum and unscaled output, joined by a second launch (3.5 to 5 us).  Where the tables are so short
+// that a workgroup can take a whole segment in less than that, each does, and there is one launch.
 #pragma once
 
 #include "attnres_cache.h"
@@ -34,7 +39,7 @@ namespace attnres {
 constexpr int kAttRows = 16;  // query rows of a workgroup
 constexpr int kAttWaves = 4;
 
-// The deal: `segs` segments (heads, blocks of rows) of each sequence, kUnit tokens a unit, unit x to
+// The deal: `segs` segments (heads, blocks of rows) of each sequence, kAttUnit tokens a unit, unit x to
 // workgroup deal_of(x).
 struct Deal {
   int total, per, more;  // units; of a workgroup; the first `more` have one more

@@ -1,14 +1,21 @@
 // The paged cache reduced to a budget: per key / value head the most attended and the
 // last tokens, copied in their order to other pages.
 //
-// Choice (one workgroup a head and kEvictSlice tokens).  Weights become keys whose unsigned order is theirs (a NaN
-// below all), held in registers; the budget-th largest is found in three rounds of 12, 10 and 10
-// bits counted in LDS (twelve first: weights lie in few octaves, and lanes that count into one
-// place wait for each other), fewer where a round leaves nothing open.  What lies above it and, of
-// what equals it, the first ones are kept: their places come from counts a wave and 64 tokens,
-// scanned once.  Bound by the latency of its rounds and barriers.
-// Copy.  Places are independent: every kept row is read and written once by the lanes of
-// its own, so nothing is ordered and nothing waits.  Bound by memory.
+// Choice.  Weights become keys whose unsigned order is theirs (a NaN below all), held in
+// registers; the budget-th largest is found in three rounds of 12, 10 and 10 bits (256 threads:
+// 11, 11 and 10) counted in LDS, fewer where a round leaves nothing open.  The first round takes most
+// bits: weights lie in few octaves, and lanes that count into one place wait for each other (four
+// copies of the counts, a quarter of the lanes each, were no faster).  What lies above the found key and, of what equals
+// it, the first ones are kept: their places come from counts a wave and 64 tokens, scanned once.
+// One workgroup a head, of 256 threads for tables of up to 2048 tokens (16 x 12 heads: 7.4 us; 1024 threads
+// 8.4) and of 1024 up to 16384; longer tables are shared by one for each 8192 tokens, a launch a round
+// (16 heads of up to 65536: 6 to 8 us each, 7.3 to place them).  Bound by latency: a launch, the chain
+// of count, page and weight, and the rounds' barriers.
+//
+// Copy.  Places are independent: every kept row is read and written once by lanes of
+// its own, so nothing is ordered and nothing waits.  Bound by memory: 102 MB of rows of 128 bytes in 20.7 us
+// (4.9 TB/s), 139 MB of rows of 256 in 30.6 (4.5; they are gathered from caches eight times as large).  Two
+// and four rows a thread at once: 22 and 27 us, 32 and 40.
 #include "attnres_cache.h"
 #include "attnres_device.h"
 
@@ -61,9 +68,9 @@ struct SelectShared {
   int above[R * TH / kWave], equal[R * TH / kWave];
 };
 
-// The next digit of the want-th largest key from the counts of its places, 2^bits of them: count(place, &n, &before),
-// `before` being those of n that lie in slices before this one.  In s.before_*: keys of theirs that are above
-// the digit and equal to it.
+// The next digit of the want-th largest key from the counts of its places, 2^bits of them: count(low, n, before) of the
+// thread's, low .. , backwards; `before` being those of n that lie in slices before this one.  In s.before_*: keys of
+// theirs that are above the digit and equal to it.
 template <bool SLICES, int R, int TH, class F>
 __device__ __forceinline__ void next_digit(int round, Found& f, SelectShared<R, TH>& s, F count) {
   const int bits = round_bits<TH>(round), mine = (1 << bits) / TH;
@@ -71,9 +78,10 @@ __device__ __forceinline__ void next_digit(int round, Found& f, SelectShared<R, 
   const int first = (1 << bits) - 1 - (int)threadIdx.x * mine;
   int n[kBins<TH> / TH], before[kBins<TH> / TH], sum = 0, sum_before = 0;
 #pragma unroll
+  for (int i = 0; i < kBins<TH> / TH; ++i) n[i] = before[i] = 0;
+  count(first - (mine - 1), n, before);
+#pragma unroll
   for (int i = 0; i < kBins<TH> / TH; ++i) {
-    n[i] = before[i] = 0;
-    if (i < mine) count(first - i, &n[i], &before[i]);
     sum += n[i];
     sum_before += before[i];
   }
@@ -200,7 +208,12 @@ __global__ __launch_bounds__(TH) void evict_select_kernel(CacheEvictParams p) {
     Found f{0, 0, p.budget - p.recent, true};
     for (int round = 0; round < 3 && f.open; ++round) {
       count_keys<R, TH>(key, 0, early, round, f, hist);
-      next_digit<false>(round, f, s, [&](int place, int* n, int*) { *n = hist[place]; });
+      next_digit<false>(round, f, s, [&](int low, int* n, int*) {
+        const int mine = (1 << round_bits<TH>(round)) / TH;
+#pragma unroll
+        for (int i = 0; i < kBins<TH> / TH; ++i)
+          if (i < mine) n[i] = hist[low + mine - 1 - i];
+      });
     }
     place(key, 0, early, f, 0, 0, kept, s);
   }
@@ -209,10 +222,10 @@ __global__ __launch_bounds__(TH) void evict_select_kernel(CacheEvictParams p) {
 // Longer tables: kSlice tokens a workgroup, a launch for each round's counts and one that places what is kept.  Each
 // launch finds the digit of the round before it, from the counts of all of the head's slices, and each workgroup
 // keeps what it has found for its next launch.
-// hist[head][slice]: 4096, 1024, 1024 places, then prefix, mask, want, open, above, equal
-constexpr int kSlots = kEvictSlots, kState = 6144;
-static_assert(kSlots >= kState + 6, "places and state");
-__device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 3072 + 1024 * round; }
+// hist[head][slice]: counts of 16 bits of 4096, 1024, 1024 places, then prefix, mask, want, open, above, equal
+constexpr int kSlots = kEvictSlots, kState = 3072;
+static_assert(kSlots >= kState + 6 && kSlots % 2 == 0 && kSlice < 1 << 16, "places and state");
+__device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 1536 + 512 * round; }
 
 // What the rounds before `round` have found; above, equal: keys of the slices before this one.
 __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int head, int slices, int slice, int round, int* above,
@@ -227,13 +240,22 @@ __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int hea
   }
   if (round > 0 && f.open) {
     const int32_t* at = p.hist + (int64_t)head * p.slices * kSlots + round_at(round - 1);
-    next_digit<true>(round - 1, f, s, [&](int place, int* n, int* before) {
+    // four places of the first round's a thread, in one load, one of the others'
+    static_assert(kBins<kBig> == 4 * kBig, "four places a thread");
+    next_digit<true>(round - 1, f, s, [&](int low, int* n, int* before) {
       for (int i0 = 0; i0 < slices; i0 += 8)  // (eight slices' loads at once)
 #pragma unroll
         for (int i = i0; i < i0 + 8; ++i) {
-          const int x = at[(int64_t)min(i, slices - 1) * kSlots + place];
-          *n += i < slices ? x : 0;
-          *before += i < slice ? x : 0;
+          const int32_t* from = at + (int64_t)min(i, slices - 1) * kSlots;
+          u32x2 x = {0, 0};
+          if (round == 1) x = *(const u32x2*)(from + low / 2);
+          else x.y = (uint32_t)((const uint16_t*)from)[low] << 16;
+          const int places[4] = {(int)(x.y >> 16), (int)(x.y & 0xffff), (int)(x.x >> 16), (int)(x.x & 0xffff)};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            n[q] += i < slices ? places[q] : 0;
+            before[q] += i < slice ? places[q] : 0;
+          }
         }
     });
     a += s.before_above;
@@ -272,7 +294,7 @@ __global__ __launch_bounds__(kBig) void evict_count_kernel(CacheEvictParams p, i
   if (!f.open) return;
   count_keys<kR, kBig>(key, j0, early, round, f, hist);
   int32_t* to = p.hist + ((int64_t)head * p.slices + slice) * kSlots + round_at(round);
-  for (int i = threadIdx.x; i < 1 << round_bits<kBig>(round); i += kBig) to[i] = hist[i];
+  for (int i = threadIdx.x; i < 1 << (round_bits<kBig>(round) - 1); i += kBig) to[i] = hist[2 * i] | hist[2 * i + 1] << 16;
 }
 
 __global__ __launch_bounds__(kBig) void evict_place_kernel(CacheEvictParams p) {
