@@ -5,7 +5,7 @@
 // head -- the heads of its group times the new tokens -- so 2 rows flops a byte in 16 bits.  4 x 4 heads of
 // 128 over 32768 to 131072 tokens, bf16: 782 MB in 135 us (5.8 TB/s; 6.2 without the ramp of the first tiles).  Rows
 // above 16 read it again, from L2, at what a CU takes (48 bytes a ns): 128 rows of a head over 4096 tokens,
-// 32 heads of 64, 33 us where 16 rows take 17.  Two and four blocks of rows in one workgroup were no faster (36 and
+// 32 heads of 64, 33 us where 16 rows take 15.  Two and four blocks of rows in one workgroup were no faster (36 and
 // 38): what is saved in loads is waited for in one wave's chain of products and exponentials.
 //
 // Products.  Query rows are columns of 16 x 16 matrix-core tiles: S^T = K Q^T with a tile's
