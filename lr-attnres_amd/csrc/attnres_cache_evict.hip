@@ -223,9 +223,9 @@ __global__ __launch_bounds__(TH) void evict_select_kernel(CacheEvictParams p) {
 // launch finds the digit of the round before it, from the counts of all of the head's slices, and each workgroup
 // keeps what it has found for its next launch.
 // hist[head][slice]: counts of 16 bits of 4096, 1024, 1024 places, then prefix, mask, want, open, above, equal
-constexpr int kSlots = kEvictSlots, kState = 3072;
+constexpr int kSlots = kEvictSlots, kState = 2048 + 2 * 512;
 static_assert(kSlots >= kState + 6 && kSlots % 2 == 0 && kSlice < 1 << 16, "places and state");
-__device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 1536 + 512 * round; }
+__device__ __forceinline__ int round_at(int round) { return round == 0 ? 0 : 2048 + 512 * (round - 1); }
 
 // What the rounds before `round` have found; above, equal: keys of the slices before this one.
 __device__ __forceinline__ Found found_before(const CacheEvictParams& p, int head, int slices, int slice, int round, int* above,
