@@ -26,7 +26,7 @@
 // evenly to a fixed number of workgroups from the lengths on the device, whatever they are:
 // no length is known to the host, and a long sequence among short ones is shared by many.  A
 // workgroup that has a head's whole length writes its rows; pieces go to the workspace as
-// maximum, sum and unscaled output, joined by a second launch (3.5 to 5 us).  Where the tables are so short
+// maximum, sum and output, joined by a second launch (3.5 to 5 us).  Where the tables are so short
 // that a workgroup can take a whole segment in less than that, each does, and there is one launch.
 #pragma once
 
@@ -144,6 +144,7 @@ struct Att {
   static constexpr int kWords = kW * kSize / 4;
   static constexpr int kPitch = HD + 4;
   static constexpr float kShift = DT::kCode == 2 ? 14.f : 0.f;
+  static constexpr float kCare = DT::kCode == 2 ? 0.f : 31.f;  // (fp16 values are far below fp32's largest)
   static constexpr int kStep = kAttWaves * kTok;               // tokens of a workgroup's round
 
   const CacheAttendParams& p;
@@ -158,6 +159,7 @@ struct Att {
   uint32_t v[kSub][4][kNi][kWords];
   sw_f4 acc[kNi][kW];
   float m, l;                    // of the lane's row: maximum of <q, k>, the lane's part of the sum
+  float low;                     // the exponents' base is further up by it: kCare after a careful pass
 
   struct Rows {
     // PAGE16: of each subtile, bytes from the head's page 0 to its first token, and whether it has a page (one that has
@@ -380,7 +382,7 @@ struct Att {
   }
 
   // a maximum as the exponents' base; of no score at all: 0, so that -inf less it stays -inf
-  __device__ __forceinline__ float base_of(float top) const { return top == -INFINITY ? 0.f : top * p.scale - kShift; }
+  __device__ __forceinline__ float base_of(float top) const { return top == -INFINITY ? 0.f : top * p.scale - kShift + low; }
 
   struct Row {       // the lane's
     float* logits;   // of token 0, or null
@@ -390,7 +392,8 @@ struct Att {
 
   // The tile of tokens t0 .., whose keys and values are on their way.  AHEAD: all rows see all of it, and the next
   // tile's are loaded where its registers become free (in every turn of the loop: a load under a condition would make
-  // each wait one for all loads).  CARE: a value that is not finite shows in the rows that see it and in no other.
+  // each wait one for all loads).  CARE: a value that is not finite shows in the rows that see it and in no other, and
+  // weights 2^31 times smaller keep sums of the largest values finite.
   template <bool AHEAD, bool CARE>
   __device__ __forceinline__ void tile(int t0, const Row& row, Rows& now, Rows& next) {
     constexpr bool CUT = !AHEAD;
@@ -547,6 +550,7 @@ struct Att {
     const int t_first = first + wave * kTok, limit = p.direct ? p.c.room : seq.n;
     if (t_first >= limit) {
       clear();
+      low = 0.f;
       n = seq.n;
       return;
     }
@@ -559,6 +563,7 @@ struct Att {
       for (int i = 0; i < kKs; ++i) q[i] ^= k32 ? 0x80000000u : 0x80008000u;
     }
     clear();
+    low = 0.f;
     have = seq.have;
     n = seq.n;
     t_lo = div_by(row0, p.by_group);
@@ -589,6 +594,7 @@ struct Att {
         for (int t = 0; t < 4; ++t) none = __builtin_fmaf(acc[i][d][t], 0.f, none);
     if (__any(none != 0.f)) {  // NaN: something was not finite
       clear();
+      low = kCare;
       for (t0 = t_first; t0 < end; t0 += kStep) {
         now = rows_of(t0, n);
         load_k(now);
@@ -608,15 +614,13 @@ __device__ __forceinline__ float att_share(float m, float top) {
 
 // Columns col .. col + 3 of query row `row` of key / value head h: zeros where it saw nothing, NaN for counts that cannot be
 template <class DT>
-__device__ __forceinline__ void att_row_out(const CacheAttendParams& p, int b, int h, int row, int col, int n, float l,
-                                            sw_f4 o) {
+__device__ __forceinline__ void att_row_out(const CacheAttendParams& p, int b, int h, int row, int col, int n, sw_f4 o) {
   const int t = div_by(row, p.by_group), hq = h * p.group + row - t * p.group, Dh = p.c.head_dim;
   const bool seen = n > 0 && (!p.c.fresh || t < p.c.fresh[b]);
   typename DT::S* out = (typename DT::S*)p.out + ((b * (int64_t)p.tokens + t) * p.q_heads + hq) * Dh + col;
-  const float inv = 1.f / l;
   float x[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = n < 0 ? __builtin_nanf("") : seen ? o[e] * inv : 0.f;
+  for (int e = 0; e < 4; ++e) x[e] = n < 0 ? __builtin_nanf("") : seen ? o[e] : 0.f;
   if (Dh % 4 == 0) {
     if (col < Dh) store_vec<DT, 4>(out, x);
   } else {
@@ -701,14 +705,14 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
 #pragma unroll
         for (int i = 0; i < kAttWaves; ++i) top = fmaxf(top, sm[i][r]);
 #pragma unroll
-        for (int i = 0; i < kAttWaves; ++i) {
-          const float f = att_share(sm[i][r], top);
-          l += f * sl[i][r];
-          o += f * *(const sw_f4*)&so[i][r][col];
-        }
+        for (int i = 0; i < kAttWaves; ++i) l += att_share(sm[i][r], top) * sl[i][r];
+        // (shares of the whole sum first: sums of the largest values would not be finite)
+        const float inv = l == 0.f && !whole ? 0.f : 1.f / l;  // (a piece that a row sees nothing of)
+#pragma unroll
+        for (int i = 0; i < kAttWaves; ++i) o += att_share(sm[i][r], top) * inv * *(const sw_f4*)&so[i][r][col];
       }
       if (whole) {
-        att_row_out<DT>(p, a.b, a.h, row0 + r, col, a.n, l, o);
+        att_row_out<DT>(p, a.b, a.h, row0 + r, col, a.n, o);
         if (p.own_weights) {
           if (col == 0) lse[r] = top + log2f(l);
         } else if (p.row_ml && col == 0) {
@@ -779,9 +783,10 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (w + i * kShares > s.w1) break;
-      const float to = fmaxf(top, m[i]), f = att_share(top, to), g = att_share(m[i], to);
-      l = f * l + g * part[i];
-      o = f * o + g * x[i];
+      const float to = fmaxf(top, m[i]), f = att_share(top, to) * l, g = att_share(m[i], to) * part[i];
+      l = f + g;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      o = f * inv * o + g * inv * x[i];
       top = to;
     }
   }
@@ -793,16 +798,17 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
   float all = top;
 #pragma unroll
   for (int i = 1; i < kShares; ++i) all = fmaxf(all, sm[i * kItems + item]);
-  float f = att_share(top, all);
-  l *= f;
-  o *= f;
+  float f[kShares], sum = 0.f;
 #pragma unroll
-  for (int i = 1; i < kShares; ++i) {
-    f = att_share(sm[i * kItems + item], all);
-    l += f * sl[i * kItems + item];
-    o += f * so[i * kItems + item];
+  for (int i = 0; i < kShares; ++i) {
+    f[i] = att_share(sm[i * kItems + item], all) * sl[i * kItems + item];
+    sum += f[i];
   }
-  att_row_out<DT>(p, b, h, row, col, n, l, o);
+  const float inv = 1.f / sum;
+  o = sw_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kShares; ++i) o += f[i] * inv * so[i * kItems + item];
+  att_row_out<DT>(p, b, h, row, col, n, o);
 }
 
 // What each cached token received: with the scores x as attention left them (base-2 logarithms),

@@ -93,6 +93,20 @@ def test_a_prompt_after_cached_tokens(dtype, T, H, K, Dh, S):
     check(c, q, cached, fresh, pass_fresh=True)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,cached", [(1, [600, 3]), (1, [9000, 2]), (5, [600, 3]), (20, [5000])])
+def test_the_largest_values(dtype, T, cached):
+    """Sums of weights times values that only their mean keeps finite."""
+    c, q, fresh = build(59, dtype, 4, 2, 64, 16, cached, T=T)
+    for b, n in enumerate(cached):
+        page, slot = c.where(b, n + T)
+        sign = torch.randint(0, 2, (n + T, 2, 64), generator=gen(b)) * 2.0 - 1.0
+        sign[:, :, :32] = 1.0
+        c.v[page, :, slot] = (sign * 0.9 * torch.finfo(DT[dtype]).max).to(DT[dtype]).to(DEV)
+    o, _ = check(c, q, cached, fresh)
+    assert bool(torch.isfinite(o).all())
+
+
 @pytest.mark.parametrize("T", [17, 40])
 def test_values_that_are_not_finite_in_a_prompt(T):
     """Each row takes what its own token sees of them, in blocks of rows and tiles of tokens that do not end together."""
