@@ -203,6 +203,13 @@ def test_received_weights(dtype, H, K, Dh, S, cached, decay):
     assert torch.equal(c.w[~touched].nan_to_num(7.0), before[~touched].nan_to_num(7.0)), "other slots are left as they were"
 
 
+@pytest.mark.parametrize("dtype,H,K,Dh,S,cached", [
+    ("bf16", 300, 1, 32, 16, [200, 3]), ("fp32", 520, 2, 16, 20, [90]), ("bf16", 4, 2, 64, 64, [6000, 100, 0]),
+    ("fp16", 2, 2, 128, 16, [131, 0, 5, 260] * 18)])
+def test_received_weights_of_many_heads_tokens_and_sequences(dtype, H, K, Dh, S, cached):
+    test_received_weights(dtype, H, K, Dh, S, cached, 0.5)
+
+
 def test_weights_of_padded_rows():
     c, q, _ = build(21, "bf16", 4, 2, 64, 16, [0, 20, 40], fresh=[0, 0, 1], weights=True)
     before = c.w.clone()

@@ -75,6 +75,16 @@ def test_generate_with_and_without_a_budget():
     assert torch.equal(out[:, 0], plain[:, 0])
 
 
+def test_generate_in_inference_mode():
+    m = model(torch.bfloat16)
+    idx = torch.randint(0, 64, (2, 30), device=DEV)
+    kw = dict(budget=24, recent=4)
+    plain = m.generate(idx, 40, cache=m.new_cache(2, page_size=8, weights=True, spare_tokens=24), **kw)
+    with torch.inference_mode():
+        inside = m.generate(idx, 40, cache=m.new_cache(2, page_size=8, weights=True, spare_tokens=24), **kw)
+    assert torch.equal(inside, plain)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_the_operators_together(dtype):
     """Prompts, steps that count what tokens receive, evictions, more steps: each call against its definition on the
