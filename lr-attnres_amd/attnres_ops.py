@@ -2252,8 +2252,8 @@ def cached_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: T
     ``q`` [B, H, T, Dh]; the cache's arguments as ``qkv_norm_rotary_cached`` takes them, with the same ``cached`` and ``fresh``
     (the counts before these T tokens; how many of them are the sequence's).  Query t of sequence b reads the tokens up to its
     own, ``j < cached[b] + t + 1``, through key / value head ``h // (H // K)``: softmax of ``scale <q, k_j>`` (``Dh ** -0.5``
-    unless given), in fp32, one rounding to the dtype.  Made for one or a few tokens: each sixteen query rows of a key / value
-    head (heads of its group times tokens) read the cache once.
+    unless given), in fp32, one rounding to the dtype.  Made for one or a few tokens: each sixteen (of large
+    calls 32) query rows of a key / value head (heads of its group times tokens) read the cache once.
 
     ``weights`` [P, K, S] (fp32, T = 1): becomes ``decay * weights`` plus the softmax weights of the head's queries, summed,
     for every token that was read; with ``decay`` 0 what was there is not read.  ``evict_cached_tokens`` goes by it.  Pages may

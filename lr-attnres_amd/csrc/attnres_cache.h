@@ -64,7 +64,8 @@ struct CacheAttendParams {
   const void* q;
   int64_t q_b_stride, q_h_stride, q_t_stride;
   int32_t tokens, q_heads;
-  int32_t group, rows, blocks;  // query heads of a key / value head; with the new tokens; 16-row blocks of them
+  int32_t group, rows, blocks;  // query heads of a key / value head; with the new tokens; blocks of them
+  int32_t row_bits;             // 4 or 5: rows of a block, 2^row_bits
   int32_t wgs;                  // of a split cache
   int32_t weight_wgs;           // that add the weights up in a launch of their own
   int32_t own_weights;          // the workgroup of a whole segment does it
@@ -77,8 +78,8 @@ struct CacheAttendParams {
   float scale;                  // of base-2 logarithms: the softmax's scale times log2(e), > 0
   float decay;
   void* out;
-  float* part;     // [2 wgs][16][tile], pieces of rows
-  float* part_ml;  // [2 wgs][16][2], their maxima and sums
+  float* part;     // [2 wgs][rows of a block][tile], pieces of rows
+  float* part_ml;  // [2 wgs][rows of a block][2], their maxima and sums
   float* row_ml;   // [batch, q_heads][2], with weights: of rows that one workgroup had
   float* logits;   // [batch, q_heads, logit_stride], with weights
   int64_t logit_stride;

@@ -4,9 +4,9 @@
 // Bound by memory: each key and value is read once for the (up to 16) query rows of its
 // head -- the heads of its group times the new tokens -- so 2 rows flops a byte in 16 bits.  4 x 4 heads of
 // 128 over 32768 to 131072 tokens, bf16: 782 MB in 135 us (5.8 TB/s; 6.2 without the ramp of the first tiles).  Rows
-// above 16 read it again, from L2, at what a CU takes (48 bytes a ns): 128 rows of a head over 4096 tokens,
-// 32 heads of 64, 33 us where 16 rows take 15.  Two and four blocks of rows in one workgroup were no faster (36 and
-// 38): what is saved in loads is waited for in one wave's chain of products and exponentials.
+// above 16 read it again, from L2, at what a CU takes (48 bytes a ns), but where that is much two blocks of 16 share a
+// workgroup's tiles: 128 rows of 16 x 2 heads of 64 over 4096 to 8192 tokens 53 -> 40 us, against 17 for 8 rows.  Four blocks
+// were no faster: what is saved in loads is waited for in one wave's chain of products and exponentials.
 //
 // Products.  Query rows are columns of 16 x 16 matrix-core tiles: S^T = K Q^T with a tile's
 // tokens as rows, then O^T = V^T P^T.  Lane l holds column l % 16 of both, so a row's maximum,
@@ -36,7 +36,6 @@
 
 namespace attnres {
 
-constexpr int kAttRows = 16;  // query rows of a workgroup
 constexpr int kAttWaves = 4;
 
 // The deal: `segs` segments (heads, blocks of rows) of each sequence, kAttUnit tokens a unit, unit x to
@@ -127,8 +126,8 @@ typedef _Float16 att_h4 __attribute__((ext_vector_type(4)));
 
 // HD: head width's tile (64, 128, 256); VB: bytes that every row starts and ends at a multiple of, and that one load
 // takes (16, or 8, 4, 2); PAGE16 (VB 16): pages of a multiple of 16 tokens, so that 16 tokens lie in one and the
-// scalar unit finds it.
-template <class DT, int HD, int VB, bool PAGE16>
+// scalar unit finds it.  RB: blocks of 16 query rows that a workgroup has.
+template <class DT, int HD, int VB, bool PAGE16, int RB>
 struct Att {
   using S = typename DT::S;
   static constexpr int kSize = sizeof(S);
@@ -148,17 +147,17 @@ struct Att {
   static constexpr int kStep = kAttWaves * kTok;               // tokens of a workgroup's round
 
   const CacheAttendParams& p;
-  int lane, wave, c, g;          // column (query row) and token group of the lane
+  int lane, wave, c, g;          // column (query row of each block) and token group of the lane
   int b, h, n, have;
   int t_lo, t_hi;                // new tokens of the rows
   int kcol[kKs], vcol0;          // first value of each key chunk; of the first value chunk
   uint32_t kofs[kKs], vofs[4][kNi]; // PAGE16: bytes from a subtile's first row
   const S *kh, *vh;              // of the head, page 0
   att_const_i32* table;          // of the sequence
-  u32x4 q[kKs], k[kSub][kKs];
+  u32x4 q[RB][kKs], k[kSub][kKs];
   uint32_t v[kSub][4][kNi][kWords];
-  sw_f4 acc[kNi][kW];
-  float m, l;                    // of the lane's row: maximum of <q, k>, the lane's part of the sum
+  sw_f4 acc[RB][kNi][kW];
+  float m[RB], l[RB];            // of the lane's rows: maximum of <q, k>, the lane's part of the sum
   float low;                     // the exponents' base is further up by it: kCare after a careful pass
 
   struct Rows {
@@ -339,21 +338,23 @@ struct Att {
     constexpr uint32_t kExp = DT::kCode == 1 ? 0x7f80u : 0x7c00u;
     return ((w & kExp) == kExp ? 0 : w & 0xffffu) | ((w >> 16 & kExp) == kExp ? 0 : w & 0xffff0000u);
   }
-  // O^T += V^T P^T over a tile, value d of chunk i of the lanes' columns.  CARE: an infinite value times the second
-  // term, which may have the other sign, is left out.
+  // O^T += V^T P^T over a tile, value d of chunk i of the lanes' columns.  CARE: values of the lane's
+  // tokens behind its `last` (16 s + t) count as 0, and an infinite value times the second term, which may have the
+  // other sign, is left out.
   template <bool CARE>
-  __device__ __forceinline__ sw_f4 weigh(const Weights& p, int i, int d, sw_f4 to) const {
+  __device__ __forceinline__ sw_f4 weigh(const Weights& p, int i, int d, sw_f4 to, int last = 0) const {
     if constexpr (k32) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        to = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[0][t][i][d]), p.e[0][t], to, 0, 0, 0);
+        to = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(CARE && t > last ? 0 : v[0][t][i][d]), p.e[0][t], to, 0, 0, 0);
     } else {
       u32x4 a;
 #pragma unroll
       for (int s = 0; s < kSub; ++s)
 #pragma unroll
         for (int t = 0; t < 4; t += 2) {
-          const uint32_t x = v[s][t][i][d / 2], y = v[s][t + 1][i][d / 2];
+          const uint32_t x = CARE && 16 * s + t > last ? 0 : v[s][t][i][d / 2];
+          const uint32_t y = CARE && 16 * s + t + 1 > last ? 0 : v[s][t + 1][i][d / 2];
           a[s * 2 + t / 2] = d % 2 ? hi_pair(x, y) : lo_pair(x, y);
         }
       u32x4 a2 = a;
@@ -384,7 +385,7 @@ struct Att {
   // a maximum as the exponents' base; of no score at all: 0, so that -inf less it stays -inf
   __device__ __forceinline__ float base_of(float top) const { return top == -INFINITY ? 0.f : top * p.scale - kShift + low; }
 
-  struct Row {       // the lane's
+  struct Row {       // one of the lane's
     float* logits;   // of token 0, or null
     int lim;         // tokens that it sees (one that is not there: whatever)
     int t;           // its new token
@@ -395,7 +396,7 @@ struct Att {
   // each wait one for all loads).  CARE: a value that is not finite shows in the rows that see it and in no other, and
   // weights 2^31 times smaller keep sums of the largest values finite.
   template <bool AHEAD, bool CARE>
-  __device__ __forceinline__ void tile(int t0, const Row& row, Rows& now, Rows& next) {
+  __device__ __forceinline__ void tile(int t0, const Row (&row)[RB], Rows& now, Rows& next) {
     constexpr bool CUT = !AHEAD;
     Rows after;
     if constexpr (AHEAD) after = rows_of(min(t0 + 2 * kStep, (n - 1) & -kTok), n);
@@ -409,54 +410,61 @@ struct Att {
           else if (kcol[i] >= p.c.head_dim) k[s][i] = u32x4{0, 0, 0, 0};
         }
     }
-    sw_f4 s4[kSub];
+    sw_f4 s4[RB][kSub];
 #pragma unroll
-    for (int s = 0; s < kSub; ++s) {
-      s4[s] = sw_f4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
-      for (int i = 0; i < kKs; ++i) sw_mfma<DT>(k[s][i], q[i], s4[s]);
-    }
+      for (int s = 0; s < kSub; ++s) {
+        s4[r][s] = sw_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kKs; ++i) sw_mfma<DT>(k[s][i], q[r][i], s4[r][s]);
+      }
     float scale[kSub];  // NaN where there is no page: the row shows it
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
       scale[s] = PAGE16 && !now.there[s] && (!CUT || t0 + 16 * s < n) ? __builtin_nanf("") : p.scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if (!PAGE16 && (unsigned)__shfl(now.page, 16 * s + g * 4 + t, kWave) >= (unsigned)p.c.pages) s4[s][t] = __builtin_nanf("");
-        if (CUT && t0 + 16 * s + g * 4 + t >= row.lim) s4[s][t] = -INFINITY;
+        const bool gone = !PAGE16 && (unsigned)__shfl(now.page, 16 * s + g * 4 + t, kWave) >= (unsigned)p.c.pages;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          if (!PAGE16 && gone) s4[r][s][t] = __builtin_nanf("");
+          if (CUT && t0 + 16 * s + g * 4 + t >= row[r].lim) s4[r][s][t] = -INFINITY;
+        }
       }
     }
     if constexpr (AHEAD) load_k(next);
-    if (row.logits) {
 #pragma unroll
-      for (int s = 0; s < kSub; ++s) *(sw_f4*)(row.logits + t0 + 16 * s + g * 4) = s4[s] * scale[s];
-    }
-    float top = s4[0][0];
+    for (int r = 0; r < RB; ++r)
+      if (row[r].logits) {
 #pragma unroll
-    for (int s = 0; s < kSub; ++s)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) top = fmaxf(top, s4[s][t]);
-    top = across(top, [](float a, float b) { return fmaxf(a, b); });
-    const float to = fmaxf(m, top);
-    if (__any(to != m)) {
-      const float was = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base_of(m) - base_of(to));
-      l *= was;
-#pragma unroll
-      for (int i = 0; i < kNi; ++i)
-#pragma unroll
-        for (int d = 0; d < kW; ++d) acc[i][d] *= was;
-      m = to;
-    }
-    const float base = base_of(to);
-    float e[kSub][4];
-#pragma unroll
-    for (int s = 0; s < kSub; ++s)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        e[s][t] = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[s][t], scale[s], -base));
-        l += e[s][t];
+        for (int s = 0; s < kSub; ++s) *(sw_f4*)(row[r].logits + t0 + 16 * s + g * 4) = s4[r][s] * scale[s];
       }
-    const Weights w = split(e);
+    float to[RB];
+    bool higher = false;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      float top = s4[r][0][0];
+#pragma unroll
+      for (int s = 0; s < kSub; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) top = fmaxf(top, s4[r][s][t]);
+      top = across(top, [](float a, float b) { return fmaxf(a, b); });
+      to[r] = fmaxf(m[r], top);
+      higher |= to[r] != m[r];
+    }
+    if (__any(higher)) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const float was = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base_of(m[r]) - base_of(to[r]));
+        l[r] *= was;
+#pragma unroll
+        for (int i = 0; i < kNi; ++i)
+#pragma unroll
+          for (int d = 0; d < kW; ++d) acc[r][i][d] *= was;
+        m[r] = to[r];
+      }
+    }
     if constexpr (CUT) {  // what lies behind the last token may be anything
 #pragma unroll
       for (int s = 0; s < kSub; ++s)
@@ -469,11 +477,28 @@ struct Att {
               for (int y = 0; y < kWords; ++y) v[s][t][i][y] = 0;
           }
     }
+    const auto weights = [&](int r) {
+      const float base = base_of(to[r]);
+      float e[kSub][4];
+#pragma unroll
+      for (int s = 0; s < kSub; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          e[s][t] = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[r][s][t], scale[s], -base));
+          l[r] += e[s][t];
+        }
+      return split(e);
+    };
     if constexpr (!CARE) {
+      Weights w[RB];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) w[r] = weights(r);
 #pragma unroll
       for (int i = 0; i < kNi; ++i)
 #pragma unroll
-        for (int d = 0; d < kW; ++d) acc[i][d] = weigh<false>(w, i, d, acc[i][d]);
+        for (int d = 0; d < kW; ++d)
+#pragma unroll
+          for (int r = 0; r < RB; ++r) acc[r][i][d] = weigh<false>(w[r], i, d, acc[r][i][d]);
       if constexpr (AHEAD) {
         load_v(next);
         now = next;
@@ -481,70 +506,77 @@ struct Att {
       }
     } else {
       // (0 times such a value is NaN: each new token's rows take a product without the values behind it)
-      for (int tt = t_hi; tt >= t_lo; --tt) {
 #pragma unroll
-        for (int s = 0; s < kSub; ++s)
+      for (int r = 0; r < RB; ++r) {
+        const Weights w = weights(r);
+        for (int tt = t_lo; tt <= t_hi; ++tt) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (t0 + 16 * s + g * 4 + t > have + tt) {
+          for (int i = 0; i < kNi; ++i)
 #pragma unroll
-              for (int i = 0; i < kNi; ++i)
+            for (int d = 0; d < kW; ++d) {
+              const sw_f4 with = weigh<true>(w, i, d, acc[r][i][d], have + tt - t0 - g * 4);
 #pragma unroll
-                for (int y = 0; y < kWords; ++y) v[s][t][i][y] = 0;
+              for (int t = 0; t < 4; ++t) acc[r][i][d][t] = row[r].t == tt ? with[t] : acc[r][i][d][t];
             }
-#pragma unroll
-        for (int i = 0; i < kNi; ++i)
-#pragma unroll
-          for (int d = 0; d < kW; ++d) {
-            const sw_f4 with = weigh<true>(w, i, d, acc[i][d]);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) acc[i][d][t] = row.t == tt ? with[t] : acc[i][d][t];
-          }
-        att_settle();
+          att_settle();
+        }
       }
     }
   }
 
   __device__ __forceinline__ void clear() {
-    m = -INFINITY;
-    l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kNi; ++i)
+    for (int r = 0; r < RB; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
 #pragma unroll
-      for (int d = 0; d < kW; ++d) acc[i][d] = sw_f4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < kNi; ++i)
+#pragma unroll
+        for (int d = 0; d < kW; ++d) acc[r][i][d] = sw_f4{0.f, 0.f, 0.f, 0.f};
+    }
   }
 
   // tokens [first, end) of the head for rows [row0, row0 + rows), of those that there are (all of them, where a workgroup
   // takes a whole segment); this wave's: tiles wave, wave + 4, ...  stage: 16 rows of LDS that nobody uses.
   __device__ __forceinline__ void piece(int row0, int rows, int first, int end, Seq seq, void* stage) {
-    const int r = row0 + c, t_row = div_by(r, p.by_group);
-    const bool valid = c < rows;
-    const int hq = h * p.group + r - t_row * p.group;
     table = (att_const_i32*)(uintptr_t)(p.c.table + b * p.c.table_stride);
     kh = (const S*)p.c.k + h * p.c.head_stride;
     vh = (const S*)p.c.v + h * p.c.head_stride;
+    int t_row[RB], hq[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int qr = row0 + 16 * r + c;
+      t_row[r] = div_by(qr, p.by_group);
+      hq[r] = h * p.group + qr - t_row[r] * p.group;
+    }
     // (before the tiles' loads: a wait for what came last waits for all of them, in every turn of the loop)
     if (VEC && p.q_vec) {
-      const S* src = (const S*)p.q + b * p.q_b_stride + hq * p.q_h_stride + t_row * p.q_t_stride;
 #pragma unroll
-      for (int i = 0; i < kKs; ++i) {
-        q[i] = u32x4{0, 0, 0, 0};
-        if (valid && kcol[i] < p.c.head_dim) q[i] = *(const u32x4*)(src + kcol[i]);
+      for (int r = 0; r < RB; ++r) {
+        const S* src = (const S*)p.q + b * p.q_b_stride + hq[r] * p.q_h_stride + t_row[r] * p.q_t_stride;
+#pragma unroll
+        for (int i = 0; i < kKs; ++i) {
+          q[r][i] = u32x4{0, 0, 0, 0};
+          if (16 * r + c < rows && kcol[i] < p.c.head_dim) q[r][i] = *(const u32x4*)(src + kcol[i]);
+        }
       }
     } else {  // (by single values, in few registers)
       S* const rows_q = (S*)stage;
-#pragma unroll 1
-      for (int i = threadIdx.x; i < kAttRows * HD; i += kAttWaves * kWave) {
-        const int qr = row0 + i / HD, col = i % HD, t = div_by(qr, p.by_group);
-        rows_q[i] = i / HD < rows && col < p.c.head_dim
-                        ? ((const S*)p.q)[b * p.q_b_stride + (h * p.group + qr - t * p.group) * p.q_h_stride +
-                                          t * p.q_t_stride + col]
-                        : (S)0;
-      }
-      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kKs; ++i) q[i] = *(const u32x4*)(rows_q + c * HD + kcol[i]);
-      __syncthreads();
+      for (int r = 0; r < RB; ++r) {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < 16 * HD; i += kAttWaves * kWave) {
+          const int at = 16 * r + i / HD, col = i % HD, t = div_by(row0 + at, p.by_group);
+          rows_q[i] = at < rows && col < p.c.head_dim
+                          ? ((const S*)p.q)[b * p.q_b_stride + (h * p.group + row0 + at - t * p.group) * p.q_h_stride +
+                                            t * p.q_t_stride + col]
+                          : (S)0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kKs; ++i) q[r][i] = *(const u32x4*)(rows_q + c * HD + kcol[i]);
+        __syncthreads();
+      }
     }
     // (the first tile's loads wait for the block table alone where the length is not known yet)
     const int t_first = first + wave * kTok, limit = p.direct ? p.c.room : seq.n;
@@ -560,7 +592,9 @@ struct Att {
     next = rows_of(min(t_first + kStep, (limit - 1) & -kTok), limit);
     if (p.negate) {
 #pragma unroll
-      for (int i = 0; i < kKs; ++i) q[i] ^= k32 ? 0x80000000u : 0x80008000u;
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i = 0; i < kKs; ++i) q[r][i] ^= k32 ? 0x80000000u : 0x80008000u;
     }
     clear();
     low = 0.f;
@@ -569,11 +603,14 @@ struct Att {
     t_lo = div_by(row0, p.by_group);
     t_hi = div_by(row0 + rows - 1, p.by_group);
     end = min(end, min(have + t_hi + 1, n));  // (behind it no row sees any)
+    const int all = have + t_lo + 1;          // tokens that every row sees
     if (t_first >= end) return;
-    const int lim = min(have + t_row + 1, n);  // of the lane's row (a row that is not there: whatever)
-    const int all = have + t_lo + 1;               // tokens that every row sees
     int t0 = t_first;
-    const Row row{p.logits && valid ? p.logits + (b * (int64_t)p.q_heads + hq) * p.logit_stride : nullptr, lim, t_row};
+    Row row[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+      row[r] = Row{p.logits && 16 * r + c < rows ? p.logits + (b * (int64_t)p.q_heads + hq[r]) * p.logit_stride : nullptr,
+                   min(have + t_row[r] + 1, n), t_row[r]};
     for (; t0 + kStep < end && t0 + kTok <= all; t0 += kStep) tile<true, false>(t0, row, now, next);
     // the last tile, and those that a row does not see all of: never many
     for (;;) {
@@ -587,11 +624,13 @@ struct Att {
     att_settle();
     float none = 0.f;
 #pragma unroll
-    for (int i = 0; i < kNi; ++i)
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
-      for (int d = 0; d < kW; ++d)
+      for (int i = 0; i < kNi; ++i)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) none = __builtin_fmaf(acc[i][d][t], 0.f, none);
+        for (int d = 0; d < kW; ++d)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) none = __builtin_fmaf(acc[r][i][d][t], 0.f, none);
     if (__any(none != 0.f)) {  // NaN: something was not finite
       clear();
       low = kCare;
@@ -602,7 +641,8 @@ struct Att {
         tile<false, true>(t0, row, now, now);
       }
     }
-    l = across(l, [](float a, float b) { return a + b; });
+#pragma unroll
+    for (int r = 0; r < RB; ++r) l[r] = across(l[r], [](float a, float b) { return a + b; });
   }
 };
 
@@ -648,13 +688,14 @@ __device__ __forceinline__ void add_own_weights(const CacheAttendParams& p, int 
   }
 }
 
-template <class DT, int HD, int VB, bool PAGE16>
-__global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_attend_kernel(CacheAttendParams p) {
-  using A = Att<DT, HD, VB, PAGE16>;
+template <class DT, int HD, int VB, bool PAGE16, int RB>
+__global__ __launch_bounds__(kAttWaves* kWave, HD == 256 || RB * HD > 128 ? 1 : 2) void cache_attend_kernel(CacheAttendParams p) {
+  using A = Att<DT, HD, VB, PAGE16, RB>;
   using S = typename DT::S;
-  __shared__ float so[kAttWaves][kAttRows][A::kPitch];
-  __shared__ float sm[kAttWaves][kAttRows], sl[kAttWaves][kAttRows];
-  __shared__ float lse[kAttRows];
+  constexpr int kRows = 16 * RB;
+  __shared__ float so[kAttWaves][16][A::kPitch];  // a block of rows after the other
+  __shared__ float sm[kAttWaves][kRows], sl[kAttWaves][kRows];
+  __shared__ float lse[kRows];
   A a(p);
   const int Dh = p.c.head_dim, segs = p.c.kv_heads * p.blocks;
   // neighbouring workgroups run on different XCDs; those of one XCD take neighbouring units
@@ -681,54 +722,61 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 ? 1 : 2) void cache_att
     const int seg = (x - b_start) / units, u0 = x - b_start - seg * units, u1 = min(units, u0 + x1 - x);
     x += u1 - u0;
     a.h = div_by(seg, p.by_blocks);
-    const int row0 = (seg - a.h * p.blocks) * kAttRows, rows = min(kAttRows, p.rows - row0);
+    const int row0 = (seg - a.h * p.blocks) * kRows, rows = min(kRows, p.rows - row0);
     const bool whole = u0 == 0 && u1 == units;
     a.piece(row0, rows, u0 * kAttUnit, p.direct ? p.c.room : u1 * kAttUnit, seq, so);
-    if (a.n > 0 && a.c < rows) {
-      if (a.g == 0) sm[a.wave][a.c] = a.m == -INFINITY ? a.m : a.base_of(a.m), sl[a.wave][a.c] = a.l;
-#pragma unroll
-      for (int i = 0; i < A::kNi; ++i)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < A::kW; e += 4)
-            *(sw_f4*)&so[a.wave][a.c][(i * 16 + a.g * 4 + t) * A::kW + e] =
-                sw_f4{a.acc[i][e][t], a.acc[i][e + 1][t], a.acc[i][e + 2][t], a.acc[i][e + 3][t]};
-    }
-    __syncthreads();
     const int64_t slot = 2 * w + (u0 == 0 ? 1 : 0);
-    for (int at = threadIdx.x; at < rows * (HD / 4); at += kAttWaves * kWave) {
-      const int r = at / (HD / 4), col = at % (HD / 4) * 4;
-      float top = -INFINITY, l = 0.f;
-      sw_f4 o = {0.f, 0.f, 0.f, 0.f};
-      if (a.n > 0) {
 #pragma unroll
-        for (int i = 0; i < kAttWaves; ++i) top = fmaxf(top, sm[i][r]);
-#pragma unroll
-        for (int i = 0; i < kAttWaves; ++i) l += att_share(sm[i][r], top) * sl[i][r];
-        // (shares of the whole sum first: sums of the largest values would not be finite)
-        const float inv = l == 0.f && !whole ? 0.f : 1.f / l;  // (a piece that a row sees nothing of)
-#pragma unroll
-        for (int i = 0; i < kAttWaves; ++i) o += att_share(sm[i][r], top) * inv * *(const sw_f4*)&so[i][r][col];
-      }
-      if (whole) {
-        att_row_out<DT>(p, a.b, a.h, row0 + r, col, a.n, o);
-        if (p.own_weights) {
-          if (col == 0) lse[r] = top + log2f(l);
-        } else if (p.row_ml && col == 0) {
-          float* ml = p.row_ml + (a.b * (int64_t)p.q_heads + a.h * p.group + row0 + r) * 2;
-          ml[0] = top;
-          ml[1] = l;
+    for (int rb = 0; rb < RB; ++rb) {
+      if (rb * 16 >= rows) break;
+      if (a.n > 0 && rb * 16 + a.c < rows) {
+        if (a.g == 0) {
+          sm[a.wave][rb * 16 + a.c] = a.m[rb] == -INFINITY ? a.m[rb] : a.base_of(a.m[rb]);
+          sl[a.wave][rb * 16 + a.c] = a.l[rb];
         }
-      } else {
-        *(sw_f4*)(p.part + (slot * kAttRows + r) * HD + col) = o;
-        if (col == 0) {
-          p.part_ml[(slot * kAttRows + r) * 2] = top;
-          p.part_ml[(slot * kAttRows + r) * 2 + 1] = l;
+#pragma unroll
+        for (int i = 0; i < A::kNi; ++i)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < A::kW; e += 4)
+              *(sw_f4*)&so[a.wave][a.c][(i * 16 + a.g * 4 + t) * A::kW + e] =
+                  sw_f4{a.acc[rb][i][e][t], a.acc[rb][i][e + 1][t], a.acc[rb][i][e + 2][t], a.acc[rb][i][e + 3][t]};
+      }
+      __syncthreads();
+      for (int at = threadIdx.x; at < min(16, rows - rb * 16) * (HD / 4); at += kAttWaves * kWave) {
+        const int in = at / (HD / 4), r = rb * 16 + in, col = at % (HD / 4) * 4;
+        float top = -INFINITY, l = 0.f;
+        sw_f4 o = {0.f, 0.f, 0.f, 0.f};
+        if (a.n > 0) {
+#pragma unroll
+          for (int i = 0; i < kAttWaves; ++i) top = fmaxf(top, sm[i][r]);
+#pragma unroll
+          for (int i = 0; i < kAttWaves; ++i) l += att_share(sm[i][r], top) * sl[i][r];
+          // (shares of the whole sum first: sums of the largest values would not be finite)
+          const float inv = l == 0.f && !whole ? 0.f : 1.f / l;  // (a piece that a row sees nothing of)
+#pragma unroll
+          for (int i = 0; i < kAttWaves; ++i) o += att_share(sm[i][r], top) * inv * *(const sw_f4*)&so[i][in][col];
+        }
+        if (whole) {
+          att_row_out<DT>(p, a.b, a.h, row0 + r, col, a.n, o);
+          if (p.own_weights) {
+            if (col == 0) lse[r] = top + log2f(l);
+          } else if (p.row_ml && col == 0) {
+            float* ml = p.row_ml + (a.b * (int64_t)p.q_heads + a.h * p.group + row0 + r) * 2;
+            ml[0] = top;
+            ml[1] = l;
+          }
+        } else {
+          *(sw_f4*)(p.part + (slot * kRows + r) * HD + col) = o;
+          if (col == 0) {
+            p.part_ml[(slot * kRows + r) * 2] = top;
+            p.part_ml[(slot * kRows + r) * 2 + 1] = l;
+          }
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
     if (p.own_weights) add_own_weights(p, a.b, a.h, rows, a.n, lse);
   }
 }
@@ -742,8 +790,8 @@ __device__ __forceinline__ Pieces pieces_of(const CacheAttendParams& p, const De
   if (p.direct) return Pieces{0, 0};
   return Pieces{deal_of(d, first), deal_of(d, first + units - 1)};
 }
-__device__ __forceinline__ int64_t piece_row(const Pieces& s, int w, int row) {
-  return (2 * w + (w == s.w0 ? 1 : 0)) * (int64_t)kAttRows + row % kAttRows;
+__device__ __forceinline__ int64_t piece_row(const CacheAttendParams& p, const Pieces& s, int w, int row) {
+  return ((int64_t)(2 * w + (w == s.w0 ? 1 : 0)) << p.row_bits) + (row & ((1 << p.row_bits) - 1));
 }
 
 // A head's pieces joined; zeros for rows that see nothing, NaN for counts that cannot be.  A workgroup for each
@@ -764,7 +812,7 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
   Pieces s{0, -1};
   if (units)
     s = pieces_of(p, d, (__builtin_amdgcn_readlane(seqs.upto, b - seqs.b0) - units) * segs +
-                            (h * p.blocks + row / kAttRows) * units, units);
+                            (h * p.blocks + (row >> p.row_bits)) * units, units);
   if (s.w0 == s.w1) return;  // one workgroup had all of it
   constexpr int kItems = HD / 4, kShares = 256 / kItems, kBatch = 4;
   const int item = threadIdx.x % kItems, share = threadIdx.x / kItems, col = item * 4;
@@ -775,7 +823,7 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
     sw_f4 x[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int64_t r = piece_row(s, min(w + i * kShares, s.w1), row);
+      const int64_t r = piece_row(p, s, min(w + i * kShares, s.w1), row);
       m[i] = p.part_ml[r * 2];
       part[i] = p.part_ml[r * 2 + 1];
       x[i] = *(const sw_f4*)(p.part + r * HD + col);
@@ -844,14 +892,14 @@ __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) 
       __syncthreads();
       for (int r = wave; r < rows; r += 256 / kWave) {
         const int row = g0 + r;
-        const Pieces s = pieces_of(p, of, b_start * p.blocks + (h * p.blocks + row / kAttRows) * units, units);
+        const Pieces s = pieces_of(p, of, b_start * p.blocks + (h * p.blocks + (row >> p.row_bits)) * units, units);
         float top = -INFINITY, l = 0.f;
         if (s.w0 == s.w1) {
           top = p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2];
           l = lane ? 0.f : p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2 + 1];
         }
         for (int w = s.w0 + lane; w <= s.w1 && s.w0 != s.w1; w += kWave) {
-          const int64_t i = piece_row(s, w, row);
+          const int64_t i = piece_row(p, s, w, row);
           const float m = p.part_ml[i * 2], to = fmaxf(top, m);
           l = att_share(top, to) * l + att_share(m, to) * p.part_ml[i * 2 + 1];
           top = to;
@@ -884,11 +932,12 @@ template <class DT, int HD>
 hipError_t run_attend(const CacheAttendParams& p, hipStream_t st) {
   const int64_t segs = (int64_t)p.c.batch * p.c.kv_heads * p.blocks;
   const dim3 grid((unsigned)(p.direct ? segs : p.wgs)), wg(kAttWaves * kWave);
-  if (p.vb == 16 && p.page16) cache_attend_kernel<DT, HD, 16, true><<<grid, wg, 0, st>>>(p);
-  else if (p.vb == 16) cache_attend_kernel<DT, HD, 16, false><<<grid, wg, 0, st>>>(p);
-  else if (p.vb == 8) cache_attend_kernel<DT, HD, 8, false><<<grid, wg, 0, st>>>(p);
-  else if (p.vb == 4) cache_attend_kernel<DT, HD, 4, false><<<grid, wg, 0, st>>>(p);
-  else if constexpr (DT::kCode != 0) cache_attend_kernel<DT, HD, 2, false><<<grid, wg, 0, st>>>(p);
+  if (p.row_bits == 5) cache_attend_kernel<DT, HD, 16, true, 2><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 16 && p.page16) cache_attend_kernel<DT, HD, 16, true, 1><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 16) cache_attend_kernel<DT, HD, 16, false, 1><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 8) cache_attend_kernel<DT, HD, 8, false, 1><<<grid, wg, 0, st>>>(p);
+  else if (p.vb == 4) cache_attend_kernel<DT, HD, 4, false, 1><<<grid, wg, 0, st>>>(p);
+  else if constexpr (DT::kCode != 0) cache_attend_kernel<DT, HD, 2, false, 1><<<grid, wg, 0, st>>>(p);
   const hipError_t err = hipGetLastError();
   const int joins = p.direct ? 0 : p.c.batch * p.c.kv_heads * p.rows;
   if (err != hipSuccess || joins + p.weight_wgs == 0) return err;

@@ -175,22 +175,29 @@ namespace {
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct AttendPlan {
-  int tile, rows, blocks, wgs, direct, page16;
+  int tile, rows, blocks, row_bits, wgs, direct, page16;
   int64_t logit_stride;
   size_t part, part_ml, row_ml, logits, need;  // offsets in the workspace, and its size
 };
 
 int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d, AttendPlan* a) {
-  const int64_t rows = d->q_heads / c->kv_heads * d->tokens, blocks = (rows + 15) / 16;
+  const int es = es_of(c->dtype);
+  const int64_t rows = d->q_heads / c->kv_heads * d->tokens, heads = c->batch * c->kv_heads;
   const int64_t room = c->table_pages * c->page_size, units = (room + kAttUnit - 1) / kAttUnit;
-  const int64_t segs = c->batch * c->kv_heads * blocks;
+  const double room_bytes = 2.0 * room * c->head_dim * es;
+  // (pages, and tokens inside one, within 32-bit offsets of each other)
+  constexpr int64_t kFar = (int64_t)1 << 32;
+  a->page16 = row_bytes(c) == 16 && c->page_size % 16 == 0 && c->page_stride < kFar / es && c->slot_stride < kFar / es / c->page_size;
+  // Each block of rows reads its head's tokens, from L2 after the first.  Blocks of 32 halve that and take longer to
+  // start, so they are for many bytes (us, 16 rows / 32: 16 x 2 heads of up to 8192 x 64 bf16, 128 rows 53 / 40, 32 rows 21.7 / 20.4;
+  // x 128 92 / 67; 28 x 14 heads of up to 1337 x 64, 56 rows 39.6 / 27.7; 4 x 4 heads of up to 4096 x 64, 2048 rows 237 / 170.  Of fewer:
+  // 4 x 2 heads of up to 4096 x 128, 128 rows 22.3 / 25.3; 8 x 2 of 400, 9.6 / 13.6.  In pages of 11 tokens 47.6 / 46.1 and 72 / 95.)
+  const int64_t blocks16 = (rows + 15) / 16;
+  a->row_bits = a->page16 && blocks16 > 1 && heads * blocks16 * room_bytes >= 256 << 20 ? 5 : 4;
+  const int64_t blocks = (rows + (1 << a->row_bits) - 1) >> a->row_bits, segs = heads * blocks;
   if (rows > INT32_MAX || segs > (1 << 23) || segs * (units > 0 ? units : 1) > INT32_MAX / 2)
     return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d, %lld cached: too many tokens", (long long)c->batch,
                     (long long)d->tokens, d->q_heads, (long long)room);
-  // (pages, and tokens inside one, within 32-bit offsets of each other)
-  constexpr int64_t kFar = (int64_t)1 << 32;
-  a->page16 = row_bytes(c) == 16 && c->page_size % 16 == 0 && c->page_stride < kFar / es_of(c->dtype) &&
-              c->slot_stride < kFar / es_of(c->dtype) / c->page_size;
   a->tile = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
   a->rows = (int)rows;
   a->blocks = (int)blocks;
@@ -204,8 +211,7 @@ int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d,
   // 64 bf16 15.4 / 14 + 4; 12 heads of 300 5.6 / 6.8 + 4; 32 segments of up to 4096 25 / 9.4 + 4; 64 of up to 8192 x 128 fp16 100 / 48
   // + 5; 15 heads of up to 700 x 40 fp32 15.5 / 10.3 + 4.)  Lengths are on the device alone, so longer tables are split though they
   // may be nearly empty, and one long sequence among short ones is shared.
-  const int es = es_of(c->dtype);
-  const double room_bytes = 2.0 * room * c->head_dim * es, rounds = (double)room / (es == 4 || a->tile == 256 ? 64 : 128);
+  const double rounds = (double)room / (es == 4 || a->tile == 256 ? 64 : 128);
   const double round_ns = a->page16 ? 650 : 1100;
   const double piece_ns = rounds * round_ns > room_bytes / 48 ? rounds * round_ns : room_bytes / 48;
   a->direct = c->pages > 0 && room_bytes <= 1 << 20 && piece_ns - segs * room_bytes / 11000.0 <= 6000;
@@ -213,9 +219,9 @@ int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d,
   a->logit_stride = (room + 31) / 32 * 32;
   size_t at = 0;
   a->part = at;
-  at += up256((size_t)2 * a->wgs * 16 * a->tile * 4);
+  at += up256(((size_t)2 * a->wgs << a->row_bits) * a->tile * 4);
   a->part_ml = at;
-  at += up256((size_t)2 * a->wgs * 16 * 2 * 4);
+  at += up256(((size_t)2 * a->wgs << a->row_bits) * 2 * 4);
   a->row_ml = at;
   if (c->weights) at += up256((size_t)c->batch * d->q_heads * 2 * 4);
   a->logits = at;
@@ -266,6 +272,7 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
     p.by_weight_wgs = fast_div(p.weight_wgs);
   }
   p.tile = a.tile;
+  p.row_bits = a.row_bits;
   p.vb = row_bytes(c);
   p.page16 = a.page16;
   p.whole = c->head_dim == a.tile;

@@ -210,6 +210,65 @@ def test_received_weights_of_many_heads_tokens_and_sequences(dtype, H, K, Dh, S,
     test_received_weights(dtype, H, K, Dh, S, cached, 0.5)
 
 
+def widen(c, rows):
+    """Columns of the table that no token is in, as many as make it a call of many bytes: blocks of 32 rows."""
+    columns = -(-(256 << 20) // (c.B * c.K * -(-rows // 16) * 2 * c.Dh * c.k.element_size() * c.S)) + 1
+    more = torch.full((c.B, max(0, columns - c.table.size(1))), -7, dtype=torch.int32, device=DEV)
+    c.table = torch.cat([c.table, more], 1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,H,K,Dh,S", [(5, 8, 2, 64, 64), (17, 1, 1, 128, 16), (9, 8, 2, 128, 32), (6, 6, 1, 256, 64), (40, 2, 2, 48, 16),
+                                        (3, 44, 2, 80, 128), (2, 20, 1, 200, 32)])
+def test_blocks_of_many_rows(dtype, T, H, K, Dh, S):
+    cached = [0, 1, 30, 127, 128, 333, 900]
+    fresh = [T, T, T - 1, 0, T, T, 1]
+    c, q, _ = build(T * Dh, dtype, H, K, Dh, S, cached, T=T, fresh=fresh)
+    widen(c, T * (H // K))
+    check(c, q, cached, fresh, pass_fresh=True)
+    check(c, q.flip(-1), cached, fresh, pass_fresh=True, scale=-0.4)
+
+
+@pytest.mark.parametrize("T", [17, 40])
+def test_what_is_not_finite_in_blocks_of_many_rows(T):
+    cached = [70, 300]
+    c, q, fresh = build(T, "bf16", 4, 2, 64, 16, cached, T=T)
+    for b, n in enumerate(cached):
+        page, slot = c.where(b, n + T)
+        for bad in (0, 9, T - 2):
+            c.v[page[n + bad], 0, slot[n + bad], bad] = -float("inf")
+            c.v[page[n + bad], 1, slot[n + bad], bad] = torch.finfo(torch.bfloat16).max
+    widen(c, 2 * T)
+    c.table[0, (70 + T) // 16 + 1:] = 10 ** 9
+    o = ops.cached_attention(q, c.k, c.v, c.table, c.cached)
+    e, bound, _ = attend_ref(c, q, cached, fresh, 64 ** -0.5)
+    fine = torch.isfinite(e)
+    assert torch.equal(torch.isfinite(o), fine) and bool((o[~fine] == -math.inf).all())
+    assert_within(o[fine], e[fine], bound[fine], "finite")
+    c.table[1, 2] = -1
+    o2 = ops.cached_attention(q, c.k, c.v, c.table, c.cached)
+    assert torch.equal(o2[0], o[0]) and bool(o2[1].isnan().all())
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.75])
+@pytest.mark.parametrize("dtype,H,K,Dh,S,cached", [("bf16", 40, 2, 64, 16, [300, 31, 1000]), ("fp32", 33, 1, 128, 32, [0, 500])])
+def test_received_weights_of_blocks_of_many_rows(dtype, H, K, Dh, S, cached, decay):
+    c, q, fresh = build(9, dtype, H, K, Dh, S, cached, weights=True)
+    if decay == 0.0:
+        c.w.fill_(float("nan"))
+    before = c.w.clone()
+    widen(c, H // K)
+    _, ps = check(c, q, cached, fresh, weights=c.w, decay=decay)
+    for b, n in enumerate(cached):
+        page, slot = c.where(b, n + 1)
+        for h in range(K):
+            rows = [ps[b, i, 0] for i in range(h * (H // K), (h + 1) * (H // K))]
+            got, old = sum(p for p, _ in rows), before[page, h, slot].double()
+            # as in test_received_weights
+            bound = got * (2 * max(s for _, s in rows) + (len(rows) + 4) * 2.0 ** -24) + (3 * 2.0 ** -24 * old if decay else 0.0) + 1e-37
+            assert_within(c.w[page, h, slot], got + (decay * old if decay else 0.0), bound, "weights")
+
+
 def test_weights_of_padded_rows():
     c, q, _ = build(21, "bf16", 4, 2, 64, 16, [0, 20, 40], fresh=[0, 0, 1], weights=True)
     before = c.w.clone()
