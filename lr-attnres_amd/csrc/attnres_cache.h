@@ -67,9 +67,9 @@ struct CacheAttendParams {
   int32_t group, rows, blocks;  // query heads of a key / value head; with the new tokens; blocks of them
   int32_t row_bits;             // 4 or 5: rows of a block, 2^row_bits
   int32_t wgs;                  // of a split cache
-  int32_t weight_wgs;           // that add the weights up in a launch of their own
+  int32_t weight_waves;         // that add the weights up in a launch of their own, four a workgroup
   int32_t own_weights;          // the workgroup of a whole segment does it
-  FastDiv by_group, by_blocks, by_segs, by_wgs, by_weight_wgs;  // segments: kv_heads * blocks
+  FastDiv by_group, by_blocks, by_segs, by_wgs, by_weight_waves;  // segments: kv_heads * blocks
   int32_t direct;               // a workgroup takes a whole segment
   int32_t tile;                 // 64 / 128 / 256: the head width it covers
   int32_t vb;                   // bytes (16, 8, 4 or a value's) that every row starts and ends at a multiple of

@@ -671,20 +671,28 @@ __device__ __forceinline__ void att_row_out(const CacheAttendParams& p, int b, i
 }
 
 // One token's weight: w_j <- decay w_j + got
-__device__ __forceinline__ void add_weight(const CacheAttendParams& p, int b, int h, int j, float got) {
+struct OldWeight {
+  float* at;  // null: no page
+  float w;    // (decay 0 reads none)
+};
+__device__ __forceinline__ OldWeight old_weight(const CacheAttendParams& p, int b, int h, int j) {
   const int at = div_by(j, p.c.by_page), page = p.c.table[b * p.c.table_stride + at];
-  if ((unsigned)page >= (unsigned)p.c.pages) return;
+  if ((unsigned)page >= (unsigned)p.c.pages) return OldWeight{nullptr, 0.f};
   float* w = p.c.w + page * p.c.w_page_stride + h * p.c.w_head_stride + (j - at * p.c.page_size);
-  *w = p.decay == 0.f ? got : p.decay * *w + got;
+  return OldWeight{w, p.decay == 0.f ? 0.f : *w};
+}
+__device__ __forceinline__ void add_weight(const CacheAttendParams& p, const OldWeight& old, float got) {
+  if (old.at) *old.at = p.decay == 0.f ? got : p.decay * old.w + got;
 }
 
 // By the workgroup that has all of the head's queries and tokens, from the scores that it has stored.
 __device__ __forceinline__ void add_own_weights(const CacheAttendParams& p, int b, int h, int rows, int n, const float* lse) {
   const float* x = p.logits + (b * (int64_t)p.q_heads + h * p.group) * p.logit_stride;
   for (int j = threadIdx.x; j < n; j += kAttWaves * kWave) {
+    const OldWeight old = old_weight(p, b, h, j);
     float sum = 0.f;
     for (int r = 0; r < rows; ++r) sum += __builtin_amdgcn_exp2f(x[r * p.logit_stride + j] - lse[r]);
-    add_weight(p, b, h, j, sum);
+    add_weight(p, old, sum);
   }
 }
 
@@ -861,17 +869,16 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
 
 // What each cached token received: with the scores x as attention left them (base-2 logarithms),
 //   w_j <- decay w_j + sum over the head's queries of 2^(x_j - lse).
-// Bound by memory: a group's scores read, the weights read and written, 4 bytes each.  Tokens are dealt
-// to workgroups as attention's units are; a row's lse comes from its pieces again, beside the join, which would
-// otherwise have to end first.
+// 4 bytes a query and token are read, and the weights read and written: bound by the latency of its loads.  A wave takes
+// a unit of tokens, two a lane, with no barrier; rows' lse come from their pieces again, beside the join, which would
+// otherwise have to end first: a lane takes one piece of one row, as many rows at a time as lanes hold.
+// (8 sequences of 4096 to 8191 tokens, 16 heads: 7 us; 9.6 with a workgroup a unit and a row's pieces over a wave.)
 __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) {
-  __shared__ float lse[256];  // of the head's rows, 256 of them at a time
-  __shared__ float half[kAttUnit];
-  static_assert(2 * kAttUnit == 256, "two threads a token");
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, segs = p.c.kv_heads;
+  constexpr int kEach = kAttUnit / kWave, kAhead = 4;  // tokens of a lane; rows whose scores are on their way together
+  const int lane = threadIdx.x & (kWave - 1), segs = p.c.kv_heads, block = 1 << p.row_bits;
   Chunk seqs;
   Seq seq{0, 0};
-  const Deal d = deal(p, segs, p.weight_wgs, p.by_weight_wgs, seqs);
+  const Deal d = deal(p, segs, p.weight_waves, p.by_weight_waves, seqs);
   const int x1 = deal_start(d, at + 1);
   Deal of;  // attention's
   of.total = d.total * p.blocks;
@@ -883,41 +890,83 @@ __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) 
       find_unit(p, segs, x, seqs, &b, &seq, &b_start, &units);
       b_end = b_start + segs * units;
     }
-    const int n = seq.n;
-    const int h = (x - b_start) / units, j = (x - b_start - h * units) * kAttUnit + threadIdx.x % kAttUnit;
-    const int part = threadIdx.x / kAttUnit;  // of the rows
-    float sum = 0.f;
-    for (int g0 = 0; g0 < p.group; g0 += 256) {
-      const int rows = min(256, p.group - g0);
-      __syncthreads();
-      for (int r = wave; r < rows; r += 256 / kWave) {
-        const int row = g0 + r;
-        const Pieces s = pieces_of(p, of, b_start * p.blocks + (h * p.blocks + (row >> p.row_bits)) * units, units);
+    const int h = (x - b_start) / units, j0 = (x - b_start - h * units) * kAttUnit + lane;
+    const float* const scores = p.logits + (b * (int64_t)p.q_heads + h * p.group) * p.logit_stride + j0;
+    const float* const row_ml = p.row_ml + (b * (int64_t)p.q_heads + h * p.group) * 2;
+    OldWeight old[kEach];
+    float sum[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      sum[e] = 0.f;
+      old[e] = j0 + e * kWave < seq.n ? old_weight(p, b, h, j0 + e * kWave) : OldWeight{nullptr, 0.f};
+    }
+    for (int r0 = 0; r0 < p.group; r0 += block) {  // rows whose pieces are the same workgroups'
+      const int rows = min(block, p.group - r0);
+      const Pieces s = pieces_of(p, of, b_start * p.blocks + (h * p.blocks + (r0 >> p.row_bits)) * units, units);
+      // lanes of a row, 2^bits: as many as it has pieces, if all rows find room
+      const int pieces = s.w1 - s.w0 + 1;
+      const int bits = pieces <= 1 ? 0 : min(32 - __clz(pieces - 1), max(0, rows > 1 ? 6 - (32 - __clz(rows - 1)) : 6));
+      for (int q0 = 0; q0 < rows; q0 += kWave >> bits) {
+        const int some = min(kWave >> bits, rows - q0), q = q0 + (lane >> bits);
+        float first[kAhead][kEach];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+            first[i][e] = i < some && j0 + e * kWave < seq.n ? scores[(r0 + q0 + i) * p.logit_stride + e * kWave] : -INFINITY;
         float top = -INFINITY, l = 0.f;
-        if (s.w0 == s.w1) {
-          top = p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2];
-          l = lane ? 0.f : p.row_ml[(b * (int64_t)p.q_heads + h * p.group + row) * 2 + 1];
-        }
-        for (int w = s.w0 + lane; w <= s.w1 && s.w0 != s.w1; w += kWave) {
-          const int64_t i = piece_row(p, s, w, row);
-          const float m = p.part_ml[i * 2], to = fmaxf(top, m);
-          l = att_share(top, to) * l + att_share(m, to) * p.part_ml[i * 2 + 1];
-          top = to;
+        if (q < rows) {
+          if (pieces <= 1) {
+            top = row_ml[(r0 + q) * 2];
+            l = row_ml[(r0 + q) * 2 + 1];
+          } else {
+            for (int w = s.w0 + (lane & ((1 << bits) - 1)); w <= s.w1; w += kAhead << bits) {
+              float m[kAhead], part[kAhead];
+#pragma unroll
+              for (int i = 0; i < kAhead; ++i) {
+                const int64_t at = piece_row(p, s, min(w + (i << bits), s.w1), r0 + q);
+                m[i] = p.part_ml[at * 2];
+                part[i] = p.part_ml[at * 2 + 1];
+              }
+#pragma unroll
+              for (int i = 0; i < kAhead; ++i) {
+                if (w + (i << bits) > s.w1) break;
+                const float to = fmaxf(top, m[i]);
+                l = att_share(top, to) * l + att_share(m[i], to) * part[i];
+                top = to;
+              }
+            }
+          }
         }
         float all = top;
-        for (int o = 1; o < kWave; o <<= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
-        l = wave_sum(att_share(top, all) * l);
-        if (lane == 0) lse[r] = all + log2f(l);
+        for (int o = 1; o < 1 << bits; o <<= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
+        l *= att_share(top, all);
+        for (int o = 1; o < 1 << bits; o <<= 1) l += __shfl_xor(l, o, kWave);
+        const float lse = all + log2f(l);
+        for (int i0 = 0; i0 < some; i0 += kAhead) {
+          float next[kAhead][kEach];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+              next[i][e] = i0 + kAhead + i < some && j0 + e * kWave < seq.n
+                               ? scores[(r0 + q0 + i0 + kAhead + i) * p.logit_stride + e * kWave] : -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i >= some) break;
+            const float base = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lse), (i0 + i) << bits));
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) sum[e] += __builtin_amdgcn_exp2f(first[i][e] - base);
+          }
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) first[i][e] = next[i][e];
+        }
       }
-      __syncthreads();
-      if (j < n)
-        for (int r = part; r < rows; r += 2)
-          sum += __builtin_amdgcn_exp2f(p.logits[(b * (int64_t)p.q_heads + h * p.group + g0 + r) * p.logit_stride + j] - lse[r]);
     }
-    if (part) half[threadIdx.x - kAttUnit] = sum;
-    __syncthreads();
-    if (part || j >= n) continue;
-    add_weight(p, b, h, j, sum + half[threadIdx.x]);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) add_weight(p, old[e], sum[e]);
   }
 }
 
@@ -925,7 +974,7 @@ __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) 
 template <class DT, int HD>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p, int joins) {
   if ((int)blockIdx.x < joins) join_row<DT, HD>(p, blockIdx.x);
-  else add_weights(p, blockIdx.x - joins);
+  else add_weights(p, (blockIdx.x - joins) * (256 / kWave) + threadIdx.x / kWave);
 }
 
 template <class DT, int HD>
@@ -940,8 +989,8 @@ hipError_t run_attend(const CacheAttendParams& p, hipStream_t st) {
   else if constexpr (DT::kCode != 0) cache_attend_kernel<DT, HD, 2, false, 1><<<grid, wg, 0, st>>>(p);
   const hipError_t err = hipGetLastError();
   const int joins = p.direct ? 0 : p.c.batch * p.c.kv_heads * p.rows;
-  if (err != hipSuccess || joins + p.weight_wgs == 0) return err;
-  cache_join_kernel<DT, HD><<<dim3((unsigned)(joins + p.weight_wgs)), dim3(256), 0, st>>>(p, joins);
+  if (err != hipSuccess || joins + p.weight_waves == 0) return err;
+  cache_join_kernel<DT, HD><<<dim3((unsigned)(joins + p.weight_waves / (256 / kWave))), dim3(256), 0, st>>>(p, joins);
   return hipGetLastError();
 }
 

@@ -268,8 +268,9 @@ extern "C" int attnres_cache_attend(const attnres_cache_desc* c, const attnres_c
   p.own_weights = c->weights && a.direct && a.blocks == 1;
   if (c->weights && !p.own_weights) {
     const int64_t units = c->batch * c->kv_heads * ((p.c.room + kAttUnit - 1) / kAttUnit);
-    p.weight_wgs = (int32_t)(units < 8 * kCus ? units : 8 * kCus);
-    p.by_weight_wgs = fast_div(p.weight_wgs);
+    const int64_t wgs = (units + 3) / 4;
+    p.weight_waves = (int32_t)(wgs < 8 * kCus ? wgs : 8 * kCus) * 4;
+    p.by_weight_waves = fast_div(p.weight_waves);
   }
   p.tile = a.tile;
   p.row_bits = a.row_bits;
