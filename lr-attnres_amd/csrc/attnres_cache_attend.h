@@ -802,17 +802,15 @@ __device__ __forceinline__ int64_t piece_row(const CacheAttendParams& p, const P
   return ((int64_t)(2 * w + (w == s.w0 ? 1 : 0)) << p.row_bits) + (row & ((1 << p.row_bits) - 1));
 }
 
-// A head's pieces joined; zeros for rows that see nothing, NaN for counts that cannot be.  A workgroup for each
-// row: its threads take four columns each, and a share of the pieces.
+// A head's pieces joined; zeros for rows that see nothing, NaN for counts that cannot be.  A workgroup's threads take
+// four columns of a row each, and a share of its pieces.
 template <class DT, int HD>
-__device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
+__device__ __forceinline__ void join_row(const CacheAttendParams& p, int at, const Deal& d, Chunk& seqs) {
   __shared__ float sm[256], sl[256];
   __shared__ sw_f4 so[256];
   const int row = at % p.rows, bh = at / p.rows, b = bh / p.c.kv_heads, h = bh - b * p.c.kv_heads;
   const int segs = p.c.kv_heads * p.blocks;
-  Chunk seqs;
-  const Deal d = deal(p, segs, p.wgs, p.by_wgs, seqs);
-  if (p.c.batch > kWave) {
+  if (b < seqs.b0 || b >= seqs.b0 + kWave) {
     seqs.load(p, 0, 0);
     while (b >= seqs.b0 + kWave) seqs.load(p, seqs.b0 + kWave, seqs.last());
   }
@@ -846,6 +844,7 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at) {
       top = to;
     }
   }
+  __syncthreads();  // (the row before it has been read)
   sm[threadIdx.x] = top;
   sl[threadIdx.x] = l;
   so[threadIdx.x] = o;
@@ -970,11 +969,21 @@ __device__ __forceinline__ void add_weights(const CacheAttendParams& p, int at) 
   }
 }
 
-// joins: workgroups that join rows; the others behind them add weights up
+// Of many rows most were one workgroup's and have nothing to join (512 new tokens of 4 x 16 heads
+// over 2000 to 4096, 32768 rows: 169 us with a workgroup each, 158 with 2048 or 1024 in all).
+constexpr int kAttJoins = 2048;  // workgroups at most
+
+// joins: workgroups that join rows, one after the other and those of a segment in many; those behind them add weights up
 template <class DT, int HD>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p, int joins) {
-  if ((int)blockIdx.x < joins) join_row<DT, HD>(p, blockIdx.x);
-  else add_weights(p, (blockIdx.x - joins) * (256 / kWave) + threadIdx.x / kWave);
+  if ((int)blockIdx.x < joins) {
+    Chunk seqs;
+    const Deal d = deal(p, p.c.kv_heads * p.blocks, p.wgs, p.by_wgs, seqs);
+    const int rows = p.c.batch * p.c.kv_heads * p.rows;
+    for (int at = blockIdx.x; at < rows; at += joins) join_row<DT, HD>(p, at, d, seqs);
+  } else {
+    add_weights(p, (blockIdx.x - joins) * (256 / kWave) + threadIdx.x / kWave);
+  }
 }
 
 template <class DT, int HD>
@@ -988,7 +997,7 @@ hipError_t run_attend(const CacheAttendParams& p, hipStream_t st) {
   else if (p.vb == 4) cache_attend_kernel<DT, HD, 4, false, 1><<<grid, wg, 0, st>>>(p);
   else if constexpr (DT::kCode != 0) cache_attend_kernel<DT, HD, 2, false, 1><<<grid, wg, 0, st>>>(p);
   const hipError_t err = hipGetLastError();
-  const int joins = p.direct ? 0 : p.c.batch * p.c.kv_heads * p.rows;
+  const int rows = p.direct ? 0 : p.c.batch * p.c.kv_heads * p.rows, joins = rows < kAttJoins ? rows : kAttJoins;
   if (err != hipSuccess || joins + p.weight_waves == 0) return err;
   cache_join_kernel<DT, HD><<<dim3((unsigned)(joins + p.weight_waves / (256 / kWave))), dim3(256), 0, st>>>(p, joins);
   return hipGetLastError();

@@ -229,6 +229,17 @@ def test_blocks_of_many_rows(dtype, T, H, K, Dh, S):
     check(c, q.flip(-1), cached, fresh, pass_fresh=True, scale=-0.4)
 
 
+@pytest.mark.parametrize("dtype,T,H,K,Dh,batch", [("bf16", 150, 8, 2, 64, 2), ("fp32", 9, 4, 2, 16, 70)])
+def test_more_rows_than_workgroups_that_join(dtype, T, H, K, Dh, batch):
+    g = gen(T)
+    cached = torch.randint(0, 400, (batch,), generator=g).tolist()
+    fresh = [T, *torch.randint(0, T + 1, (batch - 1,), generator=g).tolist()]
+    assert batch * H * T > 2048
+    c, q, _ = build(T, dtype, H, K, Dh, 16, cached, T=T, fresh=fresh)
+    widen(c, T * (H // K))
+    check(c, q, cached, fresh, pass_fresh=True)
+
+
 @pytest.mark.parametrize("T", [17, 40])
 def test_what_is_not_finite_in_blocks_of_many_rows(T):
     cached = [70, 300]
