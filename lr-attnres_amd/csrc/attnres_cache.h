@@ -54,7 +54,7 @@ struct CacheAppendParams {
   void* k;  // or null
 };
 
-// vec, lanes: as launch_qkv_rotary's
+// vec: values of a load; lanes: loads of that width that cover a head
 hipError_t launch_cache_append(int dtype, bool f32_table, const CacheAppendParams& p, int vec, int lanes, hipStream_t st);
 
 constexpr int kAttUnit = 128;  // tokens of a unit of attention's work

@@ -8,8 +8,8 @@
 // of 64 in all, bf16, 166 MB in 36 us (4.6 TB/s).  Single tokens are bound by the latency of a launch and
 // the chain count -> block table -> store, 3.5 us; the projection's loads do not wait for it.
 //
-// Layout.  As the projection's kernel: LANES lanes a head, VEC consecutive values (16
-// bytes) a lane, up to kGroups head groups a wave.  A row of a page is as long as a head, so
+// Layout.  As the projection's kernel: LANES lanes a head, vectors of VEC consecutive values (16
+// bytes where rows allow) a lane, up to kGroups head groups a wave.  A row of a page is as long as a head, so
 // stores are whole rows whatever the pages' order.
 #include "attnres_cache.h"
 #include "attnres_rotary.h"
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheApp
 }
 
 // Any alignment: one wave per head, its pairs in turn, the sum and the pairs in two passes over the row.  Single
-// values: 49 x 180 tokens of 66 heads of 86, fp16, 269 us, where pairs in the vector kernel take 106 (and 88 columns, in eights, 48).
+// values: 49 x 180 tokens of 66 heads of 86, fp16, 269 us, where pairs in the vector kernel take 66 (and 88 columns, in eights, 48).
 template <class DT, class TT>
 __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_general(CacheAppendParams p) {
   using S = typename DT::S;
@@ -209,16 +209,20 @@ hipError_t pick(const CacheAppendParams& p, int vec, int lanes, hipStream_t st) 
       if (lanes == 32) return run<DT, TT, 8, 32>(p, st);
     }
   }
+  // Narrower vectors: 16 lanes a head, several vectors each, keep four heads' loads on their way in a group (us, 16 lanes / one
+  // vector a lane: 9 x 209 tokens of 45 heads of 148, 16 bits, 19.1 / 24.3; of 32 heads of 128 in fp32 12.7 / 13.7; 49 x 180 of 66
+  // heads of 86 66 / 95; but 9 x 400 of 24 heads of 252 25 / 23.  8 lanes were slower from 100 on; with eights, two vectors a
+  // lane 45 / 43.5 for 8 x 2048 tokens of 24 heads of 128.)
   if (vec == 4) {
     if (lanes == 8) return run<DT, TT, 4, 8>(p, st);
     if (lanes == 16) return run<DT, TT, 4, 16>(p, st);
-    if (lanes == 32) return run<DT, TT, 4, 32>(p, st);
-    if (lanes == 64) return run<DT, TT, 4, 64>(p, st);
+    if (lanes == 32) return run<DT, TT, 4, 16, 2>(p, st);
+    if (lanes == 64) return run<DT, TT, 4, 16, 4>(p, st);
   }
   if (vec == 2) {
-    if (lanes == 32) return run<DT, TT, 2, 32>(p, st);
-    if (lanes == 64) return run<DT, TT, 2, 64>(p, st);
-    if (lanes == 128) return run<DT, TT, 2, 64, 2>(p, st);  // two vectors a lane
+    if (lanes == 32) return run<DT, TT, 2, 16, 2>(p, st);
+    if (lanes == 64) return run<DT, TT, 2, 16, 4>(p, st);
+    if (lanes == 128) return run<DT, TT, 2, 16, 8>(p, st);
   }
   if (vec != 1) return hipErrorInvalidValue;
   dim3 grid;

@@ -154,14 +154,13 @@ extern "C" int attnres_cache_append(const attnres_cache_desc* c, const attnres_c
   p.q = q;
   p.k = k;
   // the widest vector that every row starts at a multiple of, and the lanes that cover a
-  // head with it; vec 1 is the general kernel
+  // head with one each; vec 1 is the general kernel
   const int es = es_of(c->dtype), ts = es_of(d->table_dtype);
   int vec = 1, lanes = 1;
   for (int v = 16 / es; v >= 2 && vec == 1; v /= 2) {
     if (!rows_at(c, v) || !aligned(d->qkv, v * es) || d->batch_stride % v || d->token_stride % v || !aligned(q, v * es) ||
         !aligned(k, v * es) || !aligned(d->sin, v / 2 * ts) || !aligned(d->cos, v / 2 * ts) || d->table_row_stride % (v / 2))
       continue;
-    // (128: two vectors a lane)
     for (int n = v == 8 ? 4 : v == 4 ? 8 : 32; n <= (v == 8 ? 32 : v == 4 ? 64 : 128); n *= 2)
       if (vec == 1 && n * v >= c->head_dim) vec = v, lanes = n;
   }
