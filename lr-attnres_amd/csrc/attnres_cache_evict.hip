@@ -192,16 +192,85 @@ __device__ __forceinline__ bool no_choice(const CacheEvictParams& p, int n, int3
   return p.budget == p.recent;
 }
 
-// tables of at most R * TH tokens
-template <int R, int TH>
+// Rows i of what a head keeps: key, value and weight of each, from tokens j (none: -1), by `lanes` threads of which this
+// is `col`; per: vectors V of a row.  The loads of U rows are on their way together.
+template <class V, int U>
+__device__ __forceinline__ void copy_rows(const CacheEvictParams& p, int b, int h, const int (&i)[U], const int (&j)[U], int col,
+                                          int lanes, int per) {
+  const CachePages& c = p.c;
+  int from[U], to[U], slot[U], slot_to[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = div_by(max(j[u], 0), c.by_page), at_to = div_by(i[u], c.by_page);
+    from[u] = j[u] < 0 ? -1 : c.table[b * c.table_stride + at];
+    to[u] = j[u] < 0 ? -1 : p.new_table[b * p.new_stride + at_to];
+    slot[u] = j[u] - at * c.page_size;
+    slot_to[u] = i[u] - at_to * c.page_size;
+  }
+  bool move[U];
+  int64_t src[U], dst[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    move[u] = (unsigned)from[u] < (unsigned)c.pages && (unsigned)to[u] < (unsigned)c.pages &&
+              (from[u] != to[u] || slot[u] != slot_to[u]);
+    src[u] = (from[u] * c.page_stride + h * c.head_stride + slot[u] * c.slot_stride) * p.es;
+    dst[u] = (to[u] * c.page_stride + h * c.head_stride + slot_to[u] * c.slot_stride) * p.es;
+  }
+  for (int x = col; x < per; x += lanes) {
+    V k[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (move[u]) {
+        k[u] = ((const V*)((const char*)c.k + src[u]))[x];
+        v[u] = ((const V*)((const char*)c.v + src[u]))[x];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (move[u]) {
+        ((V*)((char*)c.k + dst[u]))[x] = k[u];
+        ((V*)((char*)c.v + dst[u]))[x] = v[u];
+      }
+  }
+  if (col == 0) {
+    float w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (move[u]) w[u] = c.w[from[u] * c.w_page_stride + h * c.w_head_stride + slot[u]];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (move[u]) c.w[to[u] * c.w_page_stride + h * c.w_head_stride + slot_to[u]] = w[u];
+  }
+}
+
+constexpr int kOwnRows = 4;  // on their way together, of a thread whose workgroup chose them
+
+// What a head keeps, by the workgroup that chose it
+template <class V, int TH>
+__device__ __forceinline__ void copy_own(const CacheEvictParams& p, int b, int h, const int* kept) {
+  const int per = p.c.head_dim * p.es / (int)sizeof(V), lanes = min(per, kWave), here = TH / lanes;
+  const int col = threadIdx.x % lanes, row = threadIdx.x / lanes;
+  if (row >= here) return;
+  int i[kOwnRows], j[kOwnRows];
+#pragma unroll
+  for (int u = 0; u < kOwnRows; ++u) {
+    i[u] = row + u * here;
+    j[u] = i[u] < p.budget ? kept[i[u]] : -1;
+  }
+  copy_rows<V, kOwnRows>(p, b, h, i, j, col, lanes, per);
+}
+
+// tables of at most R * TH tokens; OWN: the workgroup copies what it chose
+template <int R, int TH, bool OWN>
 __global__ __launch_bounds__(TH) void evict_select_kernel(CacheEvictParams p) {
   __shared__ int hist[kBins<TH>];
   __shared__ SelectShared<R, TH> s;
+  __shared__ int own[OWN ? TH * kOwnRows : 1];
   const int b = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads;
   uint32_t key[R];
   load_keys<R, TH>(p.c, b, h, 0, key);
   const int n = max(cache_count(p.c, b), 0);
-  int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
+  int32_t* const out = p.kept + (int64_t)blockIdx.x * p.budget;
+  int32_t* const kept = OWN ? own : out;
   if (h == 0 && threadIdx.x == 0) p.left[b] = min(n, p.budget);
   if (!no_choice<TH>(p, n, kept)) {
     const int early = n - p.recent;
@@ -216,6 +285,14 @@ __global__ __launch_bounds__(TH) void evict_select_kernel(CacheEvictParams p) {
       });
     }
     place(key, 0, early, f, 0, 0, kept, s);
+  }
+  if constexpr (OWN) {
+    __syncthreads();
+    if (p.vb == 16) copy_own<u32x4, TH>(p, b, h, own);
+    else if (p.vb == 8) copy_own<u32x2, TH>(p, b, h, own);
+    else if (p.vb == 4) copy_own<uint32_t, TH>(p, b, h, own);
+    else copy_own<uint16_t, TH>(p, b, h, own);
+    for (int i = threadIdx.x; i < p.budget; i += TH) out[i] = own[i];
   }
 }
 
@@ -315,26 +392,6 @@ __global__ __launch_bounds__(kBig) void evict_place_kernel(CacheEvictParams p) {
   place(key, j0, early, f, above, equal, kept, s);
 }
 
-// Row i of what a head keeps: its key, value and weight, from token j, by `lanes` threads of which this is `col`.
-template <class V>
-__device__ __forceinline__ void copy_row(const CacheEvictParams& p, int b, int h, int i, int j, int col, int lanes, int per) {
-  const CachePages& c = p.c;
-  const int at = div_by(j, c.by_page), at_to = div_by(i, c.by_page);
-  const int from = c.table[b * c.table_stride + at], to = p.new_table[b * p.new_stride + at_to];
-  if ((unsigned)from >= (unsigned)c.pages || (unsigned)to >= (unsigned)c.pages) return;
-  const int slot = j - at * c.page_size, slot_to = i - at_to * c.page_size;
-  if (from == to && slot == slot_to) return;
-  const int64_t src = (from * c.page_stride + h * c.head_stride + slot * c.slot_stride) * p.es;
-  const int64_t dst = (to * c.page_stride + h * c.head_stride + slot_to * c.slot_stride) * p.es;
-  for (int x = col; x < per; x += lanes) {
-    const V k = ((const V*)((const char*)c.k + src))[x], v = ((const V*)((const char*)c.v + src))[x];
-    ((V*)((char*)c.k + dst))[x] = k;
-    ((V*)((char*)c.v + dst))[x] = v;
-  }
-  if (col == 0)
-    c.w[to * c.w_page_stride + h * c.w_head_stride + slot_to] = c.w[from * c.w_page_stride + h * c.w_head_stride + slot];
-}
-
 // lanes: of a row (of its vectors V)
 template <class V>
 __global__ __launch_bounds__(256) void evict_copy_kernel(CacheEvictParams p, int lanes, int per, int64_t rows) {
@@ -343,7 +400,7 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(CacheEvictParams p, int
   for (int64_t row = (int64_t)blockIdx.x * here + threadIdx.x / lanes; row < rows; row += (int64_t)gridDim.x * here) {
     const int bh = (int)(row / p.budget), i = (int)(row - (int64_t)bh * p.budget);
     const int b = bh / p.c.kv_heads, h = bh % p.c.kv_heads, j = p.kept[row];
-    if (j >= 0) copy_row<V>(p, b, h, i, j, col, lanes, per);
+    if (j >= 0) copy_rows<V, 1>(p, b, h, {i}, {j}, col, lanes, per);
   }
 }
 
@@ -352,17 +409,22 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(CacheEvictParams p, int
 hipError_t launch_cache_evict(const CacheEvictParams& p, hipStream_t st) {
   const int64_t heads = (int64_t)p.c.batch * p.c.kv_heads;
   const dim3 sel((unsigned)(heads * p.slices)), wg(kBig);
+  const int per = p.c.head_dim * p.es / p.vb, lanes = per < 64 ? per : 64;
+  // A workgroup copies what it chose where its threads take all of it at once, so that no second launch waits for the first
+  // (us, one / two launches: 3 heads, 49 rows of 64 16-bit values 7.9 / 10.0; 16 x 12 heads, 128 rows 10.4 / 11.1; 40 x 16 heads
+  // 15.0 / 17.4; 16 x 8 heads, 64 rows of 128 9.9 / 10.4.  In two turns: 128 rows of 128 14.0 / 12.0, 256 of 64 14.8 / 13.6).
+  const bool own = p.c.room <= kR * kFew && p.budget <= kFew / lanes * kOwnRows;
   if (p.slices == 1) {
-    if (p.c.room <= kR * kFew) evict_select_kernel<kR, kFew><<<sel, dim3(kFew), 0, st>>>(p);
-    else if (p.c.room <= kSlice) evict_select_kernel<kR, kBig><<<sel, wg, 0, st>>>(p);
-    else evict_select_kernel<2 * kR, kBig><<<sel, wg, 0, st>>>(p);
+    if (own) evict_select_kernel<kR, kFew, true><<<sel, dim3(kFew), 0, st>>>(p);
+    else if (p.c.room <= kR * kFew) evict_select_kernel<kR, kFew, false><<<sel, dim3(kFew), 0, st>>>(p);
+    else if (p.c.room <= kSlice) evict_select_kernel<kR, kBig, false><<<sel, wg, 0, st>>>(p);
+    else evict_select_kernel<2 * kR, kBig, false><<<sel, wg, 0, st>>>(p);
   } else {
     for (int round = 0; round < 3; ++round) evict_count_kernel<<<sel, wg, 0, st>>>(p, round);
     evict_place_kernel<<<sel, wg, 0, st>>>(p);
   }
   hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  const int per = p.c.head_dim * p.es / p.vb, lanes = per < 64 ? per : 64;
+  if (err != hipSuccess || own) return err;
   const int64_t rows = heads * p.budget, blocks = (rows + 256 / lanes - 1) / (256 / lanes);
   const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
   if (p.vb == 16) evict_copy_kernel<u32x4><<<grid, dim3(256), 0, st>>>(p, lanes, per, rows);
