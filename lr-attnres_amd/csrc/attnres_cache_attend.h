@@ -844,7 +844,6 @@ __device__ __forceinline__ void join_row(const CacheAttendParams& p, int at, con
       top = to;
     }
   }
-  __syncthreads();  // (the row before it has been read)
   sm[threadIdx.x] = top;
   sl[threadIdx.x] = l;
   so[threadIdx.x] = o;
@@ -980,7 +979,12 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttendParams p, in
     Chunk seqs;
     const Deal d = deal(p, p.c.kv_heads * p.blocks, p.wgs, p.by_wgs, seqs);
     const int rows = p.c.batch * p.c.kv_heads * p.rows;
-    for (int at = blockIdx.x; at < rows; at += joins) join_row<DT, HD>(p, at, d, seqs);
+    for (int at = blockIdx.x;;) {
+      join_row<DT, HD>(p, at, d, seqs);
+      at += joins;
+      if (at >= rows) break;
+      __syncthreads();
+    }
   } else {
     add_weights(p, (blockIdx.x - joins) * (256 / kWave) + threadIdx.x / kWave);
   }
