@@ -733,10 +733,9 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 || RB * HD > 128 ? 1 : 
     const int row0 = (seg - a.h * p.blocks) * kRows, rows = min(kRows, p.rows - row0);
     const bool whole = u0 == 0 && u1 == units;
     a.piece(row0, rows, u0 * kAttUnit, p.direct ? p.c.room : u1 * kAttUnit, seq, so);
-    const int64_t slot = 2 * w + (u0 == 0 ? 1 : 0);
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      if (rb * 16 >= rows) break;
+      if (RB > 1 && rb * 16 >= rows) break;
       if (a.n > 0 && rb * 16 + a.c < rows) {
         if (a.g == 0) {
           sm[a.wave][rb * 16 + a.c] = a.m[rb] == -INFINITY ? a.m[rb] : a.base_of(a.m[rb]);
@@ -776,6 +775,7 @@ __global__ __launch_bounds__(kAttWaves* kWave, HD == 256 || RB * HD > 128 ? 1 : 
             ml[1] = l;
           }
         } else {
+          const int64_t slot = 2 * w + (u0 == 0 ? 1 : 0);
           *(sw_f4*)(p.part + (slot * kRows + r) * HD + col) = o;
           if (col == 0) {
             p.part_ml[(slot * kRows + r) * 2] = top;
