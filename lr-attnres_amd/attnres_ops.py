@@ -2121,10 +2121,11 @@ def _cache_evict_fake(k_pages, v_pages, weights, block_table, cached, new_table,
 
 
 def _int32(t: Tensor) -> Tensor:
-    """An integer tensor in int32; what it cannot hold becomes a value that no page, count or row has."""
+    """An integer tensor in int32; what it cannot hold becomes the nearest value, which no page, count or row is, nor comes to
+    with a call's new tokens (fewer than 2^31) added."""
     if t.dtype == torch.int32:
         return t
-    return (t.clamp(-1, 2 ** 31 - 1) if t.dtype == torch.int64 else t).to(torch.int32)
+    return (t.clamp(-2 ** 31, 2 ** 31 - 1) if t.dtype == torch.int64 else t).to(torch.int32)
 
 
 def _cache_ints(what: str, name: str, t: Tensor, shape: tuple) -> Tensor:
@@ -2228,6 +2229,8 @@ def qkv_norm_rotary_cached(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor
             raise RuntimeError(f"{what}: {name} must be a floating-point table, got {t.dtype}")
     if sin.shape != cos.shape:
         raise RuntimeError(f"{what}: sin {tuple(sin.shape)} and cos {tuple(cos.shape)} differ in shape")
+    if sin.size(-2) >= 2 ** 31 and positions is not None and positions.dtype == torch.int64:
+        raise RuntimeError(f"{what}: positions of 64 bits in tables of {sin.size(-2)} rows, above {2 ** 31 - 1}")
     _check_gpu([qkv, sin, cos, *(() if positions is None else (positions,))], what)
     rot = qkv.dtype if sin.dtype == cos.dtype == qkv.dtype else torch.float32
     sin, cos = (t.to(rot).reshape(-1, Dh // 2).contiguous() for t in (sin, cos))
