@@ -419,16 +419,17 @@ struct Att {
 #pragma unroll
         for (int i = 0; i < kKs; ++i) sw_mfma<DT>(k[s][i], q[r][i], s4[r][s]);
       }
-    float scale[kSub];  // NaN where there is no page: the row shows it
+    // a page that is not there shows as NaN in the rows that see its tokens: all of them, or those that are not masked
+    float scale[kSub];
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
-      scale[s] = PAGE16 && !now.there[s] && (!CUT || t0 + 16 * s < n) ? __builtin_nanf("") : p.scale;
+      scale[s] = PAGE16 && !CUT && !now.there[s] ? __builtin_nanf("") : p.scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const bool gone = !PAGE16 && (unsigned)__shfl(now.page, 16 * s + g * 4 + t, kWave) >= (unsigned)p.c.pages;
+        const bool gone = PAGE16 ? CUT && !now.there[s] : (unsigned)__shfl(now.page, 16 * s + g * 4 + t, kWave) >= (unsigned)p.c.pages;
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-          if (!PAGE16 && gone) s4[r][s][t] = __builtin_nanf("");
+          if (gone) s4[r][s][t] = __builtin_nanf("");
           if (CUT && t0 + 16 * s + g * 4 + t >= row[r].lim) s4[r][s][t] = -INFINITY;
         }
       }

@@ -64,3 +64,39 @@ def test_positions_and_counts_of_64_bits_below_zero():
     huge = sin[:1].expand(2 ** 31, -1)
     with pytest.raises(RuntimeError, match="positions of 64 bits"):
         ops.qkv_norm_rotary_cached(qkv, H, huge, huge, c.k, c.v, c.table, c.cached, positions=far64)
+
+
+def widen(c, rows):
+    """Columns of the table that no token is in, as many as make it a call of many bytes: blocks of 32 rows."""
+    columns = -(-(256 << 20) // (c.B * c.K * -(-rows // 16) * 2 * c.Dh * c.k.element_size() * c.S)) + 1
+    more = torch.full((c.B, max(0, columns - c.table.size(1))), -7, **I32)
+    c.table = torch.cat([c.table, more], 1)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype,Dh", [("bf16", 64), ("fp16", 128), ("fp32", 40)])
+@pytest.mark.parametrize("S,T", [(16, 2), (16, 20), (32, 5), (24, 2), (24, 20), (7, 9), (1, 3)])
+def test_rows_that_do_not_read_a_missing_page(S, T, dtype, Dh, wide):
+    """Rows up to the last token of a page, the next one missing: those that read it are NaN, the others as if it were there."""
+    H, K = 4, 2
+    cached = [max(0, 2 * S - 1 - T // 2), 5 * S - 1, 3]
+    g = gen(S * T)
+    c = Cache(g, DT[dtype], K, Dh, S, cached, max(cached) + T + S)
+    c.put(g, [n + T for n in cached])
+    q = queries(g, 3, H, T, Dh, DT[dtype])
+    if wide:
+        widen(c, 2 * T)
+    e, bound, _ = attend_ref(c, q, cached, [T] * 3, Dh ** -0.5)
+    good = ops.cached_attention(q, c.k, c.v, c.table, c.cached)
+    assert_within(good, e, bound, "all pages there")
+    first = [2 * S, 5 * S]  # tokens of the missing pages
+    c.table[0, 2], c.table[1, 5] = -1, c.k.size(0)
+    o = ops.cached_attention(q, c.k, c.v, c.table, c.cached)
+    for b in range(2):
+        for t in range(T):
+            if cached[b] + t >= first[b]:
+                assert bool(o[b, :, t].isnan().all()), (b, t)
+            else:
+                assert_within(o[b, :, t], e[b, :, t], bound[b, :, t], f"sequence {b}, row {t}")
+    assert cached[0] < first[0] and cached[1] < first[1] <= cached[1] + T - 1
+    assert torch.equal(o[2], good[2])
