@@ -113,12 +113,13 @@ __device__ __forceinline__ void find_unit(const CacheAttendParams& p, int segs, 
 
 #ifdef ATTNRES_CACHE_ATTEND_KERNELS
 
-// A matrix product's result must not be read for some cycles.  The compiler counts them inside a block of
-// code but has been seen to miss them over a branch (a score tile whose zeroing branch came right before it
-// was read two instructions after its product, and wrong); where a branch may come between, this waits.
+// A matrix product's result must not be read for 8 (16 bits) or 10 (fp32) issue slots.  The compiler counts them, but where
+// a branch around some code lies between it has been seen to count the way through that code alone: the short way then
+// reads too soon (a score tile whose zeroing branch came right before it was read two instructions after its product, and
+// wrong).  Branches come from plain selects too, so this waits where one may come between.
 __device__ __forceinline__ void att_settle() {
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_nop 15\n\ts_nop 15");
+  asm volatile("s_nop 15");
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -400,7 +401,6 @@ struct Att {
     constexpr bool CUT = !AHEAD;
     Rows after;
     if constexpr (AHEAD) after = rows_of(min(t0 + 2 * kStep, (n - 1) & -kTok), n);
-    // (before all of the products: no branch comes between them and what reads them)
     if (!p.whole) {
 #pragma unroll
       for (int s = 0; s < kSub; ++s)
@@ -419,6 +419,7 @@ struct Att {
 #pragma unroll
         for (int i = 0; i < kKs; ++i) sw_mfma<DT>(k[s][i], q[r][i], s4[r][s]);
       }
+    att_settle();
     // a page that is not there shows as NaN in the rows that see its tokens: all of them, or those that are not masked
     float scale[kSub];
 #pragma unroll
