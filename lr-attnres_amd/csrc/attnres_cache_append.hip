@@ -54,9 +54,9 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_kernel(CacheApp
   using TS = typename TT::S;
   constexpr int kHeads = kWave / LANES;  // heads of a group
   const int lane = threadIdx.x & (kWave - 1);
-  const int wid = (int)rot_wave();
-  const int tok = div_by(wid, by_groups);
-  if (tok >= p.n_tok) return;
+  const int64_t wave_at = rot_wave();  // (a grid of two dimensions ends behind 2^31 waves)
+  if (wave_at >= (int64_t)p.n_tok * groups) return;
+  const int wid = (int)wave_at, tok = div_by(wid, by_groups);
   const int part = wid - tok * groups;
   const int b = div_by(tok, p.by_tokens), t = tok - b * p.tokens;
   const int n_rot = p.q_heads + p.c.kv_heads, n_all = n_rot + p.c.kv_heads;
@@ -140,9 +140,9 @@ __global__ __launch_bounds__(kRotWaves* kWave) void cache_append_general(CacheAp
   using TS = typename TT::S;
   const int lane = threadIdx.x & (kWave - 1);
   const int n_rot = p.q_heads + p.c.kv_heads, n_all = n_rot + p.c.kv_heads;
-  const int wid = (int)rot_wave();
-  const int tok = wid / n_all;
-  if (tok >= p.n_tok) return;
+  const int64_t wave_at = rot_wave();  // (a grid of two dimensions ends behind 2^31 waves)
+  if (wave_at >= (int64_t)p.n_tok * n_all) return;
+  const int wid = (int)wave_at, tok = wid / n_all;
   const int h = wid - tok * n_all;
   const int b = div_by(tok, p.by_tokens), t = tok - b * p.tokens;
   const int Dh = p.c.head_dim;

@@ -100,3 +100,23 @@ def test_rows_that_do_not_read_a_missing_page(S, T, dtype, Dh, wide):
                 assert_within(o[b, :, t], e[b, :, t], bound[b, :, t], f"sequence {b}, row {t}")
     assert cached[0] < first[0] and cached[1] < first[1] <= cached[1] + T - 1
     assert torch.equal(o[2], good[2])
+
+
+def test_the_most_heads_that_a_call_takes():
+    """3 x 715827882 heads, 2 below 2^31, a wave each (rows that start anywhere): the grid's two dimensions end behind 2^31
+    waves, and those have no head."""
+    T, Dh = (2 ** 31 - 1) // 3, 2
+    flat = torch.zeros((T * 3 * Dh + 1,), dtype=torch.float16, device=DEV)
+    qkv = flat[1:].view(1, T, 3 * Dh)
+    qkv[:, :5] = torch.randn((1, 5, 3 * Dh), generator=gen(2)).to(torch.float16).to(DEV)
+    qkv[:, 5:8] = 1.0  # (padding: in no query, no page)
+    qkv[:, -3:] = 1.0
+    angle = torch.rand((8, Dh // 2), generator=gen(3))
+    sin, cos = angle.sin().to(DEV), angle.cos().to(DEV)
+    c = Cache(gen(4), torch.float16, 1, Dh, 4, [0], 8, fill=0.125)
+    q = ops.qkv_norm_rotary_cached(qkv, 1, sin, cos, c.k, c.v, c.table, c.cached, fresh=torch.tensor([5], **I32))
+    k, v = c.k.clone(), c.v.clone()
+    c.k.fill_(0.125), c.v.fill_(0.125)
+    want = ops.qkv_norm_rotary_cached(qkv[:, :5], 1, sin, cos, c.k, c.v, c.table, c.cached)
+    assert torch.equal(q[:, :, :5], want) and torch.equal(k, c.k) and torch.equal(v, c.v)
+    assert not bool(q[:, :, 5:].any())
