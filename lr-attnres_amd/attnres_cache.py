@@ -132,9 +132,10 @@ class PagedCache:
         per = -(-budget // self.page_size)
         if per * len(long) > len(self._free):
             raise RuntimeError(f"{per * len(long)} pages are needed and {len(self._free)} of {self.pages} are free")
-        owned = [list(o) for o in self._owned]
+        # (taken and given back once all layers have moved: a call that raises leaves the cache as it was)
+        free, owned = list(self._free), [list(o) for o in self._owned]
         for b in long:
-            owned[b] = [self._free.pop() for _ in range(per)]
+            owned[b] = [free.pop() for _ in range(per)]
         new = torch.full((self.batch, per), -1, dtype=torch.int32)
         for b, o in enumerate(owned):
             new[b, :min(per, len(o))] = torch.tensor(o[:per], dtype=torch.int32)
@@ -142,9 +143,9 @@ class PagedCache:
         kept = [ops.evict_cached_tokens(self.k[i], self.v[i], self.weights[i], self.table, self.cached, new, budget, recent)
                 for i in range(self.k.size(0))]
         for b in long:
-            self._free += reversed(self._owned[b])
+            free += reversed(self._owned[b])
             self.lengths[b] = budget
-        self._owned = owned
+        self._free, self._owned = free, owned
         self._write_table()
         self.cached.copy_(kept[0][1])
         return [k for k, _ in kept]

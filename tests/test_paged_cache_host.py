@@ -1,0 +1,50 @@
+"""CPU checks of the paged cache's bookkeeping where calls fail, and of what generation refuses before it has done anything."""
+
+import pytest
+import torch
+
+from attnres_cache import PagedCache
+from test_decoder_cache_host import CacheOps
+
+
+def filled(lengths, max_tokens=12, spare=6, **kw):
+    g = torch.Generator().manual_seed(5)
+    c = PagedCache(2, 2, 4, len(lengths), max_tokens, page_size=4, dtype=torch.float32, device="cpu", weights=True,
+                   spare_tokens=spare, **kw)
+    for t in (c.k, c.v, c.weights):
+        t.copy_(torch.randn(t.shape, generator=g))
+    c.reserve(lengths)
+    c.advance(lengths)
+    return c
+
+
+class Failing(CacheOps):
+    """Raises in the call of the layer given."""
+
+    def __init__(self, layer):
+        self.left = layer
+
+    def evict_cached_tokens(self, *args):
+        if self.left == 0:
+            raise RuntimeError("launch failed")
+        self.left -= 1
+        return CacheOps.evict_cached_tokens(*args)
+
+
+@pytest.mark.parametrize("layer", [0, 1])
+def test_an_eviction_that_raises_leaves_the_cache_as_it_was(layer):
+    c, want = filled([12, 3, 9]), filled([12, 3, 9])
+    before = (list(c._free), [list(o) for o in c._owned], c.table.clone(), c.cached.clone(), list(c.lengths))
+    with pytest.raises(RuntimeError, match="launch failed"):
+        c.evict(Failing(layer), 6, 2)
+    assert (c._free, c._owned, c.lengths) == (before[0], before[1], before[4])
+    assert torch.equal(c.table, before[2]) and torch.equal(c.cached, before[3])
+    # the same call again, as if it were the first
+    for a, b in zip(c.evict(CacheOps, 6, 2), want.evict(CacheOps, 6, 2)):
+        assert torch.equal(a, b)
+    assert torch.equal(c.table, want.table) and torch.equal(c.cached, want.cached) and c.lengths == want.lengths
+    for b, n in enumerate(c.lengths):
+        j = torch.arange(n)
+        page, slot = c.table[b].long()[j // 4], j % 4
+        for x, y in ((c.k, want.k), (c.v, want.v), (c.weights, want.weights)):
+            assert torch.equal(x[:, page, :, slot], y[:, page, :, slot])
