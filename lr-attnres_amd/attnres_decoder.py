@@ -300,14 +300,16 @@ class MultiHeadAttention(nn.Module):
         ops = self.ops if self.ops is not None else _default_ops()
         k, v = c.k[layer], c.v[layer]
         w = None if c.weights is None else c.weights[layer]
-        heads = ops.qkv_norm_rotary_cached(self.c_attn(x), self.n_head, self.rope.sin, self.rope.cos, k, v, step.table, c.cached,
+        qkv = self.c_attn(x)
+        dtype, qkv = qkv.dtype, qkv.to(k.dtype)
+        heads = ops.qkv_norm_rotary_cached(qkv, self.n_head, self.rope.sin, self.rope.cos, k, v, step.table, c.cached,
                                            fresh=step.fresh, positions=c.positions, qk_norm=self.qk_norm, weights=w,
                                            return_heads=step.prompt)
         if step.prompt:  # nothing is cached: attention inside the prompts alone, whose padding is behind them
             y = _attend(*heads)
         else:
             y = ops.cached_attention(heads, k, v, step.table, c.cached, fresh=step.fresh, weights=w if T == 1 else None)
-        return y.transpose(1, 2).reshape(B, T, C)
+        return y.transpose(1, 2).reshape(B, T, C).to(dtype)
 
     def forward(self, x: Tensor, step: Optional["CachedStep"] = None, layer: int = 0):
         if step is not None:
@@ -479,10 +481,13 @@ class Decoder(nn.Module):
         return self.lm_head(x)
 
     def new_cache(self, batch: int, max_tokens: Optional[int] = None, **kw) -> PagedCache:
-        """A cache for this model's layers, in its dtype and on its device."""
+        """A cache for this model's layers, on its device and in the dtype that its heads have: its parameters', or under
+        autocast that one's, unless ``dtype`` is given.  A step casts its heads to the cache's."""
         c, w = self.config, self.transformer.wte.weight
-        return PagedCache(c.n_layer, c.n_head, c.n_embd // c.n_head, batch, max_tokens or c.block_size, dtype=w.dtype,
-                          device=w.device, **kw)
+        if "dtype" not in kw:
+            kind = w.device.type
+            kw["dtype"] = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else w.dtype
+        return PagedCache(c.n_layer, c.n_head, c.n_embd // c.n_head, batch, max_tokens or c.block_size, device=w.device, **kw)
 
     def _begin_step(self, idx: Tensor, cache: PagedCache, fresh) -> CachedStep:
         B, T = idx.shape

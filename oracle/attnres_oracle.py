@@ -599,7 +599,7 @@ def qkv_norm_rotary_cached_ref(qkv, num_heads, sin, cos, k_pages, v_pages, block
     at = start.long()[:, None] + torch.arange(T)
     q, k, v = qkv_norm_rotary_ref(qkv, num_heads, sin, cos, positions=at.clamp(max=sin.numel() // sin.size(-1) - 1),
                                   num_kv_heads=K, qk_norm=qk_norm)
-    q, k = q.clone(), k.clone()
+    q, k = (t.to(qkv.dtype, copy=True) for t in (q, k))  # (tables of fp32 widen them)
     for b in range(B):
         n = T if fresh is None else int(fresh[b])
         q[b, :, n:] = 0
