@@ -19,6 +19,22 @@ import torch
 from torch import Tensor
 
 
+def send(numbers, like: Tensor) -> Tensor:
+    """Whole numbers of the host as an int32 tensor on ``like``'s device, in its stream's order: from pinned memory, so that
+    nothing waits for the GPU.  Not while a graph is captured, whose replays would read that memory again."""
+    t = torch.as_tensor(numbers, dtype=torch.int32)
+    if not like.is_cuda:
+        return t.to(like.device)
+    check_no_capture(like)
+    return t.pin_memory().to(like.device, non_blocking=True)
+
+
+def check_no_capture(like: Tensor) -> None:
+    if like.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a captured step takes no pages and no counts of its own: reserve its pages before the capture, and "
+                           "give every sequence the same number of tokens")
+
+
 class PagedCache:
     """Pages of ``layers`` layers for ``batch`` sequences of at most ``max_tokens`` cached tokens.
 
@@ -62,7 +78,7 @@ class PagedCache:
         rows = torch.full(tuple(self.table.shape), -1, dtype=torch.int32)
         for b, owned in enumerate(self._owned):
             rows[b, :len(owned)] = torch.tensor(owned, dtype=torch.int32)
-        self.table.copy_(rows)
+        self.table.copy_(send(rows, self.table))
 
     def _counts(self, fresh) -> list:
         new = [fresh] * self.batch if isinstance(fresh, int) else [int(n) for n in fresh]
@@ -83,6 +99,7 @@ class PagedCache:
         if sum(need) > len(self._free):
             raise RuntimeError(f"{sum(need)} pages are needed and {len(self._free)} of {self.pages} are free")
         if any(need):
+            check_no_capture(self.table)
             for b, n in enumerate(need):
                 self._owned[b] += [self._free.pop() for _ in range(n)]
             self._write_table()
@@ -90,8 +107,8 @@ class PagedCache:
     def advance(self, fresh) -> None:
         """``fresh`` tokens of each sequence have been written (into reserved pages)."""
         new = self._counts(fresh)
+        step = new[0] if len(set(new)) == 1 else send(new, self.cached)
         self.replayed(new)
-        step = new[0] if len(set(new)) == 1 else torch.tensor(new, dtype=torch.int32).to(self.cached.device)
         self.cached += step
         self.positions += step
 
@@ -111,11 +128,12 @@ class PagedCache:
 
     def drop(self, sequence: int) -> None:
         """Forgets a sequence: its pages are free, its next token is its first."""
+        check_no_capture(self.table)
         self._free += reversed(self._owned[sequence])
         self._owned[sequence] = []
         self.lengths[sequence] = self.next_positions[sequence] = 0
-        self.cached[sequence] = 0
-        self.positions[sequence] = 0
+        self.cached[sequence].zero_()
+        self.positions[sequence].zero_()
         self._write_table()
 
     def evict(self, ops, budget: int, recent: int = 0) -> list:
@@ -139,7 +157,7 @@ class PagedCache:
         new = torch.full((self.batch, per), -1, dtype=torch.int32)
         for b, o in enumerate(owned):
             new[b, :min(per, len(o))] = torch.tensor(o[:per], dtype=torch.int32)
-        new = new.to(self.table.device)
+        new = send(new, self.table)
         kept = [ops.evict_cached_tokens(self.k[i], self.v[i], self.weights[i], self.table, self.cached, new, budget, recent)
                 for i in range(self.k.size(0))]
         for b in long:

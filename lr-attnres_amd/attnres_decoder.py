@@ -65,7 +65,7 @@ import torch
 from torch import Tensor, nn
 from torch.nn import functional as F
 
-from attnres_cache import PagedCache
+from attnres_cache import PagedCache, send
 
 try:
     from torch.nn.attention import SDPBackend, sdpa_kernel
@@ -499,9 +499,9 @@ class Decoder(nn.Module):
         far = max(p + n for p, n in zip(cache.next_positions, new))
         if far > self.config.block_size:
             raise ValueError(f"position {far - 1} is outside block_size {self.config.block_size}")
+        counts = None if fresh is None else send(new, idx)
         cache.reserve(new)
         prompt = T > 1 and not any(cache.lengths)
-        counts = None if fresh is None else torch.tensor(new, dtype=torch.int32).to(idx.device)
         return CachedStep(cache, cache.table[:, :cache.pages_in_use()], counts, prompt)
 
     @torch.no_grad()
@@ -534,7 +534,7 @@ class Decoder(nn.Module):
             if fresh is None:
                 h = h[:, -1]
             else:
-                h = h[torch.arange(B, device=h.device), torch.tensor([n - 1 for n in fresh], device=h.device)]
+                h = h[torch.arange(B, device=h.device), send([n - 1 for n in fresh], h)]
             logits = self._logits(h)
             out[:, i] = logits.argmax(-1) if pick is None else pick(logits)
             tokens, fresh = out[:, i:i + 1], None

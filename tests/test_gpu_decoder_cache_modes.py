@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import attnres_decoder as AD
+import attnres_ops as ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -50,3 +51,53 @@ def test_generate_under_autocast(kw):
         own = m.generate(idx, 5, cache=m.new_cache(2, dtype=F32))
     assert out.shape == (2, 60) and own.shape == (2, 5)
     assert m.generate(idx, 5, cache=m.new_cache(2, dtype=BF)).shape == (2, 5)
+
+
+def test_steps_without_a_synchronization():
+    """Steps that take pages, steps of some sequences alone, evictions: nothing waits for the GPU."""
+    m = model(BF)
+    idx = torch.randint(0, 64, (3, 20), device=DEV)
+    lengths = [20, 3, 11]
+    cache = m.new_cache(3, page_size=4, weights=True, spare_tokens=40)
+
+    def work():
+        m(idx, cache=cache, fresh=lengths)
+        for _ in range(9):
+            m(idx[:, :1], cache=cache)
+        m(idx[:, :5], cache=cache, fresh=[5, 0, 2])
+        cache.evict(ops, 16, 4)
+        m(idx[:, :1], cache=cache)
+        m.generate(idx, 12, cache=cache, lengths=lengths, budget=24, recent=3)
+        for b in range(3):
+            cache.drop(b)
+
+    with torch.no_grad():
+        work()
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            work()
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+
+
+def test_a_captured_step_takes_no_pages_and_no_counts(monkeypatch):
+    """A replay would copy from host memory that has long been used again: refused, with nothing taken."""
+    m = model(BF)
+    idx = torch.randint(0, 64, (2, 6), device=DEV)
+    cache = m.new_cache(2, page_size=4, weights=True, spare_tokens=8)
+    with torch.no_grad():
+        m(idx, cache=cache)
+        before = list(cache._free), [list(o) for o in cache._owned], list(cache.lengths), cache.table.clone()
+        with monkeypatch.context() as patch:
+            patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            for call in (lambda: m(idx[:, :3], cache=cache),                       # a page more
+                         lambda: m(idx[:, :2], cache=cache, fresh=[2, 1]),         # counts
+                         lambda: cache.advance([1, 0]), lambda: cache.evict(ops, 4, 1), lambda: cache.drop(0)):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+        assert before[:3] == (cache._free, cache._owned, cache.lengths) and torch.equal(cache.table, before[3])
+        want = m(torch.cat([idx, idx[:, :3]], 1))[:, 6:]
+        got = m(idx[:, :3], cache=cache)
+    # (bf16 hidden states, as far apart as the ways of computing them are)
+    assert got.shape == want.shape and bool(torch.isfinite(got).all())
