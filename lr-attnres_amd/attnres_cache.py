@@ -7,8 +7,11 @@ table: a page number stands for that page of every layer.
 
 The host keeps the lengths and the free pages; the device has the block table and the counts that the operators read
 (``attnres_ops.qkv_norm_rotary_cached``, ``cached_attention``, ``evict_cached_tokens``), so a step needs no
-synchronization.  A step captured in a HIP graph advances the device's counts at every replay: reserve the pages of all
-of them before the capture, and tell the host with ``replayed``.
+synchronization.  What a call changes on the device it changes in the order of the current stream.
+
+A step captured in a HIP graph advances the device's counts at every replay, and the host's once, at its capture: that
+one is the first replay's.  So reserve the pages of all of them before the capture, and tell the host of every replay
+after the first with ``replayed``.
 """
 
 from __future__ import annotations
@@ -113,7 +116,8 @@ class PagedCache:
         self.positions += step
 
     def replayed(self, fresh) -> None:
-        """As ``advance``, the device's counts being advanced already: replays of a captured step."""
+        """As ``advance``, the device's counts being advanced already: by a replay of a captured step after its first (which the
+        capture itself has counted)."""
         new = self._counts(fresh)
         for b, n in enumerate(new):
             if self.lengths[b] + n > len(self._owned[b]) * self.page_size:
