@@ -17,6 +17,15 @@ extern "C" {
 #define ATTNRES_CACHE_MAX_HEAD_DIM 256
 #define ATTNRES_CACHE_MAX_TOKENS (1 << 30) /* of one sequence */
 #define ATTNRES_CACHE_MAX_SCALE 1e38f      /* (base-2 logarithms: log2(e) times it is finite) */
+/*
+ * Of one call (what the kernels count in 32 bits; more is ATTNRES_EUNSUPPORTED, but for the first ATTNRES_EINVAL):
+ */
+#define ATTNRES_CACHE_MAX_HEADS (1 << 20)       /* sequences; query heads; key / value heads */
+#define ATTNRES_CACHE_MAX_APPENDED INT32_MAX    /* batch * tokens * (q_heads + 2 kv_heads) */
+#define ATTNRES_CACHE_MAX_QUERIES (1 << 23)     /* batch * tokens * q_heads of attention */
+#define ATTNRES_CACHE_MAX_PIECES (INT32_MAX / 2) /* batch * kv_heads * blocks of 16 or 32 query rows * 128-token units of the table */
+#define ATTNRES_CACHE_MAX_EVICTED (1 << 21)     /* batch * kv_heads, times 8192-token slices of the table */
+#define ATTNRES_CACHE_MAX_KEPT INT32_MAX        /* batch * kv_heads * budget */
 
 /*
  * One layer's pages.  Token j of sequence b, head h lies at

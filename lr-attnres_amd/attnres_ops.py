@@ -2264,8 +2264,9 @@ def cached_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: T
     table has room for: give it the columns in use.
 
     A query that its sequence does not have gives zeros; a page not in [0, P) gives NaN in that sequence, in every row that
-    reads it, and a negative count or more tokens than the table has room for give NaN in all its rows.  Returns
-    [B, H, T, Dh], a view of a dense [B, T, H, Dh].  No backward.
+    reads it, and a negative count or more tokens than the table has room for give NaN in all its rows.  Calls of more
+    than 2^23 queries (B T H) are refused: split the batch or the tokens.  Returns [B, H, T, Dh], a view of a dense
+    [B, T, H, Dh].  No backward.
     """
     what = "cached_attention"
     nat = _native("cache_attend", "cache_attend")

@@ -21,12 +21,14 @@ int check_cache(const attnres_cache_desc* c) {
   if (!c) return api_fail(ATTNRES_EINVAL, "cache is NULL");
   if (c->dtype != ATTNRES_DTYPE_F32 && c->dtype != ATTNRES_DTYPE_BF16 && c->dtype != ATTNRES_DTYPE_F16)
     return api_fail(ATTNRES_EINVAL, "unknown dtype %d", c->dtype);
-  if (c->kv_heads < 1 || c->kv_heads > (1 << 20)) return api_fail(ATTNRES_EINVAL, "kv_heads=%d must be >= 1", c->kv_heads);
+  if (c->kv_heads < 1 || c->kv_heads > ATTNRES_CACHE_MAX_HEADS)
+    return api_fail(ATTNRES_EINVAL, "kv_heads=%d must be 1 .. %d", c->kv_heads, ATTNRES_CACHE_MAX_HEADS);
   if (c->head_dim < 1) return api_fail(ATTNRES_EINVAL, "head_dim=%d must be >= 1", c->head_dim);
   if (c->head_dim > ATTNRES_CACHE_MAX_HEAD_DIM)
     return api_fail(ATTNRES_EUNSUPPORTED, "head_dim=%d above %d", c->head_dim, ATTNRES_CACHE_MAX_HEAD_DIM);
   if (c->page_size < 1) return api_fail(ATTNRES_EINVAL, "page_size=%d must be >= 1", c->page_size);
-  if (c->batch < 0 || c->batch > (1 << 20)) return api_fail(ATTNRES_EINVAL, "batch=%lld", (long long)c->batch);
+  if (c->batch < 0 || c->batch > ATTNRES_CACHE_MAX_HEADS)
+    return api_fail(ATTNRES_EINVAL, "batch=%lld must be 0 .. %d", (long long)c->batch, ATTNRES_CACHE_MAX_HEADS);
   if (c->pages < 0 || c->pages > INT32_MAX) return api_fail(ATTNRES_EINVAL, "pages=%lld", (long long)c->pages);
   if (c->table_pages < 0) return api_fail(ATTNRES_EINVAL, "table_pages=%lld < 0", (long long)c->table_pages);
   if (c->table_pages > ATTNRES_CACHE_MAX_TOKENS / c->page_size)
@@ -91,10 +93,11 @@ int check_append(const attnres_cache_desc* c, const attnres_cache_append_desc* d
     return api_fail(ATTNRES_EINVAL, "table dtype %d is neither fp32 nor the cache's %d", d->table_dtype, c->dtype);
   if (d->tokens < 0 || d->tokens > (int64_t)1 << 30)
     return api_fail(ATTNRES_EINVAL, "tokens=%lld must be 0 .. 2^30", (long long)d->tokens);
-  if (d->q_heads < 1 || d->q_heads > (1 << 20)) return api_fail(ATTNRES_EINVAL, "q_heads=%d must be >= 1", d->q_heads);
+  if (d->q_heads < 1 || d->q_heads > ATTNRES_CACHE_MAX_HEADS)
+    return api_fail(ATTNRES_EINVAL, "q_heads=%d must be 1 .. %d", d->q_heads, ATTNRES_CACHE_MAX_HEADS);
   if (c->head_dim % 2) return api_fail(ATTNRES_EINVAL, "head_dim=%d must be even", c->head_dim);
   if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
-  if (c->batch * d->tokens > INT32_MAX / ((int64_t)d->q_heads + 2 * c->kv_heads))
+  if (c->batch * d->tokens > ATTNRES_CACHE_MAX_APPENDED / ((int64_t)d->q_heads + 2 * c->kv_heads))
     return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, %d + 2 * %d heads: too many", (long long)c->batch,
                     (long long)d->tokens, d->q_heads, c->kv_heads);
   if (!d->qkv || !d->sin || !d->cos) return api_fail(ATTNRES_EINVAL, "qkv / sin / cos is NULL");
@@ -112,16 +115,17 @@ int check_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d
   if (!d) return api_fail(ATTNRES_EINVAL, "desc is NULL");
   if (d->tokens < 0 || d->tokens > ATTNRES_CACHE_MAX_TOKENS)
     return api_fail(ATTNRES_EINVAL, "tokens=%lld must be 0 .. 2^30", (long long)d->tokens);
-  if (d->q_heads < 1 || d->q_heads > (1 << 20) || d->q_heads % c->kv_heads)
-    return api_fail(ATTNRES_EINVAL, "q_heads=%d must be a multiple of kv_heads=%d", d->q_heads, c->kv_heads);
+  if (d->q_heads < 1 || d->q_heads > ATTNRES_CACHE_MAX_HEADS || d->q_heads % c->kv_heads)
+    return api_fail(ATTNRES_EINVAL, "q_heads=%d must be a multiple of kv_heads=%d, at most %d", d->q_heads, c->kv_heads,
+                    ATTNRES_CACHE_MAX_HEADS);
   if (!(fabsf(d->scale) <= ATTNRES_CACHE_MAX_SCALE))
     return api_fail(ATTNRES_EINVAL, "scale must be finite, of at most %g", (double)ATTNRES_CACHE_MAX_SCALE);
   if (c->weights && d->tokens > 1) return api_fail(ATTNRES_EINVAL, "weights need a single new token, got %lld", (long long)d->tokens);
   if (c->weights && !(d->decay >= 0.f && d->decay <= 1.f)) return api_fail(ATTNRES_EINVAL, "decay must be 0 .. 1");
   if (c->batch == 0 || d->tokens == 0) return ATTNRES_OK;
-  if (c->batch * d->tokens > (1 << 23) / d->q_heads)
-    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d: too many queries", (long long)c->batch,
-                    (long long)d->tokens, d->q_heads);
+  if (c->batch * d->tokens > ATTNRES_CACHE_MAX_QUERIES / d->q_heads)
+    return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d: too many queries, above %d", (long long)c->batch,
+                    (long long)d->tokens, d->q_heads, ATTNRES_CACHE_MAX_QUERIES);
   if (!d->q) return api_fail(ATTNRES_EINVAL, "q is NULL");
   if (d->q_batch_stride < 0 || d->q_head_stride < 0 || d->q_token_stride < 0)
     return api_fail(ATTNRES_EINVAL, "q strides must be >= 0");
@@ -194,7 +198,8 @@ int plan_attend(const attnres_cache_desc* c, const attnres_cache_attend_desc* d,
   const int64_t blocks16 = (rows + 15) / 16;
   a->row_bits = a->page16 && blocks16 > 1 && heads * blocks16 * room_bytes >= 256 << 20 ? 5 : 4;
   const int64_t blocks = (rows + (1 << a->row_bits) - 1) >> a->row_bits, segs = heads * blocks;
-  if (rows > INT32_MAX || segs > (1 << 23) || segs * (units > 0 ? units : 1) > INT32_MAX / 2)
+  // (rows, and segs with them, are at most the queries)
+  if (segs * (units > 0 ? units : 1) > ATTNRES_CACHE_MAX_PIECES)
     return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, tokens=%lld, q_heads=%d, %lld cached: too many tokens", (long long)c->batch,
                     (long long)d->tokens, d->q_heads, (long long)room);
   a->tile = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
@@ -308,7 +313,7 @@ int check_evict(const attnres_cache_desc* c, int64_t budget, int64_t recent) {
   if (recent < 0 || recent > budget)
     return api_fail(ATTNRES_EINVAL, "recent=%lld must be 0 .. budget=%lld", (long long)recent, (long long)budget);
   const int64_t heads = c->batch * c->kv_heads, slices = (c->table_pages * c->page_size + kEvictSlice - 1) / kEvictSlice;
-  if (heads > (1 << 21) || heads * budget >= (int64_t)1 << 31 || heads * slices > (1 << 21))
+  if (heads > ATTNRES_CACHE_MAX_EVICTED || heads * budget > ATTNRES_CACHE_MAX_KEPT || heads * slices > ATTNRES_CACHE_MAX_EVICTED)
     return api_fail(ATTNRES_EUNSUPPORTED, "batch=%lld, kv_heads=%d, budget=%lld, %lld pages of %d: too many tokens",
                     (long long)c->batch, c->kv_heads, (long long)budget, (long long)c->table_pages, c->page_size);
   return ATTNRES_OK;
