@@ -119,12 +119,6 @@ __device__ __forceinline__ int cache_count(const CachePages& c, int b) {
   return n >= 0 && n <= c.room ? n : -1;
 }
 
-// page of token j of sequence b, -1: outside the cache
-__device__ __forceinline__ int cache_page(const CachePages& c, int b, int j) {
-  const int page = c.table[b * c.table_stride + div_by(j, c.by_page)];
-  return (unsigned)page < (unsigned)c.pages ? page : -1;
-}
-
 // over the lanes up to and with this one, by moves inside rows of 16 lanes and broadcasts of a row's last
 __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // 1, 2, 4, 8 to the right

@@ -29,6 +29,8 @@ namespace attnres {
 
 namespace {
 
+constexpr int kIters = 4;      // head groups of a wave, all loads of them in flight at once
+
 // row of the tables for token (b, t); -1: outside
 __device__ __forceinline__ int64_t rot_position(const QkvRotaryParams& p, int64_t b, int64_t t) {
   const int64_t at = p.pos ? p.pos[b * p.pos_b_stride + t * p.pos_t_stride] : p.start + t;

@@ -6,7 +6,6 @@
 namespace attnres {
 
 constexpr int kRotWaves = 4;   // waves of a workgroup
-constexpr int kIters = 4;      // head groups of a wave, all loads of them in flight at once
 
 template <class DT, int E>
 __device__ __forceinline__ void store_raw(typename DT::S* p, const Raw<DT, E>& r) {
