@@ -1,9 +1,12 @@
 """The paged cache's operators at the edges of what they are given: counts and positions that 32 bits do not hold, pages that
 some rows read and others do not, several new tokens whose rows are joined from pieces."""
 
+import ctypes
+
 import pytest
 import torch
 
+import _attnres_hip as lib
 import attnres_ops as ops
 from cache_util import Cache, assert_within, attend_ref
 
@@ -100,6 +103,44 @@ def test_rows_that_do_not_read_a_missing_page(S, T, dtype, Dh, wide):
                 assert_within(o[b, :, t], e[b, :, t], bound[b, :, t], f"sequence {b}, row {t}")
     assert cached[0] < first[0] and cached[1] < first[1] <= cached[1] + T - 1
     assert torch.equal(o[2], good[2])
+
+
+def workspace(c, q):
+    """Workspace bytes of a call, and what pieces of 256 workgroups' blocks of 16 rows take at most."""
+    d = lib.CacheAttendDesc()
+    d.q_heads, d.tokens, d.scale, d.q = q.size(1), q.size(2), 0.125, q.data_ptr()
+    n = lib.load().attnres_cache_attend_workspace_size(
+        ctypes.byref(lib.cache_desc(c.k, c.v, None, c.table, c.cached, None)), ctypes.byref(d))
+    tile = 64 if c.Dh <= 64 else 128 if c.Dh <= 128 else 256
+    return n, 2 * 256 * 16 * (tile + 2) * 4
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,H,K,Dh,S,layout", [
+    (7, 16, 4, 64, 32, "dense"), (4, 4, 4, 40, 24, "dense"), (9, 6, 2, 17, 7, "dense"), (20, 2, 1, 96, 20, "dense"),
+    (5, 8, 2, 96, 16, "dense"), (33, 2, 2, 64, 16, "tokens"), (3, 20, 2, 40, 24, "odd"), (6, 3, 1, 200, 20, "layer"),
+    (2, 1, 1, 256, 64, "dense"), (17, 2, 2, 62, 48, "dense")])
+def test_several_new_tokens_of_split_rows(dtype, T, H, K, Dh, S, layout):
+    """Tables so long that rows are read in pieces and joined, too short for blocks of 32 rows; padding among the new tokens."""
+    cached = [0, 5, 700, 2600, 131]
+    fresh = [T, 1, T - 1, T, 0]
+    g = gen(T * Dh + S)
+    c = Cache(g, DT[dtype], K, Dh, S, cached, max(cached) + T, layout)
+    c.put(g, [n + f for n, f in zip(cached, fresh)])
+    # (columns that no token is in, up to 1 MiB of keys and values a head and a little more)
+    need = -(-((1 << 20) + 4096) // (2 * Dh * c.k.element_size() * S))
+    more = torch.full((c.B, max(0, need - c.table.size(1))), 10 ** 9, **I32)
+    c.table = torch.cat([c.table, more], 1)
+    q = queries(g, c.B, H, T, Dh, DT[dtype])
+    n, most = workspace(c, q)
+    assert 0 < n <= most, "pieces, of blocks of 16 rows"
+    f = torch.tensor(fresh, **I32)
+    e, bound, _ = attend_ref(c, q, cached, fresh, Dh ** -0.5)
+    o = ops.cached_attention(q, c.k, c.v, c.table, c.cached, fresh=f)
+    assert_within(o, e, bound, "out")
+    for b, k in enumerate(fresh):
+        assert not bool(o[b, :, k:].any()), "rows that no sequence has are zeros"
+    assert torch.equal(ops.cached_attention(q, c.k, c.v, c.table, c.cached, fresh=f), o)
 
 
 def test_the_most_heads_that_a_call_takes():
