@@ -140,14 +140,18 @@ class PagedCache:
         self.positions[sequence].zero_()
         self._write_table()
 
-    def evict(self, ops, budget: int, recent: int = 0) -> list:
-        """Brings every sequence of more than ``budget`` tokens back to ``budget``: the last ``recent`` ones and, of each
-        layer's key / value head, those that received most attention.  They move into free pages; the old ones are free
-        afterwards.  Returns, for each layer, the places kept (``evict_cached_tokens``), or nothing where none was too long."""
+    def check_budget(self, budget: int, recent: int) -> None:
+        """Raises where ``evict`` could not go by them."""
         if self.weights is None:
             raise RuntimeError("evict goes by the attention that tokens received: PagedCache(weights=True)")
         if budget < 1 or not 0 <= recent <= budget:
             raise ValueError(f"budget {budget} and recent {recent} must be budget >= 1 and 0 <= recent <= budget")
+
+    def evict(self, ops, budget: int, recent: int = 0) -> list:
+        """Brings every sequence of more than ``budget`` tokens back to ``budget``: the last ``recent`` ones and, of each
+        layer's key / value head, those that received most attention.  They move into free pages; the old ones are free
+        afterwards.  Returns, for each layer, the places kept (``evict_cached_tokens``), or nothing where none was too long."""
+        self.check_budget(budget, recent)
         long = [b for b, n in enumerate(self.lengths) if n > budget]
         if not long:
             return []

@@ -522,8 +522,10 @@ class Decoder(nn.Module):
         if cache is None:
             most = min(self.config.block_size, T + max_new_tokens)
             # (with a budget, pages for a second copy of what is kept while it moves)
-            extra = {} if budget is None else dict(weights=True, spare_tokens=budget)
+            extra = {} if budget is None else dict(weights=True, spare_tokens=max(budget, 0))
             cache = self.new_cache(B, most, **extra)
+        if budget is not None:
+            cache.check_budget(budget, recent)
         far = max(p + n for p, n in zip(cache.next_positions, [T] * B if lengths is None else lengths)) + max_new_tokens - 1
         if far > self.config.block_size:
             raise ValueError(f"position {far - 1} is outside block_size {self.config.block_size}")

@@ -3,8 +3,9 @@
 import pytest
 import torch
 
+import attnres_decoder as AD
 from attnres_cache import PagedCache
-from test_decoder_cache_host import CacheOps
+from test_decoder_cache_host import CFG, CacheOps
 
 
 def filled(lengths, max_tokens=12, spare=6, **kw):
@@ -48,3 +49,22 @@ def test_an_eviction_that_raises_leaves_the_cache_as_it_was(layer):
         page, slot = c.table[b].long()[j // 4], j % 4
         for x, y in ((c.k, want.k), (c.v, want.v), (c.weights, want.weights)):
             assert torch.equal(x[:, page, :, slot], y[:, page, :, slot])
+
+
+def decoder():
+    torch.manual_seed(3)
+    return AD.Decoder(AD.DecoderConfig(**CFG), ops=CacheOps)
+
+
+@pytest.mark.parametrize("weights,budget,recent,error", [
+    (False, 8, 2, RuntimeError), (True, 0, 0, ValueError), (True, 8, 9, ValueError), (True, 8, -1, ValueError), (True, -3, 0, ValueError)])
+def test_generate_refuses_a_budget_before_its_first_token(weights, budget, recent, error):
+    m = decoder()
+    idx = torch.randint(0, 50, (2, 6))
+    cache = m.new_cache(2, page_size=4, weights=weights, spare_tokens=8)
+    with pytest.raises(error):
+        m.generate(idx, 3, cache=cache, budget=budget, recent=recent)
+    assert cache.lengths == [0, 0] and len(cache._free) == cache.pages
+    if weights:
+        with pytest.raises(error):
+            m.generate(idx, 3, budget=budget, recent=recent)
