@@ -511,8 +511,8 @@ class Decoder(nn.Module):
         [B, max_new_tokens].  The reference's model generates with a key-value cache too (``model.py:2662-2709``).
 
         ``pick`` takes logits [B, vocab] to the next tokens [B]; the largest logit's unless given.  With ``budget`` a sequence
-        that has a page's tokens more than that in the cache is brought back to it (``PagedCache.evict``, which keeps the last
-        ``recent``).  What counts is the attention of the generated tokens; a prompt's own is not added up, so that one that
+        that has a page's tokens more than that in the cache, or all that its cache takes, is brought back to it
+        (``PagedCache.evict``, which keeps the last ``recent``).  What counts is the attention of the generated tokens; a prompt's own is not added up, so that one that
         has to be cut at once keeps its beginning and its end.
         """
         B, T = idx.shape
@@ -540,7 +540,7 @@ class Decoder(nn.Module):
             logits = self._logits(h)
             out[:, i] = logits.argmax(-1) if pick is None else pick(logits)
             tokens, fresh = out[:, i:i + 1], None
-            if budget is not None and max(cache.lengths) >= budget + cache.page_size:
+            if budget is not None and max(cache.lengths) >= min(budget + cache.page_size, cache.max_tokens):
                 cache.evict(self.ops if self.ops is not None else _default_ops(), budget, recent)
         return out
 

@@ -68,3 +68,13 @@ def test_generate_refuses_a_budget_before_its_first_token(weights, budget, recen
     if weights:
         with pytest.raises(error):
             m.generate(idx, 3, budget=budget, recent=recent)
+
+
+def test_a_cache_with_less_than_a_page_above_the_budget():
+    """It is full before a sequence is a page above its budget: brought back then."""
+    m = decoder()
+    idx = torch.randint(0, 50, (2, 6))
+    cache = m.new_cache(2, 12, page_size=4, weights=True, spare_tokens=10)
+    out = m.generate(idx, 20, cache=cache, budget=10, recent=4)
+    assert out.shape == (2, 20) and max(cache.lengths) <= 12 and cache.next_positions == [25, 25]
+    assert cache.cached.tolist() == cache.lengths
