@@ -2201,7 +2201,8 @@ def qkv_norm_rotary_cached(qkv: Tensor, num_heads: int, sin: Tensor, cos: Tensor
     ``weights`` [P, K, S] (fp32): what each cached token received of attention so far, 0 for the new ones.
 
     A token that has no slot, or whose page is not in [0, P), is not written; a row outside the tables gives NaN (the values
-    of device tensors are not looked at on the host).  A page that is written to belongs to one sequence.
+    of device tensors are not looked at on the host).  A page that is written to belongs to one sequence.  Integers of any
+    kind are taken in 32 bits, the nearest where those do not hold them (so 64-bit positions need tables of less than 2^31 rows).
 
     Returns ``q`` [B, num_heads, T, Dh], dense; with ``return_heads`` also ``k`` [B, K, T, Dh], dense, and ``v`` [B, K, T, Dh],
     a view of ``qkv``: what attention inside a prompt reads.  No backward.

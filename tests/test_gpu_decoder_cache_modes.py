@@ -8,6 +8,7 @@ import torch
 
 import attnres_decoder as AD
 import attnres_ops as ops
+from attnres_cache import send
 from cache_util import append_ref, assert_within, attend_ref, evict_ref
 
 pytestmark = pytest.mark.gpu
@@ -104,6 +105,18 @@ def test_a_captured_step_takes_no_pages_and_no_counts(monkeypatch):
         got = m(idx[:, :3], cache=cache)
     # (bf16 hidden states, as far apart as the ways of computing them are)
     assert got.shape == want.shape and bool(torch.isfinite(got).all())
+
+
+def test_numbers_sent_while_the_stream_is_busy():
+    """Each from memory of its own until it has arrived, however far ahead the host is."""
+    like = torch.zeros((1,), dtype=torch.int32, device=DEV)
+    x = torch.randn((4096, 4096), device=DEV)
+    for _ in range(2):  # (the second time from memory that the first one used)
+        y = x
+        for _ in range(20):
+            y = (x @ y) * 1e-2
+        sent = [send([i, i * 7 + 1, -i], like) for i in range(500)]
+        assert torch.equal(torch.stack(sent).cpu(), torch.tensor([[i, i * 7 + 1, -i] for i in range(500)], dtype=torch.int32))
 
 
 class Checked:
