@@ -312,6 +312,9 @@ struct Att {
     if constexpr (DT::kCode == 2) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     else return pack2<DT>(a, b);
   }
+  // SHOWN: a weight too small for the first term has its smallest value there, so that an infinite value times it is
+  // infinite (fp16: 2^-38 of the largest weight, as much as the two terms may be off by anyway)
+  template <bool SHOWN>
   static __device__ __forceinline__ Weights split(const float (&e)[kSub][4]) {
     Weights w;
 #pragma unroll
@@ -320,7 +323,11 @@ struct Att {
       for (int t = 0; t < 4; t += 2) {
         w.e[s][t] = e[s][t], w.e[s][t + 1] = e[s][t + 1];
         if constexpr (!k32) {
-          const uint32_t x = terms(e[s][t], e[s][t + 1]);
+          uint32_t x = terms(e[s][t], e[s][t + 1]);
+          if constexpr (SHOWN) {
+            x |= (x & 0xffffu) == 0 && e[s][t] > 0.f ? 1u : 0u;
+            x |= x >> 16 == 0 && e[s][t + 1] > 0.f ? 0x10000u : 0u;
+          }
           w.hi[s * 2 + t / 2] = x;
           w.lo[s * 2 + t / 2] = terms(e[s][t] - bits_to_float<DT>(x & 0xffffu), e[s][t + 1] - bits_to_float<DT>(x >> 16));
         }
@@ -489,7 +496,7 @@ struct Att {
           e[s][t] = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[r][s][t], scale[s], -base));
           l[r] += e[s][t];
         }
-      return split(e);
+      return split<CARE && DT::kCode == 2>(e);
     };
     if constexpr (!CARE) {
       Weights w[RB];

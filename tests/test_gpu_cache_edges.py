@@ -161,3 +161,30 @@ def test_the_most_heads_that_a_call_takes():
     want = ops.qkv_norm_rotary_cached(qkv[:, :5], 1, sin, cos, c.k, c.v, c.table, c.cached)
     assert torch.equal(q[:, :, :5], want) and torch.equal(k, c.k) and torch.equal(v, c.v)
     assert not bool(q[:, :, 5:].any())
+
+
+@pytest.mark.parametrize("gap", [5.0, 26.0, 40.0, 60.0])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T", [1, 3])
+def test_an_infinite_value_of_a_small_weight(dtype, gap, T):
+    """exp(-gap) times an infinite value is infinite, not NaN, however much smaller than a 16-bit term it is; the other columns
+    and the rows before it are as ever."""
+    g = gen(int(gap))
+    cached = [130, 150]  # (tokens 0 .. 31 and 128 .. 159 are one wave's)
+    c = Cache(g, DT[dtype], 1, 64, 16, cached, 160)
+    c.put(g, [n + T for n in cached], std=0.125)
+    q = torch.zeros((2, 2, T, 64), dtype=DT[dtype], device=DEV)
+    q[..., 0] = 8.0  # scores are the keys' first values
+    for b, n in enumerate(cached):
+        page, slot = c.where(b, n + T)
+        c.k[page, 0, slot, 0] = 0.0
+        c.k[page[20], 0, slot[20], 0] = gap  # one token has the largest score, all others are `gap` below
+        last = n + T - 1                      # (the last new token: rows before it do not see it)
+        c.v[page[last], 0, slot[last], 7] = float("inf")
+        c.v[page[27], 0, slot[27], 9] = -float("inf")
+    e, bound, _ = attend_ref(c, q, cached, [T, T], 0.125)
+    o = ops.cached_attention(q, c.k, c.v, c.table, c.cached, scale=0.125)
+    assert bool((o[:, :, T - 1, 7] == float("inf")).all()) and bool((o[..., 9] == -float("inf")).all())
+    fine = torch.isfinite(e)
+    assert int((~fine).sum()) == 2 * 2 * (T + 1)
+    assert_within(o[fine], e[fine], bound[fine], "finite")
